@@ -187,6 +187,17 @@ namespace rocwmma
                          : "memory");
         }
 
+        // Three-dimensional form of tma_load_2d.
+        ROCWMMA_DEVICE inline void tma_load_3d(void* dst, void const* tensorMap, uint64_t* bar,
+                                               int32_t x, int32_t y, int32_t z)
+        {
+            asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+                         " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_addr(dst)),
+                         "l"(reinterpret_cast<uint64_t>(tensorMap)), "r"(smem_addr(bar)), "r"(x),
+                         "r"(y), "r"(z)
+                         : "memory");
+        }
+
         // One-dimensional form: the box starting at element x (x * element size a multiple of
         // 16 bytes).
         ROCWMMA_DEVICE inline void tma_load_1d(void* dst, void const* tensorMap, uint64_t* bar,
@@ -415,6 +426,93 @@ namespace rocwmma
                              : "memory");
         }
 
+        // ---- block-scaled 4-bit operands --------------------------------------------------
+        // Operands of kind::mxf4 / kind::mxf4nvf4: E2M1 codes, two to a byte, K-major (64
+        // values of K per instruction, 32 bytes of a row), and one 8-bit scale per 32 (E8M0) or
+        // 16 (E4M3) of them, which the instruction reads from tensor memory.
+        enum class ScaleKind : uint32_t
+        {
+            E8M0_32, // MXF4: scale_vec::2X, two scales per instruction and row
+            E4M3_16 // NVF4: scale_vec::4X, four
+        };
+
+        // Instruction descriptor of the block-scaled kinds.  `scaleId`: which byte pair of the
+        // 32-bit scale words this instruction uses (0 or 2 with two scales, 0 with four).
+        ROCWMMA_HOST_DEVICE constexpr uint32_t make_instr_desc_scaled(ScaleKind kind, uint32_t m,
+                                                                      uint32_t n, uint32_t scaleId)
+        {
+            return (scaleId << 4) /* B */ | (1u << 7) | (1u << 10) /* E2M1 */ | ((n >> 3) << 17)
+                   | ((kind == ScaleKind::E8M0_32 ? 1u : 0u) << 23) | ((m >> 7) << 27)
+                   | (scaleId << 29) /* A */;
+        }
+
+        // Shared-memory descriptor of one 512-byte scale tile (128 rows x 4 scales, stored as
+        // 32 rows of 16 bytes: word j of row r belongs to operand row 32 j + r): no swizzle,
+        // groups of 8 rows are 128 bytes apart.
+        ROCWMMA_DEVICE inline uint64_t smem_desc_scales(uint32_t addr)
+        {
+            uint64_t d = 0;
+            d |= uint64_t((addr & 0x3ffffu) >> 4);
+            d |= uint64_t(128u >> 4) << 16;
+            d |= uint64_t(128u >> 4) << 32;
+            d |= uint64_t(1) << 46;
+            return d;
+        }
+        // Copies one scale tile to four columns of tensor memory, repeated in each quarter of
+        // its lanes.  Issued by ONE thread; later tcgen05.mma of that thread see it.
+        ROCWMMA_DEVICE inline void tmem_copy_scales(uint32_t taddr, uint64_t desc)
+        {
+            asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
+                         : "memory");
+        }
+        // The same for both blocks of a pair, each from its own shared memory.
+        ROCWMMA_DEVICE inline void tmem_copy_scales_pair(uint32_t taddr, uint64_t desc)
+        {
+            asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
+                         : "memory");
+        }
+        // D[tmem] (+)= A[smem] * B[smem] with the scales of A and B at the given columns.
+        template <ScaleKind Kind>
+        ROCWMMA_DEVICE inline void mma_scaled(uint32_t dTmem, uint64_t descA, uint64_t descB,
+                                              uint32_t idesc, uint32_t scaleA, uint32_t scaleB,
+                                              uint32_t accumulate)
+        {
+            if constexpr(Kind == ScaleKind::E8M0_32)
+                asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+                             "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X "
+                             "[%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(dTmem),
+                             "l"(descA), "l"(descB), "r"(idesc), "r"(scaleA), "r"(scaleB),
+                             "r"(accumulate)
+                             : "memory");
+            else
+                asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+                             "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X "
+                             "[%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(dTmem),
+                             "l"(descA), "l"(descB), "r"(idesc), "r"(scaleA), "r"(scaleB),
+                             "r"(accumulate)
+                             : "memory");
+        }
+        template <ScaleKind Kind>
+        ROCWMMA_DEVICE inline void mma_scaled_pair(uint32_t dTmem, uint64_t descA, uint64_t descB,
+                                                   uint32_t idesc, uint32_t scaleA,
+                                                   uint32_t scaleB, uint32_t accumulate)
+        {
+            if constexpr(Kind == ScaleKind::E8M0_32)
+                asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+                             "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X "
+                             "[%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(dTmem),
+                             "l"(descA), "l"(descB), "r"(idesc), "r"(scaleA), "r"(scaleB),
+                             "r"(accumulate)
+                             : "memory");
+            else
+                asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+                             "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X "
+                             "[%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(dTmem),
+                             "l"(descA), "l"(descB), "r"(idesc), "r"(scaleA), "r"(scaleB),
+                             "r"(accumulate)
+                             : "memory");
+        }
+
         // Makes `bar` complete one arrival when all tcgen05.mma issued so far by this
         // thread have finished (implies tcgen05.fence::before_thread_sync).
         ROCWMMA_DEVICE inline void mma_commit(uint64_t* bar)
@@ -494,6 +592,17 @@ namespace rocwmma
                              smem_addr(dst)),
                          "l"(reinterpret_cast<uint64_t>(tensorMap)), "r"(barClusterAddr), "r"(x),
                          "r"(y)
+                         : "memory");
+        }
+        ROCWMMA_DEVICE inline void tma_load_3d_pair(void* dst, void const* tensorMap,
+                                                    uint32_t barClusterAddr, int32_t x, int32_t y,
+                                                    int32_t z)
+        {
+            asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global"
+                         ".mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+                             smem_addr(dst)),
+                         "l"(reinterpret_cast<uint64_t>(tensorMap)), "r"(barClusterAddr), "r"(x),
+                         "r"(y), "r"(z)
                          : "memory");
         }
         ROCWMMA_DEVICE inline void tmem_alloc_pair(uint32_t* slot, uint32_t columns)

@@ -43,7 +43,9 @@ enum b200wmma_dtype
     B200WMMA_XF32 = 5, /* xfloat32_t: fp32 storage, low 13 bits zero    */
     B200WMMA_F64  = 6, /* float64_t                                     */
     B200WMMA_I32  = 7, /* int32_t (outputs of int8 GEMM)                */
-    B200WMMA_E5M2 = 8  /* bfloat8_t, OCP e5m2                           */
+    B200WMMA_E5M2 = 8, /* bfloat8_t, OCP e5m2                           */
+    B200WMMA_MXF4 = 9, /* E2M1 codes, one E8M0 scale per 32 values (OCP microscaling) */
+    B200WMMA_NVF4 = 10 /* E2M1 codes, one E4M3 scale per 16 values      */
 };
 
 /* Memory layouts (rocwmma.hpp:74-81, 106-110). */
@@ -229,6 +231,101 @@ B200WMMA_API int b200wmma_dlrm_fwd(int dtype, const void* input, void* output, u
  */
 B200WMMA_API int b200wmma_dlrm_bwd(int dtype, const void* input, const void* upstream, void* grad,
                       void* mlp_grad, uint32_t m, uint32_t k, uint32_t batch, void* stream);
+
+/*
+ * Embedding lookup (no counterpart in the reference, whose DLRM sample starts behind it): for
+ * every token (o, i) of outer x inner
+ *     out[o * out_outer + i * out_inner + j] = scale * table[row(o, i) * ldt + j],  0 <= j < dim,
+ * in fp32, rounded once to out_dtype (F16, BF16, F32; table_dtype likewise).  The id of the token
+ * is ids[o * ids_outer + i * ids_inner], 4 or 8 bytes wide (id_bytes).  first == NULL: row = id,
+ * in a table of `rows` rows.  Otherwise the table is `inner` tables one behind the other, column i
+ * of the tokens picks from the i-th: row = first[i] + id, 0 <= id < first[i + 1] - first[i], with
+ * first[0..inner] in device memory.  An id outside its table (-1 for padding) gives a row of
+ * zeros.  With out_outer = 27 * dim and out 27 * dim-strided from the second row on, the call
+ * writes the 26 categorical features of b200wmma_dlrm_fwd's input in place.
+ * Any alignment of whole elements; rows on 16-byte boundaries and dim a multiple of 8 are fast.
+ * rows < 2^31 - 1, outer * inner < 2^31 - 4096, dim <= 2^20.
+ */
+B200WMMA_API int b200wmma_embedding(int table_dtype, int out_dtype, uint64_t rows, uint32_t dim,
+                                    uint64_t outer, uint32_t inner, const void* table, uint64_t ldt,
+                                    const void* ids, int id_bytes, uint64_t ids_outer,
+                                    uint64_t ids_inner, const int64_t* first, void* out,
+                                    uint64_t out_outer, uint64_t out_inner, double scale,
+                                    void* stream);
+
+/*
+ * Gradient of the table of b200wmma_embedding:
+ *     table_grad[r * ldt + j] = scale * sum over the tokens of row r of grad[o * grad_outer + i * grad_inner + j]
+ * (+ the old value where accumulate != 0, which leaves rows without tokens untouched; without it
+ * those are set to zero).  Sums are fp32, the result is rounded once to table_dtype.  Tokens are
+ * sorted by row and summed in an order that depends on outer, inner, dim and the ids alone: the
+ * same call gives the same bits.  `workspace`: at least b200wmma_embedding_grad_workspace(...)
+ * bytes of device memory, 256-byte aligned, which the call may overwrite and leaves no state in;
+ * calls that can run at the same time need one each.
+ */
+B200WMMA_API uint64_t b200wmma_embedding_grad_workspace(uint64_t rows, uint32_t dim, uint64_t outer,
+                                                        uint32_t inner);
+B200WMMA_API int b200wmma_embedding_grad(int grad_dtype, int table_dtype, uint64_t rows,
+                                         uint32_t dim, uint64_t outer, uint32_t inner,
+                                         const void* grad, uint64_t grad_outer,
+                                         uint64_t grad_inner, const void* ids, int id_bytes,
+                                         uint64_t ids_outer, uint64_t ids_inner,
+                                         const int64_t* first, void* table_grad, uint64_t ldt,
+                                         double scale, int accumulate, void* workspace,
+                                         uint64_t workspace_bytes, void* stream);
+
+/*
+ * 4-bit block-scaled operands (MXF4, NVF4; no counterpart in the reference, whose types end at
+ * 8 bits).  An operand of `rows` x `k` values is two buffers, both 16-byte aligned:
+ *   codes   E2M1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two to a byte, the even
+ *           column in the low four bits; a row takes b200wmma_mx_pitch(k) = ceil(k / 32) * 16
+ *           bytes, rows are a multiple of 16 bytes (`ldq`, `lda`, `ldb`, in bytes) apart;
+ *   scales  b200wmma_mx_scale_bytes(fmt, rows, k) bytes: one for each block of 32 (MXF4, E8M0)
+ *           or 16 (NVF4, E4M3) values along k, in tiles of 128 rows x 4 blocks of 512 bytes,
+ *           [row tile][block group][row % 32][row / 32 % 4][block % 4].
+ * Codes between k and the pitch and scales behind the last row or block must be zero (as
+ * b200wmma_mx_quantize writes them): the product multiplies them with each other.
+ */
+B200WMMA_API uint64_t b200wmma_mx_pitch(uint32_t k);
+/* 0 for other formats. */
+B200WMMA_API uint64_t b200wmma_mx_scale_bytes(int fmt, uint32_t rows, uint32_t k);
+
+/*
+ * Quantises `rows` x `k` values x (F16, BF16 or F32; any alignment of whole elements), stored
+ * row-major (value (r, i) at x[r * ldx + i]) or column-major (x[i * ldx + r]); the codes of a row
+ * are contiguous along k either way, so the second form makes the operand of a product that sums
+ * over the first form's rows.  With y = x * 2^-exponent (|exponent| <= 64) and a = max |y| of a block:
+ *   MXF4  scale 2^(floor(log2 a) - 2), at least 2^-127
+ *   NVF4  scale E4M3(min(a / 6, 448)), rounded to nearest even
+ *   code  E2M1(y / scale), rounded to nearest even, magnitudes over 6 become 6.
+ * The operand then stands for code * scale * 2^exponent; an NVF4 caller chooses the exponent so
+ * that a / 6 lies in E4M3's range (2^-9 to 448) and hands 2^exponent to the product as part of alpha.
+ * Blocks of zeros, and those whose scale rounds to zero, have codes of zero; a block that holds an
+ * infinity or a NaN has the NaN scale (255 / 127).  Writes every byte of `scales` and of the
+ * codes' pitch, and nothing between the pitch and ldq.  Needs no scratch memory.
+ */
+B200WMMA_API int b200wmma_mx_quantize(int fmt, int in_dtype, uint32_t rows, uint32_t k,
+                                      const void* x, uint64_t ldx, int layout, int exponent,
+                                      void* codes, uint64_t ldq, void* scales, void* stream);
+
+/* The values code * scale * 2^exponent, rounded to out_dtype (F16, BF16 or F32), row-major. */
+B200WMMA_API int b200wmma_mx_dequantize(int fmt, int out_dtype, uint32_t rows, uint32_t k,
+                                        const void* codes, uint64_t ldq, const void* scales,
+                                        int exponent, void* out, uint64_t ldo, void* stream);
+
+/*
+ * D = alpha * A * B + beta * C on 4-bit block-scaled operands of one format, through the
+ * block-cooperative path.  A is m x k; B is k x n, given as an operand of n rows x k (column-major
+ * B).  C and D are row-major, F16, BF16 or F32 (out_dtype), accumulation and the arithmetic
+ * with alpha and beta are fp32.  c may be NULL when beta == 0 and may be d.  c and d 16-byte
+ * aligned, ldc and ldd times the element size multiples of 16 bytes; any m, n, k >= 1.  The first
+ * call on a device allocates a few bytes of status memory (make it outside stream capture).
+ */
+B200WMMA_API int b200wmma_mx_gemm(int fmt, int out_dtype, uint32_t m, uint32_t n, uint32_t k,
+                                  const void* a, const void* a_scales, const void* b,
+                                  const void* b_scales, const void* c, void* d, uint64_t lda,
+                                  uint64_t ldb, uint32_t ldc, uint32_t ldd, double alpha,
+                                  double beta, void* stream);
 
 /*
  * Waits for `stream` and reports whether any kernel of this library gave up on a

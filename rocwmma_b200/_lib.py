@@ -15,13 +15,13 @@ LIB_PATH = os.path.join(_HERE, "lib", "libb200wmma.so")
 TEST_LIB_PATH = os.path.join(_HERE, "lib", "libb200wmma_test.so")
 
 # dtype / layout / status codes (enum b200wmma_dtype etc.)
-F16, BF16, E4M3, I8, F32, XF32, F64, I32, E5M2 = range(9)
+F16, BF16, E4M3, I8, F32, XF32, F64, I32, E5M2, MXF4, NVF4 = range(11)
 ROW_MAJOR, COL_MAJOR = 0, 1
 OK = 0
 ERR_INVALID_ARG, ERR_UNSUPPORTED, ERR_ALIGNMENT, ERR_CUDA, ERR_DEVICE_WAIT, ERR_TOO_LARGE = (
     -1, -2, -3, -4, -5, -6)
 
-_u32, _i, _d, _p = C.c_uint32, C.c_int, C.c_double, C.c_void_p
+_u32, _u64, _i, _d, _p = C.c_uint32, C.c_uint64, C.c_int, C.c_double, C.c_void_p
 
 # name -> (restype, argtypes); every symbol include/rocwmma_b200.h declares
 SIGNATURES = {
@@ -40,6 +40,17 @@ SIGNATURES = {
     "b200wmma_gemv": (_i, [_i, _u32, _u32, _p, _p, _p, _p, _d, _d, _u32, _p]),
     "b200wmma_dlrm_fwd": (_i, [_i, _p, _p, _u32, _u32, _u32, _p]),
     "b200wmma_dlrm_bwd": (_i, [_i, _p, _p, _p, _p, _u32, _u32, _u32, _p]),
+    "b200wmma_embedding": (_i, [_i, _i, _u64, _u32, _u64, _u32, _p, _u64, _p, _i, _u64, _u64, _p, _p, _u64,
+                                _u64, _d, _p]),
+    "b200wmma_embedding_grad_workspace": (_u64, [_u64, _u32, _u64, _u32]),
+    "b200wmma_embedding_grad": (_i, [_i, _i, _u64, _u32, _u64, _u32, _p, _u64, _u64, _p, _i, _u64, _u64, _p,
+                                     _p, _u64, _d, _i, _p, _u64, _p]),
+    "b200wmma_mx_pitch": (_u64, [_u32]),
+    "b200wmma_mx_scale_bytes": (_u64, [_i, _u32, _u32]),
+    "b200wmma_mx_quantize": (_i, [_i, _i, _u32, _u32, _p, _u64, _i, _i, _p, _u64, _p, _p]),
+    "b200wmma_mx_dequantize": (_i, [_i, _i, _u32, _u32, _p, _u64, _p, _i, _p, _u64, _p]),
+    "b200wmma_mx_gemm": (_i, [_i, _i, _u32, _u32, _u32, _p, _p, _p, _p, _p, _p, _u64, _u64, _u32, _u32,
+                              _d, _d, _p]),
     "b200wmma_check_device": (_i, [_p, C.POINTER(_u32)]),
     "b200wmma_shutdown": (_i, []),
 }

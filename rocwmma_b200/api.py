@@ -168,3 +168,241 @@ def check_device(stream=None) -> None:
 
 def shutdown() -> None:
     L.check(L.lib().b200wmma_shutdown(), "b200wmma_shutdown")
+
+
+# ---- 4-bit block-scaled operands ------------------------------------------------------------
+# An operand is a pair (codes, scales) of uint8 tensors, as the C header lays them out.
+
+def _device_of(*ts):
+    """The one device of the given tensors; they may not be spread over several."""
+    _require_cuda(*ts)
+    devices = {t.device for t in ts if t is not None}
+    if len(devices) != 1:
+        raise ValueError(f"tensors on several devices: {sorted(map(str, devices))}")
+    return devices.pop()
+
+
+class _on:
+    """Makes `device` current for a call, with its stream (the given one, or that device's
+    current one) as the value; the switch is skipped where there is nothing to switch."""
+
+    def __init__(self, device, stream):
+        self.device, self.stream = device.index, stream
+        self.back = None
+
+    def __enter__(self):
+        now = torch.cuda.current_device()
+        if now != self.device:
+            self.back = now
+            torch.cuda.set_device(self.device)
+        return _stream(self.stream)
+
+    def __exit__(self, *_):
+        if self.back is not None:
+            torch.cuda.set_device(self.back)
+
+
+def _holds(t, what, count):
+    """Whether a contiguous tensor is large enough for what a call reads or writes of it."""
+    if not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous")
+    if t.numel() < count:
+        raise ValueError(f"{what} holds {t.numel()} elements, {count} needed")
+
+
+def _is_type(t, what, dtype):
+    if t.dtype != dtype:
+        raise ValueError(f"{what} is {t.dtype}, expected {dtype}")
+
+
+def mx_pitch(k):
+    """Bytes of one row of codes."""
+    return (k + 31) // 32 * 16
+
+
+def mx_scale_bytes(fmt, rows, k):
+    """Bytes of the scales of a rows x k operand."""
+    return L.lib().b200wmma_mx_scale_bytes(fmt, rows, k)
+
+
+def _operand(fmt, rows, k, operand, ld, what):
+    codes, scales = operand
+    for t, part in ((codes, "codes"), (scales, "scales")):
+        if t.dtype != torch.uint8:
+            raise ValueError(f"{part} of {what} are {t.dtype}, expected torch.uint8")
+    _holds(codes, f"codes of {what}", (rows - 1) * ld + mx_pitch(k))
+    _holds(scales, f"scales of {what}", mx_scale_bytes(fmt, rows, k))
+
+
+def mx_quantize(fmt, in_t, rows, k, x, layout=ROW_MAJOR, exponent=0, ldx=None, ldq=None, out=None,
+                stream=None):
+    """Quantises rows x k values to MXF4 or NVF4; returns (codes, scales).
+    layout: how x is stored (its k values contiguous, or its rows); ldx in elements, ldq in bytes."""
+    ldx = ldx or _natural_ld(layout, rows, k)
+    ldq = ldq or mx_pitch(k)
+    if out is None:
+        codes = torch.empty(rows * ldq, dtype=torch.uint8, device=x.device)
+        scales = torch.empty(mx_scale_bytes(fmt, rows, k), dtype=torch.uint8, device=x.device)
+        out = codes, scales
+    device = _device_of(x, *out)
+    _is_type(x, "x", _TORCH.get(in_t))
+    _holds(x, "x", (rows - 1) * ldx + k if layout == ROW_MAJOR else (k - 1) * ldx + rows)
+    _operand(fmt, rows, k, out, ldq, "out")
+    with _on(device, stream) as s:
+        rc = L.lib().b200wmma_mx_quantize(fmt, in_t, rows, k, _ptr(x), ldx, layout, exponent,
+                                          _ptr(out[0]), ldq, _ptr(out[1]), s)
+    L.check(rc, "b200wmma_mx_quantize")
+    return out
+
+
+def mx_dequantize(fmt, out_t, rows, k, codes, scales, exponent=0, ldq=None, ldo=None, out=None,
+                  stream=None):
+    """The values an operand stands for, times 2^exponent; row-major."""
+    ldq = ldq or mx_pitch(k)
+    ldo = ldo or k
+    if out is None:
+        out = torch.empty(rows * ldo, dtype=_TORCH.get(out_t), device=codes.device)
+    device = _device_of(codes, scales, out)
+    _is_type(out, "out", _TORCH.get(out_t))
+    _holds(out, "out", (rows - 1) * ldo + k)
+    _operand(fmt, rows, k, (codes, scales), ldq, "the operand")
+    with _on(device, stream) as s:
+        rc = L.lib().b200wmma_mx_dequantize(fmt, out_t, rows, k, _ptr(codes), ldq, _ptr(scales),
+                                            exponent, _ptr(out), ldo, s)
+    L.check(rc, "b200wmma_mx_dequantize")
+    return out
+
+
+def mx_gemm(fmt, out_t, m, n, k, a, b, c, alpha, beta, lda=None, ldb=None, ldc=None, ldd=None,
+            out=None, stream=None):
+    """D = alpha*A*B + beta*C on 4-bit block-scaled operands: a = (codes, scales) of m rows x k,
+    b of n rows x k (column-major B); C/D row-major.  lda, ldb in bytes."""
+    lda = lda or mx_pitch(k)
+    ldb = ldb or mx_pitch(k)
+    ldc = ldc or n
+    ldd = ldd or n
+    d = out if out is not None else torch.empty(m * ldd, dtype=_TORCH.get(out_t), device=a[0].device)
+    device = _device_of(*a, *b, c, d)
+    _operand(fmt, m, k, a, lda, "A")
+    _operand(fmt, n, k, b, ldb, "B")
+    _is_type(d, "out", _TORCH.get(out_t))
+    _holds(d, "out", (m - 1) * ldd + n)
+    if c is not None and beta != 0:
+        _is_type(c, "c", _TORCH.get(out_t))
+        _holds(c, "c", (m - 1) * ldc + n)
+    with _on(device, stream) as s:
+        rc = L.lib().b200wmma_mx_gemm(fmt, out_t, m, n, k, _ptr(a[0]), _ptr(a[1]), _ptr(b[0]),
+                                      _ptr(b[1]), _ptr(c), _ptr(d), lda, ldb, ldc, ldd,
+                                      float(alpha), float(beta), s)
+    L.check(rc, "b200wmma_mx_gemm")
+    return d
+
+
+# ---- embedding --------------------------------------------------------------------------------
+
+_CODE = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32}
+
+
+def _value_code(t, what):
+    if t.dtype not in _CODE:
+        raise ValueError(f"{what} is {t.dtype}; float16, bfloat16 or float32 expected")
+    return _CODE[t.dtype]
+
+
+def _tokens(ids, first):
+    """(outer, inner, strides) of ids: [outer, inner], or any shape without `first`."""
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"ids are {ids.dtype}; int32 or int64 expected")
+    if first is not None:
+        if ids.dim() != 2 or first.dtype != torch.int64 or not first.is_contiguous() \
+                or first.shape != (ids.shape[1] + 1,):
+            raise ValueError("with first, ids are [outer, inner] and first inner + 1 int64 row numbers")
+    elif ids.dim() == 1:
+        ids = ids.unsqueeze(1)
+    elif ids.dim() != 2:
+        ids = ids.reshape(-1, 1)
+    return ids, ids.shape[0], ids.shape[1]
+
+
+def _rows_view(t, ids_shape, dim, what, copy):
+    """t [*ids.shape, dim] as [outer, inner, dim]; rows contiguous."""
+    if tuple(t.shape) != (*ids_shape, dim):
+        raise ValueError(f"{what} is {tuple(t.shape)}, expected {(*ids_shape, dim)}")
+    if t.dim() == 2:
+        t = t.unsqueeze(1)
+    elif t.dim() != 3:
+        if not copy and not t.is_contiguous():
+            raise ValueError(f"{what} must be contiguous for ids of this shape")
+        t = t.reshape(-1, 1, dim)
+    if dim > 1 and t.stride(2) != 1:
+        raise ValueError(f"the rows of {what} must be contiguous")
+    return t
+
+
+def embedding(table, ids, scale=1.0, first=None, out_t=None, out=None, stream=None):
+    """out[t, :] = scale * table[ids[t], :] for a table [rows, dim] (rows contiguous, any distance
+    apart) and int32 / int64 ids of any shape; ids outside the table (-1: padding) give zeros.
+    first: int64 [inner + 1] on the device; ids are [outer, inner], column i counts from row
+    first[i] up to first[i + 1].  out: [*ids.shape, dim], may be a strided view such as the
+    rows behind the dense one of dlrm_fwd's input; out_t: its type otherwise (the table's)."""
+    if table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError("table must be [rows, dim] with contiguous rows")
+    rows, dim = table.shape
+    shape = ids.shape
+    if out is None:
+        out = torch.empty(*shape, dim, dtype=table.dtype if out_t is None else _TORCH.get(out_t),
+                          device=table.device)
+    device = _device_of(table, ids, first, out)
+    tokens, outer, inner = _tokens(ids, first)
+    view = _rows_view(out, shape, dim, "out", copy=False)
+    if any(n > 1 and not step for n, step in zip(view.shape, view.stride())):
+        raise ValueError("out must not hold a row twice")
+    kinds = _value_code(table, "table"), _value_code(out, "out")
+    if not ids.numel():
+        return out
+    with _on(device, stream) as s:
+        rc = L.lib().b200wmma_embedding(
+            *kinds, rows, dim, outer, inner, _ptr(table), table.stride(0) if rows > 1 else dim, _ptr(tokens),
+            tokens.element_size(), tokens.stride(0), tokens.stride(1), _ptr(first), _ptr(view),
+            view.stride(0), view.stride(1), float(scale), s)
+    L.check(rc, "b200wmma_embedding")
+    return out
+
+
+def embedding_grad(grad, ids, rows, out_t=None, scale=1.0, first=None, out=None, accumulate=False,
+                   workspace=None, stream=None):
+    """Gradient [rows, dim] of embedding()'s table from grad [*ids.shape, dim] (strided like its
+    out).  accumulate: add to `out`, whose rows without a token stay as they are; otherwise those
+    become zero.  out_t: type of a new result (grad's).  workspace: a uint8 tensor of
+    embedding_grad_workspace(...) bytes to use instead of a new one."""
+    dim = grad.shape[-1]
+    if out is None:
+        if accumulate:
+            raise ValueError("accumulate needs out")
+        out = torch.empty(rows, dim, dtype=grad.dtype if out_t is None else _TORCH.get(out_t), device=grad.device)
+    if tuple(out.shape) != (rows, dim) or (dim > 1 and out.stride(1) != 1):
+        raise ValueError(f"out must be {(rows, dim)} with contiguous rows")
+    device = _device_of(grad, ids, first, out, workspace)
+    tokens, outer, inner = _tokens(ids, first)
+    view = _rows_view(grad, ids.shape, dim, "grad", copy=True)
+    kinds = _value_code(grad, "grad"), _value_code(out, "out")
+    if not ids.numel():
+        return out if accumulate else out.zero_()
+    with _on(device, stream) as s:
+        need = L.lib().b200wmma_embedding_grad_workspace(rows, dim, outer, inner)
+        if workspace is None:
+            with torch.cuda.stream(stream):
+                workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=device)
+        elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+            raise ValueError("workspace must be a contiguous uint8 tensor")
+        rc = L.lib().b200wmma_embedding_grad(
+            *kinds, rows, dim, outer, inner, _ptr(view), view.stride(0), view.stride(1), _ptr(tokens),
+            tokens.element_size(), tokens.stride(0), tokens.stride(1), _ptr(first), _ptr(out),
+            out.stride(0) if rows > 1 else dim, float(scale), int(accumulate), _ptr(workspace), workspace.numel(), s)
+    L.check(rc, "b200wmma_embedding_grad")
+    return out
+
+
+def embedding_grad_workspace(rows, dim, outer, inner=1):
+    """Bytes of device memory that embedding_grad works in for outer x inner tokens."""
+    return L.lib().b200wmma_embedding_grad_workspace(rows, dim, outer, inner)

@@ -1,0 +1,213 @@
+"""Embedding lookup and its gradient on the GPU against sums in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+from rocwmma_b200 import BF16, F16, F32, api
+
+pytestmark = pytest.mark.gpu
+TYPES = {F16: torch.float16, BF16: torch.bfloat16, F32: torch.float32}
+KINDS = pytest.mark.parametrize("kind", [F16, BF16, F32], ids=["f16", "bf16", "f32"])
+
+
+def _ids(shape, rows, seed, skew=1.0, padding=0.2, dtype=torch.int64):
+    g = torch.Generator().manual_seed(seed)
+    ids = (torch.rand(shape, generator=g, dtype=torch.float64) ** skew * rows).long().clamp(max=rows - 1)
+    ids = torch.where(torch.rand(shape, generator=g) < padding, -1, ids)
+    return ids.to(dtype)
+
+
+def _randn(shape, kind, seed):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(TYPES[kind])
+
+
+@KINDS
+@pytest.mark.parametrize("out_t", [F16, BF16, F32], ids=["to_f16", "to_bf16", "to_f32"])
+@pytest.mark.parametrize("tokens,rows,dim", [(1, 1, 1), (1, 7, 8), (5, 3, 3), (63, 100, 96), (64, 1000, 1001),
+                                             (1000, 50, 128), (257, 300, 2056), (20000, 40, 16)])
+def test_lookup(kind, out_t, tokens, rows, dim):
+    table, ids = _randn((rows, dim), kind, 1), _ids((tokens,), rows, 2)
+    for scale in (1.0, 0.3):
+        got = api.embedding(table.cuda(), ids.cuda(), scale=scale, out_t=out_t)
+        # a value of at most 24 bits times a 24-bit scale, rounded to fp32 and then to the output
+        want = table.float()[ids.clamp(min=0)] * np.float32(scale)
+        want = torch.where(ids[:, None] >= 0, want, 0.0).to(TYPES[out_t])
+        assert torch.equal(got.cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64], ids=["int32", "int64"])
+@pytest.mark.parametrize("dim", [128, 30])
+def test_lookup_of_several_tables_into_the_interaction(dtype, dim):
+    """Ids count within each table; the dense row in front of the picked ones is left alone."""
+    outer, sizes = 100, [3, 1, 50, 7]
+    first = torch.tensor([0, 3, 4, 54, 61])
+    table = _randn((61, dim), F16, 1)
+    ids = torch.stack([_ids((outer,), n, 3 + i) for i, n in enumerate(sizes)], 1)
+    ids[0], ids[1] = torch.tensor([3, 1, 50, 7]), torch.tensor([2, 0, 49, 6])  # one behind the end, the last
+    x = torch.full((outer, 5, dim), 7.0, dtype=torch.float16, device="cuda")
+    api.embedding(table.cuda(), ids.to(dtype).cuda(), first=first.cuda(), out=x[:, 1:])
+    want = torch.full((outer, 5, dim), 7.0, dtype=torch.float16)
+    for i, n in enumerate(sizes):
+        has = (ids[:, i] >= 0) & (ids[:, i] < n)
+        rows = table[first[i] + ids[:, i].clamp(0, n - 1)]
+        want[:, 1 + i] = torch.where(has[:, None], rows, 0.0)
+    assert torch.equal(x.cpu(), want)
+
+
+def test_lookup_strides():
+    """Rows of a wider table, transposed ids, an output with room between its rows."""
+    wide = _randn((40, 37), F32, 1)
+    ids = _ids((6, 10), 40, 2)
+    out = torch.full((6, 10, 20), 7.0, device="cuda")
+    api.embedding(wide.cuda()[:, 3:19], ids.t().contiguous().cuda().t(), out=out[:, :, 2:18], scale=2.0)
+    want = torch.full((6, 10, 20), 7.0)
+    want[:, :, 2:18] = torch.where(ids[..., None] >= 0, 2 * wide[ids.clamp(min=0), 3:19], 0.0)
+    assert torch.equal(out.cpu(), want)
+    # an id of any size outside the table picks nothing
+    far = torch.tensor([2 ** 31, 2 ** 32 + 1, -2 ** 40, 40, 39], device="cuda")
+    got = api.embedding(wide.cuda(), far).cpu()
+    assert torch.equal(got[:4], torch.zeros(4, 37)) and torch.equal(got[4], wide[39])
+
+
+def _grad_reference(grad, ids, rows, scale=1.0, old=None):
+    """(sum, sum of magnitudes, tokens) of every row in 64 bits."""
+    flat, g = ids.reshape(-1).numpy(), grad.double().reshape(-1, grad.shape[-1]).numpy()
+    total, size, count = np.zeros((rows, g.shape[1])), np.zeros((rows, g.shape[1])), np.zeros(rows)
+    ok = (flat >= 0) & (flat < rows)
+    np.add.at(total, flat[ok], g[ok])
+    np.add.at(size, flat[ok], np.abs(g[ok]))
+    np.add.at(count, flat[ok], 1)
+    return total, size, count
+
+
+def _check_grad(got, grad, ids, rows, kind, scale=1.0, old=None):
+    """Each of a row's n additions and the scaling round to fp32 (2^-24 of a partial sum, which is
+    no larger than the sum of magnitudes); one more rounding to the result's type."""
+    total, size, count = _grad_reference(grad, ids, rows)
+    scale = float(np.float32(scale))
+    want, bound = total * scale, (count + 1)[:, None] * 2.0 ** -24 * size * abs(scale)
+    if old is not None:
+        want = want + old
+        bound = bound + 2.0 ** -24 * (np.abs(old) + size * abs(scale))
+    got = got.double().cpu().numpy()
+    step = torch.finfo(TYPES[kind]).eps / 2
+    tiny = torch.finfo(TYPES[kind]).smallest_normal * torch.finfo(TYPES[kind]).eps  # subnormal results
+    err = np.abs(got - want)
+    assert (err <= bound + step * (np.abs(want) + bound) + tiny / 2).all(), err.max()
+    assert np.array_equal(got[count == 0], (old if old is not None else np.zeros_like(want))[count == 0])
+
+
+@KINDS
+@pytest.mark.parametrize("out_t", [F16, BF16, F32], ids=["to_f16", "to_bf16", "to_f32"])
+@pytest.mark.parametrize("tokens,rows,dim,skew", [(1, 1, 1, 1), (1, 5, 8, 1), (40, 1, 3, 1), (33, 70, 264, 1), (513, 90, 1001, 4),
+                                                  (4097, 300, 64, 4), (5000, 70000, 24, 1), (9000, 2, 40, 1)])
+def test_gradient(kind, out_t, tokens, rows, dim, skew):
+    grad, ids = _randn((tokens, dim), kind, 1), _ids((tokens,), rows, 2, skew)
+    for scale in (1.0, 0.3):
+        got = api.embedding_grad(grad.cuda(), ids.cuda(), rows, out_t=out_t, scale=scale)
+        _check_grad(got, grad, ids, rows, out_t, scale)
+
+
+@pytest.mark.parametrize("tokens,rows,dim", [(300000, 40, 8), (70000, 1, 16), (200000, 100000, 3)])
+def test_gradient_of_long_runs(tokens, rows, dim):
+    """Rows that most tokens share: runs over many chunks and levels; every bit the same again."""
+    grad, ids = _randn((tokens, dim), BF16, 1), _ids((tokens,), rows, 2, 6.0)
+    got = api.embedding_grad(grad.cuda(), ids.cuda(), rows, out_t=F32)
+    _check_grad(got, grad, ids, rows, F32)
+    for _ in range(3):
+        assert torch.equal(api.embedding_grad(grad.cuda(), ids.cuda(), rows, out_t=F32), got)
+
+
+def test_gradient_of_nothing():
+    """No token has a row: zeros, or what was there."""
+    grad, ids = _randn((50, 24), F32, 1).cuda(), torch.full((50,), -1, device="cuda")
+    assert not api.embedding_grad(grad, ids, 30).any()
+    old = _randn((30, 24), F32, 2).cuda()
+    got = api.embedding_grad(grad, ids, 30, out=old.clone(), accumulate=True)
+    assert torch.equal(got, old)
+    none = torch.zeros(0, dtype=torch.int64, device="cuda")
+    assert not api.embedding_grad(grad[:0], none, 30).any()
+    assert api.embedding(old, none).shape == (0, 24)
+
+
+@pytest.mark.parametrize("dim", [64, 50])
+def test_gradient_accumulates_into_views(dim):
+    """Into the first columns of a wider gradient, from the rows behind the interaction's dense one."""
+    outer, inner, rows = 70, 3, 25
+    grad = _randn((outer, inner + 1, dim), F16, 1)
+    sizes, first = [5, 12, 8], torch.tensor([0, 5, 17, 25])
+    ids = torch.stack([_ids((outer,), n, 3 + i) for i, n in enumerate(sizes)], 1)
+    old = _randn((rows, dim + 8), F32, 9)
+    wide = old.cuda()
+    got = api.embedding_grad(grad.cuda()[:, 1:], ids.int().cuda(), rows, first=first.cuda(), scale=0.5,
+                             out=wide[:, :dim], accumulate=True)
+    assert torch.equal(wide[:, dim:].cpu(), old[:, dim:])
+    flat = torch.where(ids >= 0, ids + first[:-1], -1)
+    _check_grad(got, grad[:, 1:], flat, rows, F32, 0.5, old[:, :dim].double().numpy())
+
+
+def test_gradient_is_the_lookups():
+    """<grad, embedding(table)> grows with the table as the gradient says: differences in 64 bits of a
+    function that is linear in the table."""
+    rows, dim = 30, 16
+    table, ids, g = _randn((rows, dim), F32, 1), _ids((200,), rows, 2), _randn((200, dim), F32, 3)
+    grad = api.embedding_grad(g.cuda(), ids.cuda(), rows, scale=1.5).double().cpu()
+    step = _randn((rows, dim), F32, 4)
+    up = api.embedding((table + step).cuda(), ids.cuda(), scale=1.5).double().cpu()
+    down = api.embedding((table - step).cuda(), ids.cuda(), scale=1.5).double().cpu()
+    moved = (((table + step).double() - (table - step).double()) * grad).sum()
+    # fp32 roundings: of each looked-up value (2^-24), and those of the gradient's sums (at most 200 a row)
+    size = (g.abs().double() * (up.abs() + down.abs())).sum()
+    assert abs(((up - down) * g.double()).sum() - moved) <= 202 * 2.0 ** -24 * size
+
+
+def test_dlrm_step():
+    """Lookup -> interaction -> 4-bit product, and back through the interaction to the tables."""
+    from rocwmma_b200 import MXF4
+    from tests import mx_reference as R
+
+    batch, dim, sizes = 48, 32, [4, 30, 9]
+    m = len(sizes) + 1
+    first = torch.tensor([0, 4, 34, 43])
+    table, dense = _randn((43, dim), F16, 1), _randn((batch, dim), F16, 2)
+    ids = torch.stack([_ids((batch,), n, 3 + i, padding=0) for i, n in enumerate(sizes)], 1)
+    x = torch.empty(batch, m, dim, dtype=torch.float16, device="cuda")
+    x[:, 0] = dense.cuda()
+    api.embedding(table.cuda(), ids.cuda(), first=first.cuda(), out=x[:, 1:])
+    width = dim + m * (m - 1) // 2
+    z = api.dlrm_fwd(x, m, dim, batch).view(batch, width)
+    weight = _randn((64, width), F16, 7)
+    qz = api.mx_quantize(MXF4, F16, batch, width, z)
+    qw = api.mx_quantize(MXF4, F16, 64, width, weight.cuda())
+    y = api.mx_gemm(MXF4, F32, batch, 64, width, qz, qw, None, 1.0, 0.0).view(batch, 64)
+    zv, wv = (R.quantize(MXF4, t.double().cpu().numpy())[2] for t in (z, weight))
+    bound = width * 2.0 ** -23 * (np.abs(zv) @ np.abs(wv).T)
+    assert (np.abs(y.double().cpu().numpy() - zv @ wv.T) <= bound).all()
+
+    upstream = _randn((batch, width), F16, 8).cuda()
+    _, grad = api.dlrm_bwd(x, upstream, m, dim, batch)
+    grad = grad.view(batch, m, dim)
+    total = api.embedding_grad(grad[:, 1:], ids.cuda(), 43, out_t=F32, first=first.cuda())
+    _check_grad(total, grad[:, 1:].cpu(), ids + first[:-1], 43, F32)
+
+
+def test_graph_replays_with_new_tokens_and_shares_a_workspace():
+    """Two captured gradients, one workspace, replayed one after the other."""
+    rows, dim, n = 500, 48, 3000
+    ids, grad = _ids((n,), rows, 1).cuda(), _randn((n, dim), BF16, 2).cuda()
+    work = torch.empty(api.embedding_grad_workspace(rows, dim, n), dtype=torch.uint8, device="cuda")
+    outs, graphs = [torch.empty(rows, dim, device="cuda") for _ in range(2)], []
+    api.embedding_grad(grad, ids, rows, out=outs[0], workspace=work)
+    torch.cuda.synchronize()
+    for i, out in enumerate(outs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            api.embedding_grad(grad, ids, rows, out=out, workspace=work, scale=1.0 + i)
+        graphs.append(g)
+    for seed in (3, 4):
+        ids.copy_(_ids((n,), rows, seed, 3.0))
+        grad.copy_(_randn((n, dim), BF16, seed))
+        for g in graphs:
+            g.replay()
+        for i, out in enumerate(outs):
+            _check_grad(out, grad.cpu(), ids.cpu(), rows, F32, 1.0 + i)
