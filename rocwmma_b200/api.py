@@ -16,8 +16,8 @@ from __future__ import annotations
 import torch
 
 from . import _lib as L
-from ._lib import (BF16, COL_MAJOR, E4M3, E5M2, F16, F32, F64, I8, I32, ROW_MAJOR, XF32,  # noqa: F401
-                   B200WmmaError)
+from ._lib import (BF16, COL_MAJOR, E4M3, E5M2, F16, F32, F64, I8, I32, MXF4, NVF4,  # noqa: F401
+                   ROW_MAJOR, XF32, B200WmmaError)
 
 _TORCH = {F16: torch.float16, BF16: torch.bfloat16, E4M3: torch.uint8, I8: torch.int8,
           F32: torch.float32, XF32: torch.float32, F64: torch.float64, I32: torch.int32,
@@ -173,46 +173,52 @@ def shutdown() -> None:
 # ---- 4-bit block-scaled operands ------------------------------------------------------------
 # An operand is a pair (codes, scales) of uint8 tensors, as the C header lays them out.
 
-def _device_of(*ts):
-    """The one device of the given tensors; they may not be spread over several."""
-    _require_cuda(*ts)
-    devices = {t.device for t in ts if t is not None}
-    if len(devices) != 1:
-        raise ValueError(f"tensors on several devices: {sorted(map(str, devices))}")
-    return devices.pop()
+def _device_of(first, *others):
+    """Index of the one device that the given tensors are on."""
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            raise ValueError("tensors on several devices, or not on a device at all")
+    if index < 0:
+        raise ValueError("device tensors required (this library has no CPU path)")
+    return index
 
 
-class _on:
-    """Makes `device` current for a call, with its stream (the given one, or that device's
-    current one) as the value; the switch is skipped where there is nothing to switch."""
-
-    def __init__(self, device, stream):
-        self.device, self.stream = device.index, stream
-        self.back = None
-
-    def __enter__(self):
-        now = torch.cuda.current_device()
-        if now != self.device:
-            self.back = now
-            torch.cuda.set_device(self.device)
-        return _stream(self.stream)
-
-    def __exit__(self, *_):
-        if self.back is not None:
-            torch.cuda.set_device(self.back)
-
-
-def _holds(t, what, count):
-    """Whether a contiguous tensor is large enough for what a call reads or writes of it."""
-    if not t.is_contiguous():
-        raise ValueError(f"{what} must be contiguous")
-    if t.numel() < count:
-        raise ValueError(f"{what} holds {t.numel()} elements, {count} needed")
+def _launch(entry, index, stream, *args):
+    """Calls the entry point with `stream`, or the current stream of the tensors' device, which
+    need not be the current one.  (The raw handle: making a torch.cuda.Stream of the current
+    stream takes 3 us, as long as the launch.)"""
+    if stream is None:
+        handle = torch._C._cuda_getCurrentRawStream(index)
+    elif stream.device.index != index:
+        raise ValueError(f"a stream of device {stream.device.index} for tensors on device {index}")
+    else:
+        handle = stream.cuda_stream
+    if torch.cuda.current_device() == index:
+        rc = getattr(L.lib(), entry)(*args, handle)
+    else:
+        with torch.cuda.device(index):
+            rc = getattr(L.lib(), entry)(*args, handle)
+    if rc:
+        L.check(rc, entry)
 
 
-def _is_type(t, what, dtype):
+def _empty(shape, dtype, device, stream):
+    """A new tensor whose memory `stream` (None: the current stream) may use at once."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _check(t, what, dtype, count):
+    """A contiguous tensor of the type that holds what a call reads or writes of it."""
     if t.dtype != dtype:
-        raise ValueError(f"{what} is {t.dtype}, expected {dtype}")
+        raise ValueError(f"{what}: {t.dtype}, expected {dtype}")
+    if not t.is_contiguous():
+        raise ValueError(f"{what}: must be contiguous")
+    if t.numel() < count:
+        raise ValueError(f"{what}: {t.numel()} elements, {count} needed")
 
 
 def mx_pitch(k):
@@ -220,18 +226,18 @@ def mx_pitch(k):
     return (k + 31) // 32 * 16
 
 
+_GROUP = {MXF4: 128, NVF4: 64}  # values along k of one scale tile
+
+
 def mx_scale_bytes(fmt, rows, k):
     """Bytes of the scales of a rows x k operand."""
-    return L.lib().b200wmma_mx_scale_bytes(fmt, rows, k)
+    span = _GROUP.get(fmt)
+    return (rows + 127) // 128 * ((k + span - 1) // span) * 512 if span else 0
 
 
-def _operand(fmt, rows, k, operand, ld, what):
-    codes, scales = operand
-    for t, part in ((codes, "codes"), (scales, "scales")):
-        if t.dtype != torch.uint8:
-            raise ValueError(f"{part} of {what} are {t.dtype}, expected torch.uint8")
-    _holds(codes, f"codes of {what}", (rows - 1) * ld + mx_pitch(k))
-    _holds(scales, f"scales of {what}", mx_scale_bytes(fmt, rows, k))
+def _operand(fmt, rows, k, codes, scales, ld):
+    _check(codes, "codes", torch.uint8, (rows - 1) * ld + (k + 31) // 32 * 16)
+    _check(scales, "scales", torch.uint8, mx_scale_bytes(fmt, rows, k))
 
 
 def mx_quantize(fmt, in_t, rows, k, x, layout=ROW_MAJOR, exponent=0, ldx=None, ldq=None, out=None,
@@ -241,17 +247,13 @@ def mx_quantize(fmt, in_t, rows, k, x, layout=ROW_MAJOR, exponent=0, ldx=None, l
     ldx = ldx or _natural_ld(layout, rows, k)
     ldq = ldq or mx_pitch(k)
     if out is None:
-        codes = torch.empty(rows * ldq, dtype=torch.uint8, device=x.device)
-        scales = torch.empty(mx_scale_bytes(fmt, rows, k), dtype=torch.uint8, device=x.device)
-        out = codes, scales
+        out = (_empty(rows * ldq, torch.uint8, x.device, stream),
+               _empty(mx_scale_bytes(fmt, rows, k), torch.uint8, x.device, stream))
     device = _device_of(x, *out)
-    _is_type(x, "x", _TORCH.get(in_t))
-    _holds(x, "x", (rows - 1) * ldx + k if layout == ROW_MAJOR else (k - 1) * ldx + rows)
-    _operand(fmt, rows, k, out, ldq, "out")
-    with _on(device, stream) as s:
-        rc = L.lib().b200wmma_mx_quantize(fmt, in_t, rows, k, _ptr(x), ldx, layout, exponent,
-                                          _ptr(out[0]), ldq, _ptr(out[1]), s)
-    L.check(rc, "b200wmma_mx_quantize")
+    _check(x, "x", _TORCH.get(in_t), (rows - 1) * ldx + k if layout == ROW_MAJOR else (k - 1) * ldx + rows)
+    _operand(fmt, rows, k, *out, ldq)
+    _launch("b200wmma_mx_quantize", device, stream, fmt, in_t, rows, k, x.data_ptr(), ldx, layout,
+            exponent, out[0].data_ptr(), ldq, out[1].data_ptr())
     return out
 
 
@@ -261,15 +263,12 @@ def mx_dequantize(fmt, out_t, rows, k, codes, scales, exponent=0, ldq=None, ldo=
     ldq = ldq or mx_pitch(k)
     ldo = ldo or k
     if out is None:
-        out = torch.empty(rows * ldo, dtype=_TORCH.get(out_t), device=codes.device)
+        out = _empty(rows * ldo, _TORCH.get(out_t), codes.device, stream)
     device = _device_of(codes, scales, out)
-    _is_type(out, "out", _TORCH.get(out_t))
-    _holds(out, "out", (rows - 1) * ldo + k)
-    _operand(fmt, rows, k, (codes, scales), ldq, "the operand")
-    with _on(device, stream) as s:
-        rc = L.lib().b200wmma_mx_dequantize(fmt, out_t, rows, k, _ptr(codes), ldq, _ptr(scales),
-                                            exponent, _ptr(out), ldo, s)
-    L.check(rc, "b200wmma_mx_dequantize")
+    _check(out, "out", _TORCH.get(out_t), (rows - 1) * ldo + k)
+    _operand(fmt, rows, k, codes, scales, ldq)
+    _launch("b200wmma_mx_dequantize", device, stream, fmt, out_t, rows, k, codes.data_ptr(), ldq,
+            scales.data_ptr(), exponent, out.data_ptr(), ldo)
     return out
 
 
@@ -281,20 +280,15 @@ def mx_gemm(fmt, out_t, m, n, k, a, b, c, alpha, beta, lda=None, ldb=None, ldc=N
     ldb = ldb or mx_pitch(k)
     ldc = ldc or n
     ldd = ldd or n
-    d = out if out is not None else torch.empty(m * ldd, dtype=_TORCH.get(out_t), device=a[0].device)
+    d = out if out is not None else _empty(m * ldd, _TORCH.get(out_t), a[0].device, stream)
     device = _device_of(*a, *b, c, d)
-    _operand(fmt, m, k, a, lda, "A")
-    _operand(fmt, n, k, b, ldb, "B")
-    _is_type(d, "out", _TORCH.get(out_t))
-    _holds(d, "out", (m - 1) * ldd + n)
+    _operand(fmt, m, k, *a, lda)
+    _operand(fmt, n, k, *b, ldb)
+    _check(d, "out", _TORCH.get(out_t), (m - 1) * ldd + n)
     if c is not None and beta != 0:
-        _is_type(c, "c", _TORCH.get(out_t))
-        _holds(c, "c", (m - 1) * ldc + n)
-    with _on(device, stream) as s:
-        rc = L.lib().b200wmma_mx_gemm(fmt, out_t, m, n, k, _ptr(a[0]), _ptr(a[1]), _ptr(b[0]),
-                                      _ptr(b[1]), _ptr(c), _ptr(d), lda, ldb, ldc, ldd,
-                                      float(alpha), float(beta), s)
-    L.check(rc, "b200wmma_mx_gemm")
+        _check(c, "c", _TORCH.get(out_t), (m - 1) * ldc + n)
+    _launch("b200wmma_mx_gemm", device, stream, fmt, out_t, m, n, k, a[0].data_ptr(), a[1].data_ptr(),
+            b[0].data_ptr(), b[1].data_ptr(), _ptr(c), d.data_ptr(), lda, ldb, ldc, ldd, alpha, beta)
     return d
 
 
@@ -310,7 +304,7 @@ def _value_code(t, what):
 
 
 def _tokens(ids, first):
-    """(outer, inner, strides) of ids: [outer, inner], or any shape without `first`."""
+    """ids as [outer, inner], and the two sizes; any shape without `first`."""
     if ids.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"ids are {ids.dtype}; int32 or int64 expected")
     if first is not None:
@@ -320,23 +314,30 @@ def _tokens(ids, first):
     elif ids.dim() == 1:
         ids = ids.unsqueeze(1)
     elif ids.dim() != 2:
-        ids = ids.reshape(-1, 1)
+        if not ids.is_contiguous():
+            raise ValueError("ids of this shape must be contiguous")
+        ids = ids.view(-1, 1)
     return ids, ids.shape[0], ids.shape[1]
 
 
-def _rows_view(t, ids_shape, dim, what, copy):
+def _rows_view(t, ids_shape, dim, what):
     """t [*ids.shape, dim] as [outer, inner, dim]; rows contiguous."""
     if tuple(t.shape) != (*ids_shape, dim):
         raise ValueError(f"{what} is {tuple(t.shape)}, expected {(*ids_shape, dim)}")
     if t.dim() == 2:
         t = t.unsqueeze(1)
     elif t.dim() != 3:
-        if not copy and not t.is_contiguous():
+        if not t.is_contiguous():
             raise ValueError(f"{what} must be contiguous for ids of this shape")
-        t = t.reshape(-1, 1, dim)
+        t = t.view(-1, 1, dim)
     if dim > 1 and t.stride(2) != 1:
         raise ValueError(f"the rows of {what} must be contiguous")
     return t
+
+
+def _zero(t, stream):
+    with torch.cuda.stream(stream):
+        return t.zero_()
 
 
 def embedding(table, ids, scale=1.0, first=None, out_t=None, out=None, stream=None):
@@ -350,22 +351,19 @@ def embedding(table, ids, scale=1.0, first=None, out_t=None, out=None, stream=No
     rows, dim = table.shape
     shape = ids.shape
     if out is None:
-        out = torch.empty(*shape, dim, dtype=table.dtype if out_t is None else _TORCH.get(out_t),
-                          device=table.device)
+        out = _empty((*shape, dim), table.dtype if out_t is None else _TORCH.get(out_t), table.device,
+                     stream)
     device = _device_of(table, ids, first, out)
     tokens, outer, inner = _tokens(ids, first)
-    view = _rows_view(out, shape, dim, "out", copy=False)
+    view = _rows_view(out, shape, dim, "out")
     if any(n > 1 and not step for n, step in zip(view.shape, view.stride())):
         raise ValueError("out must not hold a row twice")
     kinds = _value_code(table, "table"), _value_code(out, "out")
     if not ids.numel():
         return out
-    with _on(device, stream) as s:
-        rc = L.lib().b200wmma_embedding(
-            *kinds, rows, dim, outer, inner, _ptr(table), table.stride(0) if rows > 1 else dim, _ptr(tokens),
-            tokens.element_size(), tokens.stride(0), tokens.stride(1), _ptr(first), _ptr(view),
-            view.stride(0), view.stride(1), float(scale), s)
-    L.check(rc, "b200wmma_embedding")
+    _launch("b200wmma_embedding", device, stream, *kinds, rows, dim, outer, inner, table.data_ptr(),
+            table.stride(0) if rows > 1 else dim, tokens.data_ptr(), tokens.element_size(),
+            *tokens.stride(), _ptr(first), view.data_ptr(), *view.stride()[:2], scale)
     return out
 
 
@@ -379,27 +377,24 @@ def embedding_grad(grad, ids, rows, out_t=None, scale=1.0, first=None, out=None,
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs out")
-        out = torch.empty(rows, dim, dtype=grad.dtype if out_t is None else _TORCH.get(out_t), device=grad.device)
+        out = _empty((rows, dim), grad.dtype if out_t is None else _TORCH.get(out_t), grad.device, stream)
     if tuple(out.shape) != (rows, dim) or (dim > 1 and out.stride(1) != 1):
         raise ValueError(f"out must be {(rows, dim)} with contiguous rows")
     device = _device_of(grad, ids, first, out, workspace)
     tokens, outer, inner = _tokens(ids, first)
-    view = _rows_view(grad, ids.shape, dim, "grad", copy=True)
+    view = _rows_view(grad, ids.shape, dim, "grad")
     kinds = _value_code(grad, "grad"), _value_code(out, "out")
     if not ids.numel():
-        return out if accumulate else out.zero_()
-    with _on(device, stream) as s:
-        need = L.lib().b200wmma_embedding_grad_workspace(rows, dim, outer, inner)
-        if workspace is None:
-            with torch.cuda.stream(stream):
-                workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=device)
-        elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
-            raise ValueError("workspace must be a contiguous uint8 tensor")
-        rc = L.lib().b200wmma_embedding_grad(
-            *kinds, rows, dim, outer, inner, _ptr(view), view.stride(0), view.stride(1), _ptr(tokens),
-            tokens.element_size(), tokens.stride(0), tokens.stride(1), _ptr(first), _ptr(out),
-            out.stride(0) if rows > 1 else dim, float(scale), int(accumulate), _ptr(workspace), workspace.numel(), s)
-    L.check(rc, "b200wmma_embedding_grad")
+        return out if accumulate else _zero(out, stream)
+    if workspace is None:
+        workspace = _empty(L.lib().b200wmma_embedding_grad_workspace(rows, dim, outer, inner),
+                           torch.uint8, grad.device, stream)
+    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous uint8 tensor")
+    _launch("b200wmma_embedding_grad", device, stream, *kinds, rows, dim, outer, inner, view.data_ptr(),
+            *view.stride()[:2], tokens.data_ptr(), tokens.element_size(), *tokens.stride(), _ptr(first),
+            out.data_ptr(), out.stride(0) if rows > 1 else dim, scale, bool(accumulate), workspace.data_ptr(),
+            workspace.numel())
     return out
 
 

@@ -9,6 +9,7 @@
 #include "mx_format.cuh"
 #include "rocwmma/rocwmma_block.hpp"
 #include "runtime.cuh"
+#include "tile_schedule.cuh"
 #include <cuda.h>
 #include <mutex>
 
@@ -51,11 +52,11 @@ namespace b200wmma
 
         // alpha and beta as everywhere in this library: a rounded product each, a rounded sum.
         template <typename OutT>
-        __device__ inline OutT finish(float acc, Params const& p, OutT const* c)
+        __device__ inline OutT finish(float acc, float alpha, float beta, OutT const* c)
         {
-            float r = __fmul_rn(p.alpha, acc);
+            float r = __fmul_rn(alpha, acc);
             if(c)
-                r = __fadd_rn(r, __fmul_rn(p.beta, toFloat(*c)));
+                r = __fadd_rn(r, __fmul_rn(beta, toFloat(*c)));
             return fromFloat<OutT>(r);
         }
 
@@ -197,7 +198,7 @@ namespace b200wmma
                             {
                                 OutT const* c = p.c ? static_cast<OutT const*>(p.c) + row * p.ldc + col : nullptr;
                                 static_cast<OutT*>(p.d)[row * p.ldd + col]
-                                    = finish<OutT>(__uint_as_float(raw[j]), p, c);
+                                    = finish<OutT>(__uint_as_float(raw[j]), p.alpha, p.beta, c);
                             }
                         }
                     }
@@ -211,6 +212,353 @@ namespace b200wmma
                 __syncwarp();
                 tc_fence_after_sync();
                 tmem_dealloc(tmem, p.tmemCols);
+            }
+            if(threadIdx.x == 0 && ctl->abort.flag != 0u && p.status != nullptr)
+            {
+                atomicExch(&p.status[1], ctl->abort.code);
+                atomicExch(&p.status[0], 1u);
+            }
+        }
+
+        // ---- large products: CTA pairs -----------------------------------------------------
+        // A pair of blocks owns a 256 x 256 tile (cta_group::2): each stages its own 128 rows of
+        // A and half of the columns of B, the scales of its rows of A and those of all of B; the
+        // even block issues MMAs of M = 256.  Persistent; warp 0 loads, warp 1 multiplies, warps 2
+        // to 5 drain.
+        //
+        // Tensor memory has 512 columns: two accumulators of 256 would leave none for the scales.
+        // So the two overlap: the second starts at column ACC1, the scales of two ring slots lie
+        // behind it, and the first MMA of a tile waits only until the tile before has drained the
+        // columns that both accumulators share, which are drained first.
+        constexpr uint32_t P_TILE      = 256;
+        constexpr uint32_t P_STAGES    = 5;
+        constexpr uint32_t BOX_BYTES   = 128 * 64; // 128 rows x 64 bytes of D (or C)
+        constexpr uint32_t BOXES       = 4;
+        constexpr long long SETTLE_CYCLES = 2000000; // leaving early: copies in flight land
+
+        struct PairParams
+        {
+            void const* c;
+            void*       d;
+            uint32_t    m, n, k, ldc, ldd;
+            float       alpha, beta;
+            uint32_t    band;
+            uint32_t*   status;
+        };
+        struct PairControl
+        {
+            uint64_t   full[P_STAGES], empty[P_STAGES], accFull[2], accShared, cFull[BOXES];
+            AbortState abort;
+            uint32_t   tmemBase;
+        };
+        template <ScaleKind KIND>
+        constexpr uint32_t pairSlotBytes()
+        {
+            return 2u * CODE_BYTES + 3u * slotGroups<KIND>() * MX_TILE_BYTES;
+        }
+        template <ScaleKind KIND>
+        constexpr uint32_t pairSmemBytes()
+        {
+            return 1024u + P_STAGES * pairSlotBytes<KIND>() + BOXES * BOX_BYTES + uint32_t(sizeof(PairControl));
+        }
+
+        __device__ inline void settle()
+        {
+            const long long start = clock64();
+            while(clock64() - start < SETTLE_CYCLES)
+            {
+            }
+        }
+
+        // Drains one tile's accumulator.  A box of D is 128 rows x 64 bytes: TMEM -> registers
+        // -> shared memory in the TMA's 64-byte swizzle -> TMA store; with beta != 0 the box of C
+        // comes to the same place by TMA two boxes ahead and is combined there.  Four boxes take
+        // turns: once a store is issued, the one two before it has been read out, so that one
+        // barrier a box is enough.  A box that D's last column cuts inside a 16-byte piece is
+        // stored by the threads.
+        template <typename OutT>
+        __device__ inline bool drainTile(PairControl* ctl, uint8_t* staging, CUtensorMap const* mapC,
+                                         CUtensorMap const* mapD, PairParams const& p, uint32_t taddr,
+                                         uint32_t first, uint32_t shared, uint32_t accBar, uint32_t accPhase,
+                                         uint32_t row0, uint32_t rowIn, uint32_t col0, uint32_t& boxes,
+                                         uint32_t leaderShared)
+        {
+            constexpr uint32_t COLS   = 64 / sizeof(OutT);
+            constexpr uint32_t VEC    = 16 / sizeof(OutT);
+            constexpr uint32_t GROUPS = P_TILE / COLS;
+            const bool         leader = threadIdx.x == 64u;
+            const bool         useC   = p.c != nullptr;
+            const uint32_t     left   = p.n - col0;
+            const uint32_t     valid  = min(GROUPS, (left + COLS - 1u) / COLS);
+            const uint32_t     ragged = left < P_TILE && left % VEC != 0u ? valid - 1u : GROUPS; // box stored by threads
+            uint32_t           asked = 0, askedBoxes = boxes; // boxes of C: next group in order, next count
+            auto group = [&](uint32_t i) { return (first / COLS + i) % GROUPS; };
+            auto askForC = [&] { // leader only
+                while(asked < GROUPS && (group(asked) >= valid || group(asked) == ragged))
+                    ++asked;
+                if(asked == GROUPS)
+                    return;
+                const uint32_t b = askedBoxes % BOXES;
+                mbar_expect_tx(&ctl->cFull[b], BOX_BYTES);
+                tma_load_2d(staging + b * BOX_BYTES, mapC, &ctl->cFull[b], int32_t(col0 + group(asked) * COLS), int32_t(row0));
+                ++asked;
+                ++askedBoxes;
+            };
+            if(useC && leader)
+            {
+                askForC();
+                askForC();
+            }
+            const bool ready = mbar_wait(&ctl->accFull[accBar], accPhase, &ctl->abort, WAIT_ACC_FULL);
+            if(!named_barrier_all(1, EPI_THREADS, ready))
+                return false;
+            tc_fence_after_sync();
+            const uint32_t row = row0 + rowIn;
+#pragma unroll 1
+            for(uint32_t i = 0; i < GROUPS; ++i)
+            {
+                const uint32_t g = group(i);
+                uint32_t       raw[COLS];
+                if(g < valid)
+                {
+                    if constexpr(COLS == 32)
+                        tmem_load_32x32b_x32(taddr + g * COLS, raw);
+                    else
+                        tmem_load_32x32b_x16(taddr + g * COLS, raw);
+                    tmem_load_wait();
+                }
+                if(i + 1u == shared / COLS)
+                {
+                    // the columns that the next tile's accumulator shares are out
+                    tc_fence_before_sync();
+                    mbar_arrive_cluster(leaderShared);
+                }
+                if(g >= valid)
+                    continue;
+                if(g == ragged)
+                {
+#pragma unroll
+                    for(uint32_t e = 0; e < COLS; ++e)
+                        if(row < p.m && g * COLS + e < left)
+                        {
+                            const uint64_t col = col0 + g * COLS + e;
+                            OutT const*    c   = useC ? static_cast<OutT const*>(p.c) + uint64_t(row) * p.ldc + col : nullptr;
+                            static_cast<OutT*>(p.d)[uint64_t(row) * p.ldd + col]
+                                = finish<OutT>(__uint_as_float(raw[e]), p.alpha, p.beta, c);
+                        }
+                    continue;
+                }
+                const uint32_t b   = boxes % BOXES;
+                uint8_t*       box = staging + b * BOX_BYTES;
+                const bool landed = !useC || mbar_wait(&ctl->cFull[b], (boxes / BOXES) & 1u, &ctl->abort, WAIT_STAGE_FULL);
+#pragma unroll
+                for(uint32_t ch = 0; ch < 4u; ++ch)
+                {
+                    // 64-byte swizzle: piece index ^ (row / 2 % 4)
+                    uint4* piece = reinterpret_cast<uint4*>(box + rowIn * 64u + ((ch ^ ((rowIn >> 1) & 3u)) << 4));
+                    alignas(16) OutT v[VEC];
+                    if(useC)
+                        *reinterpret_cast<uint4*>(v) = *piece;
+#pragma unroll
+                    for(uint32_t e = 0; e < VEC; ++e)
+                        v[e] = finish<OutT>(__uint_as_float(raw[ch * VEC + e]), p.alpha, p.beta, useC ? &v[e] : nullptr);
+                    *piece = *reinterpret_cast<uint4 const*>(v);
+                }
+                fence_async_shared();
+                if(!named_barrier_all(1, EPI_THREADS, landed))
+                    return false;
+                if(leader)
+                {
+                    tma_store_2d(mapD, box, int32_t(col0 + g * COLS), int32_t(row0));
+                    tma_store_commit();
+                    tma_store_wait_read<2>();
+                    if(useC)
+                        askForC();
+                }
+                ++boxes;
+            }
+            return true;
+        }
+
+        template <ScaleKind KIND, typename OutT>
+        __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
+            mxGemmPairKernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
+                             const __grid_constant__ CUtensorMap mapScaleA,
+                             const __grid_constant__ CUtensorMap mapScaleB,
+                             const __grid_constant__ CUtensorMap mapC, const __grid_constant__ CUtensorMap mapD,
+                             const PairParams p)
+        {
+            constexpr uint32_t GROUPS     = slotGroups<KIND>();
+            constexpr uint32_t SLOT       = pairSlotBytes<KIND>();
+            constexpr uint32_t SCALE_COLS = 12u * GROUPS; // of one slot: 4 for A, 8 for B, a group
+            constexpr uint32_t SHARED     = KIND == ScaleKind::E4M3_16 ? 96u : 64u;
+            constexpr uint32_t ACC1       = 256u - SHARED;
+            static_assert(ACC1 + 256u + 2u * SCALE_COLS <= 512u, "tensor memory");
+            extern __shared__ uint8_t smemRaw[];
+            uint8_t*       ring    = smemRaw + ((1024u - (smem_addr(smemRaw) & 1023u)) & 1023u);
+            uint8_t*       staging = ring + P_STAGES * SLOT;
+            PairControl*   ctl     = reinterpret_cast<PairControl*>(staging + BOXES * BOX_BYTES);
+            const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+            const uint32_t rank = cluster_cta_rank(), pairId = blockIdx.x / 2, pairs = gridDim.x / 2;
+            const uint32_t numSlots = (p.k + SLOT_K - 1) / SLOT_K;
+            const TileSchedule sched{(p.m + P_TILE - 1u) / P_TILE, (p.n + P_TILE - 1u) / P_TILE, 0u, P_TILE, 0u, p.band, pairs, 1u};
+
+            if(threadIdx.x == 0)
+            {
+                for(uint32_t s = 0; s < P_STAGES; ++s)
+                {
+                    mbar_init(&ctl->full[s], 1);
+                    mbar_init(&ctl->empty[s], 1);
+                }
+                for(uint32_t b = 0; b < 2u; ++b)
+                    mbar_init(&ctl->accFull[b], 1);
+                mbar_init(&ctl->accShared, 2u * EPI_THREADS);
+                for(uint32_t b = 0; b < BOXES; ++b)
+                    mbar_init(&ctl->cFull[b], 1);
+                ctl->abort.flag = 0;
+                ctl->abort.code = 0;
+                mbar_init_fence();
+                tma_prefetch_descriptor(&mapA);
+                tma_prefetch_descriptor(&mapB);
+                tma_prefetch_descriptor(&mapScaleA);
+                tma_prefetch_descriptor(&mapScaleB);
+                tma_prefetch_descriptor(&mapD);
+            }
+            __syncwarp();
+            cluster_arrive_relaxed();
+            if(warp == 1)
+            {
+                tmem_alloc_pair(&ctl->tmemBase, 512);
+                tmem_relinquish_alloc_permit_pair();
+            }
+            tc_fence_before_sync();
+            __syncthreads();
+            cluster_wait(); // both blocks' barriers exist before anything signals them remotely
+            tc_fence_after_sync();
+            const uint32_t tmem = ctl->tmemBase;
+            grid_dependency_wait();
+            grid_launch_dependents();
+
+            uint32_t tm, col0, width;
+            if(warp == 0)
+            {
+                if(elect_one())
+                {
+                    uint32_t it = 0;
+                    bool     ok = true;
+                    for(uint32_t i = 0; ok && sched.get(pairId, i, tm, col0, width); ++i)
+                    {
+                        const int32_t rowA = int32_t(tm * P_TILE + rank * 128u), rowB = int32_t(col0 + rank * 128u);
+                        for(uint32_t kb = 0; kb < numSlots; ++kb, ++it)
+                        {
+                            const uint32_t s = it % P_STAGES, ph = (it / P_STAGES) & 1u;
+                            if(!mbar_wait(&ctl->empty[s], ph ^ 1u, &ctl->abort, WAIT_STAGE_EMPTY))
+                            {
+                                ok = false;
+                                break;
+                            }
+                            uint8_t* slot   = ring + s * SLOT;
+                            uint8_t* scales = slot + 2u * CODE_BYTES;
+                            if(rank == 0)
+                                mbar_expect_tx(&ctl->full[s], 2u * SLOT); // both blocks
+                            const uint32_t full = map_to_cta(smem_addr(&ctl->full[s]), 0);
+                            tma_load_2d_pair(slot, &mapA, full, int32_t(kb * 128u), rowA);
+                            tma_load_2d_pair(slot + CODE_BYTES, &mapB, full, int32_t(kb * 128u), rowB);
+                            tma_load_3d_pair(scales, &mapScaleA, full, 0, int32_t(kb * GROUPS), int32_t(tm * 2u + rank));
+                            tma_load_3d_pair(scales + GROUPS * MX_TILE_BYTES, &mapScaleB, full, 0,
+                                             int32_t(kb * GROUPS), int32_t(col0 / 128u));
+                        }
+                    }
+                    if(!ok)
+                        settle();
+                }
+            }
+            else if(warp == 1)
+            {
+                if(rank == 0 && elect_one())
+                {
+                    uint32_t it = 0;
+                    bool     ok = true;
+                    for(uint32_t i = 0; ok && sched.get(pairId, i, tm, col0, width); ++i)
+                    {
+                        // tile i - 1 has drained the columns that its accumulator shares with this one's
+                        if(i > 0u && !mbar_wait(&ctl->accShared, (i - 1u) & 1u, &ctl->abort, WAIT_ACC_EMPTY))
+                            break;
+                        tc_fence_after_sync();
+                        const uint32_t acc = tmem + (i & 1u) * ACC1;
+                        for(uint32_t kb = 0; kb < numSlots; ++kb, ++it)
+                        {
+                            const uint32_t s = it % P_STAGES, ph = (it / P_STAGES) & 1u;
+                            if(!mbar_wait(&ctl->full[s], ph, &ctl->abort, WAIT_STAGE_FULL))
+                            {
+                                ok = false;
+                                break;
+                            }
+                            tc_fence_after_sync();
+                            const uint32_t aAddr = smem_addr(ring + s * SLOT), bAddr = aAddr + CODE_BYTES;
+                            const uint32_t sAddr = bAddr + CODE_BYTES;
+                            const uint32_t scaleA = tmem + 512u - (1u + (it & 1u)) * SCALE_COLS;
+                            const uint32_t scaleB = scaleA + 4u * GROUPS;
+                            const uint32_t left  = p.k - kb * SLOT_K;
+                            const uint32_t steps = left >= SLOT_K ? SLOT_K / MMA_K : (left + MMA_K - 1u) / MMA_K;
+#pragma unroll
+                            for(uint32_t g = 0; g < GROUPS; ++g)
+                            {
+                                tmem_copy_scales_pair(scaleA + 4u * g, smem_desc_scales(sAddr + g * MX_TILE_BYTES));
+                                tmem_copy_scales_pair(scaleB + 8u * g, smem_desc_scales(sAddr + (GROUPS + g) * MX_TILE_BYTES));
+                                tmem_copy_scales_pair(scaleB + 8u * g + 4u,
+                                                      smem_desc_scales(sAddr + (2u * GROUPS + g) * MX_TILE_BYTES));
+                            }
+#pragma unroll
+                            for(uint32_t ks = 0; ks < SLOT_K / MMA_K; ++ks)
+                            {
+                                if(ks >= steps)
+                                    break;
+                                const uint32_t g  = KIND == ScaleKind::E4M3_16 ? ks : ks / 2u;
+                                const uint32_t id = KIND == ScaleKind::E4M3_16 ? 0u : (ks & 1u) * 2u;
+                                mma_scaled_pair<KIND>(acc, smem_desc_kmajor_sw128(aAddr + ks * 32u),
+                                                      smem_desc_kmajor_sw128(bAddr + ks * 32u),
+                                                      make_instr_desc_scaled(KIND, 256u, P_TILE, id), scaleA + 4u * g,
+                                                      scaleB + 8u * g, (kb > 0u || ks > 0u) ? 1u : 0u);
+                            }
+                            mma_commit_pair(&ctl->empty[s], 0x3);
+                        }
+                        if(ok)
+                            mma_commit_pair(&ctl->accFull[i & 1u], 0x3);
+                    }
+                }
+            }
+            else
+            {
+                const uint32_t quad = warp % 4, rowIn = quad * 32u + lane;
+                const uint32_t leaderShared = map_to_cta(smem_addr(&ctl->accShared), 0);
+                uint32_t       boxes = 0;
+                for(uint32_t i = 0; sched.get(pairId, i, tm, col0, width); ++i)
+                {
+                    // the second accumulator's shared columns are its first ones, the first one's its last
+                    const uint32_t buf = i & 1u;
+                    if(!drainTile<OutT>(ctl, staging, &mapC, &mapD, p, tmem + ((quad * 32u) << 16) + buf * ACC1,
+                                        buf ? 0u : ACC1, SHARED, buf, (i >> 1) & 1u, tm * P_TILE + rank * 128u, rowIn,
+                                        col0, boxes, leaderShared))
+                    {
+                        if(threadIdx.x == 64u)
+                            settle();
+                        break;
+                    }
+                }
+                if(threadIdx.x == 64u)
+                    tma_store_wait_read<0>(); // shared memory outlives the stores' reads of it
+            }
+
+            tc_fence_before_sync();
+            __syncthreads();
+            cluster_arrive_relaxed(); // neither block leaves while the other may still signal it
+            cluster_wait();
+            if(warp == 1)
+            {
+                __syncwarp();
+                tc_fence_after_sync();
+                tmem_dealloc_pair(tmem, 512);
             }
             if(threadIdx.x == 0 && ctl->abort.flag != 0u && p.status != nullptr)
             {
@@ -254,6 +602,27 @@ namespace b200wmma
             return r == CUDA_SUCCESS ? B200WMMA_OK : B200WMMA_ERR_CUDA;
         }
 
+        // Rows of C or D; box: 128 rows x 64 bytes.
+        template <typename OutT>
+        int outputMap(CUtensorMap* map, void const* base, uint32_t rows, uint32_t cols, uint32_t ld)
+        {
+            const cuuint64_t dims[2]    = {cols, rows};
+            const cuuint64_t strides[1] = {cuuint64_t(ld) * sizeof(OutT)};
+            const cuuint32_t box[2]     = {cuuint32_t(64 / sizeof(OutT)), 128};
+            const cuuint32_t estr[2]    = {1, 1};
+            EncodeFn         fn         = tensorMapEncoder();
+            if(!fn)
+                return B200WMMA_ERR_CUDA;
+            const CUtensorMapDataType type = sizeof(OutT) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                             : std::is_same<OutT, __half>::value
+                                                 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+            const CUresult r = fn(map, type, 2, const_cast<void*>(base), dims, strides, box, estr,
+                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+                                  CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+            return r == CUDA_SUCCESS ? B200WMMA_OK : B200WMMA_ERR_CUDA;
+        }
+
         template <typename KernelT>
         int optInSharedMemory(KernelT kernel, uint32_t bytes, uint32_t (&done)[64])
         {
@@ -278,8 +647,47 @@ namespace b200wmma
         };
 
         template <ScaleKind KIND, typename OutT>
+        int launchPairs(Operands const& o, Params const& q, int sms, cudaStream_t stream)
+        {
+            constexpr uint32_t GROUPS = slotGroups<KIND>();
+            const uint32_t     groups = mxGroups(KIND == ScaleKind::E4M3_16, q.k);
+            const uint64_t     tiles  = uint64_t((q.m + P_TILE - 1u) / P_TILE) * ((q.n + P_TILE - 1u) / P_TILE);
+            if(tiles > 0x7fffffffull)
+                return B200WMMA_ERR_TOO_LARGE;
+            CUtensorMap mapA, mapB, mapScaleA, mapScaleB, mapC, mapD;
+            int         rc = codeMap(&mapA, o.a, q.m, q.k, o.lda, 128);
+            if(rc == B200WMMA_OK)
+                rc = codeMap(&mapB, o.b, q.n, q.k, o.ldb, 128);
+            if(rc == B200WMMA_OK)
+                rc = scaleMap(&mapScaleA, o.aScales, q.m, groups, GROUPS, 1);
+            if(rc == B200WMMA_OK)
+                rc = scaleMap(&mapScaleB, o.bScales, q.n, groups, GROUPS, 2);
+            if(rc == B200WMMA_OK)
+                rc = outputMap<OutT>(&mapD, q.d, q.m, q.n, q.ldd);
+            mapC = mapD;
+            if(rc == B200WMMA_OK && q.c)
+                rc = outputMap<OutT>(&mapC, q.c, q.m, q.n, q.ldc);
+            if(rc != B200WMMA_OK)
+                return rc;
+            constexpr uint32_t smem = pairSmemBytes<KIND>();
+            static uint32_t    done[64] = {};
+            rc = optInSharedMemory(mxGemmPairKernel<KIND, OutT>, smem, done);
+            if(rc != B200WMMA_OK)
+                return rc;
+            const PairParams p{q.c, q.d, q.m, q.n, q.k, q.ldc, q.ldd, q.alpha, q.beta, 16u, q.status};
+            const uint32_t   pairs = uint32_t(tiles < uint64_t(sms / 2) ? tiles : uint64_t(sms / 2));
+            return cudaToStatus(launchOverlapped(mxGemmPairKernel<KIND, OutT>, dim3(2u * pairs), dim3(NUM_THREADS), smem,
+                                                 stream, mapA, mapB, mapScaleA, mapScaleB, mapC, mapD, p));
+        }
+
+        template <ScaleKind KIND, typename OutT>
         int launch(Operands const& o, Params p, cudaStream_t stream)
         {
+            const int sms = smCount();
+            if(sms < 2)
+                return B200WMMA_ERR_CUDA;
+            if(p.m > 128u)
+                return launchPairs<KIND, OutT>(o, p, sms, stream);
             constexpr uint32_t GROUPS = slotGroups<KIND>();
             const uint32_t     groups = mxGroups(KIND == ScaleKind::E4M3_16, p.k);
             p.nq                      = p.m > 128u ? 256u : p.m > 64u ? 128u : (p.m + 15u) / 16u * 16u;

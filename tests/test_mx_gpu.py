@@ -163,6 +163,15 @@ def test_gemm_alpha_beta(fmt, kind, m, n, k):
 
 
 @FORMATS
+@KINDS
+@pytest.mark.parametrize("m,n,k", [(2570, 5000, 200), (300, 20001, 328)])
+def test_gemm_many_tiles(fmt, kind, m, n, k):
+    """More tiles than the device has SMs: several to a block, the last ones ragged."""
+    _product(fmt, kind, m, n, k, 5)
+    _product(fmt, kind, m, n, k, 6, alpha=0.5, beta=-2.0, c=True)
+
+
+@FORMATS
 @pytest.mark.parametrize("m,n,k", [(1, 500, 4096), (33, 260, 2100), (300, 400, 1111)])
 def test_gemm_rounding(fmt, m, n, k):
     """Full-range operands.  Each of the k products enters a fp32 sum that the tensor core may
