@@ -12,10 +12,12 @@
 // result depends on its arguments alone: tokens are sorted by row (a stable radix sort), then
 // every run of equal rows is summed in token order, in fp32, by cutting the sorted tokens into
 // chunks; a run inside one chunk is written at once, the pieces of a run that crosses chunks go
-// to the workspace, which the next, much smaller level treats as its tokens.
+// to the workspace, which the next, much smaller level treats as its tokens.  Rows without a
+// token are cleared by blocks of their own next to those that sort, which leave HBM idle.
 #include "common.cuh"
 #include "mx_format.cuh"
 #include "rocwmma/rocwmma_block.hpp"
+#include <mutex>
 
 namespace b200wmma
 {
@@ -25,6 +27,7 @@ namespace b200wmma
     namespace
     {
         constexpr uint32_t THREADS = 256;
+        constexpr uint32_t DEVICE_THREADS = 148u * 2048u; // resident at once
         constexpr uint32_t NO_ROW  = 0x7fffffffu; // no token, or no row of the table
         constexpr uint32_t EMPTY   = 0x80000000u; // part of a run, but adds nothing to it
 
@@ -62,47 +65,12 @@ namespace b200wmma
             return row >= 0 && row < end ? uint32_t(row) : NO_ROW;
         }
 
-        // V values of a row: 16 or 32 bytes with V = 8, one element with V = 1.
+        // V neighbouring values of a row, loaded and stored as one where their alignment allows it.
         template <typename T, int V>
-        struct Piece
+        struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Piece
         {
-            static constexpr int BYTES = int(sizeof(T)) * V;
-            T                    v[V];
+            T v[V];
         };
-        template <typename T, int V>
-        __device__ inline void loadPiece(T const* p, float (&f)[V])
-        {
-            if constexpr(V == 1)
-                f[0] = toFloat(*p);
-            else
-            {
-                constexpr int N = int(sizeof(T)) * V / 16;
-                uint4         raw[N];
-#pragma unroll
-                for(int i = 0; i < N; ++i)
-                    raw[i] = reinterpret_cast<uint4 const*>(p)[i];
-#pragma unroll
-                for(int i = 0; i < V; ++i)
-                    f[i] = toFloat(reinterpret_cast<T const*>(raw)[i]);
-            }
-        }
-        template <typename T, int V>
-        __device__ inline void storePiece(T* p, float const (&f)[V])
-        {
-            if constexpr(V == 1)
-                *p = fromFloat<T>(f[0]);
-            else
-            {
-                constexpr int N = int(sizeof(T)) * V / 16;
-                alignas(16) T v[V];
-#pragma unroll
-                for(int i = 0; i < V; ++i)
-                    v[i] = fromFloat<T>(f[i]);
-#pragma unroll
-                for(int i = 0; i < N; ++i)
-                    __stcs(reinterpret_cast<uint4*>(p) + i, reinterpret_cast<uint4 const*>(v)[i]);
-            }
-        }
 
         // ---- lookup ----------------------------------------------------------------------
         struct LookupParams
@@ -112,92 +80,329 @@ namespace b200wmma
             void*       out;
             uint64_t    ldt, outOuter, outInner;
             uint32_t    pieces, lanesLog2; // pieces of a row; threads side by side on a row
+            uint32_t    perBlock; // tokens
             float       scale;
         };
 
-        // A thread moves one piece of U tokens; 2^lanesLog2 neighbours share the tokens.
-        template <typename T, typename OutT, int V, int U>
+        // A block finds the rows of its tokens first, one thread a token, then moves them, U pieces
+        // in flight a thread.
+        template <typename T, typename OutT, int V>
         __global__ void __launch_bounds__(THREADS) lookupKernel(const LookupParams p)
         {
-            const uint32_t lanes = 1u << p.lanesLog2;
-            const uint32_t piece = blockIdx.y * lanes + (threadIdx.x & (lanes - 1u));
-            const uint32_t perStep = THREADS >> p.lanesLog2;
-            const uint32_t token0  = blockIdx.x * (perStep * U) + (threadIdx.x >> p.lanesLog2);
+            constexpr uint32_t U = V == 8 ? 4 : 8;
+            __shared__ uint32_t rows[THREADS];
+            __shared__ uint64_t outs[THREADS];
+            const uint32_t token0 = blockIdx.x * p.perBlock;
+            const uint32_t here   = min(p.perBlock, p.t.count - token0);
             grid_dependency_wait();
             grid_launch_dependents();
-            if(piece >= p.pieces)
-                return;
-            float    v[U][V];
-            uint64_t at[U];
-            bool     in[U];
-#pragma unroll
-            for(int u = 0; u < U; ++u)
+            if(threadIdx.x < here)
             {
-                const uint32_t token = token0 + u * perStep;
-                in[u]                = token < p.t.count;
-                uint32_t outer = 0, inner = 0;
-                const uint32_t row = in[u] ? rowOf(p.t, token, outer, inner) : NO_ROW;
-                at[u] = uint64_t(outer) * p.outOuter + uint64_t(inner) * p.outInner + uint64_t(piece) * V;
-                if(row != NO_ROW)
-                    loadPiece<T, V>(static_cast<T const*>(p.table) + uint64_t(row) * p.ldt + uint64_t(piece) * V, v[u]);
-                else
+                uint32_t outer, inner;
+                rows[threadIdx.x] = rowOf(p.t, token0 + threadIdx.x, outer, inner);
+                outs[threadIdx.x] = uint64_t(outer) * p.outOuter + uint64_t(inner) * p.outInner;
+            }
+            __syncthreads();
+            const uint32_t lanes = 1u << p.lanesLog2, step = THREADS >> p.lanesLog2;
+            for(uint32_t piece = threadIdx.x & (lanes - 1u); piece < p.pieces; piece += lanes)
+            {
+                const uint64_t at = uint64_t(piece) * V;
+                for(uint32_t t0 = threadIdx.x >> p.lanesLog2; t0 < here; t0 += U * step)
                 {
+                    Piece<T, V> v[U];
+                    uint32_t    row[U];
 #pragma unroll
-                    for(int i = 0; i < V; ++i)
-                        v[u][i] = 0.0f;
-                }
-                // an unwritten row stays a zero: scale may be infinite or NaN
-                if(row != NO_ROW)
-                {
+                    for(uint32_t u = 0; u < U; ++u)
+                    {
+                        const uint32_t t = t0 + u * step;
+                        row[u]           = t < here ? rows[t] : NO_ROW;
+                        if(row[u] != NO_ROW)
+                            v[u] = *reinterpret_cast<Piece<T, V> const*>(static_cast<T const*>(p.table)
+                                                                         + uint64_t(row[u]) * p.ldt + at);
+                    }
 #pragma unroll
-                    for(int i = 0; i < V; ++i)
-                        v[u][i] *= p.scale;
+                    for(uint32_t u = 0; u < U; ++u)
+                    {
+                        const uint32_t t = t0 + u * step;
+                        if(t < here)
+                        {
+                            Piece<OutT, V> o;
+#pragma unroll
+                            for(int i = 0; i < V; ++i)
+                                o.v[i] = fromFloat<OutT>(row[u] != NO_ROW ? toFloat(v[u].v[i]) * p.scale : 0.0f);
+                            *reinterpret_cast<Piece<OutT, V>*>(static_cast<OutT*>(p.out) + outs[t] + at) = o;
+                        }
+                    }
                 }
             }
+        }
+
+        // ---- clearing rows without a token -------------------------------------------------
+        struct ClearParams
+        {
+            void*    table;
+            uint64_t ldt;
+            uint32_t pieces, lanesLog2; // of a row
+            uint32_t blocks; // that clear, behind those that sort; 0: nothing to clear
+        };
+
+        // The rows of [begin, end) that keep(row) does not name, by the calling block.
+        template <typename OutT, int V, typename Keep>
+        __device__ inline void clearRows(ClearParams const& c, uint64_t begin, uint64_t end, Keep keep)
+        {
+            const uint32_t lanes = 1u << c.lanesLog2;
+            Piece<OutT, V> zero;
 #pragma unroll
-            for(int u = 0; u < U; ++u)
-                if(in[u])
-                    storePiece<OutT, V>(static_cast<OutT*>(p.out) + at[u], v[u]);
+            for(int i = 0; i < V; ++i)
+                zero.v[i] = OutT(0.0f);
+            for(uint64_t row = begin + (threadIdx.x >> c.lanesLog2); row < end; row += blockDim.x >> c.lanesLog2)
+                if(!keep(row))
+                    for(uint32_t piece = threadIdx.x & (lanes - 1u); piece < c.pieces; piece += lanes)
+                        *reinterpret_cast<Piece<OutT, V>*>(static_cast<OutT*>(c.table) + row * c.ldt + uint64_t(piece) * V)
+                            = zero;
         }
 
-        // ---- sorting tokens by row ---------------------------------------------------------
-        constexpr uint32_t SORT_ITEMS  = 16; // keys of a thread
-        constexpr uint32_t SORT_TILE   = THREADS * SORT_ITEMS;
-        constexpr uint32_t RADIX       = 256;
-        constexpr uint32_t SORT_WARPS  = THREADS / 32;
-
-        // Row of every token, and a bit for every row that has one.
-        __global__ void __launch_bounds__(THREADS) keysKernel(const Tokens t, uint32_t* keys, uint32_t* touched)
+        // ---- sorting few tokens: one block --------------------------------------------------
+        constexpr uint32_t SMALL_THREADS = 1024;
+        constexpr uint32_t SMALL_ITEMS   = 16;
+        constexpr uint32_t SMALL_TOKENS  = SMALL_THREADS * SMALL_ITEMS;
+        constexpr uint32_t SMALL_WARPS   = SMALL_THREADS / 32;
+        constexpr uint32_t RADIX         = 256;
+        constexpr uint32_t CLEAR_BITS    = 65536; // rows that a clearing block looks over at a time
+        struct SmallShared
         {
+            uint32_t keys[SMALL_TOKENS];
+            uint32_t bins[SMALL_WARPS][RADIX];
+            uint32_t sums[8];
+            uint16_t tokens[SMALL_TOKENS];
+        };
+        static_assert(CLEAR_BITS / 8 <= sizeof(SmallShared::keys), "the clearing blocks' bits take the keys' place");
+
+        // Block 0 sorts all tokens in shared memory; the others clear a share of the rows each, for
+        // which they look through the tokens themselves.
+        template <typename OutT, int V>
+        __global__ void __launch_bounds__(SMALL_THREADS)
+            sortSmallKernel(const Tokens t, const ClearParams c, const uint32_t passes, uint32_t* keysOut, uint32_t* tokensOut)
+        {
+            extern __shared__ uint8_t smem[];
+            SmallShared*   sh   = reinterpret_cast<SmallShared*>(smem);
+            const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
             grid_dependency_wait();
             grid_launch_dependents();
-            const uint32_t token = blockIdx.x * THREADS + threadIdx.x;
-            if(token >= t.count)
+            uint32_t outer, inner;
+            if(blockIdx.x > 0u)
+            {
+                const uint64_t begin = uint64_t(blockIdx.x - 1u) * t.rows / c.blocks;
+                const uint64_t end   = uint64_t(blockIdx.x) * t.rows / c.blocks;
+                for(uint64_t r0 = begin; r0 < end; r0 += CLEAR_BITS)
+                {
+                    const uint32_t count = uint32_t(min(uint64_t(CLEAR_BITS), end - r0));
+                    __syncthreads();
+                    for(uint32_t i = threadIdx.x; i < (count + 31u) / 32u; i += SMALL_THREADS)
+                        sh->keys[i] = 0;
+                    __syncthreads();
+                    for(uint32_t i = threadIdx.x; i < t.count; i += SMALL_THREADS)
+                    {
+                        const uint32_t row = rowOf(t, i, outer, inner);
+                        if(row >= r0 && row - r0 < count)
+                            atomicOr(&sh->keys[uint32_t(row - r0) / 32u], 1u << (row - r0) % 32u);
+                    }
+                    __syncthreads();
+                    clearRows<OutT, V>(c, r0, r0 + count, [&](uint64_t row) {
+                        const uint32_t i = uint32_t(row - r0);
+                        return (sh->keys[i / 32u] >> (i % 32u)) & 1u;
+                    });
+                }
                 return;
-            uint32_t       outer, inner;
-            const uint32_t row = rowOf(t, token, outer, inner);
-            keys[token]        = row == NO_ROW ? t.rows : row; // behind every row
-            if(row != NO_ROW && touched)
-                atomicOr(&touched[row / 32u], 1u << (row % 32u));
+            }
+            // A warp's keys are neighbours, 32 of them a step.
+            const uint32_t items = (t.count + SMALL_THREADS - 1u) / SMALL_THREADS;
+            const uint32_t first = warp * 32u * items + lane;
+            uint32_t       key[SMALL_ITEMS], rank[SMALL_ITEMS];
+            uint16_t       token[SMALL_ITEMS];
+#pragma unroll
+            for(uint32_t i = 0; i < SMALL_ITEMS; ++i)
+            {
+                const uint32_t at = first + i * 32u;
+                key[i]            = 0;
+                token[i]          = uint16_t(at);
+                if(i < items && at < t.count)
+                {
+                    const uint32_t row = rowOf(t, at, outer, inner);
+                    key[i]             = row == NO_ROW ? t.rows : row; // behind every row
+                }
+            }
+            for(uint32_t pass = 0; pass < passes; ++pass)
+            {
+                const uint32_t shift = 8u * pass;
+                for(uint32_t i = threadIdx.x; i < SMALL_WARPS * RADIX; i += SMALL_THREADS)
+                    sh->bins[0][i] = 0;
+                __syncthreads();
+#pragma unroll
+                for(uint32_t i = 0; i < SMALL_ITEMS; ++i)
+                    if(i < items)
+                    {
+                        const bool     in    = first + i * 32u < t.count;
+                        const uint32_t digit = (key[i] >> shift) % RADIX;
+                        const uint32_t peers = __match_any_sync(0xffffffffu, in ? digit : RADIX);
+                        rank[i]              = (in ? sh->bins[warp][digit] : 0u) + __popc(peers & ((1u << lane) - 1u));
+                        __syncwarp();
+                        if(in && (peers >> lane) == 1u) // the last of its digit
+                            sh->bins[warp][digit] = rank[i] + 1u;
+                        __syncwarp();
+                    }
+                __syncthreads();
+                // thread = digit: where the keys of each warp go
+                uint32_t sum = 0, before = 0;
+                if(threadIdx.x < RADIX)
+                {
+                    for(uint32_t w = 0; w < SMALL_WARPS; ++w)
+                        sum += sh->bins[w][threadIdx.x];
+                    before = sum;
+#pragma unroll
+                    for(uint32_t d = 1; d < 32u; d *= 2u)
+                    {
+                        const uint32_t other = __shfl_up_sync(0xffffffffu, before, d);
+                        if(lane >= d)
+                            before += other;
+                    }
+                    if(lane == 31u)
+                        sh->sums[warp] = before;
+                    before -= sum;
+                }
+                __syncthreads();
+                if(threadIdx.x < RADIX)
+                {
+                    for(uint32_t w = 0; w < warp; ++w)
+                        before += sh->sums[w];
+                    for(uint32_t w = 0; w < SMALL_WARPS; ++w)
+                    {
+                        const uint32_t count      = sh->bins[w][threadIdx.x];
+                        sh->bins[w][threadIdx.x] = before;
+                        before += count;
+                    }
+                }
+                __syncthreads();
+                const bool last = pass + 1u == passes;
+#pragma unroll
+                for(uint32_t i = 0; i < SMALL_ITEMS; ++i)
+                    if(i < items && first + i * 32u < t.count)
+                    {
+                        const uint32_t to = sh->bins[warp][(key[i] >> shift) % RADIX] + rank[i];
+                        if(last)
+                        {
+                            keysOut[to]   = key[i];
+                            tokensOut[to] = token[i];
+                        }
+                        else
+                        {
+                            sh->keys[to]   = key[i];
+                            sh->tokens[to] = token[i];
+                        }
+                    }
+                if(last)
+                    break;
+                __syncthreads();
+#pragma unroll
+                for(uint32_t i = 0; i < SMALL_ITEMS; ++i)
+                    if(i < items && first + i * 32u < t.count)
+                    {
+                        key[i]   = sh->keys[first + i * 32u];
+                        token[i] = sh->tokens[first + i * 32u];
+                    }
+            }
         }
 
-        // counts[digit][tile]
-        __global__ void __launch_bounds__(THREADS)
-            countKernel(uint32_t const* keys, uint32_t n, uint32_t shift, uint32_t tiles, uint32_t* counts)
+        // ---- sorting many tokens -------------------------------------------------------------
+        constexpr uint32_t SORT_ITEMS = 16; // keys of a thread
+        constexpr uint32_t SORT_TILE  = THREADS * SORT_ITEMS;
+        constexpr uint32_t SORT_WARPS = THREADS / 32;
+
+        // What a block of a sorting kernel does that is not one of its `tiles` first: it clears its
+        // part of share `share` of `shares` of the rows.
+        struct Share
         {
-            __shared__ uint32_t bins[RADIX];
-            grid_dependency_wait();
-            grid_launch_dependents();
+            uint8_t const* touched;
+            uint32_t       rows, share, shares;
+        };
+        template <typename OutT, int V>
+        __device__ inline void clearShare(ClearParams const& c, Share const& s, uint32_t block)
+        {
+            const uint64_t begin = uint64_t(s.rows) * s.share / s.shares, count = uint64_t(s.rows) * (s.share + 1u) / s.shares - begin;
+            clearRows<OutT, V>(c, begin + count * block / c.blocks, begin + count * (block + 1u) / c.blocks,
+                               [&](uint64_t row) { return s.touched[row] != 0; });
+        }
+
+        // counts[digit][tile] += keys of the tile
+        __device__ inline void countDigits(uint32_t* bins, uint32_t const (&key)[SORT_ITEMS], uint32_t first, uint32_t n,
+                                           uint32_t shift)
+        {
             bins[threadIdx.x] = 0;
             __syncthreads();
 #pragma unroll
             for(uint32_t i = 0; i < SORT_ITEMS; ++i)
             {
-                const uint64_t at = uint64_t(blockIdx.x) * SORT_TILE + i * THREADS + threadIdx.x;
-                if(at < n)
-                    atomicAdd(&bins[(keys[at] >> shift) % RADIX], 1u);
+                // one addition for the equal digits of a warp: a hot row would queue 32
+                const bool     in    = uint64_t(first) + i * THREADS < n;
+                const uint32_t digit = in ? (key[i] >> shift) % RADIX : RADIX;
+                const uint32_t peers = __match_any_sync(0xffffffffu, digit);
+                if(in && (peers & ((1u << (threadIdx.x % 32u)) - 1u)) == 0u)
+                    atomicAdd(&bins[digit], uint32_t(__popc(peers)));
             }
             __syncthreads();
+        }
+
+        // Row of every token, a flag for every row that has one, and the first digit's counts.
+        __global__ void __launch_bounds__(THREADS)
+            keysKernel(const Tokens t, uint32_t* keys, uint8_t* touched, uint32_t tiles, uint32_t* counts)
+        {
+            __shared__ uint32_t bins[RADIX];
+            grid_dependency_wait();
+            grid_launch_dependents();
+            const uint32_t first = blockIdx.x * SORT_TILE + threadIdx.x;
+            uint32_t       key[SORT_ITEMS];
+#pragma unroll
+            for(uint32_t i = 0; i < SORT_ITEMS; ++i)
+            {
+                const uint32_t token = first + i * THREADS;
+                key[i]               = t.rows; // behind every row
+                if(token < t.count)
+                {
+                    uint32_t       outer, inner;
+                    const uint32_t row = rowOf(t, token, outer, inner);
+                    if(row != NO_ROW)
+                        key[i] = row;
+                }
+            }
+#pragma unroll
+            for(uint32_t i = 0; i < SORT_ITEMS; ++i)
+                if(first + i * THREADS < t.count)
+                {
+                    keys[first + i * THREADS] = key[i];
+                    // (read first: stores to a hot row's flag would queue up)
+                    if(touched && key[i] < t.rows && touched[key[i]] == 0)
+                        touched[key[i]] = 1;
+                }
+            countDigits(bins, key, first, t.count, 0);
+            counts[threadIdx.x * tiles + blockIdx.x] = bins[threadIdx.x];
+        }
+
+        template <typename OutT, int V>
+        __global__ void __launch_bounds__(THREADS)
+            countKernel(uint32_t const* keys, uint32_t n, uint32_t shift, uint32_t tiles, uint32_t* counts,
+                        const ClearParams c, const Share s)
+        {
+            __shared__ uint32_t bins[RADIX];
+            grid_dependency_wait();
+            grid_launch_dependents();
+            if(blockIdx.x >= tiles)
+                return clearShare<OutT, V>(c, s, blockIdx.x - tiles);
+            const uint32_t first = blockIdx.x * SORT_TILE + threadIdx.x;
+            uint32_t       key[SORT_ITEMS];
+#pragma unroll
+            for(uint32_t i = 0; i < SORT_ITEMS; ++i)
+                key[i] = first + i * THREADS < n ? keys[first + i * THREADS] : 0u;
+            countDigits(bins, key, first, n, shift);
             counts[threadIdx.x * tiles + blockIdx.x] = bins[threadIdx.x];
         }
 
@@ -253,16 +458,19 @@ namespace b200wmma
         // Moves every key of a tile, with its token, to its place among the keys of this digit:
         // those of smaller digits, of earlier tiles, of earlier warps, of earlier rows of 32 and
         // of smaller lanes come first.  tokensIn == nullptr: key i belongs to token i.
+        template <typename OutT, int V>
         __global__ void __launch_bounds__(THREADS)
             scatterKernel(uint32_t const* keysIn, uint32_t const* tokensIn, uint32_t n, uint32_t shift,
                           uint32_t tiles, uint32_t const* counts, uint32_t const* totals,
-                          uint32_t* keysOut, uint32_t* tokensOut)
+                          uint32_t* keysOut, uint32_t* tokensOut, const ClearParams c, const Share s)
         {
             __shared__ uint32_t bins[SORT_WARPS][RADIX];
             __shared__ uint32_t warps[SORT_WARPS];
             const uint32_t      warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
             grid_dependency_wait();
             grid_launch_dependents();
+            if(blockIdx.x >= tiles)
+                return clearShare<OutT, V>(c, s, blockIdx.x - tiles);
 #pragma unroll
             for(uint32_t w = 0; w < SORT_WARPS; ++w)
                 bins[w][threadIdx.x] = 0;
@@ -281,8 +489,7 @@ namespace b200wmma
                 const bool     in    = first + i * 32u < n;
                 const uint32_t digit = (key[i] >> shift) % RADIX;
                 const uint32_t peers = __match_any_sync(0xffffffffu, in ? digit : RADIX);
-                const uint32_t before = in ? bins[warp][digit] : 0u;
-                rank[i]               = before + __popc(peers & ((1u << lane) - 1u));
+                rank[i]              = (in ? bins[warp][digit] : 0u) + __popc(peers & ((1u << lane) - 1u));
                 __syncwarp();
                 if(in && (peers >> lane) == 1u) // the last of its digit
                     bins[warp][digit] = rank[i] + 1u;
@@ -318,6 +525,7 @@ namespace b200wmma
         }
 
         // ---- summing runs ------------------------------------------------------------------
+        constexpr uint32_t SUM_ITEMS = 2048; // of a block
         struct SumParams
         {
             uint32_t const* keys; // of the items, equal rows next to each other
@@ -335,148 +543,129 @@ namespace b200wmma
             float*          pieceSums; // rows of `pieces * V`
         };
 
+        // Threads side by side share a chunk of items, one piece of the row each.  The block puts
+        // its items' rows and places into shared memory first, so that the loads of U items do not
+        // wait for one another.
         template <typename T, typename OutT, int V>
         __global__ void __launch_bounds__(THREADS) sumKernel(const SumParams p)
         {
-            constexpr uint32_t U     = 8;
-            const uint32_t     lanes = 1u << p.lanesLog2;
-            const uint32_t piece = blockIdx.y * lanes + (threadIdx.x & (lanes - 1u));
-            const uint64_t chunkIdx = uint64_t(blockIdx.x) * (THREADS >> p.lanesLog2) + (threadIdx.x >> p.lanesLog2);
-            const uint64_t begin = chunkIdx * p.chunk;
+            constexpr uint32_t U = sizeof(T) * V > 16 ? 4 : V == 8 ? 8 : 16;
+            __shared__ uint32_t keys[SUM_ITEMS + 2]; // one on each side
+            __shared__ uint64_t places[SUM_ITEMS];
+            const uint32_t lanes = 1u << p.lanesLog2, groups = blockDim.x >> p.lanesLog2;
+            const uint64_t item0 = uint64_t(blockIdx.x) * groups * p.chunk;
             grid_dependency_wait();
             grid_launch_dependents();
+            for(uint32_t i = threadIdx.x; i < groups * p.chunk + 2u; i += blockDim.x)
+            {
+                const uint64_t at  = item0 + i; // of item at - 1
+                const uint32_t key = at >= 1u && at <= p.n ? p.keys[at - 1u] : NO_ROW;
+                keys[i]            = key;
+                if(i >= 1u && i <= groups * p.chunk && key < p.rows)
+                {
+                    const uint32_t token = p.tokens ? p.tokens[at - 1u] : uint32_t(at - 1u);
+                    uint32_t       outer = token, in = 0;
+                    if(p.inner > 1u)
+                    {
+                        outer = token / p.inner;
+                        in    = token - outer * p.inner;
+                    }
+                    places[i - 1u] = uint64_t(outer) * p.gradOuter + uint64_t(in) * p.gradInner;
+                }
+            }
+            __syncthreads();
+            const uint32_t piece = blockIdx.y * lanes + (threadIdx.x & (lanes - 1u));
+            const uint32_t local = (threadIdx.x >> p.lanesLog2) * p.chunk; // first item in shared memory
+            const uint64_t begin = item0 + local, chunkIdx = begin / p.chunk;
             if(piece >= p.pieces || begin >= p.n)
                 return;
-            const uint32_t end = uint32_t(min(uint64_t(p.n), begin + p.chunk));
-            const uint64_t width = uint64_t(p.pieces) * V;
-            const bool     marks = piece == 0u && p.pieceKeys != nullptr;
-            const uint32_t before = begin > 0 ? p.keys[begin - 1] & ~EMPTY : NO_ROW;
-            const uint32_t after  = end < p.n ? p.keys[end] & ~EMPTY : NO_ROW;
+            const uint32_t count  = uint32_t(min(uint64_t(p.chunk), p.n - begin));
+            const uint64_t width  = uint64_t(p.pieces) * V;
+            const uint32_t before = keys[local] & ~EMPTY, after = keys[local + count + 1u] & ~EMPTY;
+            uint32_t const* key   = keys + local + 1u;
+            T const*        grad  = static_cast<T const*>(p.grad) + uint64_t(piece) * V;
 
             float    sum[V];
-            uint32_t run = NO_ROW; // row of the current run
-            bool     fromLeft = false, left = false, right = false;
+            uint32_t run      = NO_ROW; // row of the current run
+            bool     fromLeft = false;
             uint32_t leftKey = NO_ROW, rightKey = NO_ROW;
-            auto flush = [&](bool last) {
+            auto     flush = [&](bool last) {
                 if(run >= p.rows)
                     return;
                 const bool toRight = last && after == run;
                 if(!fromLeft && !toRight)
                 {
-                    OutT* at = static_cast<OutT*>(p.table) + uint64_t(run) * p.ldt + uint64_t(piece) * V;
-                    float v[V];
+                    auto* at = reinterpret_cast<Piece<OutT, V>*>(static_cast<OutT*>(p.table) + uint64_t(run) * p.ldt
+                                                                + uint64_t(piece) * V);
+                    Piece<OutT, V> o;
                     if(p.accumulate)
                     {
-                        loadPiece<OutT, V>(at, v);
+                        const Piece<OutT, V> old = *at;
 #pragma unroll
                         for(int i = 0; i < V; ++i)
-                            v[i] = fmaf(sum[i], p.scale, v[i]);
+                            o.v[i] = fromFloat<OutT>(fmaf(sum[i], p.scale, toFloat(old.v[i])));
                     }
                     else
                     {
 #pragma unroll
                         for(int i = 0; i < V; ++i)
-                            v[i] = sum[i] * p.scale;
+                            o.v[i] = fromFloat<OutT>(sum[i] * p.scale);
                     }
-                    storePiece<OutT, V>(at, v);
+                    *at = o;
                     return;
                 }
-                float* at = p.pieceSums + (2u * chunkIdx + (fromLeft ? 0u : 1u)) * width + uint64_t(piece) * V;
+                Piece<float, V> s;
 #pragma unroll
                 for(int i = 0; i < V; ++i)
-                    at[i] = sum[i];
-                if(fromLeft)
+                    s.v[i] = sum[i];
+                *reinterpret_cast<Piece<float, V>*>(p.pieceSums + (2u * chunkIdx + (fromLeft ? 0u : 1u)) * width
+                                                    + uint64_t(piece) * V)
+                    = s;
+                if(!fromLeft)
+                    rightKey = run;
+                else
                 {
-                    left    = true;
                     leftKey = run;
                     if(toRight) // the run goes on: keep it one across this chunk's second place
                         rightKey = run | EMPTY;
                 }
-                else
-                {
-                    right    = true;
-                    rightKey = run;
-                }
             };
 
-            for(uint32_t i0 = uint32_t(begin); i0 < end; i0 += U)
+            for(uint32_t i0 = 0; i0 < count; i0 += U)
             {
-                float    v[U][V];
-                uint32_t key[U];
+                Piece<T, V> v[U];
 #pragma unroll
                 for(uint32_t u = 0; u < U; ++u)
-                {
-                    const uint32_t i = i0 + u;
-                    key[u]           = i < end ? p.keys[i] : NO_ROW | EMPTY;
-                    if((key[u] & EMPTY) == 0u && key[u] < p.rows)
+                    if(i0 + u < count && key[i0 + u] < p.rows)
+                        v[u] = *reinterpret_cast<Piece<T, V> const*>(grad + places[local + i0 + u]);
+#pragma unroll
+                for(uint32_t u = 0; u < U; ++u)
+                    if(i0 + u < count)
                     {
-                        const uint32_t token = p.tokens ? p.tokens[i] : i;
-                        uint64_t       at;
-                        if(p.inner > 1u)
+                        const uint32_t k = key[i0 + u], row = k & ~EMPTY;
+                        if(row != run)
                         {
-                            const uint32_t outer = token / p.inner;
-                            at = uint64_t(outer) * p.gradOuter + uint64_t(token - outer * p.inner) * p.gradInner;
+                            flush(false);
+                            run      = row;
+                            fromLeft = i0 + u == 0u && before == row;
+#pragma unroll
+                            for(int j = 0; j < V; ++j)
+                                sum[j] = k < p.rows ? toFloat(v[u].v[j]) : 0.0f;
                         }
-                        else
-                            at = uint64_t(token) * p.gradOuter;
-                        loadPiece<T, V>(static_cast<T const*>(p.grad) + at + uint64_t(piece) * V, v[u]);
-                    }
-                    else
-                    {
+                        else if(k < p.rows)
+                        {
 #pragma unroll
-                        for(int j = 0; j < V; ++j)
-                            v[u][j] = 0.0f;
+                            for(int j = 0; j < V; ++j)
+                                sum[j] += toFloat(v[u].v[j]);
+                        }
                     }
-                }
-#pragma unroll
-                for(uint32_t u = 0; u < U; ++u)
-                {
-                    if(i0 + u >= end)
-                        break;
-                    const uint32_t row = key[u] & ~EMPTY;
-                    if(row != run)
-                    {
-                        flush(false);
-                        run      = row;
-                        fromLeft = i0 + u == begin && before == row;
-#pragma unroll
-                        for(int j = 0; j < V; ++j)
-                            sum[j] = v[u][j];
-                    }
-                    else if((key[u] & EMPTY) == 0u)
-                    {
-#pragma unroll
-                        for(int j = 0; j < V; ++j)
-                            sum[j] += v[u][j];
-                    }
-                }
             }
             flush(true);
-            if(marks)
+            if(piece == 0u && p.pieceKeys)
             {
                 p.pieceKeys[2u * chunkIdx]      = leftKey;
                 p.pieceKeys[2u * chunkIdx + 1u] = rightKey;
             }
-        }
-
-        // Rows without a token.
-        template <typename OutT, int V>
-        __global__ void __launch_bounds__(THREADS)
-            clearKernel(OutT* table, uint64_t ldt, uint32_t rows, uint32_t pieces, uint32_t lanesLog2,
-                        uint32_t const* touched)
-        {
-            const uint32_t lanes = 1u << lanesLog2;
-            const uint64_t row   = uint64_t(blockIdx.x) * (THREADS >> lanesLog2) + (threadIdx.x >> lanesLog2);
-            grid_dependency_wait();
-            grid_launch_dependents();
-            if(row >= rows || (touched[row / 32u] >> (row % 32u)) & 1u)
-                return;
-            float zero[V];
-#pragma unroll
-            for(int i = 0; i < V; ++i)
-                zero[i] = 0.0f;
-            for(uint32_t piece = threadIdx.x & (lanes - 1u); piece < pieces; piece += lanes)
-                storePiece<OutT, V>(table + row * ldt + uint64_t(piece) * V, zero);
         }
 
         // ---- host side ---------------------------------------------------------------------
@@ -495,38 +684,41 @@ namespace b200wmma
                 ++l;
             return l;
         }
-        // Threads side by side on a row of `pieces`: enough, but no more than a block has.
-        uint32_t lanesFor(uint32_t pieces)
+        // Values of a piece: 8, 2 or 1, whatever divides dim and keeps every piece of the given
+        // tensors on its boundary.  `strides`: distances of rows, in elements.
+        template <typename... Strides>
+        uint32_t pieceSize(uint32_t dim, void const* base, uint64_t elem, uint32_t most, Strides... strides)
         {
-            const uint32_t l = log2Up(pieces);
-            return l > 8u ? 8u : l;
+            for(uint32_t v = most; v > 1u; v = v == 8u ? 2u : 1u)
+            {
+                const uint64_t bytes = v * elem < 16u ? v * elem : 16u;
+                if(dim % v == 0u && aligned(base, bytes) && ((strides * elem % bytes == 0) && ...))
+                    return v;
+            }
+            return 1;
         }
 
         template <typename T, typename OutT, int V>
-        int lookup(LookupParams p, cudaStream_t stream)
+        int lookup(LookupParams p, uint32_t dim, cudaStream_t stream)
         {
-            const uint32_t perStep = THREADS >> p.lanesLog2;
-            const uint32_t lanes   = 1u << p.lanesLog2;
-            const uint32_t across  = (p.pieces + lanes - 1u) / lanes;
-            // four tokens a thread once that still fills the device
-            const bool     many   = uint64_t(p.t.count) * across / perStep >= 4u * 148u * 8u;
-            const uint32_t each   = perStep * (many ? 4u : 1u);
-            const dim3     grid((p.t.count + each - 1u) / each, across);
-            return cudaToStatus(many ? launchOverlapped(lookupKernel<T, OutT, V, 4>, grid, dim3(THREADS), 0, stream, p)
-                                     : launchOverlapped(lookupKernel<T, OutT, V, 1>, grid, dim3(THREADS), 0, stream, p));
+            p.pieces    = dim / V;
+            p.lanesLog2 = log2Up(p.pieces) > 8u ? 8u : log2Up(p.pieces);
+            // 4096 pieces to a block (16 a thread), but blocks for every SM first
+            uint32_t per = p.pieces >= 4096u ? 1u : 4096u / p.pieces;
+            per          = per > THREADS ? THREADS : per;
+            const uint32_t spread = (p.t.count + 4u * 148u - 1u) / (4u * 148u);
+            p.perBlock            = per < spread ? per : spread;
+            return cudaToStatus(launchOverlapped(lookupKernel<T, OutT, V>, dim3((p.t.count + p.perBlock - 1u) / p.perBlock),
+                                                 dim3(THREADS), 0, stream, p));
         }
 
         template <typename T, typename OutT>
-        int lookupTyped(LookupParams p, uint32_t dim, cudaStream_t stream)
+        int lookupTyped(LookupParams const& p, uint32_t dim, cudaStream_t stream)
         {
-            // pieces of eight values where every row of the table and of the output starts on a
-            // 16-byte boundary, single values elsewhere
-            const bool wide = dim % 8u == 0u && aligned(p.table, 16) && aligned(p.out, 16)
-                              && p.ldt * sizeof(T) % 16 == 0 && p.outOuter * sizeof(OutT) % 16 == 0
-                              && p.outInner * sizeof(OutT) % 16 == 0;
-            p.pieces    = wide ? dim / 8u : dim;
-            p.lanesLog2 = lanesFor(p.pieces);
-            return wide ? lookup<T, OutT, 8>(p, stream) : lookup<T, OutT, 1>(p, stream);
+            const uint32_t v = pieceSize(dim, p.out, sizeof(OutT), pieceSize(dim, p.table, sizeof(T), 8, p.ldt), p.outOuter,
+                                         p.outInner);
+            return v == 8u ? lookup<T, OutT, 8>(p, dim, stream)
+                           : v == 2u ? lookup<T, OutT, 2>(p, dim, stream) : lookup<T, OutT, 1>(p, dim, stream);
         }
 
         template <typename T>
@@ -542,13 +734,24 @@ namespace b200wmma
             return lookupTyped<T, float>(p, dim, stream);
         }
 
-        // The workspace of the gradient; offsets in bytes.
-        constexpr uint32_t MAX_LEVELS = 8;
+        // Threads side by side on a row of the sum, and threads of its blocks.
+        uint32_t sumLanesLog2(uint32_t pieces)
+        {
+            const uint32_t l = log2Up(pieces);
+            return l > 5u ? 5u : l;
+        }
+        uint32_t sumThreads(uint32_t lanesLog2)
+        {
+            return lanesLog2 >= 3u ? THREADS : 32u << lanesLog2;
+        }
+
+        // The workspace of the gradient; offsets in bytes.  The chunks go by the sizes alone.
+        constexpr uint32_t MAX_LEVELS = 16;
         struct Plan
         {
             uint64_t keys[2], tokens[2], counts, totals, touched, bytes;
-            uint64_t touchedBytes;
             uint32_t tiles, passes, levels;
+            bool     small;
             uint32_t n[MAX_LEVELS], chunk[MAX_LEVELS];
             uint64_t pieceKeys[MAX_LEVELS], pieceSums[MAX_LEVELS];
         };
@@ -562,48 +765,62 @@ namespace b200wmma
                 at += (bytes + 255u) / 256u * 256u;
                 return here;
             };
+            w.small  = count <= SMALL_TOKENS;
             w.tiles  = uint32_t((uint64_t(count) + SORT_TILE - 1) / SORT_TILE);
             w.passes = (log2Up(rows + 1u) + 7u) / 8u; // keys 0..rows
-            if(w.passes == 0)
-                w.passes = 1;
-            w.touchedBytes = (rows + 31u) / 32u * 4u;
-            w.touched      = take(w.touchedBytes);
-            w.totals       = take(RADIX * 4u);
-            w.counts       = take(uint64_t(w.tiles) * RADIX * 4u);
-            for(int i = 0; i < 2; ++i)
+            for(int i = 0; i < (w.small ? 1 : 2); ++i)
             {
                 w.keys[i]   = take(uint64_t(count) * 4u);
                 w.tokens[i] = take(uint64_t(count) * 4u);
             }
-            uint32_t n = count;
+            if(!w.small)
+            {
+                w.touched = take(rows);
+                w.totals  = take(RADIX * 4u);
+                w.counts  = take(uint64_t(w.tiles) * RADIX * 4u);
+            }
+            const uint32_t pieces = dim % 8u == 0u ? dim / 8u : dim % 2u == 0u ? dim / 2u : dim;
+            const uint32_t lanes  = sumLanesLog2(pieces);
+            const uint32_t most   = SUM_ITEMS / (sumThreads(lanes) >> lanes); // that fit a block
+            uint32_t       n      = count;
             while(true)
             {
+                // Long chunks leave fewer pieces of runs behind, short ones make more threads:
+                // enough to fill the device first.  Higher levels are small; 64 keeps them few.
+                uint32_t chunk = 64;
+                if(w.levels == 0u)
+                    for(chunk = 8; chunk < 128u && uint64_t(n) * pieces > uint64_t(chunk) * DEVICE_THREADS;)
+                        chunk *= 2u;
+                chunk                = chunk < most ? chunk : most;
                 const uint32_t level = w.levels++;
                 w.n[level]           = n;
-                w.chunk[level]       = level == 0 ? 32u : 128u;
-                const uint32_t chunks = (n + w.chunk[level] - 1u) / w.chunk[level];
+                w.chunk[level]       = chunk;
+                const uint32_t chunks = (n + chunk - 1u) / chunk;
                 if(chunks <= 1u)
                     break;
-                n                    = 2u * chunks;
-                w.pieceKeys[level]   = take(uint64_t(n) * 4u);
-                w.pieceSums[level]   = take(uint64_t(n) * dim * 4u);
+                n                  = 2u * chunks;
+                w.pieceKeys[level] = take(uint64_t(n) * 4u);
+                w.pieceSums[level] = take(uint64_t(n) * dim * 4u);
             }
             w.bytes = at;
             return w;
         }
 
         template <typename T, typename OutT, int V>
-        int sumLevel(SumParams p, uint32_t dim, cudaStream_t stream)
+        int sumLevelPieces(SumParams p, uint32_t dim, cudaStream_t stream)
         {
             p.pieces    = dim / V;
-            p.lanesLog2 = lanesFor(p.pieces);
-            if(p.lanesLog2 > 5u)
-                p.lanesLog2 = 5u; // one chunk to a warp at most
-            const uint32_t lanes  = 1u << p.lanesLog2;
-            const uint32_t chunks = uint32_t((uint64_t(p.n) + p.chunk - 1u) / p.chunk);
-            const uint32_t per    = THREADS >> p.lanesLog2;
-            const dim3     grid((chunks + per - 1u) / per, (p.pieces + lanes - 1u) / lanes);
-            return cudaToStatus(launchOverlapped(sumKernel<T, OutT, V>, grid, dim3(THREADS), 0, stream, p));
+            p.lanesLog2 = sumLanesLog2(p.pieces);
+            const uint32_t threads = sumThreads(p.lanesLog2), lanes = 1u << p.lanesLog2;
+            const uint64_t per = uint64_t(threads >> p.lanesLog2) * p.chunk;
+            const dim3     grid(uint32_t((p.n + per - 1u) / per), (p.pieces + lanes - 1u) / lanes);
+            return cudaToStatus(launchOverlapped(sumKernel<T, OutT, V>, grid, dim3(threads), 0, stream, p));
+        }
+        template <typename T, typename OutT>
+        int sumLevel(SumParams const& p, uint32_t dim, uint32_t v, cudaStream_t stream)
+        {
+            return v == 8u ? sumLevelPieces<T, OutT, 8>(p, dim, stream)
+                           : v == 2u ? sumLevelPieces<T, OutT, 2>(p, dim, stream) : sumLevelPieces<T, OutT, 1>(p, dim, stream);
         }
 
         struct GradientCall
@@ -619,84 +836,124 @@ namespace b200wmma
             uint8_t*    workspace;
         };
 
-        template <typename T, typename OutT>
-        int gradient(GradientCall const& g, cudaStream_t stream)
-        {
-            const Plan w     = planGradient(g.t.rows, g.dim, g.t.count);
-            auto       words = [&](uint64_t at) { return reinterpret_cast<uint32_t*>(g.workspace + at); };
-            uint32_t*  touched = g.accumulate ? nullptr : words(w.touched);
-            const bool wideTable = g.dim % 8u == 0u && aligned(g.table, 16) && g.ldt * sizeof(OutT) % 16 == 0;
-            const bool wide = wideTable && aligned(g.grad, 16) && g.gradOuter * sizeof(T) % 16 == 0
-                              && g.gradInner * sizeof(T) % 16 == 0;
-#define B200WMMA_TRY(expr)          \
-    do                              \
-    {                               \
-        const int rc__ = (expr);    \
-        if(rc__ != B200WMMA_OK)     \
-            return rc__;            \
+#define B200WMMA_TRY(expr)       \
+    do                           \
+    {                            \
+        const int rc__ = (expr); \
+        if(rc__ != B200WMMA_OK)  \
+            return rc__;         \
     } while(0)
+
+        // Sorted keys and tokens into the workspace; rows without a token cleared on the way.
+        template <typename OutT, int V>
+        int sortTokens(GradientCall const& g, Plan const& w, uint32_t** keys, uint32_t** tokens, cudaStream_t stream)
+        {
+            auto        words = [&](uint64_t at) { return reinterpret_cast<uint32_t*>(g.workspace + at); };
+            ClearParams c{g.table, g.ldt, g.dim / V, 0, 0};
+            c.lanesLog2           = log2Up(c.pieces) > 8u ? 8u : log2Up(c.pieces);
+            const uint64_t bytes  = uint64_t(g.t.rows) * g.dim * sizeof(OutT);
+            if(w.small)
+            {
+                *keys   = words(w.keys[0]);
+                *tokens = words(w.tokens[0]);
+                // a block to an SM, each with 16 KB of rows at least
+                const uint64_t want = (bytes + 16383u) / 16384u;
+                c.blocks            = g.accumulate ? 0u : uint32_t(want < 147u ? want : 147u);
+                static std::mutex mutex;
+                static bool       done[64] = {};
+                {
+                    std::lock_guard<std::mutex> lock(mutex);
+                    int                         dev = 0;
+                    B200WMMA_CUDA_TRY(cudaGetDevice(&dev));
+                    if(dev >= 64 || !done[dev])
+                    {
+                        B200WMMA_CUDA_TRY(cudaFuncSetAttribute(sortSmallKernel<OutT, V>,
+                                                               cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                               int(sizeof(SmallShared))));
+                        if(dev < 64)
+                            done[dev] = true;
+                    }
+                }
+                return cudaToStatus(launchOverlapped(sortSmallKernel<OutT, V>, dim3(1u + c.blocks), dim3(SMALL_THREADS),
+                                                     sizeof(SmallShared), stream, g.t, c, w.passes, *keys, *tokens));
+            }
+            uint8_t* touched = g.accumulate ? nullptr : g.workspace + w.touched;
             if(touched)
-                B200WMMA_CUDA_TRY(cudaMemsetAsync(touched, 0, w.touchedBytes, stream));
-            B200WMMA_TRY(cudaToStatus(launchOverlapped(keysKernel, dim3((g.t.count + THREADS - 1u) / THREADS),
-                                                       dim3(THREADS), 0, stream, g.t, words(w.keys[0]), touched)));
+                B200WMMA_CUDA_TRY(cudaMemsetAsync(touched, 0, g.t.rows, stream));
+            B200WMMA_TRY(cudaToStatus(launchOverlapped(keysKernel, dim3(w.tiles), dim3(THREADS), 0, stream, g.t,
+                                                       words(w.keys[0]), touched, w.tiles, words(w.counts))));
+            Share s{touched, g.t.rows, 0, 2u * w.passes - 1u};
+            const uint64_t want = (bytes / s.shares + 65535u) / 65536u;
+            c.blocks            = g.accumulate ? 0u : uint32_t(want < 592u ? want : 592u);
+            const dim3 grid(w.tiles + c.blocks);
             for(uint32_t pass = 0; pass < w.passes; ++pass)
             {
                 const uint32_t from = pass % 2u, to = 1u - from, shift = 8u * pass;
-                B200WMMA_TRY(cudaToStatus(launchOverlapped(countKernel, dim3(w.tiles), dim3(THREADS), 0, stream,
-                                                           words(w.keys[from]), g.t.count, shift, w.tiles, words(w.counts))));
+                if(pass > 0u)
+                {
+                    B200WMMA_TRY(cudaToStatus(launchOverlapped(countKernel<OutT, V>, grid, dim3(THREADS), 0, stream,
+                                                               words(w.keys[from]), g.t.count, shift, w.tiles,
+                                                               words(w.counts), c, s)));
+                    ++s.share;
+                }
                 B200WMMA_TRY(cudaToStatus(launchOverlapped(scanKernel, dim3(RADIX), dim3(THREADS), 0, stream,
                                                            words(w.counts), w.tiles, words(w.totals))));
-                B200WMMA_TRY(cudaToStatus(launchOverlapped(scatterKernel, dim3(w.tiles), dim3(THREADS), 0, stream,
+                B200WMMA_TRY(cudaToStatus(launchOverlapped(scatterKernel<OutT, V>, grid, dim3(THREADS), 0, stream,
                                                            words(w.keys[from]), pass ? words(w.tokens[from]) : nullptr,
                                                            g.t.count, shift, w.tiles, words(w.counts), words(w.totals),
-                                                           words(w.keys[to]), words(w.tokens[to]))));
+                                                           words(w.keys[to]), words(w.tokens[to]), c, s)));
+                ++s.share;
             }
-            if(touched)
-            {
-                const uint32_t pieces = wideTable ? g.dim / 8u : g.dim, lanes = lanesFor(pieces);
-                const uint32_t blocks = uint32_t((uint64_t(g.t.rows) + (THREADS >> lanes) - 1u) / (THREADS >> lanes));
-                B200WMMA_TRY(cudaToStatus(wideTable
-                    ? launchOverlapped(clearKernel<OutT, 8>, dim3(blocks), dim3(THREADS), 0, stream,
-                                       static_cast<OutT*>(g.table), g.ldt, g.t.rows, pieces, lanes, touched)
-                    : launchOverlapped(clearKernel<OutT, 1>, dim3(blocks), dim3(THREADS), 0, stream,
-                                       static_cast<OutT*>(g.table), g.ldt, g.t.rows, pieces, lanes, touched)));
-            }
+            *keys   = words(w.keys[w.passes % 2u]);
+            *tokens = words(w.tokens[w.passes % 2u]);
+            return B200WMMA_OK;
+        }
+
+        template <typename T, typename OutT>
+        int gradient(GradientCall const& g, cudaStream_t stream)
+        {
+            const Plan     w  = planGradient(g.t.rows, g.dim, g.t.count);
+            const uint32_t vt = pieceSize(g.dim, g.table, sizeof(OutT), 8, g.ldt);
+            const uint32_t vg = pieceSize(g.dim, g.grad, sizeof(T), vt, g.gradOuter, g.gradInner);
+            uint32_t *     keys = nullptr, *tokens = nullptr;
+            B200WMMA_TRY(vt == 8u ? (sortTokens<OutT, 8>(g, w, &keys, &tokens, stream))
+                                  : vt == 2u ? (sortTokens<OutT, 2>(g, w, &keys, &tokens, stream))
+                                             : (sortTokens<OutT, 1>(g, w, &keys, &tokens, stream)));
             for(uint32_t level = 0; level < w.levels; ++level)
             {
                 const bool more = level + 1u < w.levels;
                 SumParams  p{};
-                p.n     = w.n[level];
-                p.chunk = w.chunk[level];
-                p.rows  = g.t.rows;
-                p.table = g.table;
-                p.ldt   = g.ldt;
-                p.scale = g.scale;
+                p.n          = w.n[level];
+                p.chunk      = w.chunk[level];
+                p.rows       = g.t.rows;
+                p.table      = g.table;
+                p.ldt        = g.ldt;
+                p.scale      = g.scale;
                 p.accumulate = g.accumulate ? 1u : 0u;
-                p.pieceKeys  = more ? words(w.pieceKeys[level]) : nullptr;
+                p.pieceKeys  = more ? reinterpret_cast<uint32_t*>(g.workspace + w.pieceKeys[level]) : nullptr;
                 p.pieceSums  = more ? reinterpret_cast<float*>(g.workspace + w.pieceSums[level]) : nullptr;
                 if(level == 0)
                 {
-                    p.keys      = words(w.keys[w.passes % 2u]);
-                    p.tokens    = words(w.tokens[w.passes % 2u]);
+                    p.keys      = keys;
+                    p.tokens    = tokens;
                     p.grad      = g.grad;
                     p.gradOuter = g.gradOuter;
                     p.gradInner = g.gradInner;
                     p.inner     = g.t.inner;
-                    B200WMMA_TRY(wide ? (sumLevel<T, OutT, 8>(p, g.dim, stream)) : (sumLevel<T, OutT, 1>(p, g.dim, stream)));
+                    B200WMMA_TRY((sumLevel<T, OutT>(p, g.dim, vg, stream)));
                 }
                 else
                 {
-                    p.keys      = words(w.pieceKeys[level - 1u]);
+                    p.keys      = reinterpret_cast<uint32_t*>(g.workspace + w.pieceKeys[level - 1u]);
                     p.grad      = g.workspace + w.pieceSums[level - 1u];
                     p.gradOuter = g.dim;
                     p.inner     = 1;
-                    B200WMMA_TRY(wideTable ? (sumLevel<float, OutT, 8>(p, g.dim, stream))
-                                           : (sumLevel<float, OutT, 1>(p, g.dim, stream)));
+                    B200WMMA_TRY((sumLevel<float, OutT>(p, g.dim, vt, stream)));
                 }
             }
-#undef B200WMMA_TRY
             return B200WMMA_OK;
         }
+#undef B200WMMA_TRY
 
         template <typename T>
         int gradientFrom(int out, GradientCall const& g, cudaStream_t stream)

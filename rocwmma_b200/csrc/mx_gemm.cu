@@ -26,6 +26,8 @@ namespace b200wmma
         constexpr uint32_t NUM_THREADS = 192;
         constexpr uint32_t EPI_THREADS = 128;
         constexpr uint32_t MAX_STAGES  = 8;
+        constexpr uint32_t PREFETCH_SLOTS = 16; // of a block's stretch, requested into L2 ahead
+        constexpr long long SETTLE_CYCLES = 2000000; // leaving early: copies in flight land
 
         struct Params
         {
@@ -33,15 +35,7 @@ namespace b200wmma
             void*       d;
             uint32_t    m, n, k, ldc, ldd;
             float       alpha, beta;
-            uint32_t    nq, stages, slotBytes, tilesQ, tmemCols;
             uint32_t*   status;
-        };
-
-        struct Control
-        {
-            uint64_t   full[MAX_STAGES], empty[MAX_STAGES], accFull;
-            AbortState abort;
-            uint32_t   tmemBase;
         };
 
         template <ScaleKind KIND>
@@ -60,23 +54,61 @@ namespace b200wmma
             return fromFloat<OutT>(r);
         }
 
-        // One block, one tile: 128 rows of B (the MMA's M) by nq rows of A (its N).
+        __device__ inline void settle()
+        {
+            const long long start = clock64();
+            while(clock64() - start < SETTLE_CYCLES)
+            {
+            }
+        }
+
+        // ---- thin products -----------------------------------------------------------------
+        // One of m and n is small (a decoding batch; one token): the other operand, whose rows
+        // are the MMA's M here, 128 to a block, streams from HBM once and bounds the call.  The
+        // thin operand is the MMA's N, padded to 16 rows.  A cluster of `parts` blocks shares a
+        // tile, each a stretch of K, so that the stream comes through all SMs; the partial sums
+        // meet in shared memory across the cluster (each block adds up its share of the thin
+        // rows, always in the order of the blocks) where the ring was.
+        struct ThinParams
+        {
+            void const* c;
+            void*       d;
+            uint32_t    rows, thin, k; // rows of the streamed and of the thin operand
+            uint64_t    cRow, cThin, dRow, dThin; // distance of neighbouring elements of C and D along each
+            float       alpha, beta;
+            uint32_t    nq, parts, stages, slotBytes, tmemCols;
+            uint32_t*   status;
+        };
+        struct ThinControl
+        {
+            uint64_t   full[MAX_STAGES], empty[MAX_STAGES], accFull;
+            AbortState abort;
+            uint32_t   tmemBase;
+        };
+
+        __device__ inline void storeCluster(uint32_t addr, uint32_t v)
+        {
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+        }
+
         template <ScaleKind KIND, typename OutT>
         __global__ void __launch_bounds__(NUM_THREADS)
-            mxGemmKernel(const __grid_constant__ CUtensorMap mapR,
-                         const __grid_constant__ CUtensorMap mapQ,
-                         const __grid_constant__ CUtensorMap mapScaleR,
-                         const __grid_constant__ CUtensorMap mapScaleQ, const Params p)
+            mxGemmThinKernel(const __grid_constant__ CUtensorMap mapR,
+                             const __grid_constant__ CUtensorMap mapQ,
+                             const __grid_constant__ CUtensorMap mapScaleR,
+                             const __grid_constant__ CUtensorMap mapScaleQ, const ThinParams p)
         {
             constexpr uint32_t GROUPS = slotGroups<KIND>();
             extern __shared__ uint8_t smemRaw[];
-            uint8_t* ring = smemRaw + ((1024u - (smem_addr(smemRaw) & 1023u)) & 1023u);
-            Control* ctl  = reinterpret_cast<Control*>(ring + p.stages * p.slotBytes);
+            uint8_t*     ring = smemRaw + ((1024u - (smem_addr(smemRaw) & 1023u)) & 1023u);
+            ThinControl* ctl  = reinterpret_cast<ThinControl*>(ring + p.stages * p.slotBytes);
 
             const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-            const uint32_t tileR = blockIdx.x / p.tilesQ, tileQ = blockIdx.x % p.tilesQ;
-            const uint32_t numSlots = (p.k + SLOT_K - 1) / SLOT_K;
-            const uint32_t tilesOfQ = (p.nq + 127u) / 128u; // scale row tiles of this block's A
+            const uint32_t tile = blockIdx.x / p.parts, part = blockIdx.x % p.parts; // part: rank in the cluster
+            const uint32_t allSlots = (p.k + SLOT_K - 1) / SLOT_K;
+            const uint32_t slot0 = uint32_t(uint64_t(part) * allSlots / p.parts);
+            const uint32_t numSlots = uint32_t(uint64_t(part + 1u) * allSlots / p.parts) - slot0;
+            const uint32_t tilesOfQ = (p.nq + 127u) / 128u; // scale row tiles of the thin operand
             const uint32_t qBytes   = p.nq * 128u;
 
             if(threadIdx.x == 0)
@@ -94,6 +126,14 @@ namespace b200wmma
                 tma_prefetch_descriptor(&mapQ);
                 tma_prefetch_descriptor(&mapScaleR);
                 tma_prefetch_descriptor(&mapScaleQ);
+            }
+            else if(threadIdx.x == 64u)
+            {
+                // The streamed operand's first slots are requested into L2 while the previous
+                // kernel of the stream (often the quantisation of the thin operand) still runs: a
+                // request reads nothing into the SM, and L2 is where a late write would land too.
+                for(uint32_t it = 0; it < numSlots && it < PREFETCH_SLOTS; ++it)
+                    tma_prefetch_l2_2d(&mapR, int32_t((slot0 + it) * 128u), int32_t(tile * ROW_TILE));
             }
             __syncwarp();
             if(warp == 1)
@@ -116,16 +156,19 @@ namespace b200wmma
                     {
                         const uint32_t s = it % p.stages, ph = (it / p.stages) & 1u;
                         if(!mbar_wait(&ctl->empty[s], ph ^ 1u, &ctl->abort, WAIT_STAGE_EMPTY))
+                        {
+                            settle();
                             break;
-                        uint8_t* slot   = ring + s * p.slotBytes;
-                        uint8_t* scales = slot + CODE_BYTES + qBytes;
+                        }
+                        uint8_t*       slot   = ring + s * p.slotBytes;
+                        uint8_t*       scales = slot + CODE_BYTES + qBytes;
+                        const uint32_t at     = slot0 + it;
                         mbar_expect_tx(&ctl->full[s], p.slotBytes);
-                        tma_load_2d(slot, &mapR, &ctl->full[s], int32_t(it * 128u), int32_t(tileR * ROW_TILE));
-                        tma_load_2d(slot + CODE_BYTES, &mapQ, &ctl->full[s], int32_t(it * 128u),
-                                    int32_t(tileQ * p.nq));
-                        tma_load_3d(scales, &mapScaleR, &ctl->full[s], 0, int32_t(it * GROUPS), int32_t(tileR));
+                        tma_load_2d(slot, &mapR, &ctl->full[s], int32_t(at * 128u), int32_t(tile * ROW_TILE));
+                        tma_load_2d(slot + CODE_BYTES, &mapQ, &ctl->full[s], int32_t(at * 128u), 0);
+                        tma_load_3d(scales, &mapScaleR, &ctl->full[s], 0, int32_t(at * GROUPS), int32_t(tile));
                         tma_load_3d(scales + GROUPS * MX_TILE_BYTES, &mapScaleQ, &ctl->full[s], 0,
-                                    int32_t(it * GROUPS), int32_t(tileQ * p.nq / 128u));
+                                    int32_t(at * GROUPS), 0);
                     }
                 }
             }
@@ -150,7 +193,7 @@ namespace b200wmma
                         const uint32_t qAddr = rAddr + CODE_BYTES, sAddr = qAddr + qBytes;
                         const uint32_t scaleR = scale0 + (it & 1u) * scaleCols;
                         const uint32_t scaleQ = scaleR + 4u * GROUPS;
-                        const uint32_t left   = p.k - it * SLOT_K;
+                        const uint32_t left   = p.k - (slot0 + it) * SLOT_K;
                         const uint32_t steps  = left >= SLOT_K ? SLOT_K / MMA_K : (left + MMA_K - 1) / MMA_K;
                         for(uint32_t g = 0; g < GROUPS; ++g)
                         {
@@ -176,33 +219,73 @@ namespace b200wmma
                         mma_commit(&ctl->accFull);
                 }
             }
-            else
+
+            // lanes hold rows of the streamed operand, registers rows of the thin one
+            const bool     drains = warp >= 2u;
+            const uint32_t inTile = warp % 4u * 32u + lane;
+            const uint64_t row    = uint64_t(tile) * ROW_TILE + inTile;
+            const uint32_t taddr  = tmem + ((warp % 4u * 32u) << 16);
+            const uint32_t share  = p.nq / p.parts; // thin rows that this block finishes
+            auto           put    = [&](uint32_t q, float acc) {
+                if(row < p.rows && q < p.thin)
+                {
+                    OutT const* c = p.c ? static_cast<OutT const*>(p.c) + row * p.cRow + q * p.cThin : nullptr;
+                    static_cast<OutT*>(p.d)[row * p.dRow + q * p.dThin] = finish<OutT>(acc, p.alpha, p.beta, c);
+                }
+            };
+            bool ready = false;
+            if(drains)
+                ready = mbar_wait(&ctl->accFull, 0, &ctl->abort, WAIT_ACC_FULL);
+            __syncwarp();
+            if(p.parts == 1u)
             {
-                // lanes hold rows of B (columns of D), registers rows of A (rows of D)
-                const uint32_t quad = warp % 4;
-                const uint32_t col  = tileR * ROW_TILE + quad * 32u + lane;
-                const bool     ready = mbar_wait(&ctl->accFull, 0, &ctl->abort, WAIT_ACC_FULL);
-                if(named_barrier_all(1, EPI_THREADS, ready))
+                if(drains && ready)
                 {
                     tc_fence_after_sync();
-                    for(uint32_t j0 = 0; j0 < p.nq; j0 += 16u)
+                    for(uint32_t q0 = 0; q0 < p.nq; q0 += 16u)
                     {
                         uint32_t raw[16];
-                        tmem_load_32x32b_x16(tmem + ((quad * 32u) << 16) + j0, raw);
+                        tmem_load_32x32b_x16(taddr + q0, raw);
+                        tmem_load_wait();
+#pragma unroll
+                        for(uint32_t j = 0; j < 16u; ++j)
+                            put(q0 + j, __uint_as_float(raw[j]));
+                    }
+                }
+            }
+            else
+            {
+                // every block's MMAs have read their last slot: the rings take the partial sums,
+                // [part][thin row of the share][row of the tile]
+                cluster_sync();
+                if(drains && ready)
+                {
+                    tc_fence_after_sync();
+                    const uint32_t mine = smem_addr(ring) + (part * share * ROW_TILE + inTile) * 4u;
+                    for(uint32_t q0 = 0; q0 < p.nq; q0 += 16u)
+                    {
+                        uint32_t raw[16];
+                        tmem_load_32x32b_x16(taddr + q0, raw);
                         tmem_load_wait();
 #pragma unroll
                         for(uint32_t j = 0; j < 16u; ++j)
                         {
-                            const uint64_t row = uint64_t(tileQ) * p.nq + j0 + j;
-                            if(row < p.m && col < p.n)
-                            {
-                                OutT const* c = p.c ? static_cast<OutT const*>(p.c) + row * p.ldc + col : nullptr;
-                                static_cast<OutT*>(p.d)[row * p.ldd + col]
-                                    = finish<OutT>(__uint_as_float(raw[j]), p.alpha, p.beta, c);
-                            }
+                            const uint32_t to = (q0 + j) / share;
+                            storeCluster(map_to_cta(mine + (q0 + j - to * share) * (ROW_TILE * 4u), to), raw[j]);
                         }
                     }
-                    tc_fence_before_sync();
+                }
+                cluster_sync();
+                if(drains)
+                {
+                    float const* sums = reinterpret_cast<float const*>(ring) + inTile;
+                    for(uint32_t j = 0; j < share; ++j)
+                    {
+                        float acc = sums[j * ROW_TILE];
+                        for(uint32_t o = 1; o < p.parts; ++o)
+                            acc += sums[(o * share + j) * ROW_TILE];
+                        put(part * share + j, acc);
+                    }
                 }
             }
             tc_fence_before_sync();
@@ -234,7 +317,6 @@ namespace b200wmma
         constexpr uint32_t P_STAGES    = 5;
         constexpr uint32_t BOX_BYTES   = 128 * 64; // 128 rows x 64 bytes of D (or C)
         constexpr uint32_t BOXES       = 4;
-        constexpr long long SETTLE_CYCLES = 2000000; // leaving early: copies in flight land
 
         struct PairParams
         {
@@ -260,14 +342,6 @@ namespace b200wmma
         constexpr uint32_t pairSmemBytes()
         {
             return 1024u + P_STAGES * pairSlotBytes<KIND>() + BOXES * BOX_BYTES + uint32_t(sizeof(PairControl));
-        }
-
-        __device__ inline void settle()
-        {
-            const long long start = clock64();
-            while(clock64() - start < SETTLE_CYCLES)
-            {
-            }
         }
 
         // Drains one tile's accumulator.  A box of D is 128 rows x 64 bytes: TMEM -> registers
@@ -681,45 +755,86 @@ namespace b200wmma
         }
 
         template <ScaleKind KIND, typename OutT>
-        int launch(Operands const& o, Params p, cudaStream_t stream)
+        int launchThin(Operands const& o, Params const& q, int sms, cudaStream_t stream)
+        {
+            constexpr uint32_t GROUPS = slotGroups<KIND>();
+            const uint32_t     groups = mxGroups(KIND == ScaleKind::E4M3_16, q.k);
+            const bool         thinA  = q.m <= q.n; // the thin operand is A
+            ThinParams         p{};
+            p.c      = q.c;
+            p.d      = q.d;
+            p.rows   = thinA ? q.n : q.m;
+            p.thin   = thinA ? q.m : q.n;
+            p.k      = q.k;
+            p.cRow   = thinA ? 1u : q.ldc;
+            p.cThin  = thinA ? q.ldc : 1u;
+            p.dRow   = thinA ? 1u : q.ldd;
+            p.dThin  = thinA ? q.ldd : 1u;
+            p.alpha  = q.alpha;
+            p.beta   = q.beta;
+            p.status = q.status;
+            p.nq     = (p.thin + 15u) / 16u * 16u;
+            const uint32_t tilesOfQ = (p.nq + 127u) / 128u;
+            const uint32_t slots    = (q.k + SLOT_K - 1u) / SLOT_K;
+            const uint32_t tiles    = mxRowTiles(p.rows);
+            // two blocks to an SM where their tensor memory and shared memory allow it
+            const uint32_t resident = p.nq <= 128u ? 2u : 1u;
+            p.parts                 = 8;
+            while(p.parts > 1u && (uint64_t(tiles) * p.parts > resident * uint32_t(sms) || slots < 2u * p.parts))
+                p.parts /= 2u;
+            p.slotBytes = CODE_BYTES + p.nq * 128u + GROUPS * MX_TILE_BYTES * (1u + tilesOfQ);
+            const uint32_t room  = (resident == 2u ? 112u : 224u) * 1024u - 1024u - uint32_t(sizeof(ThinControl));
+            const uint32_t mine  = (slots + p.parts - 1u) / p.parts;
+            p.stages             = room / p.slotBytes;
+            p.stages             = p.stages > MAX_STAGES ? MAX_STAGES : p.stages;
+            p.stages             = p.stages > mine ? mine : p.stages;
+            // the partial sums take the ring's place
+            while(p.parts > 1u && p.stages * p.slotBytes < p.nq * ROW_TILE * 4u)
+                ++p.stages;
+            const uint32_t cols = (p.nq + 31u) / 32u * 32u + 2u * 4u * GROUPS * (1u + tilesOfQ);
+            p.tmemCols          = 32;
+            while(p.tmemCols < cols)
+                p.tmemCols *= 2;
+            CUtensorMap mapR, mapQ, mapScaleR, mapScaleQ;
+            int         rc = codeMap(&mapR, thinA ? o.b : o.a, p.rows, p.k, thinA ? o.ldb : o.lda, ROW_TILE);
+            if(rc == B200WMMA_OK)
+                rc = codeMap(&mapQ, thinA ? o.a : o.b, p.thin, p.k, thinA ? o.lda : o.ldb, p.nq);
+            if(rc == B200WMMA_OK)
+                rc = scaleMap(&mapScaleR, thinA ? o.bScales : o.aScales, p.rows, groups, GROUPS, 1);
+            if(rc == B200WMMA_OK)
+                rc = scaleMap(&mapScaleQ, thinA ? o.aScales : o.bScales, p.thin, groups, GROUPS, tilesOfQ);
+            if(rc != B200WMMA_OK)
+                return rc;
+            const uint32_t  smem = 1024u + p.stages * p.slotBytes + uint32_t(sizeof(ThinControl));
+            static uint32_t done[64] = {};
+            rc = optInSharedMemory(mxGemmThinKernel<KIND, OutT>, smem, done);
+            if(rc != B200WMMA_OK)
+                return rc;
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim            = dim3(tiles * p.parts);
+            cfg.blockDim           = dim3(NUM_THREADS);
+            cfg.dynamicSmemBytes   = smem;
+            cfg.stream             = stream;
+            cudaLaunchAttribute attr[2];
+            attr[0].id               = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = p.parts;
+            attr[0].val.clusterDim.y = 1;
+            attr[0].val.clusterDim.z = 1;
+            attr[1].id               = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr[1].val.programmaticStreamSerializationAllowed = 1;
+            cfg.attrs    = attr;
+            cfg.numAttrs = launchOverlapEnabled() ? 2 : 1;
+            return cudaToStatus(cudaLaunchKernelEx(&cfg, mxGemmThinKernel<KIND, OutT>, mapR, mapQ, mapScaleR, mapScaleQ, p));
+        }
+
+        template <ScaleKind KIND, typename OutT>
+        int launch(Operands const& o, Params const& p, cudaStream_t stream)
         {
             const int sms = smCount();
             if(sms < 2)
                 return B200WMMA_ERR_CUDA;
-            if(p.m > 128u)
-                return launchPairs<KIND, OutT>(o, p, sms, stream);
-            constexpr uint32_t GROUPS = slotGroups<KIND>();
-            const uint32_t     groups = mxGroups(KIND == ScaleKind::E4M3_16, p.k);
-            p.nq                      = p.m > 128u ? 256u : p.m > 64u ? 128u : (p.m + 15u) / 16u * 16u;
-            const uint32_t tilesOfQ   = (p.nq + 127u) / 128u;
-            p.slotBytes               = CODE_BYTES + p.nq * 128u + GROUPS * MX_TILE_BYTES * (1u + tilesOfQ);
-            p.stages                  = 4;
-            p.tilesQ                  = uint32_t((uint64_t(p.m) + p.nq - 1) / p.nq);
-            const uint32_t cols       = (p.nq + 31u) / 32u * 32u + 2u * 4u * GROUPS * (1u + tilesOfQ);
-            p.tmemCols                = 32;
-            while(p.tmemCols < cols)
-                p.tmemCols *= 2;
-            const uint64_t blocks = uint64_t(mxRowTiles(p.n)) * p.tilesQ;
-            if(blocks > 0x7fffffffull)
-                return B200WMMA_ERR_TOO_LARGE;
-            CUtensorMap mapR, mapQ, mapScaleR, mapScaleQ;
-            int         rc = codeMap(&mapR, o.b, p.n, p.k, o.ldb, ROW_TILE);
-            if(rc == B200WMMA_OK)
-                rc = codeMap(&mapQ, o.a, p.m, p.k, o.lda, p.nq);
-            if(rc == B200WMMA_OK)
-                rc = scaleMap(&mapScaleR, o.bScales, p.n, groups, GROUPS, 1);
-            if(rc == B200WMMA_OK)
-                rc = scaleMap(&mapScaleQ, o.aScales, p.m, groups, GROUPS, tilesOfQ);
-            if(rc != B200WMMA_OK)
-                return rc;
-            const uint32_t  smem = 1024u + p.stages * p.slotBytes + uint32_t(sizeof(Control));
-            static uint32_t done[64] = {};
-            rc = optInSharedMemory(mxGemmKernel<KIND, OutT>, smem, done);
-            if(rc != B200WMMA_OK)
-                return rc;
-            return cudaToStatus(launchOverlapped(mxGemmKernel<KIND, OutT>, dim3(uint32_t(blocks)),
-                                                 dim3(NUM_THREADS), smem, stream, mapR, mapQ, mapScaleR,
-                                                 mapScaleQ, p));
+            const uint32_t thin = p.m < p.n ? p.m : p.n;
+            return thin <= 128u ? launchThin<KIND, OutT>(o, p, sms, stream) : launchPairs<KIND, OutT>(o, p, sms, stream);
         }
 
         template <typename OutT>
@@ -757,7 +872,7 @@ extern "C" int b200wmma_mx_gemm(int fmt, int out_dtype, uint32_t m, uint32_t n, 
     if(!status)
         return B200WMMA_ERR_CUDA;
     const Operands     o{a, a_scales, b, b_scales, lda, ldb};
-    const Params       p{beta != 0.0 ? c : nullptr, d, m, n, k, ldc, ldd, float(alpha), float(beta), 0, 0, 0, 0, 0, status};
+    const Params       p{beta != 0.0 ? c : nullptr, d, m, n, k, ldc, ldd, float(alpha), float(beta), status};
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch(out_dtype)
     {
