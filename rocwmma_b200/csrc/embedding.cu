@@ -9,11 +9,11 @@
 // gradient.
 //
 // Both are bound by HBM.  The gradient is made without atomics on its values, so that a call's
-// result depends on its arguments alone: tokens are sorted by row (a stable radix sort), then
-// every run of equal rows is summed in token order, in fp32, by cutting the sorted tokens into
-// chunks; a run inside one chunk is written at once, the pieces of a run that crosses chunks go
-// to the workspace, which the next, much smaller level treats as its tokens.  Rows without a
-// token are cleared by blocks of their own next to those that sort, which leave HBM idle.
+// result depends on its arguments alone: tokens are sorted by row (a stable radix sort), the
+// sorted tokens are cut into chunks, and every run of equal rows in a chunk is summed in token
+// order, in fp32.  A run inside one chunk is written at once; a run that crosses chunks leaves a
+// piece for each in the workspace, and a last kernel joins those.  Rows without a token are
+// cleared by blocks of their own beside the others.
 #include "common.cuh"
 #include "mx_format.cuh"
 #include "rocwmma/rocwmma_block.hpp"
@@ -29,7 +29,7 @@ namespace b200wmma
         constexpr uint32_t THREADS = 256;
         constexpr uint32_t DEVICE_THREADS = 148u * 2048u; // resident at once
         constexpr uint32_t NO_ROW  = 0x7fffffffu; // no token, or no row of the table
-        constexpr uint32_t EMPTY   = 0x80000000u; // part of a run, but adds nothing to it
+        constexpr uint32_t PASSES  = 0x80000000u; // with a row: a run that fills a chunk and goes on
 
         // The tokens of a call.
         struct Tokens
@@ -65,12 +65,40 @@ namespace b200wmma
             return row >= 0 && row < end ? uint32_t(row) : NO_ROW;
         }
 
-        // V neighbouring values of a row, loaded and stored as one where their alignment allows it.
+        // V neighbouring values of a row, at most 32 bytes, moved as one.
         template <typename T, int V>
-        struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Piece
+        struct alignas(sizeof(T) * V) Piece
         {
             T v[V];
         };
+        template <typename T, int V>
+        __device__ inline Piece<T, V> loadPiece(T const* at)
+        {
+            Piece<T, V> p;
+            if constexpr(sizeof(p) == 32)
+            {
+                uint32_t* w = reinterpret_cast<uint32_t*>(&p);
+                asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                             : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                             : "l"(at));
+            }
+            else
+                p = *reinterpret_cast<Piece<T, V> const*>(at);
+            return p;
+        }
+        template <typename T, int V>
+        __device__ inline void storePiece(T* at, Piece<T, V> const& p)
+        {
+            if constexpr(sizeof(p) == 32)
+            {
+                uint32_t const* w = reinterpret_cast<uint32_t const*>(&p);
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(w[0]), "r"(w[1]),
+                             "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                             : "memory");
+            }
+            else
+                *reinterpret_cast<Piece<T, V>*>(at) = p;
+        }
 
         // ---- lookup ----------------------------------------------------------------------
         struct LookupParams
@@ -117,8 +145,7 @@ namespace b200wmma
                         const uint32_t t = t0 + u * step;
                         row[u]           = t < here ? rows[t] : NO_ROW;
                         if(row[u] != NO_ROW)
-                            v[u] = *reinterpret_cast<Piece<T, V> const*>(static_cast<T const*>(p.table)
-                                                                         + uint64_t(row[u]) * p.ldt + at);
+                            v[u] = loadPiece<T, V>(static_cast<T const*>(p.table) + uint64_t(row[u]) * p.ldt + at);
                     }
 #pragma unroll
                     for(uint32_t u = 0; u < U; ++u)
@@ -130,7 +157,7 @@ namespace b200wmma
 #pragma unroll
                             for(int i = 0; i < V; ++i)
                                 o.v[i] = fromFloat<OutT>(row[u] != NO_ROW ? toFloat(v[u].v[i]) * p.scale : 0.0f);
-                            *reinterpret_cast<Piece<OutT, V>*>(static_cast<OutT*>(p.out) + outs[t] + at) = o;
+                            storePiece<OutT, V>(static_cast<OutT*>(p.out) + outs[t] + at, o);
                         }
                     }
                 }
@@ -143,7 +170,8 @@ namespace b200wmma
             void*    table;
             uint64_t ldt;
             uint32_t pieces, lanesLog2; // of a row
-            uint32_t blocks; // that clear, behind those that sort; 0: nothing to clear
+            uint32_t blocks; // that clear, behind the others; 0: nothing to clear
+            uint32_t rows, rowsPerBlock;
         };
 
         // The rows of [begin, end) that keep(row) does not name, by the calling block.
@@ -158,8 +186,7 @@ namespace b200wmma
             for(uint64_t row = begin + (threadIdx.x >> c.lanesLog2); row < end; row += blockDim.x >> c.lanesLog2)
                 if(!keep(row))
                     for(uint32_t piece = threadIdx.x & (lanes - 1u); piece < c.pieces; piece += lanes)
-                        *reinterpret_cast<Piece<OutT, V>*>(static_cast<OutT*>(c.table) + row * c.ldt + uint64_t(piece) * V)
-                            = zero;
+                        storePiece<OutT, V>(static_cast<OutT*>(c.table) + row * c.ldt + uint64_t(piece) * V, zero);
         }
 
         // ---- sorting few tokens: one block --------------------------------------------------
@@ -182,7 +209,7 @@ namespace b200wmma
         // which they look through the tokens themselves.
         template <typename OutT, int V>
         __global__ void __launch_bounds__(SMALL_THREADS)
-            sortSmallKernel(const Tokens t, const ClearParams c, const uint32_t passes, uint32_t* keysOut, uint32_t* tokensOut)
+            sortSmallKernel(const Tokens t, const ClearParams c, const uint32_t passes, uint2* sorted)
         {
             extern __shared__ uint8_t smem[];
             SmallShared*   sh   = reinterpret_cast<SmallShared*>(smem);
@@ -290,10 +317,7 @@ namespace b200wmma
                     {
                         const uint32_t to = sh->bins[warp][(key[i] >> shift) % RADIX] + rank[i];
                         if(last)
-                        {
-                            keysOut[to]   = key[i];
-                            tokensOut[to] = token[i];
-                        }
+                            sorted[to] = make_uint2(key[i], token[i]);
                         else
                         {
                             sh->keys[to]   = key[i];
@@ -318,22 +342,7 @@ namespace b200wmma
         constexpr uint32_t SORT_TILE  = THREADS * SORT_ITEMS;
         constexpr uint32_t SORT_WARPS = THREADS / 32;
 
-        // What a block of a sorting kernel does that is not one of its `tiles` first: it clears its
-        // part of share `share` of `shares` of the rows.
-        struct Share
-        {
-            uint8_t const* touched;
-            uint32_t       rows, share, shares;
-        };
-        template <typename OutT, int V>
-        __device__ inline void clearShare(ClearParams const& c, Share const& s, uint32_t block)
-        {
-            const uint64_t begin = uint64_t(s.rows) * s.share / s.shares, count = uint64_t(s.rows) * (s.share + 1u) / s.shares - begin;
-            clearRows<OutT, V>(c, begin + count * block / c.blocks, begin + count * (block + 1u) / c.blocks,
-                               [&](uint64_t row) { return s.touched[row] != 0; });
-        }
-
-        // counts[digit][tile] += keys of the tile
+        // bins[digit] = keys of the tile
         __device__ inline void countDigits(uint32_t* bins, uint32_t const (&key)[SORT_ITEMS], uint32_t first, uint32_t n,
                                            uint32_t shift)
         {
@@ -352,9 +361,9 @@ namespace b200wmma
             __syncthreads();
         }
 
-        // Row of every token, a flag for every row that has one, and the first digit's counts.
+        // Row of every token, and the first digit's counts[digit][tile].
         __global__ void __launch_bounds__(THREADS)
-            keysKernel(const Tokens t, uint32_t* keys, uint8_t* touched, uint32_t tiles, uint32_t* counts)
+            keysKernel(const Tokens t, uint32_t* keys, uint32_t tiles, uint32_t* counts)
         {
             __shared__ uint32_t bins[RADIX];
             grid_dependency_wait();
@@ -372,36 +381,24 @@ namespace b200wmma
                     const uint32_t row = rowOf(t, token, outer, inner);
                     if(row != NO_ROW)
                         key[i] = row;
+                    keys[token] = key[i];
                 }
             }
-#pragma unroll
-            for(uint32_t i = 0; i < SORT_ITEMS; ++i)
-                if(first + i * THREADS < t.count)
-                {
-                    keys[first + i * THREADS] = key[i];
-                    // (read first: stores to a hot row's flag would queue up)
-                    if(touched && key[i] < t.rows && touched[key[i]] == 0)
-                        touched[key[i]] = 1;
-                }
             countDigits(bins, key, first, t.count, 0);
             counts[threadIdx.x * tiles + blockIdx.x] = bins[threadIdx.x];
         }
 
-        template <typename OutT, int V>
         __global__ void __launch_bounds__(THREADS)
-            countKernel(uint32_t const* keys, uint32_t n, uint32_t shift, uint32_t tiles, uint32_t* counts,
-                        const ClearParams c, const Share s)
+            countKernel(uint2 const* pairs, uint32_t n, uint32_t shift, uint32_t tiles, uint32_t* counts)
         {
             __shared__ uint32_t bins[RADIX];
             grid_dependency_wait();
             grid_launch_dependents();
-            if(blockIdx.x >= tiles)
-                return clearShare<OutT, V>(c, s, blockIdx.x - tiles);
             const uint32_t first = blockIdx.x * SORT_TILE + threadIdx.x;
             uint32_t       key[SORT_ITEMS];
 #pragma unroll
             for(uint32_t i = 0; i < SORT_ITEMS; ++i)
-                key[i] = first + i * THREADS < n ? keys[first + i * THREADS] : 0u;
+                key[i] = first + i * THREADS < n ? pairs[first + i * THREADS].x : 0u;
             countDigits(bins, key, first, n, shift);
             counts[threadIdx.x * tiles + blockIdx.x] = bins[threadIdx.x];
         }
@@ -457,37 +454,46 @@ namespace b200wmma
 
         // Moves every key of a tile, with its token, to its place among the keys of this digit:
         // those of smaller digits, of earlier tiles, of earlier warps, of earlier rows of 32 and
-        // of smaller lanes come first.  tokensIn == nullptr: key i belongs to token i.
-        template <typename OutT, int V>
+        // of smaller lanes come first.  The tile is put in order in shared memory first, so that
+        // neighbouring threads write neighbouring places.  pairs == nullptr: the first pass, key i
+        // of `keys` belongs to token i.
         __global__ void __launch_bounds__(THREADS)
-            scatterKernel(uint32_t const* keysIn, uint32_t const* tokensIn, uint32_t n, uint32_t shift,
-                          uint32_t tiles, uint32_t const* counts, uint32_t const* totals,
-                          uint32_t* keysOut, uint32_t* tokensOut, const ClearParams c, const Share s)
+            scatterKernel(uint32_t const* keys, uint2 const* pairs, uint32_t n, uint32_t shift, uint32_t tiles,
+                          uint32_t const* counts, uint32_t const* totals, uint2* out)
         {
             __shared__ uint32_t bins[SORT_WARPS][RADIX];
             __shared__ uint32_t warps[SORT_WARPS];
+            __shared__ uint32_t shifts[RADIX]; // place of a digit's keys minus their place in the tile
+            __shared__ uint2    tile[SORT_TILE];
             const uint32_t      warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
             grid_dependency_wait();
             grid_launch_dependents();
-            if(blockIdx.x >= tiles)
-                return clearShare<OutT, V>(c, s, blockIdx.x - tiles);
 #pragma unroll
             for(uint32_t w = 0; w < SORT_WARPS; ++w)
                 bins[w][threadIdx.x] = 0;
             __syncthreads();
-            const uint64_t first = uint64_t(blockIdx.x) * SORT_TILE + warp * (32u * SORT_ITEMS) + lane;
-            uint32_t       key[SORT_ITEMS], rank[SORT_ITEMS];
+            const uint32_t tile0 = blockIdx.x * SORT_TILE, here = min(SORT_TILE, n - tile0);
+            const uint32_t first = warp * (32u * SORT_ITEMS) + lane;
+            uint2          pair[SORT_ITEMS];
+            uint32_t       rank[SORT_ITEMS];
 #pragma unroll
             for(uint32_t i = 0; i < SORT_ITEMS; ++i)
             {
-                const uint64_t at = first + i * 32u;
-                key[i]            = at < n ? keysIn[at] : 0xffffffffu;
+                const uint32_t at = first + i * 32u;
+                pair[i]           = make_uint2(0u, tile0 + at);
+                if(at < here)
+                {
+                    if(pairs)
+                        pair[i] = pairs[tile0 + at];
+                    else
+                        pair[i].x = keys[tile0 + at];
+                }
             }
 #pragma unroll
             for(uint32_t i = 0; i < SORT_ITEMS; ++i)
             {
-                const bool     in    = first + i * 32u < n;
-                const uint32_t digit = (key[i] >> shift) % RADIX;
+                const bool     in    = first + i * 32u < here;
+                const uint32_t digit = (pair[i].x >> shift) % RADIX;
                 const uint32_t peers = __match_any_sync(0xffffffffu, in ? digit : RADIX);
                 rank[i]              = (in ? bins[warp][digit] : 0u) + __popc(peers & ((1u << lane) - 1u));
                 __syncwarp();
@@ -496,12 +502,9 @@ namespace b200wmma
                 __syncwarp();
             }
             __syncthreads();
-            // thread = digit: where the keys of each warp go
+            // thread = digit: where the keys of each warp go in the tile, and the tile's in the whole
             {
-                uint32_t       total;
-                const uint32_t base = blockScan(totals[threadIdx.x], warps, total)
-                                      + counts[threadIdx.x * tiles + blockIdx.x];
-                uint32_t sum = base;
+                uint32_t sum = 0, total;
 #pragma unroll
                 for(uint32_t w = 0; w < SORT_WARPS; ++w)
                 {
@@ -509,18 +512,23 @@ namespace b200wmma
                     bins[w][threadIdx.x] = sum;
                     sum += count;
                 }
+                const uint32_t local = blockScan(sum, warps, total);
+#pragma unroll
+                for(uint32_t w = 0; w < SORT_WARPS; ++w)
+                    bins[w][threadIdx.x] += local;
+                shifts[threadIdx.x] = blockScan(totals[threadIdx.x], warps, total)
+                                      + counts[threadIdx.x * tiles + blockIdx.x] - local;
             }
             __syncthreads();
 #pragma unroll
             for(uint32_t i = 0; i < SORT_ITEMS; ++i)
+                if(first + i * 32u < here)
+                    tile[bins[warp][(pair[i].x >> shift) % RADIX] + rank[i]] = pair[i];
+            __syncthreads();
+            for(uint32_t i = threadIdx.x; i < here; i += THREADS)
             {
-                const uint64_t at = first + i * 32u;
-                if(at < n)
-                {
-                    const uint32_t to = bins[warp][(key[i] >> shift) % RADIX] + rank[i];
-                    keysOut[to]       = key[i];
-                    tokensOut[to]     = tokensIn ? tokensIn[at] : uint32_t(at);
-                }
+                const uint2 p = tile[i];
+                out[shifts[(p.x >> shift) % RADIX] + i] = p;
             }
         }
 
@@ -528,62 +536,112 @@ namespace b200wmma
         constexpr uint32_t SUM_ITEMS = 2048; // of a block
         struct SumParams
         {
-            uint32_t const* keys; // of the items, equal rows next to each other
-            uint32_t const* tokens; // nullptr: item i is row i of `grad`
-            void const*     grad;
-            uint64_t        gradOuter, gradInner;
-            uint32_t        inner;
-            uint32_t        n, chunk, rows;
-            uint32_t        pieces, lanesLog2;
-            void*           table;
-            uint64_t        ldt;
-            float           scale;
-            uint32_t        accumulate;
-            uint32_t*       pieceKeys; // two of each chunk: run from the left, run to the right
-            float*          pieceSums; // rows of `pieces * V`
+            uint2 const* sorted; // (row, token), equal rows next to each other
+            void const*  grad;
+            uint64_t     gradOuter, gradInner;
+            uint32_t     inner;
+            uint32_t     n, chunk, chunks, rows;
+            uint32_t     pieces, lanesLog2, slices; // pieces of a row; threads side by side on it; blocks
+            uint32_t     blocks; // that sum; those behind them clear
+            void*        table;
+            uint64_t     ldt;
+            float        scale;
+            uint32_t     accumulate;
+            uint32_t*    pieceKeys; // two of each chunk: run from the left, run to the right; nullptr: one chunk
+            float*       pieceSums; // rows of `pieces * V`
         };
+
+        // A finished row's piece.
+        template <typename OutT, int V>
+        __device__ inline void finishRow(SumParams const& p, uint32_t row, uint32_t piece, float const (&sum)[V])
+        {
+            OutT*          at = static_cast<OutT*>(p.table) + uint64_t(row) * p.ldt + uint64_t(piece) * V;
+            Piece<OutT, V> o;
+            if(p.accumulate)
+            {
+                o = loadPiece<OutT, V>(at);
+#pragma unroll
+                for(int i = 0; i < V; ++i)
+                    o.v[i] = fromFloat<OutT>(fmaf(sum[i], p.scale, toFloat(o.v[i])));
+            }
+            else
+            {
+#pragma unroll
+                for(int i = 0; i < V; ++i)
+                    o.v[i] = fromFloat<OutT>(sum[i] * p.scale);
+            }
+            storePiece<OutT, V>(at, o);
+        }
+
+        // First of the sorted items [low, high) whose row is not below `row`.
+        __device__ inline uint32_t lowerBound(uint2 const* sorted, uint32_t low, uint32_t high, uint64_t row)
+        {
+            while(low < high)
+            {
+                const uint32_t mid = low + (high - low) / 2u;
+                if(sorted[mid].x < row)
+                    low = mid + 1u;
+                else
+                    high = mid;
+            }
+            return low;
+        }
 
         // Threads side by side share a chunk of items, one piece of the row each.  The block puts
         // its items' rows and places into shared memory first, so that the loads of U items do not
         // wait for one another.
         template <typename T, typename OutT, int V>
-        __global__ void __launch_bounds__(THREADS) sumKernel(const SumParams p)
+        __global__ void __launch_bounds__(THREADS) sumKernel(const SumParams p, const ClearParams c)
         {
             constexpr uint32_t U = sizeof(T) * V > 16 ? 4 : V == 8 ? 8 : 16;
             __shared__ uint32_t keys[SUM_ITEMS + 2]; // one on each side
             __shared__ uint64_t places[SUM_ITEMS];
-            const uint32_t lanes = 1u << p.lanesLog2, groups = blockDim.x >> p.lanesLog2;
-            const uint64_t item0 = uint64_t(blockIdx.x) * groups * p.chunk;
             grid_dependency_wait();
             grid_launch_dependents();
+            if(blockIdx.x >= p.blocks)
+            {
+                const uint64_t begin = uint64_t(blockIdx.x - p.blocks) * c.rowsPerBlock;
+                const uint64_t end   = min(uint64_t(c.rows), begin + c.rowsPerBlock);
+                const uint32_t low = lowerBound(p.sorted, 0, p.n, begin), high = lowerBound(p.sorted, low, p.n, end);
+                for(uint32_t i = threadIdx.x; i < uint32_t(end - begin); i += blockDim.x)
+                {
+                    const uint32_t at = lowerBound(p.sorted, low, high, begin + i);
+                    keys[i]           = at < high && p.sorted[at].x == begin + i;
+                }
+                __syncthreads();
+                return clearRows<OutT, V>(c, begin, end, [&](uint64_t row) { return keys[row - begin] != 0u; });
+            }
+            const uint32_t lanes = 1u << p.lanesLog2, groups = blockDim.x >> p.lanesLog2;
+            const uint32_t slice = blockIdx.x % p.slices;
+            const uint64_t item0 = uint64_t(blockIdx.x / p.slices) * groups * p.chunk;
             for(uint32_t i = threadIdx.x; i < groups * p.chunk + 2u; i += blockDim.x)
             {
-                const uint64_t at  = item0 + i; // of item at - 1
-                const uint32_t key = at >= 1u && at <= p.n ? p.keys[at - 1u] : NO_ROW;
-                keys[i]            = key;
-                if(i >= 1u && i <= groups * p.chunk && key < p.rows)
+                const uint64_t at   = item0 + i; // of item at - 1
+                const uint2    pair = at >= 1u && at <= p.n ? p.sorted[at - 1u] : make_uint2(NO_ROW, 0u);
+                keys[i]             = pair.x;
+                if(i >= 1u && i <= groups * p.chunk)
                 {
-                    const uint32_t token = p.tokens ? p.tokens[at - 1u] : uint32_t(at - 1u);
-                    uint32_t       outer = token, in = 0;
+                    uint32_t outer = pair.y, in = 0;
                     if(p.inner > 1u)
                     {
-                        outer = token / p.inner;
-                        in    = token - outer * p.inner;
+                        outer = pair.y / p.inner;
+                        in    = pair.y - outer * p.inner;
                     }
                     places[i - 1u] = uint64_t(outer) * p.gradOuter + uint64_t(in) * p.gradInner;
                 }
             }
             __syncthreads();
-            const uint32_t piece = blockIdx.y * lanes + (threadIdx.x & (lanes - 1u));
+            const uint32_t piece = slice * lanes + (threadIdx.x & (lanes - 1u));
             const uint32_t local = (threadIdx.x >> p.lanesLog2) * p.chunk; // first item in shared memory
             const uint64_t begin = item0 + local, chunkIdx = begin / p.chunk;
             if(piece >= p.pieces || begin >= p.n)
                 return;
-            const uint32_t count  = uint32_t(min(uint64_t(p.chunk), p.n - begin));
-            const uint64_t width  = uint64_t(p.pieces) * V;
-            const uint32_t before = keys[local] & ~EMPTY, after = keys[local + count + 1u] & ~EMPTY;
-            uint32_t const* key   = keys + local + 1u;
-            T const*        grad  = static_cast<T const*>(p.grad) + uint64_t(piece) * V;
+            const uint32_t  count  = uint32_t(min(uint64_t(p.chunk), p.n - begin));
+            const uint64_t  width  = uint64_t(p.pieces) * V;
+            const uint32_t  before = keys[local], after = keys[local + count + 1u];
+            uint32_t const* key    = keys + local + 1u;
+            uint64_t const* place  = places + local;
+            T const*        grad   = static_cast<T const*>(p.grad) + uint64_t(piece) * V;
 
             float    sum[V];
             uint32_t run      = NO_ROW; // row of the current run
@@ -594,55 +652,30 @@ namespace b200wmma
                     return;
                 const bool toRight = last && after == run;
                 if(!fromLeft && !toRight)
-                {
-                    auto* at = reinterpret_cast<Piece<OutT, V>*>(static_cast<OutT*>(p.table) + uint64_t(run) * p.ldt
-                                                                + uint64_t(piece) * V);
-                    Piece<OutT, V> o;
-                    if(p.accumulate)
-                    {
-                        const Piece<OutT, V> old = *at;
-#pragma unroll
-                        for(int i = 0; i < V; ++i)
-                            o.v[i] = fromFloat<OutT>(fmaf(sum[i], p.scale, toFloat(old.v[i])));
-                    }
-                    else
-                    {
-#pragma unroll
-                        for(int i = 0; i < V; ++i)
-                            o.v[i] = fromFloat<OutT>(sum[i] * p.scale);
-                    }
-                    *at = o;
-                    return;
-                }
+                    return finishRow<OutT, V>(p, run, piece, sum);
                 Piece<float, V> s;
 #pragma unroll
                 for(int i = 0; i < V; ++i)
                     s.v[i] = sum[i];
-                *reinterpret_cast<Piece<float, V>*>(p.pieceSums + (2u * chunkIdx + (fromLeft ? 0u : 1u)) * width
-                                                    + uint64_t(piece) * V)
-                    = s;
-                if(!fromLeft)
-                    rightKey = run;
-                else
-                {
+                storePiece<float, V>(p.pieceSums + (2u * chunkIdx + (fromLeft ? 0u : 1u)) * width + uint64_t(piece) * V, s);
+                if(fromLeft)
                     leftKey = run;
-                    if(toRight) // the run goes on: keep it one across this chunk's second place
-                        rightKey = run | EMPTY;
-                }
+                if(toRight) // a piece of a run that starts here, or one that passes through
+                    rightKey = run | (fromLeft ? PASSES : 0u);
             };
-
+#pragma unroll 1
             for(uint32_t i0 = 0; i0 < count; i0 += U)
             {
                 Piece<T, V> v[U];
 #pragma unroll
                 for(uint32_t u = 0; u < U; ++u)
                     if(i0 + u < count && key[i0 + u] < p.rows)
-                        v[u] = *reinterpret_cast<Piece<T, V> const*>(grad + places[local + i0 + u]);
+                        v[u] = loadPiece<T, V>(grad + place[i0 + u]);
 #pragma unroll
                 for(uint32_t u = 0; u < U; ++u)
                     if(i0 + u < count)
                     {
-                        const uint32_t k = key[i0 + u], row = k & ~EMPTY;
+                        const uint32_t row = key[i0 + u];
                         if(row != run)
                         {
                             flush(false);
@@ -650,9 +683,9 @@ namespace b200wmma
                             fromLeft = i0 + u == 0u && before == row;
 #pragma unroll
                             for(int j = 0; j < V; ++j)
-                                sum[j] = k < p.rows ? toFloat(v[u].v[j]) : 0.0f;
+                                sum[j] = toFloat(v[u].v[j]);
                         }
-                        else if(k < p.rows)
+                        else
                         {
 #pragma unroll
                             for(int j = 0; j < V; ++j)
@@ -666,6 +699,83 @@ namespace b200wmma
                 p.pieceKeys[2u * chunkIdx]      = leftKey;
                 p.pieceKeys[2u * chunkIdx + 1u] = rightKey;
             }
+        }
+
+        // A block for every chunk and slice; it has work where a run starts that goes on to the
+        // right: the sum of that piece, of those of the chunks the run passes through, and of the
+        // last one's.  Groups of threads take the pieces in turn and add up in their order.
+        template <typename OutT, int V>
+        __global__ void __launch_bounds__(THREADS) joinKernel(const SumParams p)
+        {
+            constexpr uint32_t U = 4;
+            __shared__ uint32_t end;
+            __shared__ float    sums[THREADS][V + 1];
+            grid_dependency_wait();
+            grid_launch_dependents();
+            const uint32_t first = blockIdx.x / p.slices, slice = blockIdx.x % p.slices;
+            const uint32_t row = p.pieceKeys[2u * uint64_t(first) + 1u];
+            if(row >= p.rows) // none, or one that passes through
+                return;
+            for(uint32_t c0 = first + 1u;; c0 += THREADS) // the run's last chunk
+            {
+                __syncthreads();
+                if(threadIdx.x == 0u)
+                    end = 0xffffffffu;
+                __syncthreads();
+                const uint32_t c = c0 + threadIdx.x;
+                if(c >= p.chunks || p.pieceKeys[2u * uint64_t(c) + 1u] != (row | PASSES))
+                    atomicMin(&end, c);
+                __syncthreads();
+                if(end != 0xffffffffu)
+                    break;
+            }
+            const uint32_t lanes = 1u << p.lanesLog2, groups = THREADS >> p.lanesLog2;
+            const uint32_t piece = slice * lanes + (threadIdx.x & (lanes - 1u)), group = threadIdx.x >> p.lanesLog2;
+            const uint32_t count = end - first + 1u;
+            const uint64_t width = uint64_t(p.pieces) * V;
+            float          sum[V];
+#pragma unroll
+            for(int j = 0; j < V; ++j)
+                sum[j] = 0.0f;
+            if(piece < p.pieces)
+            {
+                float const* at = p.pieceSums + uint64_t(piece) * V;
+                for(uint32_t i0 = group; i0 < count; i0 += U * groups)
+                {
+                    Piece<float, V> v[U];
+#pragma unroll
+                    for(uint32_t u = 0; u < U; ++u)
+                    {
+                        const uint32_t i = i0 + u * groups;
+                        if(i < count) // the first piece went to the right, the others come from the left
+                            v[u] = loadPiece<float, V>(at + (2u * uint64_t(first + i) + (i == 0u ? 1u : 0u)) * width);
+                    }
+#pragma unroll
+                    for(uint32_t u = 0; u < U; ++u)
+                        if(i0 + u * groups < count)
+                        {
+#pragma unroll
+                            for(int j = 0; j < V; ++j)
+                                sum[j] += v[u].v[j];
+                        }
+                }
+            }
+            if(groups > 1u)
+            {
+#pragma unroll
+                for(int j = 0; j < V; ++j)
+                    sums[threadIdx.x][j] = sum[j];
+                __syncthreads();
+                if(group == 0u)
+                    for(uint32_t g = 1; g < groups && g < count; ++g)
+                    {
+#pragma unroll
+                        for(int j = 0; j < V; ++j)
+                            sum[j] += sums[(g << p.lanesLog2) + threadIdx.x][j];
+                    }
+            }
+            if(group == 0u && piece < p.pieces)
+                finishRow<OutT, V>(p, row, piece, sum);
         }
 
         // ---- host side ---------------------------------------------------------------------
@@ -691,7 +801,7 @@ namespace b200wmma
         {
             for(uint32_t v = most; v > 1u; v = v == 8u ? 2u : 1u)
             {
-                const uint64_t bytes = v * elem < 16u ? v * elem : 16u;
+                const uint64_t bytes = v * elem;
                 if(dim % v == 0u && aligned(base, bytes) && ((strides * elem % bytes == 0) && ...))
                     return v;
             }
@@ -734,11 +844,11 @@ namespace b200wmma
             return lookupTyped<T, float>(p, dim, stream);
         }
 
-        // Threads side by side on a row of the sum, and threads of its blocks.
-        uint32_t sumLanesLog2(uint32_t pieces)
+        // Threads side by side on a row of a sum, and threads of its blocks.
+        uint32_t rowLanesLog2(uint32_t pieces)
         {
             const uint32_t l = log2Up(pieces);
-            return l > 5u ? 5u : l;
+            return l > 8u ? 8u : l;
         }
         uint32_t sumThreads(uint32_t lanesLog2)
         {
@@ -746,14 +856,11 @@ namespace b200wmma
         }
 
         // The workspace of the gradient; offsets in bytes.  The chunks go by the sizes alone.
-        constexpr uint32_t MAX_LEVELS = 16;
         struct Plan
         {
-            uint64_t keys[2], tokens[2], counts, totals, touched, bytes;
-            uint32_t tiles, passes, levels;
+            uint64_t keys, pairs[2], counts, totals, pieceKeys, pieceSums, bytes;
+            uint32_t tiles, passes, chunk, chunks;
             bool     small;
-            uint32_t n[MAX_LEVELS], chunk[MAX_LEVELS];
-            uint64_t pieceKeys[MAX_LEVELS], pieceSums[MAX_LEVELS];
         };
 
         Plan planGradient(uint64_t rows, uint32_t dim, uint32_t count)
@@ -765,62 +872,33 @@ namespace b200wmma
                 at += (bytes + 255u) / 256u * 256u;
                 return here;
             };
-            w.small  = count <= SMALL_TOKENS;
-            w.tiles  = uint32_t((uint64_t(count) + SORT_TILE - 1) / SORT_TILE);
-            w.passes = (log2Up(rows + 1u) + 7u) / 8u; // keys 0..rows
-            for(int i = 0; i < (w.small ? 1 : 2); ++i)
-            {
-                w.keys[i]   = take(uint64_t(count) * 4u);
-                w.tokens[i] = take(uint64_t(count) * 4u);
-            }
+            w.small    = count <= SMALL_TOKENS;
+            w.tiles    = uint32_t((uint64_t(count) + SORT_TILE - 1) / SORT_TILE);
+            w.passes   = (log2Up(rows + 1u) + 7u) / 8u; // keys 0..rows
+            w.pairs[0] = take(uint64_t(count) * 8u);
             if(!w.small)
             {
-                w.touched = take(rows);
-                w.totals  = take(RADIX * 4u);
-                w.counts  = take(uint64_t(w.tiles) * RADIX * 4u);
+                w.pairs[1] = take(uint64_t(count) * 8u);
+                w.keys     = w.pairs[1]; // read by the first pass, which writes pairs[0]
+                w.totals   = take(RADIX * 4u);
+                w.counts   = take(uint64_t(w.tiles) * RADIX * 4u);
             }
             const uint32_t pieces = dim % 8u == 0u ? dim / 8u : dim % 2u == 0u ? dim / 2u : dim;
-            const uint32_t lanes  = sumLanesLog2(pieces);
+            const uint32_t lanes  = rowLanesLog2(pieces);
             const uint32_t most   = SUM_ITEMS / (sumThreads(lanes) >> lanes); // that fit a block
-            uint32_t       n      = count;
-            while(true)
+            // Long chunks leave fewer pieces of runs behind, short ones make more threads: twice
+            // what the device holds at once, so that the last ones do not wait long.
+            w.chunk = 8;
+            while(w.chunk < 128u && w.chunk < most && uint64_t(count) * pieces > 2u * uint64_t(w.chunk) * DEVICE_THREADS)
+                w.chunk *= 2u;
+            w.chunks = (count + w.chunk - 1u) / w.chunk;
+            if(w.chunks > 1u)
             {
-                // Long chunks leave fewer pieces of runs behind, short ones make more threads:
-                // enough to fill the device first.  Higher levels are small; 64 keeps them few.
-                uint32_t chunk = 64;
-                if(w.levels == 0u)
-                    for(chunk = 8; chunk < 128u && uint64_t(n) * pieces > uint64_t(chunk) * DEVICE_THREADS;)
-                        chunk *= 2u;
-                chunk                = chunk < most ? chunk : most;
-                const uint32_t level = w.levels++;
-                w.n[level]           = n;
-                w.chunk[level]       = chunk;
-                const uint32_t chunks = (n + chunk - 1u) / chunk;
-                if(chunks <= 1u)
-                    break;
-                n                  = 2u * chunks;
-                w.pieceKeys[level] = take(uint64_t(n) * 4u);
-                w.pieceSums[level] = take(uint64_t(n) * dim * 4u);
+                w.pieceKeys = take(uint64_t(w.chunks) * 8u);
+                w.pieceSums = take(uint64_t(w.chunks) * 2u * dim * 4u);
             }
             w.bytes = at;
             return w;
-        }
-
-        template <typename T, typename OutT, int V>
-        int sumLevelPieces(SumParams p, uint32_t dim, cudaStream_t stream)
-        {
-            p.pieces    = dim / V;
-            p.lanesLog2 = sumLanesLog2(p.pieces);
-            const uint32_t threads = sumThreads(p.lanesLog2), lanes = 1u << p.lanesLog2;
-            const uint64_t per = uint64_t(threads >> p.lanesLog2) * p.chunk;
-            const dim3     grid(uint32_t((p.n + per - 1u) / per), (p.pieces + lanes - 1u) / lanes);
-            return cudaToStatus(launchOverlapped(sumKernel<T, OutT, V>, grid, dim3(threads), 0, stream, p));
-        }
-        template <typename T, typename OutT>
-        int sumLevel(SumParams const& p, uint32_t dim, uint32_t v, cudaStream_t stream)
-        {
-            return v == 8u ? sumLevelPieces<T, OutT, 8>(p, dim, stream)
-                           : v == 2u ? sumLevelPieces<T, OutT, 2>(p, dim, stream) : sumLevelPieces<T, OutT, 1>(p, dim, stream);
         }
 
         struct GradientCall
@@ -844,69 +922,100 @@ namespace b200wmma
             return rc__;         \
     } while(0)
 
-        // Sorted keys and tokens into the workspace; rows without a token cleared on the way.
-        template <typename OutT, int V>
-        int sortTokens(GradientCall const& g, Plan const& w, uint32_t** keys, uint32_t** tokens, cudaStream_t stream)
+        ClearParams clearParams(void* table, uint64_t ldt, uint32_t rows, uint32_t pieces)
         {
-            auto        words = [&](uint64_t at) { return reinterpret_cast<uint32_t*>(g.workspace + at); };
-            ClearParams c{g.table, g.ldt, g.dim / V, 0, 0};
-            c.lanesLog2           = log2Up(c.pieces) > 8u ? 8u : log2Up(c.pieces);
-            const uint64_t bytes  = uint64_t(g.t.rows) * g.dim * sizeof(OutT);
-            if(w.small)
+            return ClearParams{table, ldt, pieces, rowLanesLog2(pieces), 0, rows, 0};
+        }
+
+        // (row, token) of every token into the workspace, sorted; few tokens: rows without one
+        // cleared on the way.
+        template <typename OutT, int V>
+        int sortFew(GradientCall const& g, Plan const& w, cudaStream_t stream)
+        {
+            ClearParams c = clearParams(g.table, g.ldt, g.t.rows, g.dim / V);
+            // a block to an SM, each with 16 KB of rows at least
+            const uint64_t want = (uint64_t(g.t.rows) * g.dim * sizeof(OutT) + 16383u) / 16384u;
+            c.blocks            = g.accumulate ? 0u : uint32_t(want < 147u ? want : 147u);
+            static std::mutex mutex;
+            static bool       done[64] = {};
             {
-                *keys   = words(w.keys[0]);
-                *tokens = words(w.tokens[0]);
-                // a block to an SM, each with 16 KB of rows at least
-                const uint64_t want = (bytes + 16383u) / 16384u;
-                c.blocks            = g.accumulate ? 0u : uint32_t(want < 147u ? want : 147u);
-                static std::mutex mutex;
-                static bool       done[64] = {};
+                std::lock_guard<std::mutex> lock(mutex);
+                int                         dev = 0;
+                B200WMMA_CUDA_TRY(cudaGetDevice(&dev));
+                if(dev >= 64 || !done[dev])
                 {
-                    std::lock_guard<std::mutex> lock(mutex);
-                    int                         dev = 0;
-                    B200WMMA_CUDA_TRY(cudaGetDevice(&dev));
-                    if(dev >= 64 || !done[dev])
-                    {
-                        B200WMMA_CUDA_TRY(cudaFuncSetAttribute(sortSmallKernel<OutT, V>,
-                                                               cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                               int(sizeof(SmallShared))));
-                        if(dev < 64)
-                            done[dev] = true;
-                    }
+                    B200WMMA_CUDA_TRY(cudaFuncSetAttribute(sortSmallKernel<OutT, V>,
+                                                           cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                           int(sizeof(SmallShared))));
+                    if(dev < 64)
+                        done[dev] = true;
                 }
-                return cudaToStatus(launchOverlapped(sortSmallKernel<OutT, V>, dim3(1u + c.blocks), dim3(SMALL_THREADS),
-                                                     sizeof(SmallShared), stream, g.t, c, w.passes, *keys, *tokens));
             }
-            uint8_t* touched = g.accumulate ? nullptr : g.workspace + w.touched;
-            if(touched)
-                B200WMMA_CUDA_TRY(cudaMemsetAsync(touched, 0, g.t.rows, stream));
-            B200WMMA_TRY(cudaToStatus(launchOverlapped(keysKernel, dim3(w.tiles), dim3(THREADS), 0, stream, g.t,
-                                                       words(w.keys[0]), touched, w.tiles, words(w.counts))));
-            Share s{touched, g.t.rows, 0, 2u * w.passes - 1u};
-            const uint64_t want = (bytes / s.shares + 65535u) / 65536u;
-            c.blocks            = g.accumulate ? 0u : uint32_t(want < 592u ? want : 592u);
-            const dim3 grid(w.tiles + c.blocks);
+            return cudaToStatus(launchOverlapped(sortSmallKernel<OutT, V>, dim3(1u + c.blocks), dim3(SMALL_THREADS),
+                                                 sizeof(SmallShared), stream, g.t, c, w.passes,
+                                                 reinterpret_cast<uint2*>(g.workspace + w.pairs[0])));
+        }
+
+        int sortMany(GradientCall const& g, Plan const& w, uint2** sorted, cudaStream_t stream)
+        {
+            auto       words = [&](uint64_t at) { return reinterpret_cast<uint32_t*>(g.workspace + at); };
+            auto       pairs = [&](uint32_t i) { return reinterpret_cast<uint2*>(g.workspace + w.pairs[i]); };
+            const dim3 grid(w.tiles);
+            B200WMMA_TRY(cudaToStatus(launchOverlapped(keysKernel, grid, dim3(THREADS), 0, stream, g.t, words(w.keys),
+                                                       w.tiles, words(w.counts))));
             for(uint32_t pass = 0; pass < w.passes; ++pass)
             {
-                const uint32_t from = pass % 2u, to = 1u - from, shift = 8u * pass;
+                uint2* from = pass ? pairs((pass - 1u) % 2u) : nullptr;
                 if(pass > 0u)
-                {
-                    B200WMMA_TRY(cudaToStatus(launchOverlapped(countKernel<OutT, V>, grid, dim3(THREADS), 0, stream,
-                                                               words(w.keys[from]), g.t.count, shift, w.tiles,
-                                                               words(w.counts), c, s)));
-                    ++s.share;
-                }
+                    B200WMMA_TRY(cudaToStatus(launchOverlapped(countKernel, grid, dim3(THREADS), 0, stream, from,
+                                                               g.t.count, 8u * pass, w.tiles, words(w.counts))));
                 B200WMMA_TRY(cudaToStatus(launchOverlapped(scanKernel, dim3(RADIX), dim3(THREADS), 0, stream,
                                                            words(w.counts), w.tiles, words(w.totals))));
-                B200WMMA_TRY(cudaToStatus(launchOverlapped(scatterKernel<OutT, V>, grid, dim3(THREADS), 0, stream,
-                                                           words(w.keys[from]), pass ? words(w.tokens[from]) : nullptr,
-                                                           g.t.count, shift, w.tiles, words(w.counts), words(w.totals),
-                                                           words(w.keys[to]), words(w.tokens[to]), c, s)));
-                ++s.share;
+                B200WMMA_TRY(cudaToStatus(launchOverlapped(scatterKernel, grid, dim3(THREADS), 0, stream, words(w.keys),
+                                                           from, g.t.count, 8u * pass, w.tiles, words(w.counts),
+                                                           words(w.totals), pairs(pass % 2u))));
             }
-            *keys   = words(w.keys[w.passes % 2u]);
-            *tokens = words(w.tokens[w.passes % 2u]);
+            *sorted = pairs((w.passes - 1u) % 2u);
             return B200WMMA_OK;
+        }
+
+        // The sums of chunks, with pieces of `V` values, and rows cleared beside them where the
+        // sort has not done that.
+        template <typename T, typename OutT, int V>
+        int sumChunks(GradientCall const& g, Plan const& w, SumParams p, cudaStream_t stream)
+        {
+            p.pieces    = g.dim / V;
+            p.lanesLog2 = rowLanesLog2(p.pieces);
+            p.slices    = (p.pieces + (1u << p.lanesLog2) - 1u) >> p.lanesLog2;
+            const uint32_t threads = sumThreads(p.lanesLog2);
+            const uint64_t per     = uint64_t(threads >> p.lanesLog2) * p.chunk;
+            const uint64_t blocks  = (p.n + per - 1u) / per * p.slices;
+            // rows may lie on wider boundaries than those of the gradient: clear by the narrower
+            ClearParams c = clearParams(g.table, g.ldt, g.t.rows, p.pieces);
+            c.lanesLog2   = c.lanesLog2 < log2Up(threads) ? c.lanesLog2 : log2Up(threads);
+            if(!w.small && !g.accumulate)
+            {
+                const uint64_t rowBytes = uint64_t(g.dim) * sizeof(OutT);
+                c.rowsPerBlock          = rowBytes >= 65536u ? 1u : uint32_t(65536u / rowBytes);
+                c.rowsPerBlock          = c.rowsPerBlock > 1024u ? 1024u : c.rowsPerBlock;
+                c.blocks                = (g.t.rows + c.rowsPerBlock - 1u) / c.rowsPerBlock;
+            }
+            if(blocks + c.blocks > 0x7fffffffull)
+                return B200WMMA_ERR_TOO_LARGE;
+            p.blocks = uint32_t(blocks);
+            return cudaToStatus(launchOverlapped(sumKernel<T, OutT, V>, dim3(p.blocks + c.blocks), dim3(threads), 0, stream, p, c));
+        }
+
+        template <typename OutT, int V>
+        int joinPieces(GradientCall const& g, SumParams p, cudaStream_t stream)
+        {
+            p.pieces    = g.dim / V;
+            p.lanesLog2 = rowLanesLog2(p.pieces);
+            p.slices    = (p.pieces + (1u << p.lanesLog2) - 1u) >> p.lanesLog2;
+            const uint64_t blocks = uint64_t(p.chunks) * p.slices;
+            if(blocks > 0x7fffffffull)
+                return B200WMMA_ERR_TOO_LARGE;
+            return cudaToStatus(launchOverlapped(joinKernel<OutT, V>, dim3(uint32_t(blocks)), dim3(THREADS), 0, stream, p));
         }
 
         template <typename T, typename OutT>
@@ -915,42 +1024,36 @@ namespace b200wmma
             const Plan     w  = planGradient(g.t.rows, g.dim, g.t.count);
             const uint32_t vt = pieceSize(g.dim, g.table, sizeof(OutT), 8, g.ldt);
             const uint32_t vg = pieceSize(g.dim, g.grad, sizeof(T), vt, g.gradOuter, g.gradInner);
-            uint32_t *     keys = nullptr, *tokens = nullptr;
-            B200WMMA_TRY(vt == 8u ? (sortTokens<OutT, 8>(g, w, &keys, &tokens, stream))
-                                  : vt == 2u ? (sortTokens<OutT, 2>(g, w, &keys, &tokens, stream))
-                                             : (sortTokens<OutT, 1>(g, w, &keys, &tokens, stream)));
-            for(uint32_t level = 0; level < w.levels; ++level)
+            uint2*         sorted = reinterpret_cast<uint2*>(g.workspace + w.pairs[0]);
+            if(w.small)
+                B200WMMA_TRY(vt == 8u ? (sortFew<OutT, 8>(g, w, stream))
+                                      : vt == 2u ? (sortFew<OutT, 2>(g, w, stream)) : (sortFew<OutT, 1>(g, w, stream)));
+            else
+                B200WMMA_TRY(sortMany(g, w, &sorted, stream));
+            SumParams p{};
+            p.sorted     = sorted;
+            p.grad       = g.grad;
+            p.gradOuter  = g.gradOuter;
+            p.gradInner  = g.gradInner;
+            p.inner      = g.t.inner;
+            p.n          = g.t.count;
+            p.chunk      = w.chunk;
+            p.chunks     = w.chunks;
+            p.rows       = g.t.rows;
+            p.table      = g.table;
+            p.ldt        = g.ldt;
+            p.scale      = g.scale;
+            p.accumulate = g.accumulate ? 1u : 0u;
+            if(w.chunks > 1u)
             {
-                const bool more = level + 1u < w.levels;
-                SumParams  p{};
-                p.n          = w.n[level];
-                p.chunk      = w.chunk[level];
-                p.rows       = g.t.rows;
-                p.table      = g.table;
-                p.ldt        = g.ldt;
-                p.scale      = g.scale;
-                p.accumulate = g.accumulate ? 1u : 0u;
-                p.pieceKeys  = more ? reinterpret_cast<uint32_t*>(g.workspace + w.pieceKeys[level]) : nullptr;
-                p.pieceSums  = more ? reinterpret_cast<float*>(g.workspace + w.pieceSums[level]) : nullptr;
-                if(level == 0)
-                {
-                    p.keys      = keys;
-                    p.tokens    = tokens;
-                    p.grad      = g.grad;
-                    p.gradOuter = g.gradOuter;
-                    p.gradInner = g.gradInner;
-                    p.inner     = g.t.inner;
-                    B200WMMA_TRY((sumLevel<T, OutT>(p, g.dim, vg, stream)));
-                }
-                else
-                {
-                    p.keys      = reinterpret_cast<uint32_t*>(g.workspace + w.pieceKeys[level - 1u]);
-                    p.grad      = g.workspace + w.pieceSums[level - 1u];
-                    p.gradOuter = g.dim;
-                    p.inner     = 1;
-                    B200WMMA_TRY((sumLevel<float, OutT>(p, g.dim, vt, stream)));
-                }
+                p.pieceKeys = reinterpret_cast<uint32_t*>(g.workspace + w.pieceKeys);
+                p.pieceSums = reinterpret_cast<float*>(g.workspace + w.pieceSums);
             }
+            B200WMMA_TRY(vg == 8u ? (sumChunks<T, OutT, 8>(g, w, p, stream))
+                                  : vg == 2u ? (sumChunks<T, OutT, 2>(g, w, p, stream)) : (sumChunks<T, OutT, 1>(g, w, p, stream)));
+            if(w.chunks > 1u)
+                B200WMMA_TRY(vt == 8u ? (joinPieces<OutT, 8>(g, p, stream))
+                                      : vt == 2u ? (joinPieces<OutT, 2>(g, p, stream)) : (joinPieces<OutT, 1>(g, p, stream)));
             return B200WMMA_OK;
         }
 #undef B200WMMA_TRY
