@@ -41,7 +41,7 @@ namespace b200wmma
             uint32_t       wide; // 64-bit ids
         };
 
-        __device__ inline uint32_t rowOf(Tokens const& t, uint32_t token, uint32_t& outer, uint32_t& inner)
+        __device__ inline int64_t idOf(Tokens const& t, uint32_t token, uint32_t& outer, uint32_t& inner)
         {
             outer = token;
             inner = 0;
@@ -51,18 +51,24 @@ namespace b200wmma
                 inner = token - outer * t.inner;
             }
             const uint64_t at = uint64_t(outer) * t.idsOuter + uint64_t(inner) * t.idsInner;
-            const int64_t  id = t.wide ? static_cast<int64_t const*>(t.ids)[at]
-                                       : int64_t(static_cast<int32_t const*>(t.ids)[at]);
-            int64_t row = id, end = t.rows;
+            return t.wide ? static_cast<int64_t const*>(t.ids)[at] : int64_t(static_cast<int32_t const*>(t.ids)[at]);
+        }
+        __device__ inline uint32_t rowOf(Tokens const& t, int64_t id, uint32_t inner)
+        {
+            int64_t begin = 0, end = t.rows;
             if(t.first)
             {
-                const int64_t begin = t.first[inner];
-                end                 = t.first[inner + 1];
-                row                 = begin + id;
-                if(begin < 0 || end > int64_t(t.rows) || id < 0 || id >= end - begin)
+                begin = t.first[inner];
+                end   = t.first[inner + 1];
+                if(begin < 0 || end > int64_t(t.rows))
                     return NO_ROW;
             }
-            return row >= 0 && row < end ? uint32_t(row) : NO_ROW;
+            return id >= 0 && id < end - begin ? uint32_t(begin + id) : NO_ROW;
+        }
+        __device__ inline uint32_t rowOf(Tokens const& t, uint32_t token, uint32_t& outer, uint32_t& inner)
+        {
+            const int64_t id = idOf(t, token, outer, inner);
+            return rowOf(t, id, inner);
         }
 
         // V neighbouring values of a row, at most 32 bytes, moved as one.
@@ -189,6 +195,21 @@ namespace b200wmma
                         storePiece<OutT, V>(static_cast<OutT*>(c.table) + row * c.ldt + uint64_t(piece) * V, zero);
         }
 
+        // Lanes of the warp with the same digit of eight bits, among those that are `in`.  (Eight
+        // ballots: match.any took most of the scattering kernel's time.)
+        __device__ inline uint32_t sameDigit(uint32_t digit, bool in)
+        {
+            uint32_t same = __ballot_sync(0xffffffffu, in);
+#pragma unroll
+            for(uint32_t b = 0; b < 8u; ++b)
+            {
+                const bool     set  = (digit >> b) & 1u;
+                const uint32_t vote = __ballot_sync(0xffffffffu, set);
+                same &= set ? vote : ~vote;
+            }
+            return same;
+        }
+
         // ---- sorting few tokens: one block --------------------------------------------------
         constexpr uint32_t SMALL_THREADS = 1024;
         constexpr uint32_t SMALL_ITEMS   = 16;
@@ -271,7 +292,7 @@ namespace b200wmma
                     {
                         const bool     in    = first + i * 32u < t.count;
                         const uint32_t digit = (key[i] >> shift) % RADIX;
-                        const uint32_t peers = __match_any_sync(0xffffffffu, in ? digit : RADIX);
+                        const uint32_t peers = sameDigit(digit, in);
                         rank[i]              = (in ? sh->bins[warp][digit] : 0u) + __popc(peers & ((1u << lane) - 1u));
                         __syncwarp();
                         if(in && (peers >> lane) == 1u) // the last of its digit
@@ -353,8 +374,8 @@ namespace b200wmma
             {
                 // one addition for the equal digits of a warp: a hot row would queue 32
                 const bool     in    = uint64_t(first) + i * THREADS < n;
-                const uint32_t digit = in ? (key[i] >> shift) % RADIX : RADIX;
-                const uint32_t peers = __match_any_sync(0xffffffffu, digit);
+                const uint32_t digit = (key[i] >> shift) % RADIX;
+                const uint32_t peers = sameDigit(digit, in);
                 if(in && (peers & ((1u << (threadIdx.x % 32u)) - 1u)) == 0u)
                     atomicAdd(&bins[digit], uint32_t(__popc(peers)));
             }
@@ -369,7 +390,14 @@ namespace b200wmma
             grid_dependency_wait();
             grid_launch_dependents();
             const uint32_t first = blockIdx.x * SORT_TILE + threadIdx.x;
-            uint32_t       key[SORT_ITEMS];
+            uint32_t       key[SORT_ITEMS], outer, inner[SORT_ITEMS];
+            int64_t        id[SORT_ITEMS];
+#pragma unroll
+            for(uint32_t i = 0; i < SORT_ITEMS; ++i)
+            {
+                const uint32_t token = first + i * THREADS;
+                id[i]                = token < t.count ? idOf(t, token, outer, inner[i]) : -1;
+            }
 #pragma unroll
             for(uint32_t i = 0; i < SORT_ITEMS; ++i)
             {
@@ -377,8 +405,7 @@ namespace b200wmma
                 key[i]               = t.rows; // behind every row
                 if(token < t.count)
                 {
-                    uint32_t       outer, inner;
-                    const uint32_t row = rowOf(t, token, outer, inner);
+                    const uint32_t row = rowOf(t, id[i], inner[i]);
                     if(row != NO_ROW)
                         key[i] = row;
                     keys[token] = key[i];
@@ -494,7 +521,7 @@ namespace b200wmma
             {
                 const bool     in    = first + i * 32u < here;
                 const uint32_t digit = (pair[i].x >> shift) % RADIX;
-                const uint32_t peers = __match_any_sync(0xffffffffu, in ? digit : RADIX);
+                const uint32_t peers = sameDigit(digit, in);
                 rank[i]              = (in ? bins[warp][digit] : 0u) + __popc(peers & ((1u << lane) - 1u));
                 __syncwarp();
                 if(in && (peers >> lane) == 1u) // the last of its digit
@@ -533,7 +560,8 @@ namespace b200wmma
         }
 
         // ---- summing runs ------------------------------------------------------------------
-        constexpr uint32_t SUM_ITEMS = 2048; // of a block
+        constexpr uint32_t SUM_ITEMS = 1024; // of a block
+        constexpr uint32_t RING_BYTES = 128; // of a thread: pieces on their way
         struct SumParams
         {
             uint2 const* sorted; // (row, token), equal rows next to each other
@@ -587,15 +615,62 @@ namespace b200wmma
             return low;
         }
 
+        // A thread's ring of pieces that cp.async brings: nobody else reads them, so there is nothing to
+        // synchronise, and the loads hold no registers while they fly.  (With the pieces of eight
+        // items in registers the kernel ran 512 threads to an SM and 2.3 TB/s.)
+        template <typename T, int V>
+        struct Ring
+        {
+            // (single 16-bit values travel in the aligned word that holds them)
+            static constexpr uint32_t BYTES = sizeof(T) * V < 4 ? 4 : sizeof(T) * V;
+            static constexpr uint32_t PART  = BYTES > 16 ? 16 : BYTES; // of one copy
+            static constexpr uint32_t DEPTH = RING_BYTES / BYTES > 16 ? 16 : RING_BYTES / BYTES;
+
+            // slot s of the calling thread; the threads of a block lie side by side
+            static __device__ uint8_t* at(uint8_t* ring, uint32_t s, uint32_t part)
+            {
+                return ring + ((s * (BYTES / PART) + part) * THREADS + threadIdx.x) * PART;
+            }
+            static __device__ void load(uint8_t* ring, uint32_t s, T const* from)
+            {
+                uint64_t src = reinterpret_cast<uint64_t>(from);
+                if constexpr(sizeof(T) * V < 4)
+                    src &= ~uint64_t(3);
+#pragma unroll
+                for(uint32_t part = 0; part < BYTES / PART; ++part)
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(
+                                     uint32_t(__cvta_generic_to_shared(at(ring, s, part)))),
+                                 "l"(src + part * PART), "n"(PART)
+                                 : "memory");
+            }
+            static __device__ Piece<T, V> get(uint8_t* ring, uint32_t s, uint64_t place)
+            {
+                Piece<T, V> p;
+                if constexpr(sizeof(T) * V < 4)
+                    p.v[0] = reinterpret_cast<T const*>(at(ring, s, 0))[place / sizeof(T) % 2u];
+                else
+                {
+                    struct alignas(PART) Part
+                    {
+                        uint8_t b[PART];
+                    };
+#pragma unroll
+                    for(uint32_t part = 0; part < BYTES / PART; ++part)
+                        reinterpret_cast<Part*>(&p)[part] = *reinterpret_cast<Part const*>(at(ring, s, part));
+                }
+                return p;
+            }
+        };
+
         // Threads side by side share a chunk of items, one piece of the row each.  The block puts
-        // its items' rows and places into shared memory first, so that the loads of U items do not
-        // wait for one another.
+        // its items' rows and places into shared memory first, so that no load waits for another.
         template <typename T, typename OutT, int V>
         __global__ void __launch_bounds__(THREADS) sumKernel(const SumParams p, const ClearParams c)
         {
-            constexpr uint32_t U = sizeof(T) * V > 16 ? 4 : V == 8 ? 8 : 16;
+            using R = Ring<T, V>;
             __shared__ uint32_t keys[SUM_ITEMS + 2]; // one on each side
             __shared__ uint64_t places[SUM_ITEMS];
+            __shared__ alignas(16) uint8_t ring[R::DEPTH * R::BYTES * THREADS];
             grid_dependency_wait();
             grid_launch_dependents();
             if(blockIdx.x >= p.blocks)
@@ -647,53 +722,56 @@ namespace b200wmma
             uint32_t run      = NO_ROW; // row of the current run
             bool     fromLeft = false;
             uint32_t leftKey = NO_ROW, rightKey = NO_ROW;
-            auto     flush = [&](bool last) {
-                if(run >= p.rows)
-                    return;
-                const bool toRight = last && after == run;
-                if(!fromLeft && !toRight)
-                    return finishRow<OutT, V>(p, run, piece, sum);
-                Piece<float, V> s;
-#pragma unroll
-                for(int i = 0; i < V; ++i)
-                    s.v[i] = sum[i];
-                storePiece<float, V>(p.pieceSums + (2u * chunkIdx + (fromLeft ? 0u : 1u)) * width + uint64_t(piece) * V, s);
-                if(fromLeft)
-                    leftKey = run;
-                if(toRight) // a piece of a run that starts here, or one that passes through
-                    rightKey = run | (fromLeft ? PASSES : 0u);
+            auto     load = [&](uint32_t i) {
+                if(i < count && key[i] < p.rows)
+                    R::load(ring, i % R::DEPTH, grad + place[i]);
+                asm volatile("cp.async.commit_group;" ::: "memory");
             };
-#pragma unroll 1
-            for(uint32_t i0 = 0; i0 < count; i0 += U)
+#pragma unroll
+            for(uint32_t i = 0; i < R::DEPTH; ++i)
+                load(i);
+            for(uint32_t i = 0;; ++i)
             {
-                Piece<T, V> v[U];
-#pragma unroll
-                for(uint32_t u = 0; u < U; ++u)
-                    if(i0 + u < count && key[i0 + u] < p.rows)
-                        v[u] = loadPiece<T, V>(grad + place[i0 + u]);
-#pragma unroll
-                for(uint32_t u = 0; u < U; ++u)
-                    if(i0 + u < count)
+                const uint32_t row = i < count ? key[i] : NO_ROW;
+                if(row != run || i == count)
+                {
+                    // the end of a run
+                    if(run < p.rows)
                     {
-                        const uint32_t row = key[i0 + u];
-                        if(row != run)
-                        {
-                            flush(false);
-                            run      = row;
-                            fromLeft = i0 + u == 0u && before == row;
-#pragma unroll
-                            for(int j = 0; j < V; ++j)
-                                sum[j] = toFloat(v[u].v[j]);
-                        }
+                        const bool toRight = i == count && after == run;
+                        if(!fromLeft && !toRight)
+                            finishRow<OutT, V>(p, run, piece, sum);
                         else
                         {
+                            Piece<float, V> s;
 #pragma unroll
                             for(int j = 0; j < V; ++j)
-                                sum[j] += toFloat(v[u].v[j]);
+                                s.v[j] = sum[j];
+                            storePiece<float, V>(p.pieceSums + (2u * chunkIdx + (fromLeft ? 0u : 1u)) * width + uint64_t(piece) * V, s);
+                            if(fromLeft)
+                                leftKey = run;
+                            if(toRight) // a piece of a run that starts here, or one that passes through
+                                rightKey = run | (fromLeft ? PASSES : 0u);
                         }
                     }
+                    if(i == count)
+                        break;
+                    run      = row;
+                    fromLeft = i == 0u && before == row;
+#pragma unroll
+                    for(int j = 0; j < V; ++j)
+                        sum[j] = 0.0f;
+                }
+                asm volatile("cp.async.wait_group %0;" ::"n"(R::DEPTH - 1) : "memory");
+                if(row < p.rows)
+                {
+                    const Piece<T, V> v = R::get(ring, i % R::DEPTH, reinterpret_cast<uint64_t>(grad + place[i]));
+#pragma unroll
+                    for(int j = 0; j < V; ++j)
+                        sum[j] += toFloat(v.v[j]);
+                }
+                load(i + R::DEPTH);
             }
-            flush(true);
             if(piece == 0u && p.pieceKeys)
             {
                 p.pieceKeys[2u * chunkIdx]      = leftKey;
@@ -701,81 +779,114 @@ namespace b200wmma
             }
         }
 
-        // A block for every chunk and slice; it has work where a run starts that goes on to the
-        // right: the sum of that piece, of those of the chunks the run passes through, and of the
-        // last one's.  Groups of threads take the pieces in turn and add up in their order.
+        // Joins the runs that cross chunks.  A group of threads side by side has a chunk: where a run
+        // starts there that goes on to the right, the row is the sum of that piece, of those of the
+        // chunks that the run passes through, and of the last one's, in this order.  Runs of more
+        // than JOIN_FEW pieces are left to the whole block: its groups take the pieces in turn.
+        constexpr uint32_t JOIN_FEW = 16;
+
         template <typename OutT, int V>
         __global__ void __launch_bounds__(THREADS) joinKernel(const SumParams p)
         {
             constexpr uint32_t U = 4;
-            __shared__ uint32_t end;
+            __shared__ uint32_t longs[THREADS], longCount, end;
             __shared__ float    sums[THREADS][V + 1];
+            if(threadIdx.x == 0u)
+                longCount = 0;
+            __syncthreads();
             grid_dependency_wait();
             grid_launch_dependents();
-            const uint32_t first = blockIdx.x / p.slices, slice = blockIdx.x % p.slices;
-            const uint32_t row = p.pieceKeys[2u * uint64_t(first) + 1u];
-            if(row >= p.rows) // none, or one that passes through
-                return;
-            for(uint32_t c0 = first + 1u;; c0 += THREADS) // the run's last chunk
-            {
-                __syncthreads();
-                if(threadIdx.x == 0u)
-                    end = 0xffffffffu;
-                __syncthreads();
-                const uint32_t c = c0 + threadIdx.x;
-                if(c >= p.chunks || p.pieceKeys[2u * uint64_t(c) + 1u] != (row | PASSES))
-                    atomicMin(&end, c);
-                __syncthreads();
-                if(end != 0xffffffffu)
-                    break;
-            }
             const uint32_t lanes = 1u << p.lanesLog2, groups = THREADS >> p.lanesLog2;
-            const uint32_t piece = slice * lanes + (threadIdx.x & (lanes - 1u)), group = threadIdx.x >> p.lanesLog2;
-            const uint32_t count = end - first + 1u;
+            const uint32_t slice = blockIdx.x % p.slices;
+            const uint32_t lane = threadIdx.x & (lanes - 1u), group = threadIdx.x >> p.lanesLog2;
+            const uint32_t piece = slice * lanes + lane;
             const uint64_t width = uint64_t(p.pieces) * V;
+            float const*   at    = p.pieceSums + uint64_t(piece) * V;
+            auto           rightKey = [&](uint32_t c) { return p.pieceKeys[2u * uint64_t(c) + 1u]; };
             float          sum[V];
+            // pieces begin, begin + step, ... of a run of `count` that starts in chunk `first`
+            auto add = [&](uint32_t first, uint32_t begin, uint32_t count, uint32_t step) {
 #pragma unroll
-            for(int j = 0; j < V; ++j)
-                sum[j] = 0.0f;
-            if(piece < p.pieces)
-            {
-                float const* at = p.pieceSums + uint64_t(piece) * V;
-                for(uint32_t i0 = group; i0 < count; i0 += U * groups)
+                for(int j = 0; j < V; ++j)
+                    sum[j] = 0.0f;
+                for(uint32_t i0 = begin; i0 < count; i0 += U * step)
                 {
                     Piece<float, V> v[U];
 #pragma unroll
                     for(uint32_t u = 0; u < U; ++u)
                     {
-                        const uint32_t i = i0 + u * groups;
+                        const uint32_t i = i0 + u * step;
                         if(i < count) // the first piece went to the right, the others come from the left
                             v[u] = loadPiece<float, V>(at + (2u * uint64_t(first + i) + (i == 0u ? 1u : 0u)) * width);
                     }
 #pragma unroll
                     for(uint32_t u = 0; u < U; ++u)
-                        if(i0 + u * groups < count)
+                        if(i0 + u * step < count)
                         {
 #pragma unroll
                             for(int j = 0; j < V; ++j)
                                 sum[j] += v[u].v[j];
                         }
                 }
-            }
-            if(groups > 1u)
+            };
+            const uint64_t mine = uint64_t(blockIdx.x / p.slices) * groups + group;
+            if(mine + 1u < p.chunks)
             {
-#pragma unroll
-                for(int j = 0; j < V; ++j)
-                    sums[threadIdx.x][j] = sum[j];
-                __syncthreads();
-                if(group == 0u)
-                    for(uint32_t g = 1; g < groups && g < count; ++g)
+                const uint32_t first = uint32_t(mine), row = rightKey(first);
+                if(row < p.rows) // a run starts here and goes on
+                {
+                    uint32_t count = 2;
+                    while(count <= JOIN_FEW && rightKey(first + count - 1u) == (row | PASSES))
+                        ++count;
+                    if(count > JOIN_FEW)
                     {
-#pragma unroll
-                        for(int j = 0; j < V; ++j)
-                            sum[j] += sums[(g << p.lanesLog2) + threadIdx.x][j];
+                        if(lane == 0u)
+                            longs[atomicAdd(&longCount, 1u)] = first;
                     }
+                    else if(piece < p.pieces)
+                    {
+                        add(first, 0, count, 1);
+                        finishRow<OutT, V>(p, row, piece, sum);
+                    }
+                }
             }
-            if(group == 0u && piece < p.pieces)
-                finishRow<OutT, V>(p, row, piece, sum);
+            __syncthreads();
+            for(uint32_t l = 0; l < longCount; ++l)
+            {
+                const uint32_t first = longs[l], row = rightKey(first);
+                for(uint32_t c0 = first + 1u;; c0 += THREADS) // the run's last chunk
+                {
+                    __syncthreads();
+                    if(threadIdx.x == 0u)
+                        end = 0xffffffffu;
+                    __syncthreads();
+                    const uint32_t c = c0 + threadIdx.x;
+                    if(c >= p.chunks || rightKey(c) != (row | PASSES))
+                        atomicMin(&end, c);
+                    __syncthreads();
+                    if(end != 0xffffffffu)
+                        break;
+                }
+                const uint32_t count = end - first + 1u;
+                if(piece < p.pieces)
+                    add(first, group, count, groups);
+                if(groups > 1u)
+                {
+#pragma unroll
+                    for(int j = 0; j < V; ++j)
+                        sums[threadIdx.x][j] = sum[j];
+                    __syncthreads();
+                    if(group == 0u)
+                        for(uint32_t g = 1; g < groups && g < count; ++g)
+                        {
+#pragma unroll
+                            for(int j = 0; j < V; ++j)
+                                sum[j] += sums[(g << p.lanesLog2) + threadIdx.x][j];
+                        }
+                }
+                if(group == 0u && piece < p.pieces)
+                    finishRow<OutT, V>(p, row, piece, sum);
+            }
         }
 
         // ---- host side ---------------------------------------------------------------------
@@ -793,6 +904,12 @@ namespace b200wmma
             while((1ull << l) < v)
                 ++l;
             return l;
+        }
+        // Threads side by side on a row.
+        uint32_t rowLanesLog2(uint32_t pieces)
+        {
+            const uint32_t l = log2Up(pieces);
+            return l > 8u ? 8u : l;
         }
         // Values of a piece: 8, 2 or 1, whatever divides dim and keeps every piece of the given
         // tensors on its boundary.  `strides`: distances of rows, in elements.
@@ -812,7 +929,7 @@ namespace b200wmma
         int lookup(LookupParams p, uint32_t dim, cudaStream_t stream)
         {
             p.pieces    = dim / V;
-            p.lanesLog2 = log2Up(p.pieces) > 8u ? 8u : log2Up(p.pieces);
+            p.lanesLog2 = rowLanesLog2(p.pieces);
             // 4096 pieces to a block (16 a thread), but blocks for every SM first
             uint32_t per = p.pieces >= 4096u ? 1u : 4096u / p.pieces;
             per          = per > THREADS ? THREADS : per;
@@ -844,12 +961,7 @@ namespace b200wmma
             return lookupTyped<T, float>(p, dim, stream);
         }
 
-        // Threads side by side on a row of a sum, and threads of its blocks.
-        uint32_t rowLanesLog2(uint32_t pieces)
-        {
-            const uint32_t l = log2Up(pieces);
-            return l > 8u ? 8u : l;
-        }
+        // Threads of a block of the sum.
         uint32_t sumThreads(uint32_t lanesLog2)
         {
             return lanesLog2 >= 3u ? THREADS : 32u << lanesLog2;
@@ -997,7 +1109,7 @@ namespace b200wmma
             {
                 const uint64_t rowBytes = uint64_t(g.dim) * sizeof(OutT);
                 c.rowsPerBlock          = rowBytes >= 65536u ? 1u : uint32_t(65536u / rowBytes);
-                c.rowsPerBlock          = c.rowsPerBlock > 1024u ? 1024u : c.rowsPerBlock;
+                c.rowsPerBlock          = c.rowsPerBlock > SUM_ITEMS ? SUM_ITEMS : c.rowsPerBlock;
                 c.blocks                = (g.t.rows + c.rowsPerBlock - 1u) / c.rowsPerBlock;
             }
             if(blocks + c.blocks > 0x7fffffffull)
@@ -1012,7 +1124,8 @@ namespace b200wmma
             p.pieces    = g.dim / V;
             p.lanesLog2 = rowLanesLog2(p.pieces);
             p.slices    = (p.pieces + (1u << p.lanesLog2) - 1u) >> p.lanesLog2;
-            const uint64_t blocks = uint64_t(p.chunks) * p.slices;
+            const uint32_t groups = THREADS >> p.lanesLog2;
+            const uint64_t blocks = (uint64_t(p.chunks) + groups - 1u) / groups * p.slices;
             if(blocks > 0x7fffffffull)
                 return B200WMMA_ERR_TOO_LARGE;
             return cudaToStatus(launchOverlapped(joinKernel<OutT, V>, dim3(uint32_t(blocks)), dim3(THREADS), 0, stream, p));
