@@ -298,46 +298,48 @@ _CODE = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32}
 
 
 def _value_code(t, what):
-    if t.dtype not in _CODE:
+    code = _CODE.get(t.dtype)
+    if code is None:
         raise ValueError(f"{what} is {t.dtype}; float16, bfloat16 or float32 expected")
-    return _CODE[t.dtype]
+    return code
 
 
 def _tokens(ids, first):
-    """ids as [outer, inner], and the two sizes; any shape without `first`."""
-    if ids.dtype not in (torch.int32, torch.int64):
+    """(outer, inner, id bytes, outer stride, inner stride) of ids; outer x inner tokens."""
+    if ids.dtype == torch.int64:
+        size = 8
+    elif ids.dtype == torch.int32:
+        size = 4
+    else:
         raise ValueError(f"ids are {ids.dtype}; int32 or int64 expected")
+    dims = ids.dim()
     if first is not None:
-        if ids.dim() != 2 or first.dtype != torch.int64 or not first.is_contiguous() \
+        if dims != 2 or first.dtype != torch.int64 or not first.is_contiguous() \
                 or first.shape != (ids.shape[1] + 1,):
             raise ValueError("with first, ids are [outer, inner] and first inner + 1 int64 row numbers")
-    elif ids.dim() == 1:
-        ids = ids.unsqueeze(1)
-    elif ids.dim() != 2:
+    elif dims == 1:
+        return ids.shape[0], 1, size, ids.stride(0), 0
+    elif dims != 2:
         if not ids.is_contiguous():
             raise ValueError("ids of this shape must be contiguous")
-        ids = ids.view(-1, 1)
-    return ids, ids.shape[0], ids.shape[1]
+        return ids.numel(), 1, size, 1, 0
+    return (*ids.shape, size, *ids.stride())
 
 
-def _rows_view(t, ids_shape, dim, what):
-    """t [*ids.shape, dim] as [outer, inner, dim]; rows contiguous."""
-    if tuple(t.shape) != (*ids_shape, dim):
+def _rows_of(t, ids_shape, dim, what):
+    """Distances of t's rows along outer and inner, for t [*ids.shape, dim] with contiguous rows."""
+    if t.shape != (*ids_shape, dim):
         raise ValueError(f"{what} is {tuple(t.shape)}, expected {(*ids_shape, dim)}")
-    if t.dim() == 2:
-        t = t.unsqueeze(1)
-    elif t.dim() != 3:
-        if not t.is_contiguous():
-            raise ValueError(f"{what} must be contiguous for ids of this shape")
-        t = t.view(-1, 1, dim)
-    if dim > 1 and t.stride(2) != 1:
+    strides = t.stride()
+    if dim > 1 and strides[-1] != 1:
         raise ValueError(f"the rows of {what} must be contiguous")
-    return t
-
-
-def _zero(t, stream):
-    with torch.cuda.stream(stream):
-        return t.zero_()
+    if len(strides) == 3:
+        return strides[:2]
+    if len(strides) == 2:
+        return strides[0], 0
+    if not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous for ids of this shape")
+    return dim, 0
 
 
 def embedding(table, ids, scale=1.0, first=None, out_t=None, out=None, stream=None):
@@ -346,24 +348,24 @@ def embedding(table, ids, scale=1.0, first=None, out_t=None, out=None, stream=No
     first: int64 [inner + 1] on the device; ids are [outer, inner], column i counts from row
     first[i] up to first[i + 1].  out: [*ids.shape, dim], may be a strided view such as the
     rows behind the dense one of dlrm_fwd's input; out_t: its type otherwise (the table's)."""
-    if table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise ValueError("table must be [rows, dim] with contiguous rows")
     rows, dim = table.shape
+    ldt, step = table.stride()
+    if dim > 1 and step != 1:
+        raise ValueError("the rows of table must be contiguous")
     shape = ids.shape
     if out is None:
         out = _empty((*shape, dim), table.dtype if out_t is None else _TORCH.get(out_t), table.device,
                      stream)
     device = _device_of(table, ids, first, out)
-    tokens, outer, inner = _tokens(ids, first)
-    view = _rows_view(out, shape, dim, "out")
-    if any(n > 1 and not step for n, step in zip(view.shape, view.stride())):
+    outer, inner, size, ids_outer, ids_inner = _tokens(ids, first)
+    out_outer, out_inner = _rows_of(out, shape, dim, "out")
+    if (not out_outer and outer > 1) or (not out_inner and inner > 1):
         raise ValueError("out must not hold a row twice")
     kinds = _value_code(table, "table"), _value_code(out, "out")
-    if not ids.numel():
-        return out
-    _launch("b200wmma_embedding", device, stream, *kinds, rows, dim, outer, inner, table.data_ptr(),
-            table.stride(0) if rows > 1 else dim, tokens.data_ptr(), tokens.element_size(),
-            *tokens.stride(), _ptr(first), view.data_ptr(), *view.stride()[:2], scale)
+    if outer and inner:
+        _launch("b200wmma_embedding", device, stream, *kinds, rows, dim, outer, inner, table.data_ptr(),
+                ldt if rows > 1 else dim, ids.data_ptr(), size, ids_outer, ids_inner, _ptr(first),
+                out.data_ptr(), out_outer, out_inner, scale)
     return out
 
 
@@ -378,22 +380,26 @@ def embedding_grad(grad, ids, rows, out_t=None, scale=1.0, first=None, out=None,
         if accumulate:
             raise ValueError("accumulate needs out")
         out = _empty((rows, dim), grad.dtype if out_t is None else _TORCH.get(out_t), grad.device, stream)
-    if tuple(out.shape) != (rows, dim) or (dim > 1 and out.stride(1) != 1):
+    ldt, step = out.stride()
+    if out.shape != (rows, dim) or (dim > 1 and step != 1):
         raise ValueError(f"out must be {(rows, dim)} with contiguous rows")
     device = _device_of(grad, ids, first, out, workspace)
-    tokens, outer, inner = _tokens(ids, first)
-    view = _rows_view(grad, ids.shape, dim, "grad")
+    outer, inner, size, ids_outer, ids_inner = _tokens(ids, first)
+    grad_outer, grad_inner = _rows_of(grad, ids.shape, dim, "grad")
     kinds = _value_code(grad, "grad"), _value_code(out, "out")
-    if not ids.numel():
-        return out if accumulate else _zero(out, stream)
+    if not (outer and inner):
+        if not accumulate:
+            with torch.cuda.stream(stream):
+                out.zero_()
+        return out
     if workspace is None:
         workspace = _empty(L.lib().b200wmma_embedding_grad_workspace(rows, dim, outer, inner),
                            torch.uint8, grad.device, stream)
     elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
         raise ValueError("workspace must be a contiguous uint8 tensor")
-    _launch("b200wmma_embedding_grad", device, stream, *kinds, rows, dim, outer, inner, view.data_ptr(),
-            *view.stride()[:2], tokens.data_ptr(), tokens.element_size(), *tokens.stride(), _ptr(first),
-            out.data_ptr(), out.stride(0) if rows > 1 else dim, scale, bool(accumulate), workspace.data_ptr(),
+    _launch("b200wmma_embedding_grad", device, stream, *kinds, rows, dim, outer, inner, grad.data_ptr(),
+            grad_outer, grad_inner, ids.data_ptr(), size, ids_outer, ids_inner, _ptr(first),
+            out.data_ptr(), ldt if rows > 1 else dim, scale, accumulate, workspace.data_ptr(),
             workspace.numel())
     return out
 

@@ -10,11 +10,11 @@
 // is what the formats are: nothing else here rounds.  y / s is exact for MXF4 (a power of two);
 // for NVF4 see scaledBy().
 //
-// Both directions are bound by HBM: 2 + 17/32 bytes per 16-bit value.  A block of 256 threads
-// takes 128 rows x 128 columns, so that the scale tiles it makes (512 bytes each) leave whole.
+// Both directions are bound by HBM: 2 + 17/32 bytes per 16-bit value.
 #include "common.cuh"
 #include "mx_format.cuh"
 #include "rocwmma/rocwmma_block.hpp"
+#include <cstring>
 
 namespace b200wmma
 {
@@ -23,40 +23,85 @@ namespace b200wmma
 
     namespace
     {
-        constexpr uint32_t TILE_K  = 128;
-        constexpr uint32_t THREADS = 256;
+        constexpr uint32_t TILE_K    = 128;
+        constexpr uint32_t THREADS   = 256;
+        constexpr uint32_t SLAB_ROWS = 32; // rows of a block: one 32-bit word of each scale tile row
 
-        // Eight consecutive values of a row, those at and behind `left` read as zero.
-        template <typename T, bool VEC>
-        __device__ inline void load8(T const* p, uint32_t left, float (&v)[8])
+        // Eight consecutive values of a row as they are stored.
+        template <typename T>
+        struct alignas(16) Raw8
         {
-            if(VEC && left >= 8u)
-            {
-                constexpr int N = int(sizeof(T) * 8 / 16);
-                uint4         raw[N];
+            T v[8];
+        };
+        template <typename T>
+        __device__ inline Raw8<T> zero8()
+        {
+            Raw8<T> r;
 #pragma unroll
-                for(int i = 0; i < N; ++i)
-                    raw[i] = reinterpret_cast<uint4 const*>(p)[i];
-                T const* t = reinterpret_cast<T const*>(raw);
+            for(int i = 0; i < 8; ++i)
+                r.v[i] = T(0.0f);
+            return r;
+        }
+        template <typename T>
+        __device__ inline Raw8<T> load8(T const* p)
+        {
+            Raw8<T> r;
 #pragma unroll
-                for(int i = 0; i < 8; ++i)
-                    v[i] = toFloat(t[i]);
-            }
-            else
-            {
-#pragma unroll
-                for(int i = 0; i < 8; ++i)
-                    v[i] = uint32_t(i) < left ? toFloat(p[i]) : 0.0f;
-            }
+            for(int i = 0; i < int(sizeof(T) * 8 / 16); ++i)
+                reinterpret_cast<uint4*>(&r)[i] = reinterpret_cast<uint4 const*>(p)[i];
+            return r;
         }
 
-        // Largest |v| as bits: ordered like the values, a NaN above the infinity.
-        __device__ inline uint32_t topBits(float v, uint32_t top)
+        // Largest |v| of values as the bits of a float: ordered like the values, a NaN above the
+        // infinity.  16-bit types compare two magnitudes at a time, as integers.
+        template <typename T>
+        __device__ inline uint32_t wordTop(uint32_t top, T const (&v)[2])
         {
-            return max(top, __float_as_uint(v) & 0x7fffffffu);
+            uint32_t w;
+            memcpy(&w, v, 4);
+            return __vmaxu2(top, w & 0x7fff7fffu);
         }
+        __device__ inline float topFloat(uint32_t bits, __half)
+        {
+            return __half2float(__ushort_as_half(uint16_t(bits)));
+        }
+        __device__ inline float topFloat(uint32_t bits, __nv_bfloat16)
+        {
+            return __uint_as_float(bits << 16);
+        }
+        // A running maximum; merged over lanes or places, then turned into a float.
+        template <typename T>
+        struct Top
+        {
+            uint32_t bits = 0;
+            __device__ void two(T a, T b)
+            {
+                if constexpr(sizeof(T) == 2)
+                {
+                    const T v[2] = {a, b};
+                    bits         = wordTop(bits, v);
+                }
+                else
+                    bits = max(bits, max(__float_as_uint(a) & 0x7fffffffu, __float_as_uint(b) & 0x7fffffffu));
+            }
+            __device__ void lanes(uint32_t with)
+            {
+                const uint32_t other = __shfl_xor_sync(0xffffffffu, bits, with);
+                if constexpr(sizeof(T) == 2)
+                    bits = __vmaxu2(bits, other);
+                else
+                    bits = max(bits, other);
+            }
+            __device__ float value() const
+            {
+                if constexpr(sizeof(T) == 2)
+                    return topFloat(max(bits & 0xffffu, bits >> 16), T());
+                else
+                    return __uint_as_float(bits);
+            }
+        };
 
-        // The scale of a block whose largest magnitude has these bits.
+        // The scale of a block whose largest magnitude is `top`.
         struct Scale
         {
             uint32_t byte;
@@ -64,23 +109,22 @@ namespace b200wmma
             float    value;
         };
         template <bool NV>
-        __device__ inline Scale scaleOf(uint32_t top)
+        __device__ inline Scale scaleOf(float top)
         {
-            const bool fine = top < 0x7f800000u;
+            const bool fine = top < __uint_as_float(0x7f800000u); // false for a NaN
             Scale      s;
             if constexpr(NV)
             {
-                const float want = fminf(__fdiv_rn(__uint_as_float(fine ? top : 0u), 6.0f), 448.0f);
-                const uint32_t byte = toE4m3(want);
+                const uint32_t byte = toE4m3(fminf(__fdiv_rn(fine ? top : 0.0f, 6.0f), 448.0f));
                 s.value             = fromE4m3(byte);
                 s.inverse           = byte != 0u ? __frcp_rn(s.value) : 0.0f;
                 s.byte              = fine ? byte : 0x7fu;
             }
             else
             {
-                const uint32_t e    = (fine ? top : 0u) >> 23;
+                const uint32_t e    = __float_as_uint(fine ? top : 0.0f) >> 23;
                 const uint32_t byte = e > 2u ? e - 2u : 0u;
-                s.value             = fromE8m0(byte);
+                s.value             = 0.0f;
                 s.inverse           = fine ? __uint_as_float((254u - byte) << 23) : 0.0f;
                 s.byte              = fine ? byte : 255u;
             }
@@ -107,23 +151,85 @@ namespace b200wmma
                 return s.inverse != 0.0f ? __fdiv_rn(y, s.value) : 0.0f;
         }
 
-        // Inputs in which a NaN may meet an inverse of zero would make a NaN, whose code is not
-        // zero; codes of such blocks are cleared as words.
+        // Eight codes.  (A NaN or an infinity times an inverse of zero would not give codes of zero:
+        // those of such blocks are cleared as words.)
         template <typename T, bool NV>
-        __device__ inline uint32_t codes8(float const (&y)[8], Scale const& s)
+        __device__ inline uint32_t codes8(T const (&x)[8], Scale const& s, float factor)
         {
             float v[8];
 #pragma unroll
             for(int i = 0; i < 8; ++i)
-                v[i] = scaledBy<T, NV>(y[i], s);
+                v[i] = toFloat(x[i]);
+            if(factor != 1.0f)
+            {
+#pragma unroll
+                for(int i = 0; i < 8; ++i)
+                    v[i] *= factor;
+            }
+#pragma unroll
+            for(int i = 0; i < 8; ++i)
+                v[i] = scaledBy<T, NV>(v[i], s);
             const uint32_t c = e2m1x8(v);
             return s.inverse != 0.0f ? c : 0u;
         }
 
+        // Byte of (row, block) in a scale tile of its row.
         __device__ inline uint32_t scaleOffset(uint32_t row, uint32_t block)
         {
             return (block / 4u) * MX_TILE_BYTES + (row % 32u) * 16u + (row / 32u % 4u) * 4u
                    + block % 4u;
+        }
+
+        // A row of a tile whose values do not start on 16-byte boundaries in global memory passes
+        // through shared memory, where it lies as far from a boundary as it does there: whole
+        // 16-byte pieces move as such, only those that the row shares with its neighbours or with
+        // the next tile move value by value.
+        template <typename T>
+        struct StagedRow
+        {
+            static constexpr uint32_t PER   = 16 / sizeof(T); // values of a piece
+            static constexpr uint32_t PITCH = (TILE_K + PER) * sizeof(T);
+            static constexpr uint32_t PIECES = TILE_K / PER + 1u;
+
+            static __device__ uint32_t shift(T const* row)
+            {
+                return uint32_t(reinterpret_cast<uintptr_t>(row) % 16u) / uint32_t(sizeof(T));
+            }
+        };
+        // Threads of the block move rows of `count` values, row r of the tile at global(r), to or
+        // from shared memory.
+        template <typename T, bool LOAD, typename Row>
+        __device__ inline void moveStaged(uint8_t* staged, uint32_t rows, uint32_t count, Row global)
+        {
+            using S = StagedRow<T>;
+            for(uint32_t i = threadIdx.x; i < rows * S::PIECES; i += THREADS)
+            {
+                const uint32_t r = i / S::PIECES, piece = i % S::PIECES;
+                T*             row   = global(r);
+                const uint32_t shift = S::shift(row);
+                const uint32_t first = piece * S::PER; // of the piece, counted from the boundary
+                T*             here  = reinterpret_cast<T*>(staged + r * S::PITCH) + first;
+                T*             there = row + (int32_t(first) - int32_t(shift));
+                if(first >= shift && first + S::PER <= shift + count)
+                {
+                    if(LOAD)
+                        *reinterpret_cast<uint4*>(here) = *reinterpret_cast<uint4 const*>(there);
+                    else
+                        *reinterpret_cast<uint4*>(there) = *reinterpret_cast<uint4 const*>(here);
+                }
+                else
+                {
+#pragma unroll
+                    for(uint32_t j = 0; j < S::PER; ++j)
+                        if(first + j >= shift && first + j < shift + count)
+                        {
+                            if(LOAD)
+                                here[j] = there[j];
+                            else
+                                there[j] = here[j];
+                        }
+                }
+            }
         }
 
         struct QuantizeParams
@@ -137,74 +243,105 @@ namespace b200wmma
             float       factor; // 2^-exponent
         };
 
-        // The scale tiles of one 128 x 128 tile, from shared memory, whole.
-        template <bool NV>
-        __device__ inline void storeScales(QuantizeParams const& p, uint8_t const* scales,
-                                           uint32_t tileRow, uint32_t tileK)
-        {
-            constexpr uint32_t GROUPS = TILE_K / (4u * mxBlock(NV));
-            const uint32_t     at     = threadIdx.x * 16u;
-            const uint32_t     group  = tileK * GROUPS + at / MX_TILE_BYTES;
-            if(at < GROUPS * MX_TILE_BYTES && group < p.groups)
-                *reinterpret_cast<uint4*>(p.scales + (uint64_t(tileRow) * p.groups + group) * MX_TILE_BYTES
-                                          + at % MX_TILE_BYTES)
-                    = *reinterpret_cast<uint4 const*>(scales + at);
-        }
-
-        // x row-major: k is contiguous.  Sixteen threads read 128 values of a row, eight each;
-        // a block's largest magnitude comes from its two (NVF4) or four (MXF4) threads.
+        // x row-major: k is contiguous.  A block takes 32 rows x 128 columns: sixteen threads read
+        // 128 values of a row, eight each, and a block's largest magnitude comes from its two
+        // (NVF4) or four (MXF4) threads; those with the scales of four blocks write them as a word.
         template <typename T, bool NV, bool VEC>
         __global__ void __launch_bounds__(THREADS) quantizeRowsKernel(const QuantizeParams p)
         {
+            constexpr int      STEPS  = SLAB_ROWS / (THREADS / 16);
             constexpr uint32_t GROUPS = TILE_K / (4u * mxBlock(NV));
-            constexpr int      STEPS  = 128 / (THREADS / 16);
-            __shared__ alignas(16) uint8_t scales[GROUPS * MX_TILE_BYTES];
-            const uint32_t tileRow = blockIdx.x / p.tilesK, tileK = blockIdx.x % p.tilesK;
+            const uint32_t slab = blockIdx.x / p.tilesK, tileK = blockIdx.x % p.tilesK;
             const uint32_t col = threadIdx.x % 16u * 8u, rowIn = threadIdx.x / 16u;
-            const uint32_t k0 = tileK * TILE_K + col;
-            const uint32_t left = k0 < p.k ? p.k - k0 : 0u;
+            const uint32_t k0   = tileK * TILE_K + col, count = min(TILE_K, p.k - tileK * TILE_K);
+            const uint64_t row0 = uint64_t(slab) * SLAB_ROWS;
+            const uint32_t rows = row0 < p.rows ? uint32_t(min(uint64_t(SLAB_ROWS), p.rows - row0)) : 0u;
+            T const*       x    = static_cast<T const*>(p.x) + row0 * p.ldx + tileK * TILE_K;
             grid_dependency_wait();
             grid_launch_dependents();
-#pragma unroll
-            for(int half = 0; half < 2; ++half)
+            Raw8<T> raw[STEPS];
+            if constexpr(VEC)
             {
-                float y[STEPS / 2][8];
-#pragma unroll
-                for(int i = 0; i < STEPS / 2; ++i)
+                if(rows == SLAB_ROWS && count == TILE_K)
                 {
-                    const uint64_t row = uint64_t(tileRow) * 128u + (half * (STEPS / 2) + i) * 16u + rowIn;
-                    load8<T, VEC>(static_cast<T const*>(p.x) + row * p.ldx + k0, row < p.rows ? left : 0u, y[i]);
+#pragma unroll
+                    for(int i = 0; i < STEPS; ++i)
+                        raw[i] = load8(x + (i * 16u + rowIn) * p.ldx + col);
                 }
-#pragma unroll
-                for(int i = 0; i < STEPS / 2; ++i)
+                else
                 {
-                    const uint32_t r   = (half * (STEPS / 2) + i) * 16u + rowIn;
-                    const uint64_t row = uint64_t(tileRow) * 128u + r;
-                    uint32_t       top = 0;
 #pragma unroll
-                    for(int j = 0; j < 8; ++j)
+                    for(int i = 0; i < STEPS; ++i)
                     {
-                        y[i][j] *= p.factor;
-                        top = topBits(y[i][j], top);
+                        const uint32_t r = i * 16u + rowIn;
+                        T const*       at = x + r * p.ldx + col;
+                        raw[i]            = zero8<T>();
+                        if(r < rows && col + 8u <= count)
+                            raw[i] = load8(at);
+                        else if(r < rows)
+                        {
+#pragma unroll
+                            for(uint32_t j = 0; j < 8u; ++j)
+                                if(col + j < count)
+                                    raw[i].v[j] = at[j];
+                        }
                     }
-                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    if constexpr(!NV)
-                        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    const Scale    s    = scaleOf<NV>(top);
-                    const uint32_t code = codes8<T, NV>(y[i], s);
-                    if(col % mxBlock(NV) == 0u)
-                        scales[scaleOffset(r, col / mxBlock(NV))] = uint8_t(s.byte);
-                    if(row < p.rows && k0 / 2u < mxPitch(p.k))
-                        *reinterpret_cast<uint32_t*>(p.codes + row * p.ldq + k0 / 2u) = code;
                 }
             }
-            __syncthreads();
-            storeScales<NV>(p, scales, tileRow, tileK);
+            else
+            {
+                __shared__ alignas(16) uint8_t staged[SLAB_ROWS * StagedRow<T>::PITCH];
+                auto rowAt = [&](uint32_t r) { return const_cast<T*>(x) + r * p.ldx; };
+                moveStaged<T, true>(staged, rows, count, rowAt);
+                __syncthreads();
+#pragma unroll
+                for(int i = 0; i < STEPS; ++i)
+                {
+                    const uint32_t r = i * 16u + rowIn;
+                    raw[i]           = zero8<T>();
+                    if(r < rows)
+                    {
+                        T const* at = reinterpret_cast<T const*>(staged + r * StagedRow<T>::PITCH)
+                                      + StagedRow<T>::shift(rowAt(r)) + col;
+#pragma unroll
+                        for(uint32_t j = 0; j < 8u; ++j)
+                            if(col + j < count)
+                                raw[i].v[j] = at[j];
+                    }
+                }
+            }
+#pragma unroll
+            for(int i = 0; i < STEPS; ++i)
+            {
+                const uint32_t r = i * 16u + rowIn;
+                Top<T>         top;
+#pragma unroll
+                for(int j = 0; j < 8; j += 2)
+                    top.two(raw[i].v[j], raw[i].v[j + 1]);
+                top.lanes(1);
+                if constexpr(!NV)
+                    top.lanes(2);
+                const Scale    s    = scaleOf<NV>(top.value() * p.factor);
+                const uint32_t code = codes8<T, NV>(raw[i].v, s, p.factor);
+                if(r < rows && k0 / 2u < mxPitch(p.k))
+                    *reinterpret_cast<uint32_t*>(p.codes + (row0 + r) * p.ldq + k0 / 2u) = code;
+                // the bytes of four blocks, a word of the scale tile's row
+                constexpr uint32_t LANES = mxBlock(NV) / 8u; // of a block
+                uint32_t           word  = s.byte << (8u * (threadIdx.x / LANES % 4u));
+                word |= __shfl_xor_sync(0xffffffffu, word, LANES);
+                word |= __shfl_xor_sync(0xffffffffu, word, 2u * LANES);
+                const uint32_t group = tileK * GROUPS + col / (4u * mxBlock(NV));
+                if(threadIdx.x % (4u * LANES) == 0u && group < p.groups)
+                    *reinterpret_cast<uint32_t*>(p.scales + (uint64_t(slab / 4u) * p.groups + group) * MX_TILE_BYTES
+                                                 + scaleOffset(slab % 4u * SLAB_ROWS + r, 0))
+                        = word;
+            }
         }
 
-        // x column-major: the rows are contiguous.  A thread takes two neighbouring rows and 32
-        // values of k of each, so that a warp reads 64 consecutive values at a time and no
-        // maximum crosses a thread; the codes pass through shared memory to leave as rows.
+        // x column-major: the rows are contiguous.  A block takes 128 rows x 128 columns, a thread
+        // two neighbouring rows and 32 values of k of each, so that a warp reads 64 consecutive
+        // values at a time and no maximum crosses a thread; the codes pass through shared memory
+        // to leave as rows, the scale tiles to leave whole.
         template <typename T, bool NV, bool VEC>
         __global__ void __launch_bounds__(THREADS) quantizeColumnsKernel(const QuantizeParams p)
         {
@@ -213,38 +350,39 @@ namespace b200wmma
             constexpr uint32_t PITCH  = 80; // of a staged row: 64 bytes of codes, 16 of padding
             __shared__ alignas(16) uint8_t scales[GROUPS * MX_TILE_BYTES];
             __shared__ alignas(16) uint8_t staged[128 * PITCH];
+            struct alignas(2 * sizeof(T)) Pair
+            {
+                T v[2];
+            };
             const uint32_t tileRow = blockIdx.x / p.tilesK, tileK = blockIdx.x % p.tilesK;
             const uint32_t r = threadIdx.x % 64u * 2u, kIn = threadIdx.x / 64u * 32u;
             const uint64_t row = uint64_t(tileRow) * 128u + r;
             const uint32_t k0  = tileK * TILE_K + kIn;
+            const uint32_t count = k0 < p.k ? min(32u, p.k - k0) : 0u;
             grid_dependency_wait();
             grid_launch_dependents();
-            T        v[32][2];
-            T const* x = static_cast<T const*>(p.x) + row;
+            Pair     v[32];
+            T const* x = static_cast<T const*>(p.x) + row + uint64_t(k0) * p.ldx;
 #pragma unroll
-            for(int i = 0; i < 32; ++i)
+            for(uint32_t i = 0; i < 32u; ++i)
+                v[i].v[0] = v[i].v[1] = T(0.0f);
+            if(VEC && row + 1u < p.rows)
             {
-                const bool in = k0 < p.k && uint32_t(i) < p.k - k0;
-                T const*   at = x + (uint64_t(k0) + uint32_t(i)) * p.ldx;
-                if constexpr(VEC)
+#pragma unroll
+                for(uint32_t i = 0; i < 32u; ++i)
+                    if(i < count)
+                        v[i] = *reinterpret_cast<Pair const*>(x + i * p.ldx);
+            }
+            else
+            {
+                const bool one = row < p.rows, two = row + 1u < p.rows;
+#pragma unroll
+                for(uint32_t i = 0; i < 32u; ++i)
                 {
-                    using Pair = typename std::conditional<sizeof(T) == 2, uint32_t, uint2>::type;
-                    Pair w{};
-                    if(in && row + 1u < p.rows)
-                        w = *reinterpret_cast<Pair const*>(at);
-                    else if(in && row < p.rows)
-                    {
-                        const T one[2] = {at[0], T(0.0f)};
-                        w              = *reinterpret_cast<Pair const*>(one);
-                    }
-                    const T* pair = reinterpret_cast<T const*>(&w);
-                    v[i][0]       = pair[0];
-                    v[i][1]       = pair[1];
-                }
-                else
-                {
-                    v[i][0] = in && row < p.rows ? at[0] : T(0.0f);
-                    v[i][1] = in && row + 1u < p.rows ? at[1] : T(0.0f);
+                    if(i < count && one)
+                        v[i].v[0] = x[i * p.ldx];
+                    if(i < count && two)
+                        v[i].v[1] = x[i * p.ldx + 1u];
                 }
             }
 #pragma unroll
@@ -254,19 +392,19 @@ namespace b200wmma
 #pragma unroll
                 for(int b = 0; b < 32 / B; ++b)
                 {
-                    uint32_t top = 0;
+                    Top<T> top;
 #pragma unroll
-                    for(int i = 0; i < B; ++i)
-                        top = topBits(toFloat(v[b * B + i][j]) * p.factor, top);
-                    const Scale s = scaleOf<NV>(top);
+                    for(int i = 0; i < B; i += 2)
+                        top.two(v[b * B + i].v[j], v[b * B + i + 1].v[j]);
+                    const Scale s = scaleOf<NV>(top.value() * p.factor);
 #pragma unroll
                     for(int w = 0; w < B / 8; ++w)
                     {
-                        float y[8];
+                        T y[8];
 #pragma unroll
                         for(int i = 0; i < 8; ++i)
-                            y[i] = toFloat(v[b * B + w * 8 + i][j]) * p.factor;
-                        words[b * (B / 8) + w] = codes8<T, NV>(y, s);
+                            y[i] = v[b * B + w * 8 + i].v[j];
+                        words[b * (B / 8) + w] = codes8<T, NV>(y, s, p.factor);
                     }
                     scales[scaleOffset(r + j, kIn / B + b)] = uint8_t(s.byte);
                 }
@@ -274,9 +412,16 @@ namespace b200wmma
                     = make_uint4(words[0], words[1], words[2], words[3]);
             }
             __syncthreads();
-            storeScales<NV>(p, scales, tileRow, tileK);
+            {
+                const uint32_t at = threadIdx.x * 16u, group = tileK * GROUPS + at / MX_TILE_BYTES;
+                if(at < GROUPS * MX_TILE_BYTES && group < p.groups)
+                    *reinterpret_cast<uint4*>(p.scales + (uint64_t(tileRow) * p.groups + group) * MX_TILE_BYTES
+                                              + at % MX_TILE_BYTES)
+                        = *reinterpret_cast<uint4 const*>(scales + at);
+            }
             // four threads a row
             const uint64_t pitch = mxPitch(p.k);
+#pragma unroll
             for(uint32_t i = threadIdx.x; i < 128u * 4u; i += THREADS)
             {
                 const uint32_t rr = i / 4u;
@@ -299,60 +444,86 @@ namespace b200wmma
             float          factor; // 2^exponent
         };
 
+        // A block takes 32 rows x 128 columns, a thread eight codes of two rows.
         template <typename T, bool NV, bool VEC>
         __global__ void __launch_bounds__(THREADS) dequantizeKernel(const DequantizeParams p)
         {
-            constexpr int  STEPS   = 128 / (THREADS / 16);
-            const uint32_t tileRow = blockIdx.x / p.tilesK, tileK = blockIdx.x % p.tilesK;
-            const uint32_t k0 = tileK * TILE_K + threadIdx.x % 16u * 8u, rowIn = threadIdx.x / 16u;
+            constexpr int  STEPS = SLAB_ROWS / (THREADS / 16);
+            const uint32_t slab = blockIdx.x / p.tilesK, tileK = blockIdx.x % p.tilesK;
+            const uint32_t col = threadIdx.x % 16u * 8u, rowIn = threadIdx.x / 16u;
+            const uint32_t k0   = tileK * TILE_K + col, count = min(TILE_K, p.k - tileK * TILE_K);
+            const uint64_t row0 = uint64_t(slab) * SLAB_ROWS;
+            const uint32_t rows = row0 < p.rows ? uint32_t(min(uint64_t(SLAB_ROWS), p.rows - row0)) : 0u;
+            T*             out  = static_cast<T*>(p.out) + row0 * p.ldo + tileK * TILE_K;
             grid_dependency_wait();
             grid_launch_dependents();
-            if(k0 >= p.k)
-                return;
             uint32_t word[STEPS], byte[STEPS];
 #pragma unroll
             for(int i = 0; i < STEPS; ++i)
             {
-                const uint32_t r   = i * 16u + rowIn;
-                const uint64_t row = uint64_t(tileRow) * 128u + r;
+                const uint32_t r = i * 16u + rowIn;
                 word[i] = byte[i] = 0;
-                if(row < p.rows)
+                if(r < rows && col < count)
                 {
-                    word[i] = *reinterpret_cast<uint32_t const*>(p.codes + row * p.ldq + k0 / 2u);
-                    byte[i] = p.scales[uint64_t(tileRow) * p.groups * MX_TILE_BYTES
-                                       + uint64_t(k0 / mxBlock(NV) / 4u) * MX_TILE_BYTES
-                                       + scaleOffset(r, k0 / mxBlock(NV) % 4u)];
+                    word[i] = *reinterpret_cast<uint32_t const*>(p.codes + (row0 + r) * p.ldq + k0 / 2u);
+                    byte[i] = p.scales[(uint64_t(slab / 4u) * p.groups + k0 / mxBlock(NV) / 4u) * MX_TILE_BYTES
+                                       + scaleOffset(slab % 4u * SLAB_ROWS + r, k0 / mxBlock(NV) % 4u)];
                 }
             }
-#pragma unroll
-            for(int i = 0; i < STEPS; ++i)
-            {
-                const uint64_t row = uint64_t(tileRow) * 128u + i * 16u + rowIn;
-                if(row >= p.rows)
-                    continue;
+            auto values = [&](int i) {
                 // code * s is exact (three bits times at most four); so is the power of two,
                 // short of the subnormals
                 const float s = NV ? fromE4m3(byte[i]) : fromE8m0(byte[i]);
                 float       v[8];
                 e2m1x8ToFloat(word[i], v);
-                alignas(16) T out[8];
+                Raw8<T> o;
 #pragma unroll
                 for(int j = 0; j < 8; ++j)
-                    out[j] = fromFloat<T>(v[j] * s * p.factor);
-                T* at = static_cast<T*>(p.out) + row * p.ldo + k0;
-                if(VEC && k0 + 8u <= p.k)
-                {
+                    o.v[j] = fromFloat<T>(v[j] * s * p.factor);
+                return o;
+            };
+            if constexpr(VEC)
+            {
 #pragma unroll
-                    for(int j = 0; j < int(sizeof(T) * 8 / 16); ++j)
-                        reinterpret_cast<uint4*>(at)[j] = reinterpret_cast<uint4 const*>(out)[j];
-                }
-                else
+                for(int i = 0; i < STEPS; ++i)
                 {
+                    const uint32_t r  = i * 16u + rowIn;
+                    const Raw8<T>  o  = values(i);
+                    T*             at = out + r * p.ldo + col;
+                    if(r < rows && col + 8u <= count)
+                    {
 #pragma unroll
-                    for(int j = 0; j < 8; ++j)
-                        if(k0 + j < p.k)
-                            at[j] = out[j];
+                        for(int j = 0; j < int(sizeof(T) * 8 / 16); ++j)
+                            reinterpret_cast<uint4*>(at)[j] = reinterpret_cast<uint4 const*>(&o)[j];
+                    }
+                    else if(r < rows)
+                    {
+#pragma unroll
+                        for(uint32_t j = 0; j < 8u; ++j)
+                            if(col + j < count)
+                                at[j] = o.v[j];
+                    }
                 }
+            }
+            else
+            {
+                __shared__ alignas(16) uint8_t staged[SLAB_ROWS * StagedRow<T>::PITCH];
+                auto rowAt = [&](uint32_t r) { return out + r * p.ldo; };
+#pragma unroll
+                for(int i = 0; i < STEPS; ++i)
+                {
+                    const uint32_t r = i * 16u + rowIn;
+                    const Raw8<T>  o = values(i);
+                    if(r < rows)
+                    {
+                        T* at = reinterpret_cast<T*>(staged + r * StagedRow<T>::PITCH) + StagedRow<T>::shift(rowAt(r)) + col;
+#pragma unroll
+                        for(int j = 0; j < 8; ++j)
+                            at[j] = o.v[j];
+                    }
+                }
+                __syncthreads();
+                moveStaged<T, false>(staged, rows, count, rowAt);
             }
         }
 
@@ -364,11 +535,12 @@ namespace b200wmma
         template <typename T>
         int quantize(bool nv, bool columns, QuantizeParams const& p, uint32_t blocks, cudaStream_t stream)
         {
-            // Wide loads where every row (or pair of rows) starts on their boundary.
+            // Wide loads where every row (or pair of rows) starts on their boundary.  A block takes
+            // 32 rows (rows contiguous along k) or 128; `blocks` counts tiles of 128.
             const uint64_t width = columns ? 2 * sizeof(T) : 16;
             const bool     vec   = aligned(p.x, width) && p.ldx * sizeof(T) % width == 0;
             auto launch = [&](auto kernel) {
-                return cudaToStatus(launchOverlapped(kernel, dim3(blocks), dim3(THREADS), 0, stream, p));
+                return cudaToStatus(launchOverlapped(kernel, dim3(columns ? blocks : 4u * blocks), dim3(THREADS), 0, stream, p));
             };
             if(columns)
                 return nv ? (vec ? launch(quantizeColumnsKernel<T, true, true>) : launch(quantizeColumnsKernel<T, true, false>))
@@ -381,8 +553,10 @@ namespace b200wmma
         int dequantize(bool nv, DequantizeParams const& p, uint32_t blocks, cudaStream_t stream)
         {
             const bool vec = aligned(p.out, 16) && p.ldo * sizeof(T) % 16 == 0;
+            // a block takes 32 rows; slabs without a row have nothing to do
+            const uint32_t slabs = blocks / p.tilesK * 4u - (p.rows % 128u ? (127u - (p.rows - 1u) % 128u) / 32u : 0u);
             auto launch = [&](auto kernel) {
-                return cudaToStatus(launchOverlapped(kernel, dim3(blocks), dim3(THREADS), 0, stream, p));
+                return cudaToStatus(launchOverlapped(kernel, dim3(slabs * p.tilesK), dim3(THREADS), 0, stream, p));
             };
             return nv ? (vec ? launch(dequantizeKernel<T, true, true>) : launch(dequantizeKernel<T, true, false>))
                       : (vec ? launch(dequantizeKernel<T, false, true>) : launch(dequantizeKernel<T, false, false>));
@@ -401,7 +575,7 @@ namespace b200wmma
             if(!aligned(codes, 16) || !aligned(scales, 16) || ldq % 16 || !aligned(values, dtypeSize(dtype)))
                 return B200WMMA_ERR_ALIGNMENT;
             *blocks = uint64_t(mxRowTiles(rows)) * ((uint64_t(k) + TILE_K - 1) / TILE_K);
-            if(*blocks > 0x7fffffffull)
+            if(*blocks > 0x1fffffffull)
                 return B200WMMA_ERR_TOO_LARGE;
             return B200WMMA_OK;
         }
