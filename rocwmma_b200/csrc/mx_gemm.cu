@@ -26,7 +26,7 @@ namespace b200wmma
         constexpr uint32_t NUM_THREADS = 192;
         constexpr uint32_t EPI_THREADS = 128;
         constexpr uint32_t MAX_STAGES  = 8;
-        constexpr uint32_t PREFETCH_SLOTS = 16; // of a block's stretch, requested into L2 ahead
+        constexpr uint32_t PREFETCH_SLOTS = 8; // of a block's stretch, requested into L2 ahead
         constexpr long long SETTLE_CYCLES = 2000000; // leaving early: copies in flight land
 
         struct Params
@@ -42,6 +42,30 @@ namespace b200wmma
         constexpr uint32_t slotGroups() // scale tiles of 128 rows in a ring slot
         {
             return KIND == ScaleKind::E4M3_16 ? 4u : 2u;
+        }
+
+        // Loads and MMAs are issued by one thread each, whose instructions follow one another at four
+        // or more cycles: a division by the ring's depth, or a descriptor put together anew, costs as
+        // much as an MMA.  So slots are counted with a position that wraps, and descriptors are one
+        // 32-bit sum (their upper halves never change).
+        struct RingPosition
+        {
+            uint32_t slot = 0, phase = 0, offset = 0; // offset of the slot in shared memory
+            __device__ void next(uint32_t stages, uint32_t slotBytes)
+            {
+                ++slot;
+                offset += slotBytes;
+                if(slot == stages)
+                {
+                    slot   = 0;
+                    offset = 0;
+                    phase ^= 1u;
+                }
+            }
+        };
+        __device__ inline uint64_t descAt(uint64_t base, uint32_t bytes)
+        {
+            return (base & 0xffffffff00000000ull) | (uint32_t(base) + (bytes >> 4));
         }
 
         // alpha and beta as everywhere in this library: a rounded product each, a rounded sum.
@@ -77,6 +101,8 @@ namespace b200wmma
             uint64_t    cRow, cThin, dRow, dThin; // distance of neighbouring elements of C and D along each
             float       alpha, beta;
             uint32_t    nq, parts, stages, slotBytes, tmemCols;
+            void const* r; // codes of the streamed operand, for requests ahead
+            uint64_t    ldr;
             uint32_t*   status;
         };
         struct ThinControl
@@ -89,6 +115,35 @@ namespace b200wmma
         __device__ inline void storeCluster(uint32_t addr, uint32_t v)
         {
             asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+        }
+
+        // Four neighbouring elements of D, or the first `count` of them.  `wide`: D and C lie on the
+        // boundary of four.
+        template <typename OutT>
+        __device__ inline void putFour(OutT* d, OutT const* c, ThinParams const& p, bool wide, uint32_t count, float4 acc)
+        {
+            struct alignas(4 * sizeof(OutT)) Four
+            {
+                OutT v[4];
+            };
+            const float a[4] = {acc.x, acc.y, acc.z, acc.w};
+            if(wide && count >= 4u)
+            {
+                Four o;
+                if(c)
+                    o = *reinterpret_cast<Four const*>(c);
+#pragma unroll
+                for(int i = 0; i < 4; ++i)
+                    o.v[i] = finish<OutT>(a[i], p.alpha, p.beta, c ? &o.v[i] : nullptr);
+                *reinterpret_cast<Four*>(d) = o;
+            }
+            else
+            {
+#pragma unroll
+                for(uint32_t i = 0; i < 4u; ++i)
+                    if(i < count)
+                        d[i] = finish<OutT>(a[i], p.alpha, p.beta, c ? c + i : nullptr);
+            }
         }
 
         template <ScaleKind KIND, typename OutT>
@@ -127,13 +182,20 @@ namespace b200wmma
                 tma_prefetch_descriptor(&mapScaleR);
                 tma_prefetch_descriptor(&mapScaleQ);
             }
-            else if(threadIdx.x == 64u)
+            else if(warp >= 2u)
             {
                 // The streamed operand's first slots are requested into L2 while the previous
                 // kernel of the stream (often the quantisation of the thin operand) still runs: a
                 // request reads nothing into the SM, and L2 is where a late write would land too.
-                for(uint32_t it = 0; it < numSlots && it < PREFETCH_SLOTS; ++it)
-                    tma_prefetch_l2_2d(&mapR, int32_t((slot0 + it) * 128u), int32_t(tile * ROW_TILE));
+                // (Not by TMA: the loads would queue up behind the requests, 1 us for 16 slots.)
+                const uint64_t row = uint64_t(tile) * ROW_TILE + threadIdx.x - 64u;
+                if(row < p.rows)
+                    for(uint32_t it = 0; it < numSlots && it < PREFETCH_SLOTS; ++it)
+                    {
+                        const uint64_t at = uint64_t(slot0 + it) * 128u;
+                        if(at * 2u < p.k)
+                            prefetch_l2(static_cast<uint8_t const*>(p.r) + row * p.ldr + at);
+                    }
             }
             __syncwarp();
             if(warp == 1)
@@ -152,23 +214,23 @@ namespace b200wmma
             {
                 if(elect_one())
                 {
-                    for(uint32_t it = 0; it < numSlots; ++it)
+                    RingPosition at;
+                    int32_t      x = int32_t(slot0 * 128u), group = int32_t(slot0 * GROUPS);
+                    for(uint32_t it = 0; it < numSlots; ++it, x += 128, group += int32_t(GROUPS))
                     {
-                        const uint32_t s = it % p.stages, ph = (it / p.stages) & 1u;
-                        if(!mbar_wait(&ctl->empty[s], ph ^ 1u, &ctl->abort, WAIT_STAGE_EMPTY))
+                        uint64_t* full = &ctl->full[at.slot];
+                        if(!mbar_wait(&ctl->empty[at.slot], at.phase ^ 1u, &ctl->abort, WAIT_STAGE_EMPTY))
                         {
                             settle();
                             break;
                         }
-                        uint8_t*       slot   = ring + s * p.slotBytes;
-                        uint8_t*       scales = slot + CODE_BYTES + qBytes;
-                        const uint32_t at     = slot0 + it;
-                        mbar_expect_tx(&ctl->full[s], p.slotBytes);
-                        tma_load_2d(slot, &mapR, &ctl->full[s], int32_t(at * 128u), int32_t(tile * ROW_TILE));
-                        tma_load_2d(slot + CODE_BYTES, &mapQ, &ctl->full[s], int32_t(at * 128u), 0);
-                        tma_load_3d(scales, &mapScaleR, &ctl->full[s], 0, int32_t(at * GROUPS), int32_t(tile));
-                        tma_load_3d(scales + GROUPS * MX_TILE_BYTES, &mapScaleQ, &ctl->full[s], 0,
-                                    int32_t(at * GROUPS), 0);
+                        uint8_t* slot = ring + at.offset;
+                        mbar_expect_tx(full, p.slotBytes);
+                        tma_load_2d(slot, &mapR, full, x, int32_t(tile * ROW_TILE));
+                        tma_load_2d(slot + CODE_BYTES, &mapQ, full, x, 0);
+                        tma_load_3d(slot + CODE_BYTES + qBytes, &mapScaleR, full, 0, group, int32_t(tile));
+                        tma_load_3d(slot + CODE_BYTES + qBytes + GROUPS * MX_TILE_BYTES, &mapScaleQ, full, 0, group, 0);
+                        at.next(p.stages, p.slotBytes);
                     }
                 }
             }
@@ -178,114 +240,157 @@ namespace b200wmma
                 {
                     // accumulator, then the scales of two ring slots in turn
                     const uint32_t scaleCols = 4u * GROUPS * (1u + tilesOfQ);
-                    const uint32_t scale0    = tmem + (p.nq + 31u) / 32u * 32u;
-                    bool           ok        = true;
-                    for(uint32_t it = 0; it < numSlots; ++it)
+                    uint32_t       scale = tmem + (p.nq + 31u) / 32u * 32u, otherScale = scale + scaleCols;
+                    const uint32_t base  = smem_addr(ring);
+                    const uint64_t descR = smem_desc_kmajor_sw128(base), descQ = descAt(descR, CODE_BYTES);
+                    const uint64_t descS = smem_desc_scales(base + CODE_BYTES + qBytes);
+                    const uint32_t idesc = make_instr_desc_scaled(KIND, ROW_TILE, p.nq, 0);
+                    RingPosition   at;
+                    uint32_t       left = p.k - slot0 * SLOT_K, more = 0;
+                    bool           ok = true;
+                    for(uint32_t it = 0; it < numSlots; ++it, left -= SLOT_K)
                     {
-                        const uint32_t s = it % p.stages, ph = (it / p.stages) & 1u;
-                        if(!mbar_wait(&ctl->full[s], ph, &ctl->abort, WAIT_STAGE_FULL))
+                        if(!mbar_wait(&ctl->full[at.slot], at.phase, &ctl->abort, WAIT_STAGE_FULL))
                         {
                             ok = false;
                             break;
                         }
                         tc_fence_after_sync();
-                        const uint32_t rAddr = smem_addr(ring + s * p.slotBytes);
-                        const uint32_t qAddr = rAddr + CODE_BYTES, sAddr = qAddr + qBytes;
-                        const uint32_t scaleR = scale0 + (it & 1u) * scaleCols;
-                        const uint32_t scaleQ = scaleR + 4u * GROUPS;
-                        const uint32_t left   = p.k - (slot0 + it) * SLOT_K;
-                        const uint32_t steps  = left >= SLOT_K ? SLOT_K / MMA_K : (left + MMA_K - 1) / MMA_K;
+                        const uint64_t dS = descAt(descS, at.offset);
+#pragma unroll
                         for(uint32_t g = 0; g < GROUPS; ++g)
                         {
-                            tmem_copy_scales(scaleR + 4u * g, smem_desc_scales(sAddr + g * MX_TILE_BYTES));
-                            for(uint32_t t = 0; t < tilesOfQ; ++t)
-                                tmem_copy_scales(scaleQ + 4u * (g * tilesOfQ + t),
-                                                 smem_desc_scales(sAddr + (GROUPS * (1u + t) + g) * MX_TILE_BYTES));
+                            tmem_copy_scales(scale + 4u * g, descAt(dS, g * MX_TILE_BYTES));
+                            if(tilesOfQ == 1u)
+                                tmem_copy_scales(scale + 4u * (GROUPS + g), descAt(dS, (GROUPS + g) * MX_TILE_BYTES));
+                            else
+                                for(uint32_t t = 0; t < tilesOfQ; ++t)
+                                    tmem_copy_scales(scale + 4u * (GROUPS + g * tilesOfQ + t),
+                                                     descAt(dS, (GROUPS * (1u + t) + g) * MX_TILE_BYTES));
                         }
-                        for(uint32_t ks = 0; ks < steps; ++ks)
-                        {
+                        const uint64_t dR = descAt(descR, at.offset), dQ = descAt(descQ, at.offset);
+                        auto step = [&](uint32_t ks) {
                             // MXF4 takes a tile's four scales in two steps, NVF4 in one
                             const uint32_t g  = KIND == ScaleKind::E4M3_16 ? ks : ks / 2u;
                             const uint32_t id = KIND == ScaleKind::E4M3_16 ? 0u : (ks & 1u) * 2u;
-                            mma_scaled<KIND>(tmem, smem_desc_kmajor_sw128(rAddr + ks * 32u),
-                                             smem_desc_kmajor_sw128(qAddr + ks * 32u),
-                                             make_instr_desc_scaled(KIND, ROW_TILE, p.nq, id),
-                                             scaleR + 4u * g, scaleQ + 4u * g * tilesOfQ,
-                                             (it > 0u || ks > 0u) ? 1u : 0u);
+                            mma_scaled<KIND>(tmem, descAt(dR, ks * 32u), descAt(dQ, ks * 32u), idesc | id << 4 | id << 29,
+                                             scale + 4u * g, scale + 4u * (GROUPS + g * tilesOfQ), more);
+                            more = 1;
+                        };
+                        if(left >= SLOT_K)
+                        {
+#pragma unroll
+                            for(uint32_t ks = 0; ks < SLOT_K / MMA_K; ++ks)
+                                step(ks);
                         }
-                        mma_commit(&ctl->empty[s]);
+                        else
+                            for(uint32_t ks = 0; ks * MMA_K < left; ++ks)
+                                step(ks);
+                        mma_commit(&ctl->empty[at.slot]);
+                        const uint32_t swap = scale;
+                        scale               = otherScale;
+                        otherScale          = swap;
+                        at.next(p.stages, p.slotBytes);
                     }
                     if(ok)
                         mma_commit(&ctl->accFull);
                 }
             }
 
-            // lanes hold rows of the streamed operand, registers rows of the thin one
+            // Every block puts its sums, as [part][thin row of the share][row of the tile], into the
+            // ring of the block that finishes them (a lane has a row of the tile, registers hold thin
+            // rows); then four values that D has side by side are one thread's.
             const bool     drains = warp >= 2u;
-            const uint32_t inTile = warp % 4u * 32u + lane;
-            const uint64_t row    = uint64_t(tile) * ROW_TILE + inTile;
-            const uint32_t taddr  = tmem + ((warp % 4u * 32u) << 16);
-            const uint32_t share  = p.nq / p.parts; // thin rows that this block finishes
-            auto           put    = [&](uint32_t q, float acc) {
-                if(row < p.rows && q < p.thin)
-                {
-                    OutT const* c = p.c ? static_cast<OutT const*>(p.c) + row * p.cRow + q * p.cThin : nullptr;
-                    static_cast<OutT*>(p.d)[row * p.dRow + q * p.dThin] = finish<OutT>(acc, p.alpha, p.beta, c);
-                }
-            };
-            bool ready = false;
+            const uint32_t share  = p.nq / p.parts; // thin rows that a block finishes
+            bool           ready  = false;
             if(drains)
                 ready = mbar_wait(&ctl->accFull, 0, &ctl->abort, WAIT_ACC_FULL);
             __syncwarp();
-            if(p.parts == 1u)
+            if(p.parts > 1u)
+                cluster_sync(); // every block's MMAs have read their last slot
+            if(drains && ready)
             {
-                if(drains && ready)
+                tc_fence_after_sync();
+                const uint32_t inTile = warp % 4u * 32u + lane, taddr = tmem + ((warp % 4u * 32u) << 16);
+                const uint32_t mine   = smem_addr(ring) + (part * share * ROW_TILE + inTile) * 4u;
+                uint32_t       to = 0, local = 0, addr = p.parts > 1u ? map_to_cta(mine, 0) : mine;
+                for(uint32_t q0 = 0; q0 < p.nq; q0 += 16u)
                 {
-                    tc_fence_after_sync();
-                    for(uint32_t q0 = 0; q0 < p.nq; q0 += 16u)
-                    {
-                        uint32_t raw[16];
-                        tmem_load_32x32b_x16(taddr + q0, raw);
-                        tmem_load_wait();
+                    uint32_t raw[16];
+                    tmem_load_32x32b_x16(taddr + q0, raw);
+                    tmem_load_wait();
 #pragma unroll
-                        for(uint32_t j = 0; j < 16u; ++j)
-                            put(q0 + j, __uint_as_float(raw[j]));
-                    }
-                }
-            }
-            else
-            {
-                // every block's MMAs have read their last slot: the rings take the partial sums,
-                // [part][thin row of the share][row of the tile]
-                cluster_sync();
-                if(drains && ready)
-                {
-                    tc_fence_after_sync();
-                    const uint32_t mine = smem_addr(ring) + (part * share * ROW_TILE + inTile) * 4u;
-                    for(uint32_t q0 = 0; q0 < p.nq; q0 += 16u)
+                    for(uint32_t j = 0; j < 16u; ++j)
                     {
-                        uint32_t raw[16];
-                        tmem_load_32x32b_x16(taddr + q0, raw);
-                        tmem_load_wait();
-#pragma unroll
-                        for(uint32_t j = 0; j < 16u; ++j)
+                        storeCluster(addr, raw[j]);
+                        addr += ROW_TILE * 4u;
+                        if(p.parts > 1u && ++local == share && ++to < p.parts)
                         {
-                            const uint32_t to = (q0 + j) / share;
-                            storeCluster(map_to_cta(mine + (q0 + j - to * share) * (ROW_TILE * 4u), to), raw[j]);
+                            local = 0;
+                            addr  = map_to_cta(mine, to);
                         }
                     }
                 }
+                tc_fence_before_sync();
+            }
+            if(p.parts > 1u)
                 cluster_sync();
-                if(drains)
+            else
+                __syncthreads();
+            {
+                float const*   sums  = reinterpret_cast<float const*>(ring);
+                const uint32_t first = part * share; // thin row
+                const uint32_t mine  = first < p.thin ? min(share, p.thin - first) : 0u;
+                const uint64_t row0  = uint64_t(tile) * ROW_TILE;
+                const uint32_t left  = uint32_t(min(uint64_t(ROW_TILE), p.rows - row0));
+                OutT*          d     = static_cast<OutT*>(p.d) + row0 * p.dRow + first * p.dThin;
+                OutT const*    c     = p.c ? static_cast<OutT const*>(p.c) + row0 * p.cRow + first * p.cThin : nullptr;
+                if(p.dRow == 1u)
                 {
-                    float const* sums = reinterpret_cast<float const*>(ring) + inTile;
-                    for(uint32_t j = 0; j < share; ++j)
+                    // a warp takes a row of D, a lane four columns
+                    constexpr uint32_t WARPS = NUM_THREADS / 32u;
+                    const uint32_t     r     = 4u * lane;
+                    if(r < left)
                     {
-                        float acc = sums[j * ROW_TILE];
-                        for(uint32_t o = 1; o < p.parts; ++o)
-                            acc += sums[(o * share + j) * ROW_TILE];
-                        put(part * share + j, acc);
+                        d += r + warp * p.dThin;
+                        c = c ? c + r + warp * p.cThin : nullptr;
+                        float const* at = sums + warp * ROW_TILE + r;
+#pragma unroll 4
+                        for(uint32_t q = warp; q < mine; q += WARPS)
+                        {
+                            float4 acc = *reinterpret_cast<float4 const*>(at);
+                            for(uint32_t o = 1; o < p.parts; ++o)
+                            {
+                                const float4 more = *reinterpret_cast<float4 const*>(at + o * share * ROW_TILE);
+                                acc.x += more.x;
+                                acc.y += more.y;
+                                acc.z += more.z;
+                                acc.w += more.w;
+                            }
+                            putFour<OutT>(d, c, p, true, left - r, acc);
+                            at += WARPS * ROW_TILE;
+                            d += WARPS * p.dThin;
+                            c = c ? c + WARPS * p.cThin : nullptr;
+                        }
                     }
+                }
+                else if(threadIdx.x < left)
+                {
+                    // a thread takes a row of D, four columns at a time
+                    const uint32_t r = threadIdx.x;
+                    d += r * p.dRow;
+                    c = c ? c + r * p.cRow : nullptr;
+                    auto total = [&](uint32_t q) {
+                        if(q >= mine)
+                            return 0.0f;
+                        float acc = sums[q * ROW_TILE + r];
+                        for(uint32_t o = 1; o < p.parts; ++o)
+                            acc += sums[(o * share + q) * ROW_TILE + r];
+                        return acc;
+                    };
+                    for(uint32_t q = 0; q < mine; q += 4u)
+                        putFour<OutT>(d + q, c ? c + q : nullptr, p, first % 4u == 0u, mine - q,
+                                      make_float4(total(q), total(q + 1u), total(q + 2u), total(q + 3u)));
                 }
             }
             tc_fence_before_sync();
@@ -518,29 +623,31 @@ namespace b200wmma
             {
                 if(elect_one())
                 {
-                    uint32_t it = 0;
-                    bool     ok = true;
+                    const uint32_t leaderFull = map_to_cta(smem_addr(&ctl->full[0]), 0);
+                    RingPosition   at;
+                    bool           ok = true;
                     for(uint32_t i = 0; ok && sched.get(pairId, i, tm, col0, width); ++i)
                     {
                         const int32_t rowA = int32_t(tm * P_TILE + rank * 128u), rowB = int32_t(col0 + rank * 128u);
-                        for(uint32_t kb = 0; kb < numSlots; ++kb, ++it)
+                        const int32_t tileA = int32_t(tm * 2u + rank), tileB = int32_t(col0 / 128u);
+                        int32_t       x = 0, group = 0;
+                        for(uint32_t kb = 0; kb < numSlots; ++kb, x += 128, group += int32_t(GROUPS))
                         {
-                            const uint32_t s = it % P_STAGES, ph = (it / P_STAGES) & 1u;
-                            if(!mbar_wait(&ctl->empty[s], ph ^ 1u, &ctl->abort, WAIT_STAGE_EMPTY))
+                            if(!mbar_wait(&ctl->empty[at.slot], at.phase ^ 1u, &ctl->abort, WAIT_STAGE_EMPTY))
                             {
                                 ok = false;
                                 break;
                             }
-                            uint8_t* slot   = ring + s * SLOT;
-                            uint8_t* scales = slot + 2u * CODE_BYTES;
+                            uint8_t*       slot = ring + at.offset;
+                            const uint32_t full = leaderFull + at.slot * 8u;
                             if(rank == 0)
-                                mbar_expect_tx(&ctl->full[s], 2u * SLOT); // both blocks
-                            const uint32_t full = map_to_cta(smem_addr(&ctl->full[s]), 0);
-                            tma_load_2d_pair(slot, &mapA, full, int32_t(kb * 128u), rowA);
-                            tma_load_2d_pair(slot + CODE_BYTES, &mapB, full, int32_t(kb * 128u), rowB);
-                            tma_load_3d_pair(scales, &mapScaleA, full, 0, int32_t(kb * GROUPS), int32_t(tm * 2u + rank));
-                            tma_load_3d_pair(scales + GROUPS * MX_TILE_BYTES, &mapScaleB, full, 0,
-                                             int32_t(kb * GROUPS), int32_t(col0 / 128u));
+                                mbar_expect_tx(&ctl->full[at.slot], 2u * SLOT); // both blocks
+                            tma_load_2d_pair(slot, &mapA, full, x, rowA);
+                            tma_load_2d_pair(slot + CODE_BYTES, &mapB, full, x, rowB);
+                            tma_load_3d_pair(slot + 2u * CODE_BYTES, &mapScaleA, full, 0, group, tileA);
+                            tma_load_3d_pair(slot + 2u * CODE_BYTES + GROUPS * MX_TILE_BYTES, &mapScaleB, full, 0, group,
+                                             tileB);
+                            at.next(P_STAGES, SLOT);
                         }
                     }
                     if(!ok)
@@ -551,51 +658,60 @@ namespace b200wmma
             {
                 if(rank == 0 && elect_one())
                 {
-                    uint32_t it = 0;
-                    bool     ok = true;
+                    const uint32_t base  = smem_addr(ring);
+                    const uint64_t descA = smem_desc_kmajor_sw128(base), descB = descAt(descA, CODE_BYTES);
+                    const uint64_t descS = smem_desc_scales(base + 2u * CODE_BYTES);
+                    uint32_t       scale = tmem + 512u - SCALE_COLS, otherScale = scale - SCALE_COLS;
+                    RingPosition   at;
+                    bool           ok = true;
                     for(uint32_t i = 0; ok && sched.get(pairId, i, tm, col0, width); ++i)
                     {
                         // tile i - 1 has drained the columns that its accumulator shares with this one's
                         if(i > 0u && !mbar_wait(&ctl->accShared, (i - 1u) & 1u, &ctl->abort, WAIT_ACC_EMPTY))
                             break;
                         tc_fence_after_sync();
-                        const uint32_t acc = tmem + (i & 1u) * ACC1;
-                        for(uint32_t kb = 0; kb < numSlots; ++kb, ++it)
+                        const uint32_t acc  = tmem + (i & 1u) * ACC1;
+                        uint32_t       left = p.k, more = 0;
+                        for(uint32_t kb = 0; kb < numSlots; ++kb, left -= SLOT_K)
                         {
-                            const uint32_t s = it % P_STAGES, ph = (it / P_STAGES) & 1u;
-                            if(!mbar_wait(&ctl->full[s], ph, &ctl->abort, WAIT_STAGE_FULL))
+                            if(!mbar_wait(&ctl->full[at.slot], at.phase, &ctl->abort, WAIT_STAGE_FULL))
                             {
                                 ok = false;
                                 break;
                             }
                             tc_fence_after_sync();
-                            const uint32_t aAddr = smem_addr(ring + s * SLOT), bAddr = aAddr + CODE_BYTES;
-                            const uint32_t sAddr = bAddr + CODE_BYTES;
-                            const uint32_t scaleA = tmem + 512u - (1u + (it & 1u)) * SCALE_COLS;
-                            const uint32_t scaleB = scaleA + 4u * GROUPS;
-                            const uint32_t left  = p.k - kb * SLOT_K;
-                            const uint32_t steps = left >= SLOT_K ? SLOT_K / MMA_K : (left + MMA_K - 1u) / MMA_K;
+                            const uint64_t dS = descAt(descS, at.offset);
 #pragma unroll
                             for(uint32_t g = 0; g < GROUPS; ++g)
                             {
-                                tmem_copy_scales_pair(scaleA + 4u * g, smem_desc_scales(sAddr + g * MX_TILE_BYTES));
-                                tmem_copy_scales_pair(scaleB + 8u * g, smem_desc_scales(sAddr + (GROUPS + g) * MX_TILE_BYTES));
-                                tmem_copy_scales_pair(scaleB + 8u * g + 4u,
-                                                      smem_desc_scales(sAddr + (2u * GROUPS + g) * MX_TILE_BYTES));
+                                tmem_copy_scales_pair(scale + 4u * g, descAt(dS, g * MX_TILE_BYTES));
+                                tmem_copy_scales_pair(scale + 4u * GROUPS + 8u * g, descAt(dS, (GROUPS + g) * MX_TILE_BYTES));
+                                tmem_copy_scales_pair(scale + 4u * GROUPS + 8u * g + 4u,
+                                                      descAt(dS, (2u * GROUPS + g) * MX_TILE_BYTES));
                             }
-#pragma unroll
-                            for(uint32_t ks = 0; ks < SLOT_K / MMA_K; ++ks)
-                            {
-                                if(ks >= steps)
-                                    break;
+                            const uint64_t dA = descAt(descA, at.offset), dB = descAt(descB, at.offset);
+                            auto           step = [&](uint32_t ks) {
                                 const uint32_t g  = KIND == ScaleKind::E4M3_16 ? ks : ks / 2u;
                                 const uint32_t id = KIND == ScaleKind::E4M3_16 ? 0u : (ks & 1u) * 2u;
-                                mma_scaled_pair<KIND>(acc, smem_desc_kmajor_sw128(aAddr + ks * 32u),
-                                                      smem_desc_kmajor_sw128(bAddr + ks * 32u),
-                                                      make_instr_desc_scaled(KIND, 256u, P_TILE, id), scaleA + 4u * g,
-                                                      scaleB + 8u * g, (kb > 0u || ks > 0u) ? 1u : 0u);
+                                mma_scaled_pair<KIND>(acc, descAt(dA, ks * 32u), descAt(dB, ks * 32u),
+                                                      make_instr_desc_scaled(KIND, 256u, P_TILE, id), scale + 4u * g,
+                                                      scale + 4u * GROUPS + 8u * g, more);
+                                more = 1;
+                            };
+                            if(left >= SLOT_K)
+                            {
+#pragma unroll
+                                for(uint32_t ks = 0; ks < SLOT_K / MMA_K; ++ks)
+                                    step(ks);
                             }
-                            mma_commit_pair(&ctl->empty[s], 0x3);
+                            else
+                                for(uint32_t ks = 0; ks * MMA_K < left; ++ks)
+                                    step(ks);
+                            mma_commit_pair(&ctl->empty[at.slot], 0x3);
+                            const uint32_t swap = scale;
+                            scale               = otherScale;
+                            otherScale          = swap;
+                            at.next(P_STAGES, SLOT);
                         }
                         if(ok)
                             mma_commit_pair(&ctl->accFull[i & 1u], 0x3);
@@ -773,23 +889,28 @@ namespace b200wmma
             p.alpha  = q.alpha;
             p.beta   = q.beta;
             p.status = q.status;
+            p.r      = thinA ? o.b : o.a;
+            p.ldr    = thinA ? o.ldb : o.lda;
             p.nq     = (p.thin + 15u) / 16u * 16u;
             const uint32_t tilesOfQ = (p.nq + 127u) / 128u;
             const uint32_t slots    = (q.k + SLOT_K - 1u) / SLOT_K;
             const uint32_t tiles    = mxRowTiles(p.rows);
-            // two blocks to an SM where their tensor memory and shared memory allow it
-            const uint32_t resident = p.nq <= 128u ? 2u : 1u;
+            // K is split until the blocks fill the device: twice over for up to 32 thin rows (1 x 8192 x
+            // 8192 MXF4: 8.5 us in the kernel with 4 parts, 9.3 with 2, 11.4 with 1), once for more,
+            // whose sums cost more to exchange (64 x 16384 x 4096 NVF4: TODO).
+            const uint32_t resident = p.nq <= 32u ? 2u : 1u;
             p.parts                 = 8;
             while(p.parts > 1u && (uint64_t(tiles) * p.parts > resident * uint32_t(sms) || slots < 2u * p.parts))
                 p.parts /= 2u;
             p.slotBytes = CODE_BYTES + p.nq * 128u + GROUPS * MX_TILE_BYTES * (1u + tilesOfQ);
-            const uint32_t room  = (resident == 2u ? 112u : 224u) * 1024u - 1024u - uint32_t(sizeof(ThinControl));
+            // a block leaves room for another on its SM: of this kernel or of the next one
+            const uint32_t room  = 112u * 1024u - uint32_t(sizeof(ThinControl)) - 1024u;
             const uint32_t mine  = (slots + p.parts - 1u) / p.parts;
             p.stages             = room / p.slotBytes;
             p.stages             = p.stages > MAX_STAGES ? MAX_STAGES : p.stages;
             p.stages             = p.stages > mine ? mine : p.stages;
-            // the partial sums take the ring's place
-            while(p.parts > 1u && p.stages * p.slotBytes < p.nq * ROW_TILE * 4u)
+            // the sums take the ring's place
+            while(p.stages * p.slotBytes < p.nq * ROW_TILE * 4u)
                 ++p.stages;
             const uint32_t cols = (p.nq + 31u) / 32u * 32u + 2u * 4u * GROUPS * (1u + tilesOfQ);
             p.tmemCols          = 32;
