@@ -5,13 +5,17 @@
 Produces, next to this file:
     lib/libb200wmma.so        the product: kernels + C ABI (include/rocwmma_b200.h)
     lib/libb200wmma_test.so   device-API unit-test kernels used only by tests/
+    _bind.so                  the Python binding of the calls where ctypes would take longer than
+                              the kernels (csrc/bind.cpp; g++, torch's headers)
 """
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -66,6 +70,26 @@ def _link(objs, name, force):
     return so
 
 
+def _bind(force):
+    """The Python binding, linked with libb200wmma.so and with torch's libraries (which `import
+    torch` has loaded before the binding is)."""
+    src, so = os.path.join(CSRC, "bind.cpp"), os.path.join(HERE, "_bind.so")
+    if force or _stale(so, [src, os.path.join(ROOT, "include", "rocwmma_b200.h")]):
+        torch = os.path.dirname(importlib.util.find_spec("torch").origin)
+        cuda = os.path.dirname(os.path.dirname(NVCC))
+        cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-fvisibility=hidden", "-shared",
+               "-I", os.path.join(ROOT, "include"), "-I", os.path.join(cuda, "include"),
+               "-isystem", os.path.join(torch, "include"),
+               "-isystem", os.path.join(torch, "include", "torch", "csrc", "api", "include"),
+               "-I", sysconfig.get_paths()["include"], src, "-o", so,
+               "-L", LIB, "-lb200wmma", "-L", os.path.join(torch, "lib"), "-ltorch_python", "-ltorch",
+               "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN/lib"]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"g++ failed for bind.cpp:\n{r.stdout}\n{r.stderr}")
+    return so
+
+
 def build(force: bool = False, verbose: bool = False):
     os.makedirs(OBJ, exist_ok=True)
     os.makedirs(LIB, exist_ok=True)
@@ -73,6 +97,7 @@ def build(force: bool = False, verbose: bool = False):
     with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
         objs = dict(zip(srcs, ex.map(lambda s: _compile(s, force), srcs)))
     prod = _link([objs[s] for s in PRODUCT if s in objs], "libb200wmma.so", force)
+    _bind(force)
     test = None
     if all(s in objs for s in TESTLIB):
         test = _link([objs[s] for s in TESTLIB], "libb200wmma_test.so", force)
