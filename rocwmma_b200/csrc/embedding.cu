@@ -17,7 +17,9 @@
 #include "common.cuh"
 #include "mx_format.cuh"
 #include "rocwmma/rocwmma_block.hpp"
+#include <cstring>
 #include <mutex>
+#include <type_traits>
 
 namespace b200wmma
 {
@@ -160,9 +162,20 @@ namespace b200wmma
                         if(t < here)
                         {
                             Piece<OutT, V> o;
+                            if(row[u] == NO_ROW)
+                            {
 #pragma unroll
-                            for(int i = 0; i < V; ++i)
-                                o.v[i] = fromFloat<OutT>(row[u] != NO_ROW ? toFloat(v[u].v[i]) * p.scale : 0.0f);
+                                for(int i = 0; i < V; ++i)
+                                    o.v[i] = OutT(0.0f);
+                            }
+                            else if(std::is_same<T, OutT>::value && p.scale == 1.0f)
+                                memcpy(&o, &v[u], sizeof(o)); // (65536 x 26 x 128 f16: 88 us with the conversions, COPY_US without)
+                            else
+                            {
+#pragma unroll
+                                for(int i = 0; i < V; ++i)
+                                    o.v[i] = fromFloat<OutT>(toFloat(v[u].v[i]) * p.scale);
+                            }
                             storePiece<OutT, V>(static_cast<OutT*>(p.out) + outs[t] + at, o);
                         }
                     }
@@ -195,13 +208,13 @@ namespace b200wmma
                         storePiece<OutT, V>(static_cast<OutT*>(c.table) + row * c.ldt + uint64_t(piece) * V, zero);
         }
 
-        // Lanes of the warp with the same digit of eight bits, among those that are `in`.  (Eight
-        // ballots: match.any took most of the scattering kernel's time.)
-        __device__ inline uint32_t sameDigit(uint32_t digit, bool in)
+        // Lanes of the warp with the same digit of `bits` bits, among those that are `in`.  (A ballot
+        // for each bit: match.any took most of the scattering kernel's time.)
+        __device__ inline uint32_t sameDigit(uint32_t digit, bool in, uint32_t bits)
         {
             uint32_t same = __ballot_sync(0xffffffffu, in);
-#pragma unroll
-            for(uint32_t b = 0; b < 8u; ++b)
+#pragma unroll 10
+            for(uint32_t b = 0; b < bits; ++b)
             {
                 const bool     set  = (digit >> b) & 1u;
                 const uint32_t vote = __ballot_sync(0xffffffffu, set);
@@ -292,7 +305,7 @@ namespace b200wmma
                     {
                         const bool     in    = first + i * 32u < t.count;
                         const uint32_t digit = (key[i] >> shift) % RADIX;
-                        const uint32_t peers = sameDigit(digit, in);
+                        const uint32_t peers = sameDigit(digit, in, 8);
                         rank[i]              = (in ? sh->bins[warp][digit] : 0u) + __popc(peers & ((1u << lane) - 1u));
                         __syncwarp();
                         if(in && (peers >> lane) == 1u) // the last of its digit
@@ -359,34 +372,48 @@ namespace b200wmma
         }
 
         // ---- sorting many tokens -------------------------------------------------------------
+        // Digits of up to ten bits: two passes for tables of up to a million rows.
         constexpr uint32_t SORT_ITEMS = 16; // keys of a thread
         constexpr uint32_t SORT_TILE  = THREADS * SORT_ITEMS;
         constexpr uint32_t SORT_WARPS = THREADS / 32;
+        constexpr uint32_t SORT_BITS  = 10;
+        constexpr uint32_t SORT_RADIX = 1u << SORT_BITS;
+        struct Digit
+        {
+            uint32_t shift, bits;
+            __device__ uint32_t of(uint32_t key) const
+            {
+                return (key >> shift) & ((1u << bits) - 1u);
+            }
+        };
 
         // bins[digit] = keys of the tile
         __device__ inline void countDigits(uint32_t* bins, uint32_t const (&key)[SORT_ITEMS], uint32_t first, uint32_t n,
-                                           uint32_t shift)
+                                           Digit digit, uint32_t tiles, uint32_t* counts)
         {
-            bins[threadIdx.x] = 0;
+            const uint32_t radix = 1u << digit.bits;
+            for(uint32_t d = threadIdx.x; d < radix; d += THREADS)
+                bins[d] = 0;
             __syncthreads();
 #pragma unroll
             for(uint32_t i = 0; i < SORT_ITEMS; ++i)
             {
                 // one addition for the equal digits of a warp: a hot row would queue 32
                 const bool     in    = uint64_t(first) + i * THREADS < n;
-                const uint32_t digit = (key[i] >> shift) % RADIX;
-                const uint32_t peers = sameDigit(digit, in);
+                const uint32_t peers = sameDigit(digit.of(key[i]), in, digit.bits);
                 if(in && (peers & ((1u << (threadIdx.x % 32u)) - 1u)) == 0u)
-                    atomicAdd(&bins[digit], uint32_t(__popc(peers)));
+                    atomicAdd(&bins[digit.of(key[i])], uint32_t(__popc(peers)));
             }
             __syncthreads();
+            for(uint32_t d = threadIdx.x; d < radix; d += THREADS)
+                counts[uint64_t(d) * tiles + blockIdx.x] = bins[d];
         }
 
         // Row of every token, and the first digit's counts[digit][tile].
         __global__ void __launch_bounds__(THREADS)
-            keysKernel(const Tokens t, uint32_t* keys, uint32_t tiles, uint32_t* counts)
+            keysKernel(const Tokens t, uint32_t* keys, uint32_t tiles, const Digit digit, uint32_t* counts)
         {
-            __shared__ uint32_t bins[RADIX];
+            __shared__ uint32_t bins[SORT_RADIX];
             grid_dependency_wait();
             grid_launch_dependents();
             const uint32_t first = blockIdx.x * SORT_TILE + threadIdx.x;
@@ -411,14 +438,13 @@ namespace b200wmma
                     keys[token] = key[i];
                 }
             }
-            countDigits(bins, key, first, t.count, 0);
-            counts[threadIdx.x * tiles + blockIdx.x] = bins[threadIdx.x];
+            countDigits(bins, key, first, t.count, digit, tiles, counts);
         }
 
         __global__ void __launch_bounds__(THREADS)
-            countKernel(uint2 const* pairs, uint32_t n, uint32_t shift, uint32_t tiles, uint32_t* counts)
+            countKernel(uint2 const* pairs, uint32_t n, const Digit digit, uint32_t tiles, uint32_t* counts)
         {
-            __shared__ uint32_t bins[RADIX];
+            __shared__ uint32_t bins[SORT_RADIX];
             grid_dependency_wait();
             grid_launch_dependents();
             const uint32_t first = blockIdx.x * SORT_TILE + threadIdx.x;
@@ -426,8 +452,7 @@ namespace b200wmma
 #pragma unroll
             for(uint32_t i = 0; i < SORT_ITEMS; ++i)
                 key[i] = first + i * THREADS < n ? pairs[first + i * THREADS].x : 0u;
-            countDigits(bins, key, first, n, shift);
-            counts[threadIdx.x * tiles + blockIdx.x] = bins[threadIdx.x];
+            countDigits(bins, key, first, n, digit, tiles, counts);
         }
 
         // Exclusive sum of a value over the block's threads, and the total.
@@ -484,20 +509,26 @@ namespace b200wmma
         // of smaller lanes come first.  The tile is put in order in shared memory first, so that
         // neighbouring threads write neighbouring places.  pairs == nullptr: the first pass, key i
         // of `keys` belongs to token i.
+        struct ScatterShared
+        {
+            uint2    tile[SORT_TILE];
+            uint16_t bins[SORT_WARPS][SORT_RADIX];
+            uint32_t shifts[SORT_RADIX]; // place of a digit's keys minus their place in the tile
+            uint32_t warps[SORT_WARPS];
+        };
+
         __global__ void __launch_bounds__(THREADS)
-            scatterKernel(uint32_t const* keys, uint2 const* pairs, uint32_t n, uint32_t shift, uint32_t tiles,
+            scatterKernel(uint32_t const* keys, uint2 const* pairs, uint32_t n, const Digit digit, uint32_t tiles,
                           uint32_t const* counts, uint32_t const* totals, uint2* out)
         {
-            __shared__ uint32_t bins[SORT_WARPS][RADIX];
-            __shared__ uint32_t warps[SORT_WARPS];
-            __shared__ uint32_t shifts[RADIX]; // place of a digit's keys minus their place in the tile
-            __shared__ uint2    tile[SORT_TILE];
-            const uint32_t      warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
+            constexpr uint32_t PER = SORT_RADIX / THREADS; // digits of a thread
+            extern __shared__ uint8_t smem[];
+            ScatterShared* sh   = reinterpret_cast<ScatterShared*>(smem);
+            const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, radix = 1u << digit.bits;
             grid_dependency_wait();
             grid_launch_dependents();
-#pragma unroll
-            for(uint32_t w = 0; w < SORT_WARPS; ++w)
-                bins[w][threadIdx.x] = 0;
+            for(uint32_t i = threadIdx.x; i < SORT_WARPS * SORT_RADIX / 2u; i += THREADS)
+                reinterpret_cast<uint32_t*>(sh->bins)[i] = 0;
             __syncthreads();
             const uint32_t tile0 = blockIdx.x * SORT_TILE, here = min(SORT_TILE, n - tile0);
             const uint32_t first = warp * (32u * SORT_ITEMS) + lane;
@@ -520,42 +551,60 @@ namespace b200wmma
             for(uint32_t i = 0; i < SORT_ITEMS; ++i)
             {
                 const bool     in    = first + i * 32u < here;
-                const uint32_t digit = (pair[i].x >> shift) % RADIX;
-                const uint32_t peers = sameDigit(digit, in);
-                rank[i]              = (in ? bins[warp][digit] : 0u) + __popc(peers & ((1u << lane) - 1u));
+                const uint32_t d     = digit.of(pair[i].x);
+                const uint32_t peers = sameDigit(d, in, digit.bits);
+                rank[i]              = (in ? sh->bins[warp][d] : 0u) + __popc(peers & ((1u << lane) - 1u));
                 __syncwarp();
                 if(in && (peers >> lane) == 1u) // the last of its digit
-                    bins[warp][digit] = rank[i] + 1u;
+                    sh->bins[warp][d] = uint16_t(rank[i] + 1u);
                 __syncwarp();
             }
             __syncthreads();
-            // thread = digit: where the keys of each warp go in the tile, and the tile's in the whole
+            // thread = neighbouring digits: where the keys of each warp go in the tile, and the tile's
+            // in the whole
             {
-                uint32_t sum = 0, total;
+                const uint32_t d0 = threadIdx.x * PER;
+                uint32_t       sums[PER], all[PER], total, mine = 0, whole = 0;
 #pragma unroll
-                for(uint32_t w = 0; w < SORT_WARPS; ++w)
+                for(uint32_t j = 0; j < PER; ++j)
                 {
-                    const uint32_t count = bins[w][threadIdx.x];
-                    bins[w][threadIdx.x] = sum;
-                    sum += count;
-                }
-                const uint32_t local = blockScan(sum, warps, total);
+                    sums[j] = 0;
 #pragma unroll
-                for(uint32_t w = 0; w < SORT_WARPS; ++w)
-                    bins[w][threadIdx.x] += local;
-                shifts[threadIdx.x] = blockScan(totals[threadIdx.x], warps, total)
-                                      + counts[threadIdx.x * tiles + blockIdx.x] - local;
+                    for(uint32_t w = 0; w < SORT_WARPS; ++w)
+                        sums[j] += sh->bins[w][d0 + j];
+                    mine += sums[j];
+                    all[j] = d0 + j < radix ? totals[d0 + j] : 0u;
+                    whole += all[j];
+                }
+                uint32_t local  = blockScan(mine, sh->warps, total);
+                uint32_t global = blockScan(whole, sh->warps, total);
+#pragma unroll
+                for(uint32_t j = 0; j < PER; ++j)
+                {
+                    uint32_t at = local;
+#pragma unroll
+                    for(uint32_t w = 0; w < SORT_WARPS; ++w)
+                    {
+                        const uint32_t count = sh->bins[w][d0 + j];
+                        sh->bins[w][d0 + j]  = uint16_t(at);
+                        at += count;
+                    }
+                    if(d0 + j < radix)
+                        sh->shifts[d0 + j] = global + counts[uint64_t(d0 + j) * tiles + blockIdx.x] - local;
+                    local += sums[j];
+                    global += all[j];
+                }
             }
             __syncthreads();
 #pragma unroll
             for(uint32_t i = 0; i < SORT_ITEMS; ++i)
                 if(first + i * 32u < here)
-                    tile[bins[warp][(pair[i].x >> shift) % RADIX] + rank[i]] = pair[i];
+                    sh->tile[sh->bins[warp][digit.of(pair[i].x)] + rank[i]] = pair[i];
             __syncthreads();
             for(uint32_t i = threadIdx.x; i < here; i += THREADS)
             {
-                const uint2 p = tile[i];
-                out[shifts[(p.x >> shift) % RADIX] + i] = p;
+                const uint2 p = sh->tile[i];
+                out[sh->shifts[digit.of(p.x)] + i] = p;
             }
         }
 
@@ -638,10 +687,14 @@ namespace b200wmma
                     src &= ~uint64_t(3);
 #pragma unroll
                 for(uint32_t part = 0; part < BYTES / PART; ++part)
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(
-                                     uint32_t(__cvta_generic_to_shared(at(ring, s, part)))),
-                                 "l"(src + part * PART), "n"(PART)
-                                 : "memory");
+                {
+                    const uint32_t to = uint32_t(__cvta_generic_to_shared(at(ring, s, part)));
+                    if constexpr(PART == 16) // past L1, which has no use for them
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(src + part * PART) : "memory");
+                    else
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(src + part * PART), "n"(PART)
+                                     : "memory");
+                }
             }
             static __device__ Piece<T, V> get(uint8_t* ring, uint32_t s, uint64_t place)
             {
@@ -668,8 +721,8 @@ namespace b200wmma
         __global__ void __launch_bounds__(THREADS) sumKernel(const SumParams p, const ClearParams c)
         {
             using R = Ring<T, V>;
-            __shared__ uint32_t keys[SUM_ITEMS + 2]; // one on each side
-            __shared__ uint64_t places[SUM_ITEMS];
+            __shared__ uint32_t rows[SUM_ITEMS + 2]; // of the items, and one on each side
+            __shared__ uint64_t places[SUM_ITEMS + 2]; // of their gradients, in elements
             __shared__ alignas(16) uint8_t ring[R::DEPTH * R::BYTES * THREADS];
             grid_dependency_wait();
             grid_launch_dependents();
@@ -681,10 +734,10 @@ namespace b200wmma
                 for(uint32_t i = threadIdx.x; i < uint32_t(end - begin); i += blockDim.x)
                 {
                     const uint32_t at = lowerBound(p.sorted, low, high, begin + i);
-                    keys[i]           = at < high && p.sorted[at].x == begin + i;
+                    rows[i]           = at < high && p.sorted[at].x == begin + i;
                 }
                 __syncthreads();
-                return clearRows<OutT, V>(c, begin, end, [&](uint64_t row) { return keys[row - begin] != 0u; });
+                return clearRows<OutT, V>(c, begin, end, [&](uint64_t row) { return rows[row - begin] != 0u; });
             }
             const uint32_t lanes = 1u << p.lanesLog2, groups = blockDim.x >> p.lanesLog2;
             const uint32_t slice = blockIdx.x % p.slices;
@@ -693,17 +746,14 @@ namespace b200wmma
             {
                 const uint64_t at   = item0 + i; // of item at - 1
                 const uint2    pair = at >= 1u && at <= p.n ? p.sorted[at - 1u] : make_uint2(NO_ROW, 0u);
-                keys[i]             = pair.x;
-                if(i >= 1u && i <= groups * p.chunk)
+                uint32_t       outer = pair.y, in = 0;
+                if(p.inner > 1u)
                 {
-                    uint32_t outer = pair.y, in = 0;
-                    if(p.inner > 1u)
-                    {
-                        outer = pair.y / p.inner;
-                        in    = pair.y - outer * p.inner;
-                    }
-                    places[i - 1u] = uint64_t(outer) * p.gradOuter + uint64_t(in) * p.gradInner;
+                    outer = pair.y / p.inner;
+                    in    = pair.y - outer * p.inner;
                 }
+                rows[i]   = pair.x;
+                places[i] = uint64_t(outer) * p.gradOuter + uint64_t(in) * p.gradInner;
             }
             __syncthreads();
             const uint32_t piece = slice * lanes + (threadIdx.x & (lanes - 1u));
@@ -713,9 +763,9 @@ namespace b200wmma
                 return;
             const uint32_t  count  = uint32_t(min(uint64_t(p.chunk), p.n - begin));
             const uint64_t  width  = uint64_t(p.pieces) * V;
-            const uint32_t  before = keys[local], after = keys[local + count + 1u];
-            uint32_t const* key    = keys + local + 1u;
-            uint64_t const* place  = places + local;
+            const uint32_t  before = rows[local], after = rows[local + count + 1u];
+            uint32_t const* rowAt  = rows + local + 1u;
+            uint64_t const* place  = places + local + 1u;
             T const*        grad   = static_cast<T const*>(p.grad) + uint64_t(piece) * V;
 
             float    sum[V];
@@ -723,7 +773,7 @@ namespace b200wmma
             bool     fromLeft = false;
             uint32_t leftKey = NO_ROW, rightKey = NO_ROW;
             auto     load = [&](uint32_t i) {
-                if(i < count && key[i] < p.rows)
+                if(i < count && rowAt[i] < p.rows)
                     R::load(ring, i % R::DEPTH, grad + place[i]);
                 asm volatile("cp.async.commit_group;" ::: "memory");
             };
@@ -732,7 +782,7 @@ namespace b200wmma
                 load(i);
             for(uint32_t i = 0;; ++i)
             {
-                const uint32_t row = i < count ? key[i] : NO_ROW;
+                const uint32_t row = i < count ? rowAt[i] : NO_ROW;
                 if(row != run || i == count)
                 {
                     // the end of a run
@@ -765,7 +815,7 @@ namespace b200wmma
                 asm volatile("cp.async.wait_group %0;" ::"n"(R::DEPTH - 1) : "memory");
                 if(row < p.rows)
                 {
-                    const Piece<T, V> v = R::get(ring, i % R::DEPTH, reinterpret_cast<uint64_t>(grad + place[i]));
+                    const Piece<T, V> v = R::get(ring, i % R::DEPTH, sizeof(T) * V < 4 ? reinterpret_cast<uint64_t>(grad + place[i]) : 0u);
 #pragma unroll
                     for(int j = 0; j < V; ++j)
                         sum[j] += toFloat(v.v[j]);
@@ -788,7 +838,7 @@ namespace b200wmma
         template <typename OutT, int V>
         __global__ void __launch_bounds__(THREADS) joinKernel(const SumParams p)
         {
-            constexpr uint32_t U = 4;
+            constexpr uint32_t U = 8;
             __shared__ uint32_t longs[THREADS], longCount, end;
             __shared__ float    sums[THREADS][V + 1];
             if(threadIdx.x == 0u)
@@ -971,7 +1021,7 @@ namespace b200wmma
         struct Plan
         {
             uint64_t keys, pairs[2], counts, totals, pieceKeys, pieceSums, bytes;
-            uint32_t tiles, passes, chunk, chunks;
+            uint32_t tiles, passes, digitBits, chunk, chunks; // digits: of many tokens
             bool     small;
         };
 
@@ -986,14 +1036,16 @@ namespace b200wmma
             };
             w.small    = count <= SMALL_TOKENS;
             w.tiles    = uint32_t((uint64_t(count) + SORT_TILE - 1) / SORT_TILE);
-            w.passes   = (log2Up(rows + 1u) + 7u) / 8u; // keys 0..rows
+            const uint32_t bits = log2Up(rows + 1u), most1 = w.small ? 8u : SORT_BITS; // keys 0..rows
+            w.passes    = (bits + most1 - 1u) / most1;
+            w.digitBits = (bits + w.passes - 1u) / w.passes;
             w.pairs[0] = take(uint64_t(count) * 8u);
             if(!w.small)
             {
                 w.pairs[1] = take(uint64_t(count) * 8u);
                 w.keys     = w.pairs[1]; // read by the first pass, which writes pairs[0]
-                w.totals   = take(RADIX * 4u);
-                w.counts   = take(uint64_t(w.tiles) * RADIX * 4u);
+                w.totals   = take(SORT_RADIX * 4u);
+                w.counts   = take((uint64_t(w.tiles) << w.digitBits) * 4u);
             }
             const uint32_t pieces = dim % 8u == 0u ? dim / 8u : dim % 2u == 0u ? dim / 2u : dim;
             const uint32_t lanes  = rowLanesLog2(pieces);
@@ -1034,6 +1086,22 @@ namespace b200wmma
             return rc__;         \
     } while(0)
 
+        // More than 48 KB of shared memory: a property of the kernel on each device.
+        template <typename KernelT>
+        int optIn(KernelT kernel, size_t bytes, std::mutex& mutex, bool (&done)[64])
+        {
+            std::lock_guard<std::mutex> lock(mutex);
+            int                         dev = 0;
+            B200WMMA_CUDA_TRY(cudaGetDevice(&dev));
+            if(dev >= 64 || !done[dev])
+            {
+                B200WMMA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
+                if(dev < 64)
+                    done[dev] = true;
+            }
+            return B200WMMA_OK;
+        }
+
         ClearParams clearParams(void* table, uint64_t ldt, uint32_t rows, uint32_t pieces)
         {
             return ClearParams{table, ldt, pieces, rowLanesLog2(pieces), 0, rows, 0};
@@ -1050,19 +1118,7 @@ namespace b200wmma
             c.blocks            = g.accumulate ? 0u : uint32_t(want < 147u ? want : 147u);
             static std::mutex mutex;
             static bool       done[64] = {};
-            {
-                std::lock_guard<std::mutex> lock(mutex);
-                int                         dev = 0;
-                B200WMMA_CUDA_TRY(cudaGetDevice(&dev));
-                if(dev >= 64 || !done[dev])
-                {
-                    B200WMMA_CUDA_TRY(cudaFuncSetAttribute(sortSmallKernel<OutT, V>,
-                                                           cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                           int(sizeof(SmallShared))));
-                    if(dev < 64)
-                        done[dev] = true;
-                }
-            }
+            B200WMMA_TRY(optIn(sortSmallKernel<OutT, V>, sizeof(SmallShared), mutex, done));
             return cudaToStatus(launchOverlapped(sortSmallKernel<OutT, V>, dim3(1u + c.blocks), dim3(SMALL_THREADS),
                                                  sizeof(SmallShared), stream, g.t, c, w.passes,
                                                  reinterpret_cast<uint2*>(g.workspace + w.pairs[0])));
@@ -1072,20 +1128,24 @@ namespace b200wmma
         {
             auto       words = [&](uint64_t at) { return reinterpret_cast<uint32_t*>(g.workspace + at); };
             auto       pairs = [&](uint32_t i) { return reinterpret_cast<uint2*>(g.workspace + w.pairs[i]); };
+            static std::mutex mutex;
+            static bool       done[64] = {};
+            B200WMMA_TRY(optIn(scatterKernel, sizeof(ScatterShared), mutex, done));
             const dim3 grid(w.tiles);
+            auto       digit = [&](uint32_t pass) { return Digit{w.digitBits * pass, w.digitBits}; };
             B200WMMA_TRY(cudaToStatus(launchOverlapped(keysKernel, grid, dim3(THREADS), 0, stream, g.t, words(w.keys),
-                                                       w.tiles, words(w.counts))));
+                                                       w.tiles, digit(0), words(w.counts))));
             for(uint32_t pass = 0; pass < w.passes; ++pass)
             {
                 uint2* from = pass ? pairs((pass - 1u) % 2u) : nullptr;
                 if(pass > 0u)
                     B200WMMA_TRY(cudaToStatus(launchOverlapped(countKernel, grid, dim3(THREADS), 0, stream, from,
-                                                               g.t.count, 8u * pass, w.tiles, words(w.counts))));
-                B200WMMA_TRY(cudaToStatus(launchOverlapped(scanKernel, dim3(RADIX), dim3(THREADS), 0, stream,
+                                                               g.t.count, digit(pass), w.tiles, words(w.counts))));
+                B200WMMA_TRY(cudaToStatus(launchOverlapped(scanKernel, dim3(1u << w.digitBits), dim3(THREADS), 0, stream,
                                                            words(w.counts), w.tiles, words(w.totals))));
-                B200WMMA_TRY(cudaToStatus(launchOverlapped(scatterKernel, grid, dim3(THREADS), 0, stream, words(w.keys),
-                                                           from, g.t.count, 8u * pass, w.tiles, words(w.counts),
-                                                           words(w.totals), pairs(pass % 2u))));
+                B200WMMA_TRY(cudaToStatus(launchOverlapped(scatterKernel, grid, dim3(THREADS), sizeof(ScatterShared),
+                                                           stream, words(w.keys), from, g.t.count, digit(pass), w.tiles,
+                                                           words(w.counts), words(w.totals), pairs(pass % 2u))));
             }
             *sorted = pairs((w.passes - 1u) % 2u);
             return B200WMMA_OK;
@@ -1122,7 +1182,10 @@ namespace b200wmma
         int joinPieces(GradientCall const& g, SumParams p, cudaStream_t stream)
         {
             p.pieces    = g.dim / V;
-            p.lanesLog2 = rowLanesLog2(p.pieces);
+            // at most a warp to a piece, so that a block has eight groups for the long runs (16384
+            // tokens of 4096, where the most frequent one has 75 pieces: JOIN_BEFORE us with 256
+            // threads to a row, JOIN_AFTER with 32)
+            p.lanesLog2 = rowLanesLog2(p.pieces) < 5u ? rowLanesLog2(p.pieces) : 5u;
             p.slices    = (p.pieces + (1u << p.lanesLog2) - 1u) >> p.lanesLog2;
             const uint32_t groups = THREADS >> p.lanesLog2;
             const uint64_t blocks = (uint64_t(p.chunks) + groups - 1u) / groups * p.slices;

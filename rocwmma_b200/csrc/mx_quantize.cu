@@ -15,6 +15,7 @@
 #include "mx_format.cuh"
 #include "rocwmma/rocwmma_block.hpp"
 #include <cstring>
+#include <type_traits>
 
 namespace b200wmma
 {
@@ -240,46 +241,89 @@ namespace b200wmma
             uint64_t    ldq; // bytes
             uint64_t    ldx; // elements
             uint32_t    rows, k, groups, tilesK;
+            uint32_t    tilesPerBlock; // rows only
             float       factor; // 2^-exponent
         };
 
-        // x row-major: k is contiguous.  A block takes 32 rows x 128 columns: sixteen threads read
-        // 128 values of a row, eight each, and a block's largest magnitude comes from its two
-        // (NVF4) or four (MXF4) threads; those with the scales of four blocks write them as a word.
+        // Columns that a block's threads take at a time, and how many such tiles a block has: more of
+        // them spread what a block sets up over more values, but the device is filled first.
+        inline uint32_t tilesPerBlock(uint64_t tiles, uint32_t tilesK)
+        {
+            const uint64_t per = tiles / (2u * 8u * 148u); // eight blocks to an SM, twice
+            return uint32_t(per < 1u ? 1u : per > 8u ? 8u : per < tilesK ? per : tilesK);
+        }
+
+        // x row-major: k is contiguous.  A block takes 32 rows x 128 columns at a time: sixteen
+        // threads read 128 values of a row, eight each, and a block's largest magnitude comes from
+        // its two (NVF4) or four (MXF4) threads; those with the scales of four blocks write them as
+        // a word.  The values of the next tile are on their way while those of one are worked on.
         template <typename T, bool NV, bool VEC>
         __global__ void __launch_bounds__(THREADS) quantizeRowsKernel(const QuantizeParams p)
         {
-            constexpr int      STEPS  = SLAB_ROWS / (THREADS / 16);
-            constexpr uint32_t GROUPS = TILE_K / (4u * mxBlock(NV));
-            const uint32_t slab = blockIdx.x / p.tilesK, tileK = blockIdx.x % p.tilesK;
+            constexpr uint32_t STEPS  = SLAB_ROWS / (THREADS / 16);
+            constexpr uint32_t GROUPS = TILE_K / (4u * mxBlock(NV)), LANES = mxBlock(NV) / 8u; // of a block
+            const uint32_t across = (p.tilesK + p.tilesPerBlock - 1u) / p.tilesPerBlock;
+            const uint32_t slab = blockIdx.x / across, tile0 = blockIdx.x % across * p.tilesPerBlock;
+            const uint32_t tiles = min(p.tilesPerBlock, p.tilesK - tile0);
             const uint32_t col = threadIdx.x % 16u * 8u, rowIn = threadIdx.x / 16u;
-            const uint32_t k0   = tileK * TILE_K + col, count = min(TILE_K, p.k - tileK * TILE_K);
             const uint64_t row0 = uint64_t(slab) * SLAB_ROWS;
             const uint32_t rows = row0 < p.rows ? uint32_t(min(uint64_t(SLAB_ROWS), p.rows - row0)) : 0u;
-            T const*       x    = static_cast<T const*>(p.x) + row0 * p.ldx + tileK * TILE_K;
-            grid_dependency_wait();
-            grid_launch_dependents();
-            Raw8<T> raw[STEPS];
-            if constexpr(VEC)
+            // this thread's places in its rows: rowIn and rowIn + 16
+            T const*       x[STEPS];
+            uint8_t*       codes[STEPS];
+            uint8_t*       scales[STEPS];
+            const uint64_t k0 = uint64_t(tile0) * TILE_K + col;
+#pragma unroll
+            for(uint32_t i = 0; i < STEPS; ++i)
             {
-                if(rows == SLAB_ROWS && count == TILE_K)
+                const uint32_t r = i * 16u + rowIn;
+                x[i]      = static_cast<T const*>(p.x) + (row0 + r) * p.ldx + k0;
+                codes[i]  = p.codes + (row0 + r) * p.ldq + k0 / 2u;
+                scales[i] = p.scales + (uint64_t(slab / 4u) * p.groups + k0 / (4u * mxBlock(NV))) * MX_TILE_BYTES
+                            + scaleOffset(slab % 4u * SLAB_ROWS + r, 0);
+            }
+            uint32_t       left  = p.k > k0 ? uint32_t(p.k - k0) : 0u; // columns from the thread's first on
+            uint32_t       pitch = mxPitch(p.k) > k0 / 2u ? uint32_t(mxPitch(p.k) - k0 / 2u) : 0u; // bytes
+            uint32_t       group = uint32_t(k0 / (4u * mxBlock(NV)));
+            __shared__ alignas(16) uint8_t staged[VEC ? 16 : SLAB_ROWS * StagedRow<T>::PITCH];
+            auto fetch = [&](uint32_t t, Raw8<T>(&raw)[STEPS]) {
+                const uint32_t done = t * TILE_K;
+#pragma unroll
+                for(uint32_t i = 0; i < STEPS; ++i)
+                    raw[i] = zero8<T>();
+                if constexpr(VEC)
                 {
 #pragma unroll
-                    for(int i = 0; i < STEPS; ++i)
-                        raw[i] = load8(x + (i * 16u + rowIn) * p.ldx + col);
+                    for(uint32_t i = 0; i < STEPS; ++i)
+                        if(i * 16u + rowIn < rows && left >= done + 8u)
+                            raw[i] = load8(x[i] + done);
+                    if(left > done && left < done + 8u)
+                    {
+#pragma unroll
+                        for(uint32_t i = 0; i < STEPS; ++i)
+#pragma unroll
+                            for(uint32_t j = 0; j < 8u; ++j)
+                                if(i * 16u + rowIn < rows && done + j < left)
+                                    raw[i].v[j] = x[i][done + j];
+                    }
                 }
                 else
                 {
+                    const uint32_t count = min(TILE_K, p.k - (tile0 + t) * TILE_K);
+                    auto rowAt = [&](uint32_t r) {
+                        return const_cast<T*>(static_cast<T const*>(p.x)) + (row0 + r) * p.ldx + uint64_t(tile0 + t) * TILE_K;
+                    };
+                    __syncthreads();
+                    moveStaged<T, true>(staged, rows, count, rowAt);
+                    __syncthreads();
 #pragma unroll
-                    for(int i = 0; i < STEPS; ++i)
+                    for(uint32_t i = 0; i < STEPS; ++i)
                     {
                         const uint32_t r = i * 16u + rowIn;
-                        T const*       at = x + r * p.ldx + col;
-                        raw[i]            = zero8<T>();
-                        if(r < rows && col + 8u <= count)
-                            raw[i] = load8(at);
-                        else if(r < rows)
+                        if(r < rows)
                         {
+                            T const* at = reinterpret_cast<T const*>(staged + r * StagedRow<T>::PITCH)
+                                          + StagedRow<T>::shift(rowAt(r)) + col;
 #pragma unroll
                             for(uint32_t j = 0; j < 8u; ++j)
                                 if(col + j < count)
@@ -287,89 +331,72 @@ namespace b200wmma
                         }
                     }
                 }
-            }
-            else
+            };
+            grid_dependency_wait();
+            grid_launch_dependents();
+            Raw8<T> raw[STEPS], next[STEPS];
+            fetch(0, next);
+            for(uint32_t t = 0; t < tiles; ++t)
             {
-                __shared__ alignas(16) uint8_t staged[SLAB_ROWS * StagedRow<T>::PITCH];
-                auto rowAt = [&](uint32_t r) { return const_cast<T*>(x) + r * p.ldx; };
-                moveStaged<T, true>(staged, rows, count, rowAt);
-                __syncthreads();
 #pragma unroll
-                for(int i = 0; i < STEPS; ++i)
+                for(uint32_t i = 0; i < STEPS; ++i)
+                    raw[i] = next[i];
+                if(t + 1u < tiles)
+                    fetch(t + 1u, next);
+#pragma unroll
+                for(uint32_t i = 0; i < STEPS; ++i)
                 {
-                    const uint32_t r = i * 16u + rowIn;
-                    raw[i]           = zero8<T>();
-                    if(r < rows)
-                    {
-                        T const* at = reinterpret_cast<T const*>(staged + r * StagedRow<T>::PITCH)
-                                      + StagedRow<T>::shift(rowAt(r)) + col;
+                    Top<T> top;
 #pragma unroll
-                        for(uint32_t j = 0; j < 8u; ++j)
-                            if(col + j < count)
-                                raw[i].v[j] = at[j];
-                    }
+                    for(int j = 0; j < 8; j += 2)
+                        top.two(raw[i].v[j], raw[i].v[j + 1]);
+                    top.lanes(1);
+                    if constexpr(!NV)
+                        top.lanes(2);
+                    const Scale    s    = scaleOf<NV>(top.value() * p.factor);
+                    const uint32_t code = codes8<T, NV>(raw[i].v, s, p.factor);
+                    if(i * 16u + rowIn < rows && t * (TILE_K / 2u) < pitch)
+                        *reinterpret_cast<uint32_t*>(codes[i] + t * (TILE_K / 2u)) = code;
+                    // the bytes of four blocks, a word of the scale tile's row
+                    uint32_t word = s.byte << (8u * (threadIdx.x / LANES % 4u));
+                    word |= __shfl_xor_sync(0xffffffffu, word, LANES);
+                    word |= __shfl_xor_sync(0xffffffffu, word, 2u * LANES);
+                    if(threadIdx.x % (4u * LANES) == 0u && group + t * GROUPS < p.groups)
+                        *reinterpret_cast<uint32_t*>(scales[i] + t * (GROUPS * MX_TILE_BYTES)) = word;
                 }
-            }
-#pragma unroll
-            for(int i = 0; i < STEPS; ++i)
-            {
-                const uint32_t r = i * 16u + rowIn;
-                Top<T>         top;
-#pragma unroll
-                for(int j = 0; j < 8; j += 2)
-                    top.two(raw[i].v[j], raw[i].v[j + 1]);
-                top.lanes(1);
-                if constexpr(!NV)
-                    top.lanes(2);
-                const Scale    s    = scaleOf<NV>(top.value() * p.factor);
-                const uint32_t code = codes8<T, NV>(raw[i].v, s, p.factor);
-                if(r < rows && k0 / 2u < mxPitch(p.k))
-                    *reinterpret_cast<uint32_t*>(p.codes + (row0 + r) * p.ldq + k0 / 2u) = code;
-                // the bytes of four blocks, a word of the scale tile's row
-                constexpr uint32_t LANES = mxBlock(NV) / 8u; // of a block
-                uint32_t           word  = s.byte << (8u * (threadIdx.x / LANES % 4u));
-                word |= __shfl_xor_sync(0xffffffffu, word, LANES);
-                word |= __shfl_xor_sync(0xffffffffu, word, 2u * LANES);
-                const uint32_t group = tileK * GROUPS + col / (4u * mxBlock(NV));
-                if(threadIdx.x % (4u * LANES) == 0u && group < p.groups)
-                    *reinterpret_cast<uint32_t*>(p.scales + (uint64_t(slab / 4u) * p.groups + group) * MX_TILE_BYTES
-                                                 + scaleOffset(slab % 4u * SLAB_ROWS + r, 0))
-                        = word;
             }
         }
 
-        // x column-major: the rows are contiguous.  A block takes 128 rows x 128 columns, a thread
-        // two neighbouring rows and 32 values of k of each, so that a warp reads 64 consecutive
-        // values at a time and no maximum crosses a thread; the codes pass through shared memory
-        // to leave as rows, the scale tiles to leave whole.
+        // x column-major: the rows are contiguous.  A block takes 128 rows x four blocks of k (a scale
+        // tile), a thread two neighbouring rows and one block of k of each, so that a warp reads 64
+        // consecutive values at a time and no maximum crosses a thread; the codes pass through
+        // shared memory to leave as rows, the scale tile to leave whole.
         template <typename T, bool NV, bool VEC>
-        __global__ void __launch_bounds__(THREADS) quantizeColumnsKernel(const QuantizeParams p)
+        __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 4 : 3) quantizeColumnsKernel(const QuantizeParams p)
         {
-            constexpr uint32_t GROUPS = TILE_K / (4u * mxBlock(NV));
-            constexpr int      B      = int(mxBlock(NV));
-            constexpr uint32_t PITCH  = 80; // of a staged row: 64 bytes of codes, 16 of padding
-            __shared__ alignas(16) uint8_t scales[GROUPS * MX_TILE_BYTES];
+            constexpr uint32_t B     = mxBlock(NV);
+            constexpr uint32_t BYTES = 4 * B / 2, PITCH = BYTES + 16; // of a staged row of codes
+            __shared__ alignas(16) uint8_t scales[MX_TILE_BYTES];
             __shared__ alignas(16) uint8_t staged[128 * PITCH];
             struct alignas(2 * sizeof(T)) Pair
             {
                 T v[2];
             };
-            const uint32_t tileRow = blockIdx.x / p.tilesK, tileK = blockIdx.x % p.tilesK;
-            const uint32_t r = threadIdx.x % 64u * 2u, kIn = threadIdx.x / 64u * 32u;
-            const uint64_t row = uint64_t(tileRow) * 128u + r;
-            const uint32_t k0  = tileK * TILE_K + kIn;
-            const uint32_t count = k0 < p.k ? min(32u, p.k - k0) : 0u;
+            const uint32_t tileRow = blockIdx.x / p.groups, group = blockIdx.x % p.groups;
+            const uint32_t r = threadIdx.x % 64u * 2u, blockIn = threadIdx.x / 64u;
+            const uint64_t row = uint64_t(tileRow) * 128u + r, k0 = (uint64_t(group) * 4u + blockIn) * B;
+            const uint32_t count = k0 < p.k ? uint32_t(min(uint64_t(B), p.k - k0)) : 0u;
             grid_dependency_wait();
             grid_launch_dependents();
-            Pair     v[32];
-            T const* x = static_cast<T const*>(p.x) + row + uint64_t(k0) * p.ldx;
+            Pair     v[B];
+            T const* x = static_cast<T const*>(p.x) + row + k0 * p.ldx;
 #pragma unroll
-            for(uint32_t i = 0; i < 32u; ++i)
+            for(uint32_t i = 0; i < B; ++i)
                 v[i].v[0] = v[i].v[1] = T(0.0f);
             if(VEC && row + 1u < p.rows)
             {
 #pragma unroll
-                for(uint32_t i = 0; i < 32u; ++i)
+                for(uint32_t i = 0; i < B; ++i)
                     if(i < count)
                         v[i] = *reinterpret_cast<Pair const*>(x + i * p.ldx);
             }
@@ -377,7 +404,7 @@ namespace b200wmma
             {
                 const bool one = row < p.rows, two = row + 1u < p.rows;
 #pragma unroll
-                for(uint32_t i = 0; i < 32u; ++i)
+                for(uint32_t i = 0; i < B; ++i)
                 {
                     if(i < count && one)
                         v[i].v[0] = x[i * p.ldx];
@@ -388,48 +415,43 @@ namespace b200wmma
 #pragma unroll
             for(int j = 0; j < 2; ++j)
             {
-                uint32_t words[4];
+                Top<T> top;
 #pragma unroll
-                for(int b = 0; b < 32 / B; ++b)
+                for(uint32_t i = 0; i < B; i += 2)
+                    top.two(v[i].v[j], v[i + 1].v[j]);
+                const Scale s = scaleOf<NV>(top.value() * p.factor);
+                uint32_t    words[B / 8];
+#pragma unroll
+                for(uint32_t w = 0; w < B / 8; ++w)
                 {
-                    Top<T> top;
+                    T y[8];
 #pragma unroll
-                    for(int i = 0; i < B; i += 2)
-                        top.two(v[b * B + i].v[j], v[b * B + i + 1].v[j]);
-                    const Scale s = scaleOf<NV>(top.value() * p.factor);
-#pragma unroll
-                    for(int w = 0; w < B / 8; ++w)
-                    {
-                        T y[8];
-#pragma unroll
-                        for(int i = 0; i < 8; ++i)
-                            y[i] = v[b * B + w * 8 + i].v[j];
-                        words[b * (B / 8) + w] = codes8<T, NV>(y, s, p.factor);
-                    }
-                    scales[scaleOffset(r + j, kIn / B + b)] = uint8_t(s.byte);
+                    for(uint32_t i = 0; i < 8; ++i)
+                        y[i] = v[w * 8 + i].v[j];
+                    words[w] = codes8<T, NV>(y, s, p.factor);
                 }
-                *reinterpret_cast<uint4*>(staged + (r + j) * PITCH + kIn / 2u)
-                    = make_uint4(words[0], words[1], words[2], words[3]);
+                scales[scaleOffset(r + j, blockIn)] = uint8_t(s.byte);
+                uint32_t* to = reinterpret_cast<uint32_t*>(staged + (r + j) * PITCH + blockIn * (B / 2));
+#pragma unroll
+                for(uint32_t w = 0; w < B / 8; ++w)
+                    to[w] = words[w];
             }
             __syncthreads();
-            {
-                const uint32_t at = threadIdx.x * 16u, group = tileK * GROUPS + at / MX_TILE_BYTES;
-                if(at < GROUPS * MX_TILE_BYTES && group < p.groups)
-                    *reinterpret_cast<uint4*>(p.scales + (uint64_t(tileRow) * p.groups + group) * MX_TILE_BYTES
-                                              + at % MX_TILE_BYTES)
-                        = *reinterpret_cast<uint4 const*>(scales + at);
-            }
-            // four threads a row
-            const uint64_t pitch = mxPitch(p.k);
+            const uint32_t at = threadIdx.x * 16u;
+            if(at < MX_TILE_BYTES)
+                *reinterpret_cast<uint4*>(p.scales + (uint64_t(tileRow) * p.groups + group) * MX_TILE_BYTES + at)
+                    = *reinterpret_cast<uint4 const*>(scales + at);
+            // sixteen bytes a thread
+            constexpr uint32_t PIECES = BYTES / 16u;
+            const uint64_t     pitch  = mxPitch(p.k);
 #pragma unroll
-            for(uint32_t i = threadIdx.x; i < 128u * 4u; i += THREADS)
+            for(uint32_t i = threadIdx.x; i < 128u * PIECES; i += THREADS)
             {
-                const uint32_t rr = i / 4u;
-                const uint64_t at = uint64_t(tileK) * (TILE_K / 2) + i % 4u * 16u;
-                const uint64_t out = uint64_t(tileRow) * 128u + rr;
-                if(out < p.rows && at < pitch)
-                    *reinterpret_cast<uint4*>(p.codes + out * p.ldq + at)
-                        = *reinterpret_cast<uint4 const*>(staged + rr * PITCH + i % 4u * 16u);
+                const uint32_t rr  = i / PIECES;
+                const uint64_t col = uint64_t(group) * BYTES + i % PIECES * 16u, out = uint64_t(tileRow) * 128u + rr;
+                if(out < p.rows && col < pitch)
+                    *reinterpret_cast<uint4*>(p.codes + out * p.ldq + col)
+                        = *reinterpret_cast<uint4 const*>(staged + rr * PITCH + i % PIECES * 16u);
             }
         }
 
@@ -441,89 +463,147 @@ namespace b200wmma
             uint64_t       ldq; // bytes
             uint64_t       ldo; // elements
             uint32_t       rows, k, groups, tilesK;
+            uint32_t       tilesPerBlock;
             float          factor; // 2^exponent
         };
 
-        // A block takes 32 rows x 128 columns, a thread eight codes of two rows.
-        template <typename T, bool NV, bool VEC>
-        __global__ void __launch_bounds__(THREADS) dequantizeKernel(const DequantizeParams p)
+        // Eight values: code * s is exact (three bits times at most four); so is the power of two, short
+        // of the subnormals.
+        template <typename T, bool NV>
+        __device__ inline Raw8<T> values8(uint32_t codes, uint32_t byte, float factor)
         {
-            constexpr int  STEPS = SLAB_ROWS / (THREADS / 16);
-            const uint32_t slab = blockIdx.x / p.tilesK, tileK = blockIdx.x % p.tilesK;
-            const uint32_t col = threadIdx.x % 16u * 8u, rowIn = threadIdx.x / 16u;
-            const uint32_t k0   = tileK * TILE_K + col, count = min(TILE_K, p.k - tileK * TILE_K);
-            const uint64_t row0 = uint64_t(slab) * SLAB_ROWS;
-            const uint32_t rows = row0 < p.rows ? uint32_t(min(uint64_t(SLAB_ROWS), p.rows - row0)) : 0u;
-            T*             out  = static_cast<T*>(p.out) + row0 * p.ldo + tileK * TILE_K;
-            grid_dependency_wait();
-            grid_launch_dependents();
-            uint32_t word[STEPS], byte[STEPS];
+            const float s = NV ? fromE4m3(byte) : fromE8m0(byte);
+            float       v[8];
+            e2m1x8ToFloat(codes, v);
 #pragma unroll
-            for(int i = 0; i < STEPS; ++i)
+            for(int j = 0; j < 8; ++j)
+                v[j] *= s;
+            if(factor != 1.0f)
             {
-                const uint32_t r = i * 16u + rowIn;
-                word[i] = byte[i] = 0;
-                if(r < rows && col < count)
-                {
-                    word[i] = *reinterpret_cast<uint32_t const*>(p.codes + (row0 + r) * p.ldq + k0 / 2u);
-                    byte[i] = p.scales[(uint64_t(slab / 4u) * p.groups + k0 / mxBlock(NV) / 4u) * MX_TILE_BYTES
-                                       + scaleOffset(slab % 4u * SLAB_ROWS + r, k0 / mxBlock(NV) % 4u)];
-                }
-            }
-            auto values = [&](int i) {
-                // code * s is exact (three bits times at most four); so is the power of two,
-                // short of the subnormals
-                const float s = NV ? fromE4m3(byte[i]) : fromE8m0(byte[i]);
-                float       v[8];
-                e2m1x8ToFloat(word[i], v);
-                Raw8<T> o;
 #pragma unroll
                 for(int j = 0; j < 8; ++j)
-                    o.v[j] = fromFloat<T>(v[j] * s * p.factor);
-                return o;
-            };
-            if constexpr(VEC)
+                    v[j] *= factor;
+            }
+            Raw8<T> o;
+            if constexpr(std::is_same<T, float>::value)
             {
 #pragma unroll
-                for(int i = 0; i < STEPS; ++i)
-                {
-                    const uint32_t r  = i * 16u + rowIn;
-                    const Raw8<T>  o  = values(i);
-                    T*             at = out + r * p.ldo + col;
-                    if(r < rows && col + 8u <= count)
-                    {
-#pragma unroll
-                        for(int j = 0; j < int(sizeof(T) * 8 / 16); ++j)
-                            reinterpret_cast<uint4*>(at)[j] = reinterpret_cast<uint4 const*>(&o)[j];
-                    }
-                    else if(r < rows)
-                    {
-#pragma unroll
-                        for(uint32_t j = 0; j < 8u; ++j)
-                            if(col + j < count)
-                                at[j] = o.v[j];
-                    }
-                }
+                for(int j = 0; j < 8; ++j)
+                    o.v[j] = v[j];
             }
             else
             {
-                __shared__ alignas(16) uint8_t staged[SLAB_ROWS * StagedRow<T>::PITCH];
-                auto rowAt = [&](uint32_t r) { return out + r * p.ldo; };
 #pragma unroll
-                for(int i = 0; i < STEPS; ++i)
+                for(int j = 0; j < 8; j += 2)
+                    if constexpr(std::is_same<T, __half>::value)
+                        reinterpret_cast<__half2*>(&o)[j / 2] = __floats2half2_rn(v[j], v[j + 1]);
+                    else
+                        reinterpret_cast<__nv_bfloat162*>(&o)[j / 2] = __floats2bfloat162_rn(v[j], v[j + 1]);
+            }
+            return o;
+        }
+
+        // A block takes 32 rows x 128 columns at a time, a thread eight codes of two rows; the codes
+        // of the next tile are on their way meanwhile.
+        template <typename T, bool NV, bool VEC>
+        __global__ void __launch_bounds__(THREADS) dequantizeKernel(const DequantizeParams p)
+        {
+            constexpr uint32_t STEPS  = SLAB_ROWS / (THREADS / 16);
+            constexpr uint32_t GROUPS = TILE_K / (4u * mxBlock(NV));
+            const uint32_t across = (p.tilesK + p.tilesPerBlock - 1u) / p.tilesPerBlock;
+            const uint32_t slab = blockIdx.x / across, tile0 = blockIdx.x % across * p.tilesPerBlock;
+            const uint32_t tiles = min(p.tilesPerBlock, p.tilesK - tile0);
+            const uint32_t col = threadIdx.x % 16u * 8u, rowIn = threadIdx.x / 16u;
+            const uint64_t row0 = uint64_t(slab) * SLAB_ROWS, k0 = uint64_t(tile0) * TILE_K + col;
+            const uint32_t rows = row0 < p.rows ? uint32_t(min(uint64_t(SLAB_ROWS), p.rows - row0)) : 0u;
+            const uint32_t left = p.k > k0 ? uint32_t(p.k - k0) : 0u; // columns from the thread's first on
+            uint8_t const* codes[STEPS];
+            uint8_t const* scales[STEPS];
+            T*             out[STEPS];
+#pragma unroll
+            for(uint32_t i = 0; i < STEPS; ++i)
+            {
+                const uint32_t r = i * 16u + rowIn;
+                codes[i]  = p.codes + (row0 + r) * p.ldq + k0 / 2u;
+                scales[i] = p.scales + (uint64_t(slab / 4u) * p.groups + k0 / (4u * mxBlock(NV))) * MX_TILE_BYTES
+                            + scaleOffset(slab % 4u * SLAB_ROWS + r, uint32_t(k0 / mxBlock(NV) % 4u));
+                out[i] = static_cast<T*>(p.out) + (row0 + r) * p.ldo + k0;
+            }
+            auto fetch = [&](uint32_t t, uint32_t(&word)[STEPS], uint32_t(&byte)[STEPS]) {
+#pragma unroll
+                for(uint32_t i = 0; i < STEPS; ++i)
                 {
-                    const uint32_t r = i * 16u + rowIn;
-                    const Raw8<T>  o = values(i);
-                    if(r < rows)
+                    word[i] = byte[i] = 0;
+                    if(i * 16u + rowIn < rows && left > t * TILE_K)
                     {
-                        T* at = reinterpret_cast<T*>(staged + r * StagedRow<T>::PITCH) + StagedRow<T>::shift(rowAt(r)) + col;
-#pragma unroll
-                        for(int j = 0; j < 8; ++j)
-                            at[j] = o.v[j];
+                        word[i] = *reinterpret_cast<uint32_t const*>(codes[i] + t * (TILE_K / 2u));
+                        byte[i] = scales[i][t * (GROUPS * MX_TILE_BYTES)];
                     }
                 }
-                __syncthreads();
-                moveStaged<T, false>(staged, rows, count, rowAt);
+            };
+            __shared__ alignas(16) uint8_t staged[VEC ? 16 : SLAB_ROWS * StagedRow<T>::PITCH];
+            grid_dependency_wait();
+            grid_launch_dependents();
+            uint32_t word[STEPS], byte[STEPS], nextWord[STEPS], nextByte[STEPS];
+            fetch(0, nextWord, nextByte);
+            for(uint32_t t = 0; t < tiles; ++t)
+            {
+                const uint32_t done = t * TILE_K;
+#pragma unroll
+                for(uint32_t i = 0; i < STEPS; ++i)
+                {
+                    word[i] = nextWord[i];
+                    byte[i] = nextByte[i];
+                }
+                if(t + 1u < tiles)
+                    fetch(t + 1u, nextWord, nextByte);
+                if constexpr(VEC)
+                {
+#pragma unroll
+                    for(uint32_t i = 0; i < STEPS; ++i)
+                    {
+                        const Raw8<T> o  = values8<T, NV>(word[i], byte[i], p.factor);
+                        T*            at = out[i] + done;
+                        if(i * 16u + rowIn >= rows || left <= done)
+                            continue;
+                        if(left >= done + 8u)
+                        {
+#pragma unroll
+                            for(int j = 0; j < int(sizeof(T) * 8 / 16); ++j)
+                                reinterpret_cast<uint4*>(at)[j] = reinterpret_cast<uint4 const*>(&o)[j];
+                        }
+                        else
+                        {
+#pragma unroll
+                            for(uint32_t j = 0; j < 8u; ++j)
+                                if(done + j < left)
+                                    at[j] = o.v[j];
+                        }
+                    }
+                }
+                else
+                {
+                    const uint32_t count = min(TILE_K, p.k - (tile0 + t) * TILE_K);
+                    auto rowAt = [&](uint32_t r) {
+                        return static_cast<T*>(p.out) + (row0 + r) * p.ldo + uint64_t(tile0 + t) * TILE_K;
+                    };
+                    __syncthreads();
+#pragma unroll
+                    for(uint32_t i = 0; i < STEPS; ++i)
+                    {
+                        const uint32_t r = i * 16u + rowIn;
+                        const Raw8<T>  o = values8<T, NV>(word[i], byte[i], p.factor);
+                        if(r < rows)
+                        {
+                            T* at = reinterpret_cast<T*>(staged + r * StagedRow<T>::PITCH) + StagedRow<T>::shift(rowAt(r)) + col;
+#pragma unroll
+                            for(int j = 0; j < 8; ++j)
+                                at[j] = o.v[j];
+                        }
+                    }
+                    __syncthreads();
+                    moveStaged<T, false>(staged, rows, count, rowAt);
+                }
             }
         }
 
@@ -532,15 +612,25 @@ namespace b200wmma
             return reinterpret_cast<uintptr_t>(p) % bytes == 0;
         }
 
-        template <typename T>
-        int quantize(bool nv, bool columns, QuantizeParams const& p, uint32_t blocks, cudaStream_t stream)
+        // Slabs of 32 rows that hold a row, or (`whole`) whose scales are written: those of whole
+        // tiles of 128.
+        uint32_t slabsOf(uint32_t rows, bool whole)
         {
-            // Wide loads where every row (or pair of rows) starts on their boundary.  A block takes
-            // 32 rows (rows contiguous along k) or 128; `blocks` counts tiles of 128.
+            return whole ? mxRowTiles(rows) * 4u : uint32_t((uint64_t(rows) + SLAB_ROWS - 1u) / SLAB_ROWS);
+        }
+
+        template <typename T>
+        int quantize(bool nv, bool columns, QuantizeParams p, cudaStream_t stream)
+        {
+            // Wide loads where every row (or pair of rows) starts on their boundary.
             const uint64_t width = columns ? 2 * sizeof(T) : 16;
             const bool     vec   = aligned(p.x, width) && p.ldx * sizeof(T) % width == 0;
+            const uint32_t slabs = slabsOf(p.rows, true);
+            p.tilesPerBlock      = tilesPerBlock(uint64_t(slabs) * p.tilesK, p.tilesK);
+            const uint32_t blocks = columns ? mxRowTiles(p.rows) * p.groups
+                                            : slabs * ((p.tilesK + p.tilesPerBlock - 1u) / p.tilesPerBlock);
             auto launch = [&](auto kernel) {
-                return cudaToStatus(launchOverlapped(kernel, dim3(columns ? blocks : 4u * blocks), dim3(THREADS), 0, stream, p));
+                return cudaToStatus(launchOverlapped(kernel, dim3(blocks), dim3(THREADS), 0, stream, p));
             };
             if(columns)
                 return nv ? (vec ? launch(quantizeColumnsKernel<T, true, true>) : launch(quantizeColumnsKernel<T, true, false>))
@@ -550,13 +640,14 @@ namespace b200wmma
         }
 
         template <typename T>
-        int dequantize(bool nv, DequantizeParams const& p, uint32_t blocks, cudaStream_t stream)
+        int dequantize(bool nv, DequantizeParams p, cudaStream_t stream)
         {
-            const bool vec = aligned(p.out, 16) && p.ldo * sizeof(T) % 16 == 0;
-            // a block takes 32 rows; slabs without a row have nothing to do
-            const uint32_t slabs = blocks / p.tilesK * 4u - (p.rows % 128u ? (127u - (p.rows - 1u) % 128u) / 32u : 0u);
+            const bool     vec   = aligned(p.out, 16) && p.ldo * sizeof(T) % 16 == 0;
+            const uint32_t slabs = slabsOf(p.rows, false);
+            p.tilesPerBlock      = tilesPerBlock(uint64_t(slabs) * p.tilesK, p.tilesK);
+            const uint32_t blocks = slabs * ((p.tilesK + p.tilesPerBlock - 1u) / p.tilesPerBlock);
             auto launch = [&](auto kernel) {
-                return cudaToStatus(launchOverlapped(kernel, dim3(slabs * p.tilesK), dim3(THREADS), 0, stream, p));
+                return cudaToStatus(launchOverlapped(kernel, dim3(blocks), dim3(THREADS), 0, stream, p));
             };
             return nv ? (vec ? launch(dequantizeKernel<T, true, true>) : launch(dequantizeKernel<T, true, false>))
                       : (vec ? launch(dequantizeKernel<T, false, true>) : launch(dequantizeKernel<T, false, false>));
@@ -565,7 +656,7 @@ namespace b200wmma
         // What both directions check; OK or a status.
         int checkOperand(int fmt, int dtype, uint32_t rows, uint32_t k, void const* values,
                          uint64_t ld, uint64_t span, int exponent, void const* codes, uint64_t ldq,
-                         void const* scales, uint64_t* blocks)
+                         void const* scales)
         {
             if(!values || !codes || !scales || rows == 0 || k == 0 || ld < span || ldq < mxPitch(k)
                || exponent < -64 || exponent > 64)
@@ -574,8 +665,8 @@ namespace b200wmma
                 return B200WMMA_ERR_UNSUPPORTED;
             if(!aligned(codes, 16) || !aligned(scales, 16) || ldq % 16 || !aligned(values, dtypeSize(dtype)))
                 return B200WMMA_ERR_ALIGNMENT;
-            *blocks = uint64_t(mxRowTiles(rows)) * ((uint64_t(k) + TILE_K - 1) / TILE_K);
-            if(*blocks > 0x1fffffffull)
+            // blocks of a launch, four slabs to a tile of 128 rows
+            if(uint64_t(mxRowTiles(rows)) * ((uint64_t(k) + TILE_K - 1) / TILE_K) > 0x1fffffffull)
                 return B200WMMA_ERR_TOO_LARGE;
             return B200WMMA_OK;
         }
@@ -605,46 +696,44 @@ int b200wmma_mx_quantize(int fmt, int in_dtype, uint32_t rows, uint32_t k, const
     const bool columns = layout == B200WMMA_COL_MAJOR;
     if(layout != B200WMMA_ROW_MAJOR && !columns)
         return B200WMMA_ERR_INVALID_ARG;
-    uint64_t  blocks = 0;
     const int rc = checkOperand(fmt, in_dtype, rows, k, x, ldx, columns ? rows : k, exponent, codes,
-                                ldq, scales, &blocks);
+                                ldq, scales);
     if(rc != B200WMMA_OK)
         return rc;
     const bool           nv = fmt == B200WMMA_NVF4;
     const QuantizeParams p{x, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), ldq, ldx,
                            rows, k, mxGroups(nv, k), uint32_t((uint64_t(k) + TILE_K - 1) / TILE_K),
-                           ldexpf(1.0f, -exponent)};
+                           0, ldexpf(1.0f, -exponent)};
     const cudaStream_t   s = static_cast<cudaStream_t>(stream);
     switch(in_dtype)
     {
     case B200WMMA_F16:
-        return quantize<__half>(nv, columns, p, uint32_t(blocks), s);
+        return quantize<__half>(nv, columns, p, s);
     case B200WMMA_BF16:
-        return quantize<__nv_bfloat16>(nv, columns, p, uint32_t(blocks), s);
+        return quantize<__nv_bfloat16>(nv, columns, p, s);
     }
-    return quantize<float>(nv, columns, p, uint32_t(blocks), s);
+    return quantize<float>(nv, columns, p, s);
 }
 
 int b200wmma_mx_dequantize(int fmt, int out_dtype, uint32_t rows, uint32_t k, const void* codes,
                            uint64_t ldq, const void* scales, int exponent, void* out, uint64_t ldo,
                            void* stream)
 {
-    uint64_t  blocks = 0;
-    const int rc = checkOperand(fmt, out_dtype, rows, k, out, ldo, k, exponent, codes, ldq, scales, &blocks);
+    const int rc = checkOperand(fmt, out_dtype, rows, k, out, ldo, k, exponent, codes, ldq, scales);
     if(rc != B200WMMA_OK)
         return rc;
     const bool             nv = fmt == B200WMMA_NVF4;
     const DequantizeParams p{static_cast<uint8_t const*>(codes), static_cast<uint8_t const*>(scales),
                              out, ldq, ldo, rows, k, mxGroups(nv, k),
-                             uint32_t((uint64_t(k) + TILE_K - 1) / TILE_K), ldexpf(1.0f, exponent)};
+                             uint32_t((uint64_t(k) + TILE_K - 1) / TILE_K), 0, ldexpf(1.0f, exponent)};
     const cudaStream_t     s = static_cast<cudaStream_t>(stream);
     switch(out_dtype)
     {
     case B200WMMA_F16:
-        return dequantize<__half>(nv, p, uint32_t(blocks), s);
+        return dequantize<__half>(nv, p, s);
     case B200WMMA_BF16:
-        return dequantize<__nv_bfloat16>(nv, p, uint32_t(blocks), s);
+        return dequantize<__nv_bfloat16>(nv, p, s);
     }
-    return dequantize<float>(nv, p, uint32_t(blocks), s);
+    return dequantize<float>(nv, p, s);
 }
 }
