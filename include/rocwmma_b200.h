@@ -294,7 +294,8 @@ B200WMMA_API uint64_t b200wmma_mx_scale_bytes(int fmt, uint32_t rows, uint32_t k
  * Quantises `rows` x `k` values x (F16, BF16 or F32; any alignment of whole elements), stored
  * row-major (value (r, i) at x[r * ldx + i]) or column-major (x[i * ldx + r]); the codes of a row
  * are contiguous along k either way, so the second form makes the operand of a product that sums
- * over the first form's rows.  With y = x * 2^-exponent (|exponent| <= 64) and a = max |y| of a block:
+ * over the first form's rows.  With y = x * 2^-exponent, in fp32, (|exponent| <= 64) and a = max |y|
+ * of a block:
  *   MXF4  scale 2^(floor(log2 a) - 2), at least 2^-127
  *   NVF4  scale E4M3(min(a / 6, 448)), rounded to nearest even
  *   code  E2M1(y / scale), rounded to nearest even, magnitudes over 6 become 6.

@@ -24,7 +24,6 @@ namespace b200wmma
         constexpr uint32_t ROW_TILE    = 128;
         constexpr uint32_t CODE_BYTES  = ROW_TILE * 128;
         constexpr uint32_t NUM_THREADS = 192;
-        constexpr uint32_t EPI_THREADS = 128;
         constexpr uint32_t MAX_STAGES  = 8;
         constexpr uint32_t PREFETCH_SLOTS = 8; // of a block's stretch, requested into L2 ahead
         constexpr long long SETTLE_CYCLES = 2000000; // leaving early: copies in flight land
@@ -412,7 +411,7 @@ namespace b200wmma
         // A pair of blocks owns a 256 x 256 tile (cta_group::2): each stages its own 128 rows of
         // A and half of the columns of B, the scales of its rows of A and those of all of B; the
         // even block issues MMAs of M = 256.  Persistent; warp 0 loads, warp 1 multiplies, warps 2
-        // to 5 drain.
+        // to 9 drain, warp 10 moves boxes of C and D.
         //
         // Tensor memory has 512 columns: two accumulators of 256 would leave none for the scales.
         // So the two overlap: the second starts at column ACC1, the scales of two ring slots lie
@@ -422,6 +421,8 @@ namespace b200wmma
         constexpr uint32_t P_STAGES    = 5;
         constexpr uint32_t BOX_BYTES   = 128 * 64; // 128 rows x 64 bytes of D (or C)
         constexpr uint32_t BOXES       = 4;
+        constexpr uint32_t P_THREADS   = 352;
+        constexpr uint32_t DRAIN_WARPS = 8;
 
         struct PairParams
         {
@@ -434,7 +435,8 @@ namespace b200wmma
         };
         struct PairControl
         {
-            uint64_t   full[P_STAGES], empty[P_STAGES], accFull[2], accShared, cFull[BOXES];
+            uint64_t   full[P_STAGES], empty[P_STAGES], accFull[2], accShared;
+            uint64_t   cFull[BOXES], boxFull[BOXES], boxFree[BOXES];
             AbortState abort;
             uint32_t   tmemBase;
         };
@@ -449,118 +451,179 @@ namespace b200wmma
             return 1024u + P_STAGES * pairSlotBytes<KIND>() + BOXES * BOX_BYTES + uint32_t(sizeof(PairControl));
         }
 
-        // Drains one tile's accumulator.  A box of D is 128 rows x 64 bytes: TMEM -> registers
-        // -> shared memory in the TMA's 64-byte swizzle -> TMA store; with beta != 0 the box of C
-        // comes to the same place by TMA two boxes ahead and is combined there.  Four boxes take
-        // turns: once a store is issued, the one two before it has been read out, so that one
-        // barrier a box is enough.  A box that D's last column cuts inside a 16-byte piece is
-        // stored by the threads.
+        // The boxes of one tile, 128 rows x 64 bytes of D each, in the order in which they are drained:
+        // from column `first` on, around the tile's end.  Those that hold a whole number of 16-byte
+        // pieces of D pass through shared memory (`staged`); one that D's last column cuts inside a
+        // piece is stored by the draining threads.
         template <typename OutT>
-        __device__ inline bool drainTile(PairControl* ctl, uint8_t* staging, CUtensorMap const* mapC,
-                                         CUtensorMap const* mapD, PairParams const& p, uint32_t taddr,
-                                         uint32_t first, uint32_t shared, uint32_t accBar, uint32_t accPhase,
-                                         uint32_t row0, uint32_t rowIn, uint32_t col0, uint32_t& boxes,
-                                         uint32_t leaderShared)
+        struct Boxes
         {
-            constexpr uint32_t COLS   = 64 / sizeof(OutT);
-            constexpr uint32_t VEC    = 16 / sizeof(OutT);
-            constexpr uint32_t GROUPS = P_TILE / COLS;
-            const bool         leader = threadIdx.x == 64u;
-            const bool         useC   = p.c != nullptr;
-            const uint32_t     left   = p.n - col0;
-            const uint32_t     valid  = min(GROUPS, (left + COLS - 1u) / COLS);
-            const uint32_t     ragged = left < P_TILE && left % VEC != 0u ? valid - 1u : GROUPS; // box stored by threads
-            uint32_t           asked = 0, askedBoxes = boxes; // boxes of C: next group in order, next count
-            auto group = [&](uint32_t i) { return (first / COLS + i) % GROUPS; };
-            auto askForC = [&] { // leader only
-                while(asked < GROUPS && (group(asked) >= valid || group(asked) == ragged))
-                    ++asked;
-                if(asked == GROUPS)
-                    return;
-                const uint32_t b = askedBoxes % BOXES;
-                mbar_expect_tx(&ctl->cFull[b], BOX_BYTES);
-                tma_load_2d(staging + b * BOX_BYTES, mapC, &ctl->cFull[b], int32_t(col0 + group(asked) * COLS), int32_t(row0));
-                ++asked;
-                ++askedBoxes;
-            };
-            if(useC && leader)
+            static constexpr uint32_t COLS  = 64 / sizeof(OutT);
+            static constexpr uint32_t VEC   = 16 / sizeof(OutT);
+            static constexpr uint32_t COUNT = P_TILE / COLS;
+            uint32_t first, left, valid, ragged;
+            __device__ Boxes(PairParams const& p, uint32_t col0, uint32_t firstCol)
+                : first(firstCol / COLS), left(p.n - col0), valid(min(COUNT, (left + COLS - 1u) / COLS)),
+                  ragged(left < P_TILE && left % VEC != 0u ? valid - 1u : COUNT)
             {
-                askForC();
-                askForC();
             }
-            const bool ready = mbar_wait(&ctl->accFull[accBar], accPhase, &ctl->abort, WAIT_ACC_FULL);
-            if(!named_barrier_all(1, EPI_THREADS, ready))
+            __device__ uint32_t at(uint32_t i) const
+            {
+                return (first + i) % COUNT;
+            }
+            __device__ bool staged(uint32_t box) const
+            {
+                return box < valid && box != ragged;
+            }
+        };
+
+        // Warp 10, one thread: boxes of D go out by TMA as the draining warps fill them; with C, boxes
+        // of it come in by TMA to where D's will be, up to four ahead.
+        template <typename OutT>
+        __device__ inline bool moveBoxes(PairControl* ctl, uint8_t* staging, CUtensorMap const* mapC, CUtensorMap const* mapD,
+                                         PairParams const& p, uint32_t first, uint32_t row0, uint32_t col0, uint32_t& count)
+        {
+            using B = Boxes<OutT>;
+            const B    boxes(p, col0, first);
+            const bool useC = p.c != nullptr;
+            uint32_t   asked = 0, askedCount = count;
+            auto       askForC = [&] {
+                while(asked < B::COUNT && !boxes.staged(boxes.at(asked)))
+                    ++asked;
+                if(asked == B::COUNT)
+                    return;
+                const uint32_t b = askedCount % BOXES;
+                mbar_expect_tx(&ctl->cFull[b], BOX_BYTES);
+                tma_load_2d(staging + b * BOX_BYTES, mapC, &ctl->cFull[b], int32_t(col0 + boxes.at(asked) * B::COLS), int32_t(row0));
+                ++asked;
+                ++askedCount;
+            };
+            if(useC) // the boxes of the tile before have been read out
+                for(uint32_t b = 0; b < BOXES; ++b)
+                    askForC();
+            for(uint32_t i = 0; i < B::COUNT; ++i)
+            {
+                const uint32_t box = boxes.at(i);
+                if(!boxes.staged(box))
+                    continue;
+                const uint32_t b = count % BOXES;
+                if(!mbar_wait(&ctl->boxFull[b], (count / BOXES) & 1u, &ctl->abort, WAIT_ACC_FULL))
+                    return false;
+                tma_store_2d(mapD, staging + b * BOX_BYTES, int32_t(col0 + box * B::COLS), int32_t(row0));
+                tma_store_commit();
+                if(useC)
+                {
+                    tma_store_wait_read<0>();
+                    askForC();
+                }
+                else
+                {
+                    // the store before has been read out (the first box of all has none before it)
+                    tma_store_wait_read<1>();
+                    if(count > 0u)
+                        mbar_arrive(&ctl->boxFree[(count - 1u) % BOXES]);
+                }
+                ++count;
+            }
+            if(useC)
+                tma_store_wait_read<0>();
+            return true;
+        }
+
+        // Drains one tile's accumulator: TMEM -> registers -> shared memory in the TMA's 64-byte
+        // swizzle, in place of C's box where there is one.  Two sets of four warps take boxes in
+        // turn.  (Four warps, with one of their threads moving the boxes as well: 4.7 us for the last
+        // tile of 256 columns bf16, 11 us f32 with C; so: DRAIN_US.)
+        template <typename OutT, bool C>
+        __device__ inline bool drainTile(PairControl* ctl, uint8_t* staging, PairParams const& p, uint32_t taddr, uint32_t set,
+                                         uint32_t first, uint32_t shared, uint32_t accBar, uint32_t accPhase, uint32_t row0,
+                                         uint32_t rowIn, uint32_t col0, uint32_t& count, uint32_t leaderShared)
+        {
+            using B = Boxes<OutT>;
+            constexpr uint32_t COLS = B::COLS, VEC = B::VEC;
+            const B            boxes(p, col0, first);
+            const uint32_t     row = row0 + rowIn, lastShared = shared / COLS - 1u - (shared / COLS - 1u + set) % 2u;
+            if constexpr(C)
+            {
+                // the row's part of C into L2 while the tile is multiplied
+                if(row < p.m)
+                {
+                    uint8_t const* c = static_cast<uint8_t const*>(p.c) + (uint64_t(row) * p.ldc + col0) * sizeof(OutT);
+                    const uint32_t bytes = min(P_TILE, boxes.left) * uint32_t(sizeof(OutT));
+                    for(uint32_t at = set * 128u; at < bytes; at += 256u)
+                        prefetch_l2(c + at);
+                }
+            }
+            if(!__all_sync(0xffffffffu, mbar_wait(&ctl->accFull[accBar], accPhase, &ctl->abort, WAIT_ACC_FULL)))
                 return false;
             tc_fence_after_sync();
-            const uint32_t row = row0 + rowIn;
 #pragma unroll 1
-            for(uint32_t i = 0; i < GROUPS; ++i)
+            for(uint32_t i = 0; i < B::COUNT; ++i)
             {
-                const uint32_t g = group(i);
-                uint32_t       raw[COLS];
-                if(g < valid)
+                const uint32_t box = boxes.at(i), mine = count;
+                count += boxes.staged(box) ? 1u : 0u;
+                if(i % 2u != set)
+                    continue;
+                uint32_t raw[COLS];
+                if(box < boxes.valid)
                 {
                     if constexpr(COLS == 32)
-                        tmem_load_32x32b_x32(taddr + g * COLS, raw);
+                        tmem_load_32x32b_x32(taddr + box * COLS, raw);
                     else
-                        tmem_load_32x32b_x16(taddr + g * COLS, raw);
+                        tmem_load_32x32b_x16(taddr + box * COLS, raw);
                     tmem_load_wait();
                 }
-                if(i + 1u == shared / COLS)
+                if(i == lastShared)
                 {
-                    // the columns that the next tile's accumulator shares are out
+                    // this warp's part of the columns that the next tile's accumulator shares is out
                     tc_fence_before_sync();
-                    mbar_arrive_cluster(leaderShared);
+                    if(rowIn % 32u == 0u)
+                        mbar_arrive_cluster(leaderShared);
                 }
-                if(g >= valid)
+                if(box >= boxes.valid)
                     continue;
-                if(g == ragged)
+                if(box == boxes.ragged)
                 {
 #pragma unroll
                     for(uint32_t e = 0; e < COLS; ++e)
-                        if(row < p.m && g * COLS + e < left)
+                        if(row < p.m && box * COLS + e < boxes.left)
                         {
-                            const uint64_t col = col0 + g * COLS + e;
-                            OutT const*    c   = useC ? static_cast<OutT const*>(p.c) + uint64_t(row) * p.ldc + col : nullptr;
+                            const uint64_t col = col0 + box * COLS + e;
+                            OutT const*    c   = C ? static_cast<OutT const*>(p.c) + uint64_t(row) * p.ldc + col : nullptr;
                             static_cast<OutT*>(p.d)[uint64_t(row) * p.ldd + col]
                                 = finish<OutT>(__uint_as_float(raw[e]), p.alpha, p.beta, c);
                         }
                     continue;
                 }
-                const uint32_t b   = boxes % BOXES;
-                uint8_t*       box = staging + b * BOX_BYTES;
-                const bool landed = !useC || mbar_wait(&ctl->cFull[b], (boxes / BOXES) & 1u, &ctl->abort, WAIT_STAGE_FULL);
+                const uint32_t b = mine % BOXES, use = (mine / BOXES) & 1u;
+                const bool     open = C ? mbar_wait(&ctl->cFull[b], use, &ctl->abort, WAIT_STAGE_FULL)
+                                        : mbar_wait(&ctl->boxFree[b], use ^ 1u, &ctl->abort, WAIT_DRAIN);
+                if(!__all_sync(0xffffffffu, open))
+                    return false;
+                uint8_t* at = staging + b * BOX_BYTES + rowIn * 64u;
 #pragma unroll
                 for(uint32_t ch = 0; ch < 4u; ++ch)
                 {
                     // 64-byte swizzle: piece index ^ (row / 2 % 4)
-                    uint4* piece = reinterpret_cast<uint4*>(box + rowIn * 64u + ((ch ^ ((rowIn >> 1) & 3u)) << 4));
+                    uint4* piece = reinterpret_cast<uint4*>(at + ((ch ^ ((rowIn >> 1) & 3u)) << 4));
                     alignas(16) OutT v[VEC];
-                    if(useC)
+                    if constexpr(C)
                         *reinterpret_cast<uint4*>(v) = *piece;
 #pragma unroll
                     for(uint32_t e = 0; e < VEC; ++e)
-                        v[e] = finish<OutT>(__uint_as_float(raw[ch * VEC + e]), p.alpha, p.beta, useC ? &v[e] : nullptr);
+                        v[e] = finish<OutT>(__uint_as_float(raw[ch * VEC + e]), p.alpha, p.beta, C ? &v[e] : nullptr);
                     *piece = *reinterpret_cast<uint4 const*>(v);
                 }
                 fence_async_shared();
-                if(!named_barrier_all(1, EPI_THREADS, landed))
-                    return false;
-                if(leader)
-                {
-                    tma_store_2d(mapD, box, int32_t(col0 + g * COLS), int32_t(row0));
-                    tma_store_commit();
-                    tma_store_wait_read<2>();
-                    if(useC)
-                        askForC();
-                }
-                ++boxes;
+                __syncwarp();
+                if(rowIn % 32u == 0u)
+                    mbar_arrive(&ctl->boxFull[b]);
             }
             return true;
         }
 
         template <ScaleKind KIND, typename OutT>
-        __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
+        __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
             mxGemmPairKernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
                              const __grid_constant__ CUtensorMap mapScaleA,
                              const __grid_constant__ CUtensorMap mapScaleB,
@@ -591,9 +654,13 @@ namespace b200wmma
                 }
                 for(uint32_t b = 0; b < 2u; ++b)
                     mbar_init(&ctl->accFull[b], 1);
-                mbar_init(&ctl->accShared, 2u * EPI_THREADS);
+                mbar_init(&ctl->accShared, 2u * DRAIN_WARPS);
                 for(uint32_t b = 0; b < BOXES; ++b)
+                {
                     mbar_init(&ctl->cFull[b], 1);
+                    mbar_init(&ctl->boxFull[b], DRAIN_WARPS / 2u);
+                    mbar_init(&ctl->boxFree[b], 1);
+                }
                 ctl->abort.flag = 0;
                 ctl->abort.code = 0;
                 mbar_init_fence();
@@ -718,26 +785,32 @@ namespace b200wmma
                     }
                 }
             }
-            else
+            else if(warp < 2u + DRAIN_WARPS)
             {
-                const uint32_t quad = warp % 4, rowIn = quad * 32u + lane;
+                const uint32_t quad = warp % 4, rowIn = quad * 32u + lane, set = (warp - 2u) / 4u;
                 const uint32_t leaderShared = map_to_cta(smem_addr(&ctl->accShared), 0);
-                uint32_t       boxes = 0;
-                for(uint32_t i = 0; sched.get(pairId, i, tm, col0, width); ++i)
+                uint32_t       count = 0;
+                bool           ok    = true;
+                for(uint32_t i = 0; ok && sched.get(pairId, i, tm, col0, width); ++i)
                 {
                     // the second accumulator's shared columns are its first ones, the first one's its last
-                    const uint32_t buf = i & 1u;
-                    if(!drainTile<OutT>(ctl, staging, &mapC, &mapD, p, tmem + ((quad * 32u) << 16) + buf * ACC1,
-                                        buf ? 0u : ACC1, SHARED, buf, (i >> 1) & 1u, tm * P_TILE + rank * 128u, rowIn,
-                                        col0, boxes, leaderShared))
-                    {
-                        if(threadIdx.x == 64u)
-                            settle();
-                        break;
-                    }
+                    const uint32_t buf = i & 1u, taddr = tmem + ((quad * 32u) << 16) + buf * ACC1;
+                    const uint32_t first = buf ? 0u : ACC1, row0 = tm * P_TILE + rank * 128u;
+                    ok = p.c ? drainTile<OutT, true>(ctl, staging, p, taddr, set, first, SHARED, buf, (i >> 1) & 1u, row0, rowIn,
+                                                     col0, count, leaderShared)
+                             : drainTile<OutT, false>(ctl, staging, p, taddr, set, first, SHARED, buf, (i >> 1) & 1u, row0, rowIn,
+                                                      col0, count, leaderShared);
                 }
-                if(threadIdx.x == 64u)
-                    tma_store_wait_read<0>(); // shared memory outlives the stores' reads of it
+            }
+            else if(elect_one())
+            {
+                uint32_t count = 0;
+                bool     ok    = true;
+                for(uint32_t i = 0; ok && sched.get(pairId, i, tm, col0, width); ++i)
+                    ok = moveBoxes<OutT>(ctl, staging, &mapC, &mapD, p, i & 1u ? 0u : ACC1, tm * P_TILE + rank * 128u, col0, count);
+                if(!ok)
+                    settle();
+                tma_store_wait_read<0>(); // shared memory outlives the stores' reads of it
             }
 
             tc_fence_before_sync();
@@ -866,7 +939,7 @@ namespace b200wmma
                 return rc;
             const PairParams p{q.c, q.d, q.m, q.n, q.k, q.ldc, q.ldd, q.alpha, q.beta, 16u, q.status};
             const uint32_t   pairs = uint32_t(tiles < uint64_t(sms / 2) ? tiles : uint64_t(sms / 2));
-            return cudaToStatus(launchOverlapped(mxGemmPairKernel<KIND, OutT>, dim3(2u * pairs), dim3(NUM_THREADS), smem,
+            return cudaToStatus(launchOverlapped(mxGemmPairKernel<KIND, OutT>, dim3(2u * pairs), dim3(P_THREADS), smem,
                                                  stream, mapA, mapB, mapScaleA, mapScaleB, mapC, mapD, p));
         }
 

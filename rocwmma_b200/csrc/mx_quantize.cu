@@ -28,150 +28,195 @@ namespace b200wmma
         constexpr uint32_t THREADS   = 256;
         constexpr uint32_t SLAB_ROWS = 32; // rows of a block: one 32-bit word of each scale tile row
 
-        // Eight consecutive values of a row as they are stored.
+        // Sixteen consecutive values of a row as they are stored.
+        constexpr uint32_t RUN = 16;
         template <typename T>
-        struct alignas(16) Raw8
+        struct alignas(32) Run
         {
-            T v[8];
+            T v[RUN];
         };
         template <typename T>
-        __device__ inline Raw8<T> zero8()
+        __device__ inline Run<T> zeroRun()
         {
-            Raw8<T> r;
+            Run<T> r;
 #pragma unroll
-            for(int i = 0; i < 8; ++i)
+            for(uint32_t i = 0; i < RUN; ++i)
                 r.v[i] = T(0.0f);
             return r;
         }
         template <typename T>
-        __device__ inline Raw8<T> load8(T const* p)
+        __device__ inline Run<T> loadRun(T const* p)
         {
-            Raw8<T> r;
+            Run<T>    r;
+            uint32_t* w = reinterpret_cast<uint32_t*>(&r);
 #pragma unroll
-            for(int i = 0; i < int(sizeof(T) * 8 / 16); ++i)
-                reinterpret_cast<uint4*>(&r)[i] = reinterpret_cast<uint4 const*>(p)[i];
+            for(uint32_t i = 0; i < sizeof(r) / 4u; i += 8u)
+                asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                             : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]), "=r"(w[i + 4]),
+                               "=r"(w[i + 5]), "=r"(w[i + 6]), "=r"(w[i + 7])
+                             : "l"(reinterpret_cast<uint32_t const*>(p) + i));
             return r;
         }
+        template <typename T>
+        __device__ inline void storeRun(T* p, Run<T> const& r)
+        {
+            uint32_t const* w = reinterpret_cast<uint32_t const*>(&r);
+#pragma unroll
+            for(uint32_t i = 0; i < sizeof(r) / 4u; i += 8u)
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<uint32_t*>(p) + i),
+                             "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]),
+                             "r"(w[i + 6]), "r"(w[i + 7])
+                             : "memory");
+        }
 
-        // Largest |v| of values as the bits of a float: ordered like the values, a NaN above the
-        // infinity.  16-bit types compare two magnitudes at a time, as integers.
+        // Values are worked on as the 32-bit words they come in, two to a word if they have 16 bits:
+        // taken out one by one, they cost twice the instructions that the arithmetic does.
         template <typename T>
-        __device__ inline uint32_t wordTop(uint32_t top, T const (&v)[2])
+        struct Words
         {
-            uint32_t w;
-            memcpy(&w, v, 4);
-            return __vmaxu2(top, w & 0x7fff7fffu);
-        }
-        __device__ inline float topFloat(uint32_t bits, __half)
-        {
-            return __half2float(__ushort_as_half(uint16_t(bits)));
-        }
-        __device__ inline float topFloat(uint32_t bits, __nv_bfloat16)
-        {
-            return __uint_as_float(bits << 16);
-        }
-        // A running maximum; merged over lanes or places, then turned into a float.
-        template <typename T>
-        struct Top
-        {
-            uint32_t bits = 0;
-            __device__ void two(T a, T b)
+            static constexpr uint32_t PER = 4 / sizeof(T); // values of a word
+            static __device__ float value(uint32_t w, uint32_t) // of 32 bits
             {
-                if constexpr(sizeof(T) == 2)
-                {
-                    const T v[2] = {a, b};
-                    bits         = wordTop(bits, v);
-                }
-                else
-                    bits = max(bits, max(__float_as_uint(a) & 0x7fffffffu, __float_as_uint(b) & 0x7fffffffu));
+                return __uint_as_float(w);
             }
-            __device__ void lanes(uint32_t with)
+            // running maximum of magnitudes, place by place; a NaN stays one
+            static __device__ uint32_t top(uint32_t most, uint32_t w)
             {
-                const uint32_t other = __shfl_xor_sync(0xffffffffu, bits, with);
-                if constexpr(sizeof(T) == 2)
-                    bits = __vmaxu2(bits, other);
-                else
-                    bits = max(bits, other);
+                return max(most, w & 0x7fffffffu);
             }
-            __device__ float value() const
+        };
+        template <typename T, typename T2>
+        struct Words16
+        {
+            static constexpr uint32_t PER = 2;
+            static __device__ uint32_t top(uint32_t most, uint32_t w)
             {
-                if constexpr(sizeof(T) == 2)
-                    return topFloat(max(bits & 0xffffu, bits >> 16), T());
-                else
-                    return __uint_as_float(bits);
+                const T2 m = __hmax2_nan(*reinterpret_cast<T2*>(&most), __habs2(*reinterpret_cast<T2*>(&w)));
+                return *reinterpret_cast<uint32_t const*>(&m);
+            }
+        };
+        template <>
+        struct Words<__nv_bfloat16> : Words16<__nv_bfloat16, __nv_bfloat162>
+        {
+            static __device__ float value(uint32_t w, uint32_t place)
+            {
+                return __uint_as_float(place ? w & 0xffff0000u : w << 16);
+            }
+        };
+        template <>
+        struct Words<__half> : Words16<__half, __half2>
+        {
+            static __device__ float value(uint32_t w, uint32_t place)
+            {
+                const float2 f = __half22float2(*reinterpret_cast<__half2*>(&w));
+                return place ? f.y : f.x;
             }
         };
 
-        // The scale of a block whose largest magnitude is `top`.
+        // The scale of a block whose largest magnitude is `top`, for values x with y = x * factor.
         struct Scale
         {
             uint32_t byte;
-            float    inverse; // MXF4: exactly 1 / s; NVF4: 1 / s rounded; 0: codes are zero
+            float    times; // factor / s (NVF4: 1 / s rounded); 0: codes are zero
             float    value;
         };
         template <bool NV>
-        __device__ inline Scale scaleOf(float top)
+        __device__ inline Scale scaleOf(float top, float factor)
         {
-            const bool fine = top < __uint_as_float(0x7f800000u); // false for a NaN
-            Scale      s;
+            const float y    = top * factor;
+            const bool  fine = y < __uint_as_float(0x7f800000u); // false for a NaN
+            Scale       s;
             if constexpr(NV)
             {
-                const uint32_t byte = toE4m3(fminf(__fdiv_rn(fine ? top : 0.0f, 6.0f), 448.0f));
+                const uint32_t byte = toE4m3(fminf(__fdiv_rn(fine ? y : 0.0f, 6.0f), 448.0f));
                 s.value             = fromE4m3(byte);
-                s.inverse           = byte != 0u ? __frcp_rn(s.value) : 0.0f;
+                s.times             = byte != 0u ? __frcp_rn(s.value) * factor : 0.0f;
                 s.byte              = fine ? byte : 0x7fu;
             }
             else
             {
-                const uint32_t e    = __float_as_uint(fine ? top : 0.0f) >> 23;
+                const uint32_t e    = __float_as_uint(fine ? y : 0.0f) >> 23;
                 const uint32_t byte = e > 2u ? e - 2u : 0u;
                 s.value             = 0.0f;
-                s.inverse           = fine ? __uint_as_float((254u - byte) << 23) : 0.0f;
-                s.byte              = fine ? byte : 255u;
+                s.times = fine ? __uint_as_float((254u - byte) << 23) * factor : 0.0f;
+                s.byte  = fine ? byte : 255u;
             }
             return s;
         }
-
-        // y / s, exact as far as the rounding to E2M1 can see.  For NVF4 the borders between two
-        // codes are multiples m s of a 4-bit s by a 3-bit m: at most seven significant bits.  A
-        // quotient from 16-bit values (at most eleven bits) is on a border or at least 2^-11 of
-        // its size away from it, so y * (1 / s), which is off by less than 2^-22, is rounded to
-        // 14 bits: what lay on a border is there again, and nothing else gets there.  For 32-bit
-        // values the division is rounded correctly, which keeps the order to every border.
-        template <typename T, bool NV>
-        __device__ inline float scaledBy(float y, Scale const& s)
+        // Whether x * times is (x * factor) / s: not where times, about 4 / top, left fp32's range, as it
+        // does for blocks of values below 2^-125 with a factor of more than one.
+        __device__ inline bool safe(Scale const& s)
         {
-            if constexpr(!NV)
-                return y * s.inverse;
-            else if constexpr(sizeof(T) == 2)
-            {
-                const uint32_t q = __float_as_uint(y * s.inverse);
-                return __uint_as_float((q + 0x200u) & ~0x3ffu);
-            }
-            else
-                return s.inverse != 0.0f ? __fdiv_rn(y, s.value) : 0.0f;
+            const uint32_t e = __float_as_uint(s.times) >> 23;
+            return e - 1u < 254u || s.times == 0.0f;
         }
 
-        // Eight codes.  (A NaN or an infinity times an inverse of zero would not give codes of zero:
-        // those of such blocks are cleared as words.)
+        // Eight values to codes: y / s, exact as far as the rounding to E2M1 can see.  MXF4 divides by a
+        // power of two.  For NVF4 the borders between two codes are multiples m s of a 4-bit s by a
+        // 3-bit m: at most seven significant bits.  A quotient from 16-bit values (at most eleven
+        // bits) is on a border or at least 2^-11 of its size away from it, so x * (1 / s), which is
+        // off by less than 2^-22, is rounded to 14 bits: what lay on a border is there again, and
+        // nothing else gets there.  For 32-bit values the division is rounded correctly, which
+        // keeps the order to every border.
+        // (A NaN or an infinity times zero would not give codes of zero: those of blocks without a
+        // usable scale are cleared as words.)
         template <typename T, bool NV>
-        __device__ inline uint32_t codes8(T const (&x)[8], Scale const& s, float factor)
+        __device__ inline uint32_t codes8(float (&v)[8], Scale const& s, float factor)
         {
-            float v[8];
 #pragma unroll
             for(int i = 0; i < 8; ++i)
-                v[i] = toFloat(x[i]);
-            if(factor != 1.0f)
+            {
+                if constexpr(!NV)
+                    v[i] *= s.times;
+                else if constexpr(sizeof(T) == 2)
+                    v[i] = __uint_as_float((__float_as_uint(v[i] * s.times) + 0x200u) & ~0x3ffu);
+                else
+                    v[i] = s.times != 0.0f ? __fdiv_rn(v[i] * factor, s.value) : 0.0f;
+            }
+            const uint32_t c = e2m1x8(v);
+            return s.times != 0.0f ? c : 0u;
+        }
+        // The same in two steps, for blocks that safe() excludes.
+        template <bool NV>
+        __device__ inline uint32_t codes8Slow(float (&v)[8], Scale const& s, float factor)
+        {
+            Scale one = s;
+            one.times = NV ? 1.0f : __uint_as_float((254u - s.byte) << 23);
+#pragma unroll
+            for(int i = 0; i < 8; ++i)
+                v[i] = NV ? __fdiv_rn(v[i] * factor, s.value) : v[i] * factor;
+            return codes8<float, false>(v, one, 1.0f);
+        }
+
+        // Eight values as words to codes, for blocks that safe() admits.
+        template <typename T, bool NV>
+        __device__ inline uint32_t codesOf(uint32_t const* w, Scale const& s, float factor)
+        {
+            using W = Words<T>;
+            float v[8];
+            if constexpr(std::is_same<T, __nv_bfloat16>::value && !NV)
+            {
+                // times a power of two, two at a time: exact in bf16 (short of its subnormals, whose
+                // codes are zero)
+                const __nv_bfloat162 times = __float2bfloat162_rn(s.times); // exactly
+#pragma unroll
+                for(uint32_t j = 0; j < 4; ++j)
+                {
+                    const __nv_bfloat162 y  = __hmul2(*reinterpret_cast<__nv_bfloat162 const*>(&w[j]), times);
+                    const uint32_t       yw = *reinterpret_cast<uint32_t const*>(&y);
+                    v[2 * j]                = W::value(yw, 0);
+                    v[2 * j + 1]            = W::value(yw, 1);
+                }
+                const uint32_t c = e2m1x8(v);
+                return s.times != 0.0f ? c : 0u;
+            }
+            else
             {
 #pragma unroll
-                for(int i = 0; i < 8; ++i)
-                    v[i] *= factor;
+                for(uint32_t j = 0; j < 8; ++j)
+                    v[j] = W::value(w[j / W::PER], j % W::PER);
+                return codes8<T, NV>(v, s, factor);
             }
-#pragma unroll
-            for(int i = 0; i < 8; ++i)
-                v[i] = scaledBy<T, NV>(v[i], s);
-            const uint32_t c = e2m1x8(v);
-            return s.inverse != 0.0f ? c : 0u;
         }
 
         // Byte of (row, block) in a scale tile of its row.
@@ -253,117 +298,111 @@ namespace b200wmma
             return uint32_t(per < 1u ? 1u : per > 8u ? 8u : per < tilesK ? per : tilesK);
         }
 
-        // x row-major: k is contiguous.  A block takes 32 rows x 128 columns at a time: sixteen
-        // threads read 128 values of a row, eight each, and a block's largest magnitude comes from
-        // its two (NVF4) or four (MXF4) threads; those with the scales of four blocks write them as
-        // a word.  The values of the next tile are on their way while those of one are worked on.
+        // x row-major: k is contiguous.  A block takes 32 rows x 128 columns at a time: eight threads
+        // have 128 values of a row, sixteen each, which is a block (NVF4) or half of one (MXF4);
+        // those with the scales of four blocks write them as a word.  The values of the next tile
+        // are on their way while those of one are worked on.  (8192 x 8192 bf16 MXF4, 171 MB: 64 us
+        // with eight values a thread and maxima found as integers, ROWS_US so.)
         template <typename T, bool NV, bool VEC>
         __global__ void __launch_bounds__(THREADS) quantizeRowsKernel(const QuantizeParams p)
         {
-            constexpr uint32_t STEPS  = SLAB_ROWS / (THREADS / 16);
-            constexpr uint32_t GROUPS = TILE_K / (4u * mxBlock(NV)), LANES = mxBlock(NV) / 8u; // of a block
+            using W                   = Words<T>;
+            constexpr uint32_t GROUPS = TILE_K / (4u * mxBlock(NV)), LANES = mxBlock(NV) / RUN; // of a block
             const uint32_t across = (p.tilesK + p.tilesPerBlock - 1u) / p.tilesPerBlock;
             const uint32_t slab = blockIdx.x / across, tile0 = blockIdx.x % across * p.tilesPerBlock;
             const uint32_t tiles = min(p.tilesPerBlock, p.tilesK - tile0);
-            const uint32_t col = threadIdx.x % 16u * 8u, rowIn = threadIdx.x / 16u;
-            const uint64_t row0 = uint64_t(slab) * SLAB_ROWS;
+            const uint32_t col = threadIdx.x % 8u * RUN, r = threadIdx.x / 8u;
+            const uint64_t row0 = uint64_t(slab) * SLAB_ROWS, row = row0 + r, k0 = uint64_t(tile0) * TILE_K + col;
             const uint32_t rows = row0 < p.rows ? uint32_t(min(uint64_t(SLAB_ROWS), p.rows - row0)) : 0u;
-            // this thread's places in its rows: rowIn and rowIn + 16
-            T const*       x[STEPS];
-            uint8_t*       codes[STEPS];
-            uint8_t*       scales[STEPS];
-            const uint64_t k0 = uint64_t(tile0) * TILE_K + col;
-#pragma unroll
-            for(uint32_t i = 0; i < STEPS; ++i)
-            {
-                const uint32_t r = i * 16u + rowIn;
-                x[i]      = static_cast<T const*>(p.x) + (row0 + r) * p.ldx + k0;
-                codes[i]  = p.codes + (row0 + r) * p.ldq + k0 / 2u;
-                scales[i] = p.scales + (uint64_t(slab / 4u) * p.groups + k0 / (4u * mxBlock(NV))) * MX_TILE_BYTES
-                            + scaleOffset(slab % 4u * SLAB_ROWS + r, 0);
-            }
-            uint32_t       left  = p.k > k0 ? uint32_t(p.k - k0) : 0u; // columns from the thread's first on
-            uint32_t       pitch = mxPitch(p.k) > k0 / 2u ? uint32_t(mxPitch(p.k) - k0 / 2u) : 0u; // bytes
-            uint32_t       group = uint32_t(k0 / (4u * mxBlock(NV)));
+            T const*       x      = static_cast<T const*>(p.x) + row * p.ldx + k0;
+            uint8_t*       codes  = p.codes + row * p.ldq + k0 / 2u;
+            uint8_t*       scales = p.scales + (uint64_t(slab / 4u) * p.groups + k0 / (4u * mxBlock(NV))) * MX_TILE_BYTES
+                              + scaleOffset(slab % 4u * SLAB_ROWS + r, 0);
+            const uint32_t left  = r < rows && p.k > k0 ? uint32_t(p.k - k0) : 0u; // values from the first on
+            const uint32_t pitch = r < rows && mxPitch(p.k) > k0 / 2u ? uint32_t(mxPitch(p.k) - k0 / 2u) : 0u; // bytes
+            const uint32_t group = uint32_t(k0 / (4u * mxBlock(NV)));
             __shared__ alignas(16) uint8_t staged[VEC ? 16 : SLAB_ROWS * StagedRow<T>::PITCH];
-            auto fetch = [&](uint32_t t, Raw8<T>(&raw)[STEPS]) {
+            auto fetch = [&](uint32_t t) {
                 const uint32_t done = t * TILE_K;
-#pragma unroll
-                for(uint32_t i = 0; i < STEPS; ++i)
-                    raw[i] = zero8<T>();
+                Run<T>         raw;
                 if constexpr(VEC)
                 {
+                    if(left >= done + RUN)
+                        return loadRun(x + done);
+                    raw = zeroRun<T>();
 #pragma unroll
-                    for(uint32_t i = 0; i < STEPS; ++i)
-                        if(i * 16u + rowIn < rows && left >= done + 8u)
-                            raw[i] = load8(x[i] + done);
-                    if(left > done && left < done + 8u)
-                    {
-#pragma unroll
-                        for(uint32_t i = 0; i < STEPS; ++i)
-#pragma unroll
-                            for(uint32_t j = 0; j < 8u; ++j)
-                                if(i * 16u + rowIn < rows && done + j < left)
-                                    raw[i].v[j] = x[i][done + j];
-                    }
+                    for(uint32_t j = 0; j < RUN; ++j)
+                        if(done + j < left)
+                            raw.v[j] = x[done + j];
                 }
                 else
                 {
                     const uint32_t count = min(TILE_K, p.k - (tile0 + t) * TILE_K);
-                    auto rowAt = [&](uint32_t r) {
-                        return const_cast<T*>(static_cast<T const*>(p.x)) + (row0 + r) * p.ldx + uint64_t(tile0 + t) * TILE_K;
+                    auto rowAt = [&](uint32_t i) {
+                        return const_cast<T*>(static_cast<T const*>(p.x)) + (row0 + i) * p.ldx + uint64_t(tile0 + t) * TILE_K;
                     };
                     __syncthreads();
                     moveStaged<T, true>(staged, rows, count, rowAt);
                     __syncthreads();
-#pragma unroll
-                    for(uint32_t i = 0; i < STEPS; ++i)
+                    raw = zeroRun<T>();
+                    if(r < rows)
                     {
-                        const uint32_t r = i * 16u + rowIn;
-                        if(r < rows)
-                        {
-                            T const* at = reinterpret_cast<T const*>(staged + r * StagedRow<T>::PITCH)
-                                          + StagedRow<T>::shift(rowAt(r)) + col;
+                        T const* at = reinterpret_cast<T const*>(staged + r * StagedRow<T>::PITCH) + StagedRow<T>::shift(rowAt(r)) + col;
 #pragma unroll
-                            for(uint32_t j = 0; j < 8u; ++j)
-                                if(col + j < count)
-                                    raw[i].v[j] = at[j];
-                        }
+                        for(uint32_t j = 0; j < RUN; ++j)
+                            if(col + j < count)
+                                raw.v[j] = at[j];
                     }
                 }
+                return raw;
             };
             grid_dependency_wait();
             grid_launch_dependents();
-            Raw8<T> raw[STEPS], next[STEPS];
-            fetch(0, next);
+            Run<T> next = fetch(0);
             for(uint32_t t = 0; t < tiles; ++t)
             {
-#pragma unroll
-                for(uint32_t i = 0; i < STEPS; ++i)
-                    raw[i] = next[i];
+                const Run<T> raw = next;
                 if(t + 1u < tiles)
-                    fetch(t + 1u, next);
+                    next = fetch(t + 1u);
+                uint32_t const* w   = reinterpret_cast<uint32_t const*>(&raw);
+                uint32_t        top = 0;
 #pragma unroll
-                for(uint32_t i = 0; i < STEPS; ++i)
+                for(uint32_t j = 0; j < RUN / W::PER; ++j)
+                    top = W::top(top, w[j]);
+                if constexpr(!NV)
+                    top = W::top(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                if constexpr(W::PER == 2)
+                    top = W::top(top, top << 16 | top >> 16);
+                const Scale s = scaleOf<NV>(W::value(top, 0), p.factor);
+                uint32_t    code[RUN / 8];
+                if(safe(s))
                 {
-                    Top<T> top;
 #pragma unroll
-                    for(int j = 0; j < 8; j += 2)
-                        top.two(raw[i].v[j], raw[i].v[j + 1]);
-                    top.lanes(1);
-                    if constexpr(!NV)
-                        top.lanes(2);
-                    const Scale    s    = scaleOf<NV>(top.value() * p.factor);
-                    const uint32_t code = codes8<T, NV>(raw[i].v, s, p.factor);
-                    if(i * 16u + rowIn < rows && t * (TILE_K / 2u) < pitch)
-                        *reinterpret_cast<uint32_t*>(codes[i] + t * (TILE_K / 2u)) = code;
-                    // the bytes of four blocks, a word of the scale tile's row
-                    uint32_t word = s.byte << (8u * (threadIdx.x / LANES % 4u));
-                    word |= __shfl_xor_sync(0xffffffffu, word, LANES);
-                    word |= __shfl_xor_sync(0xffffffffu, word, 2u * LANES);
-                    if(threadIdx.x % (4u * LANES) == 0u && group + t * GROUPS < p.groups)
-                        *reinterpret_cast<uint32_t*>(scales[i] + t * (GROUPS * MX_TILE_BYTES)) = word;
+                    for(uint32_t c = 0; c < RUN / 8; ++c)
+                        code[c] = codesOf<T, NV>(w + c * (8 / W::PER), s, p.factor);
                 }
+                else
+                {
+#pragma unroll
+                    for(uint32_t c = 0; c < RUN / 8; ++c)
+                    {
+                        float v[8];
+#pragma unroll
+                        for(uint32_t j = 0; j < 8; ++j)
+                            v[j] = W::value(w[(c * 8 + j) / W::PER], j % W::PER);
+                        code[c] = codes8Slow<NV>(v, s, p.factor);
+                    }
+                }
+                if(t * (TILE_K / 2u) < pitch)
+                    *reinterpret_cast<uint2*>(codes) = make_uint2(code[0], code[1]);
+                codes += TILE_K / 2u;
+                // the bytes of four blocks, a word of the scale tile's row
+                uint32_t word = s.byte << (8u * (threadIdx.x / LANES % 4u));
+                word |= __shfl_xor_sync(0xffffffffu, word, LANES);
+                word |= __shfl_xor_sync(0xffffffffu, word, 2u * LANES);
+                if(threadIdx.x % (4u * LANES) == 0u && group + t * GROUPS < p.groups)
+                    *reinterpret_cast<uint32_t*>(scales) = word;
+                scales += GROUPS * MX_TILE_BYTES;
             }
         }
 
@@ -372,16 +411,19 @@ namespace b200wmma
         // consecutive values at a time and no maximum crosses a thread; the codes pass through
         // shared memory to leave as rows, the scale tile to leave whole.
         template <typename T, bool NV, bool VEC>
-        __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 4 : 3) quantizeColumnsKernel(const QuantizeParams p)
+        __global__ void __launch_bounds__(THREADS, NV ? 4 : 2) quantizeColumnsKernel(const QuantizeParams p)
         {
             constexpr uint32_t B     = mxBlock(NV);
             constexpr uint32_t BYTES = 4 * B / 2, PITCH = BYTES + 16; // of a staged row of codes
             __shared__ alignas(16) uint8_t scales[MX_TILE_BYTES];
             __shared__ alignas(16) uint8_t staged[128 * PITCH];
+            using W = Words<T>;
+            constexpr uint32_t PAIR = 2 / W::PER; // words of two values
             struct alignas(2 * sizeof(T)) Pair
             {
-                T v[2];
+                uint32_t w[PAIR];
             };
+            static_assert(sizeof(Pair) == 2 * sizeof(T), "two values");
             const uint32_t tileRow = blockIdx.x / p.groups, group = blockIdx.x % p.groups;
             const uint32_t r = threadIdx.x % 64u * 2u, blockIn = threadIdx.x / 64u;
             const uint64_t row = uint64_t(tileRow) * 128u + r, k0 = (uint64_t(group) * 4u + blockIn) * B;
@@ -392,7 +434,7 @@ namespace b200wmma
             T const* x = static_cast<T const*>(p.x) + row + k0 * p.ldx;
 #pragma unroll
             for(uint32_t i = 0; i < B; ++i)
-                v[i].v[0] = v[i].v[1] = T(0.0f);
+                v[i] = Pair{};
             if(VEC && row + 1u < p.rows)
             {
 #pragma unroll
@@ -406,35 +448,39 @@ namespace b200wmma
 #pragma unroll
                 for(uint32_t i = 0; i < B; ++i)
                 {
+                    T both[2] = {T(0.0f), T(0.0f)};
                     if(i < count && one)
-                        v[i].v[0] = x[i * p.ldx];
+                        both[0] = x[i * p.ldx];
                     if(i < count && two)
-                        v[i].v[1] = x[i * p.ldx + 1u];
+                        both[1] = x[i * p.ldx + 1u];
+                    memcpy(&v[i], both, sizeof(both));
                 }
             }
+            uint32_t tops[PAIR] = {}; // of 16 bits: both rows' in a word
 #pragma unroll
-            for(int j = 0; j < 2; ++j)
+            for(uint32_t i = 0; i < B; ++i)
+#pragma unroll
+                for(uint32_t j = 0; j < PAIR; ++j)
+                    tops[j] = W::top(tops[j], v[i].w[j]);
+#pragma unroll
+            for(uint32_t j = 0; j < 2; ++j)
             {
-                Top<T> top;
-#pragma unroll
-                for(uint32_t i = 0; i < B; i += 2)
-                    top.two(v[i].v[j], v[i + 1].v[j]);
-                const Scale s = scaleOf<NV>(top.value() * p.factor);
+                const Scale s = scaleOf<NV>(W::value(tops[j / W::PER], j % W::PER), p.factor);
                 uint32_t    words[B / 8];
 #pragma unroll
-                for(uint32_t w = 0; w < B / 8; ++w)
+                for(uint32_t c = 0; c < B / 8; ++c)
                 {
-                    T y[8];
+                    float y[8];
 #pragma unroll
                     for(uint32_t i = 0; i < 8; ++i)
-                        y[i] = v[w * 8 + i].v[j];
-                    words[w] = codes8<T, NV>(y, s, p.factor);
+                        y[i] = W::value(v[c * 8 + i].w[j / W::PER], j % W::PER);
+                    words[c] = safe(s) ? codes8<T, NV>(y, s, p.factor) : codes8Slow<NV>(y, s, p.factor);
                 }
                 scales[scaleOffset(r + j, blockIn)] = uint8_t(s.byte);
                 uint32_t* to = reinterpret_cast<uint32_t*>(staged + (r + j) * PITCH + blockIn * (B / 2));
 #pragma unroll
-                for(uint32_t w = 0; w < B / 8; ++w)
-                    to[w] = words[w];
+                for(uint32_t c = 0; c < B / 8; ++c)
+                    to[c] = words[c];
             }
             __syncthreads();
             const uint32_t at = threadIdx.x * 16u;
@@ -469,137 +515,92 @@ namespace b200wmma
 
         // Eight values: code * s is exact (three bits times at most four); so is the power of two, short
         // of the subnormals.
-        template <typename T, bool NV>
-        __device__ inline Raw8<T> values8(uint32_t codes, uint32_t byte, float factor)
+        template <typename T>
+        __device__ inline void values8(uint32_t codes, float s, float factor, T* out)
         {
-            const float s = NV ? fromE4m3(byte) : fromE8m0(byte);
-            float       v[8];
+            float v[8];
             e2m1x8ToFloat(codes, v);
 #pragma unroll
             for(int j = 0; j < 8; ++j)
-                v[j] *= s;
-            if(factor != 1.0f)
-            {
+                v[j] = v[j] * s * factor;
 #pragma unroll
-                for(int j = 0; j < 8; ++j)
-                    v[j] *= factor;
-            }
-            Raw8<T> o;
-            if constexpr(std::is_same<T, float>::value)
-            {
-#pragma unroll
-                for(int j = 0; j < 8; ++j)
-                    o.v[j] = v[j];
-            }
-            else
-            {
-#pragma unroll
-                for(int j = 0; j < 8; j += 2)
-                    if constexpr(std::is_same<T, __half>::value)
-                        reinterpret_cast<__half2*>(&o)[j / 2] = __floats2half2_rn(v[j], v[j + 1]);
-                    else
-                        reinterpret_cast<__nv_bfloat162*>(&o)[j / 2] = __floats2bfloat162_rn(v[j], v[j + 1]);
-            }
-            return o;
+            for(int j = 0; j < 8; j += 2)
+                if constexpr(std::is_same<T, __half>::value)
+                    reinterpret_cast<__half2*>(out)[j / 2] = __floats2half2_rn(v[j], v[j + 1]);
+                else if constexpr(std::is_same<T, __nv_bfloat16>::value)
+                    reinterpret_cast<__nv_bfloat162*>(out)[j / 2] = __floats2bfloat162_rn(v[j], v[j + 1]);
+                else
+                {
+                    out[j]     = v[j];
+                    out[j + 1] = v[j + 1];
+                }
         }
 
-        // A block takes 32 rows x 128 columns at a time, a thread eight codes of two rows; the codes
-        // of the next tile are on their way meanwhile.
+        // A block takes 32 rows x 128 columns at a time, a thread sixteen codes; those of the next
+        // tile are on their way meanwhile.
         template <typename T, bool NV, bool VEC>
         __global__ void __launch_bounds__(THREADS) dequantizeKernel(const DequantizeParams p)
         {
-            constexpr uint32_t STEPS  = SLAB_ROWS / (THREADS / 16);
             constexpr uint32_t GROUPS = TILE_K / (4u * mxBlock(NV));
             const uint32_t across = (p.tilesK + p.tilesPerBlock - 1u) / p.tilesPerBlock;
             const uint32_t slab = blockIdx.x / across, tile0 = blockIdx.x % across * p.tilesPerBlock;
             const uint32_t tiles = min(p.tilesPerBlock, p.tilesK - tile0);
-            const uint32_t col = threadIdx.x % 16u * 8u, rowIn = threadIdx.x / 16u;
-            const uint64_t row0 = uint64_t(slab) * SLAB_ROWS, k0 = uint64_t(tile0) * TILE_K + col;
+            const uint32_t col = threadIdx.x % 8u * RUN, r = threadIdx.x / 8u;
+            const uint64_t row0 = uint64_t(slab) * SLAB_ROWS, row = row0 + r, k0 = uint64_t(tile0) * TILE_K + col;
             const uint32_t rows = row0 < p.rows ? uint32_t(min(uint64_t(SLAB_ROWS), p.rows - row0)) : 0u;
-            const uint32_t left = p.k > k0 ? uint32_t(p.k - k0) : 0u; // columns from the thread's first on
-            uint8_t const* codes[STEPS];
-            uint8_t const* scales[STEPS];
-            T*             out[STEPS];
-#pragma unroll
-            for(uint32_t i = 0; i < STEPS; ++i)
-            {
-                const uint32_t r = i * 16u + rowIn;
-                codes[i]  = p.codes + (row0 + r) * p.ldq + k0 / 2u;
-                scales[i] = p.scales + (uint64_t(slab / 4u) * p.groups + k0 / (4u * mxBlock(NV))) * MX_TILE_BYTES
-                            + scaleOffset(slab % 4u * SLAB_ROWS + r, uint32_t(k0 / mxBlock(NV) % 4u));
-                out[i] = static_cast<T*>(p.out) + (row0 + r) * p.ldo + k0;
-            }
-            auto fetch = [&](uint32_t t, uint32_t(&word)[STEPS], uint32_t(&byte)[STEPS]) {
-#pragma unroll
-                for(uint32_t i = 0; i < STEPS; ++i)
-                {
-                    word[i] = byte[i] = 0;
-                    if(i * 16u + rowIn < rows && left > t * TILE_K)
-                    {
-                        word[i] = *reinterpret_cast<uint32_t const*>(codes[i] + t * (TILE_K / 2u));
-                        byte[i] = scales[i][t * (GROUPS * MX_TILE_BYTES)];
-                    }
-                }
-            };
+            const uint32_t left = r < rows && p.k > k0 ? uint32_t(p.k - k0) : 0u; // values from the first on
+            uint8_t const* codes  = p.codes + row * p.ldq + k0 / 2u;
+            uint8_t const* scales = p.scales + (uint64_t(slab / 4u) * p.groups + k0 / (4u * mxBlock(NV))) * MX_TILE_BYTES
+                                    + scaleOffset(slab % 4u * SLAB_ROWS + r, uint32_t(k0 / mxBlock(NV) % 4u));
+            T*             out    = static_cast<T*>(p.out) + row * p.ldo + k0;
             __shared__ alignas(16) uint8_t staged[VEC ? 16 : SLAB_ROWS * StagedRow<T>::PITCH];
             grid_dependency_wait();
             grid_launch_dependents();
-            uint32_t word[STEPS], byte[STEPS], nextWord[STEPS], nextByte[STEPS];
-            fetch(0, nextWord, nextByte);
+            uint2    nextCode{};
+            uint32_t nextByte = 0;
+            auto     fetch    = [&](uint32_t t) {
+                if(left > t * TILE_K)
+                {
+                    nextCode = *reinterpret_cast<uint2 const*>(codes + t * (TILE_K / 2u));
+                    nextByte = scales[t * (GROUPS * MX_TILE_BYTES)];
+                }
+            };
+            fetch(0);
             for(uint32_t t = 0; t < tiles; ++t)
             {
                 const uint32_t done = t * TILE_K;
-#pragma unroll
-                for(uint32_t i = 0; i < STEPS; ++i)
-                {
-                    word[i] = nextWord[i];
-                    byte[i] = nextByte[i];
-                }
+                const uint2    code = nextCode;
+                const float    s    = NV ? fromE4m3(nextByte) : fromE8m0(nextByte);
                 if(t + 1u < tiles)
-                    fetch(t + 1u, nextWord, nextByte);
+                    fetch(t + 1u);
+                Run<T> o;
+                values8<T>(code.x, s, p.factor, o.v);
+                values8<T>(code.y, s, p.factor, o.v + 8);
                 if constexpr(VEC)
                 {
-#pragma unroll
-                    for(uint32_t i = 0; i < STEPS; ++i)
+                    if(left >= done + RUN)
+                        storeRun(out + done, o);
+                    else
                     {
-                        const Raw8<T> o  = values8<T, NV>(word[i], byte[i], p.factor);
-                        T*            at = out[i] + done;
-                        if(i * 16u + rowIn >= rows || left <= done)
-                            continue;
-                        if(left >= done + 8u)
-                        {
 #pragma unroll
-                            for(int j = 0; j < int(sizeof(T) * 8 / 16); ++j)
-                                reinterpret_cast<uint4*>(at)[j] = reinterpret_cast<uint4 const*>(&o)[j];
-                        }
-                        else
-                        {
-#pragma unroll
-                            for(uint32_t j = 0; j < 8u; ++j)
-                                if(done + j < left)
-                                    at[j] = o.v[j];
-                        }
+                        for(uint32_t j = 0; j < RUN; ++j)
+                            if(done + j < left)
+                                out[done + j] = o.v[j];
                     }
                 }
                 else
                 {
                     const uint32_t count = min(TILE_K, p.k - (tile0 + t) * TILE_K);
-                    auto rowAt = [&](uint32_t r) {
-                        return static_cast<T*>(p.out) + (row0 + r) * p.ldo + uint64_t(tile0 + t) * TILE_K;
+                    auto rowAt = [&](uint32_t i) {
+                        return static_cast<T*>(p.out) + (row0 + i) * p.ldo + uint64_t(tile0 + t) * TILE_K;
                     };
                     __syncthreads();
-#pragma unroll
-                    for(uint32_t i = 0; i < STEPS; ++i)
+                    if(r < rows)
                     {
-                        const uint32_t r = i * 16u + rowIn;
-                        const Raw8<T>  o = values8<T, NV>(word[i], byte[i], p.factor);
-                        if(r < rows)
-                        {
-                            T* at = reinterpret_cast<T*>(staged + r * StagedRow<T>::PITCH) + StagedRow<T>::shift(rowAt(r)) + col;
+                        T* at = reinterpret_cast<T*>(staged + r * StagedRow<T>::PITCH) + StagedRow<T>::shift(rowAt(r)) + col;
 #pragma unroll
-                            for(int j = 0; j < 8; ++j)
-                                at[j] = o.v[j];
-                        }
+                        for(uint32_t j = 0; j < RUN; ++j)
+                            at[j] = o.v[j];
                     }
                     __syncthreads();
                     moveStaged<T, false>(staged, rows, count, rowAt);
@@ -623,7 +624,7 @@ namespace b200wmma
         int quantize(bool nv, bool columns, QuantizeParams p, cudaStream_t stream)
         {
             // Wide loads where every row (or pair of rows) starts on their boundary.
-            const uint64_t width = columns ? 2 * sizeof(T) : 16;
+            const uint64_t width = columns ? 2 * sizeof(T) : 32;
             const bool     vec   = aligned(p.x, width) && p.ldx * sizeof(T) % width == 0;
             const uint32_t slabs = slabsOf(p.rows, true);
             p.tilesPerBlock      = tilesPerBlock(uint64_t(slabs) * p.tilesK, p.tilesK);
@@ -642,7 +643,7 @@ namespace b200wmma
         template <typename T>
         int dequantize(bool nv, DequantizeParams p, cudaStream_t stream)
         {
-            const bool     vec   = aligned(p.out, 16) && p.ldo * sizeof(T) % 16 == 0;
+            const bool     vec   = aligned(p.out, 32) && p.ldo * sizeof(T) % 32 == 0;
             const uint32_t slabs = slabsOf(p.rows, false);
             p.tilesPerBlock      = tilesPerBlock(uint64_t(slabs) * p.tilesK, p.tilesK);
             const uint32_t blocks = slabs * ((p.tilesK + p.tilesPerBlock - 1u) / p.tilesPerBlock);

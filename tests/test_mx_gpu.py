@@ -92,6 +92,20 @@ def test_quantize_extremes(fmt):
 
 
 @FORMATS
+@pytest.mark.parametrize("kind", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("layout", [ROW_MAJOR, COL_MAJOR], ids=["rows", "columns"])
+def test_quantize_tiny_values_with_an_exponent(fmt, kind, layout):
+    """Down to fp32's subnormals, brought into range by the exponent: factor / scale may overflow."""
+    rows = torch.arange(-148, -90, dtype=torch.float64)
+    x = (torch.rand(rows.numel(), 64, generator=torch.Generator().manual_seed(1), dtype=torch.float64) - 0.5)
+    x = (x * 2.0 ** rows[:, None]).to(TYPES[kind])
+    dev = (x.t().contiguous() if layout == COL_MAJOR else x).cuda()
+    for e in (-64, -60, -31):
+        q = api.mx_quantize(fmt, kind, *x.shape, dev, layout=layout, exponent=e)
+        _check_operand(fmt, *x.shape, q, x, e)
+
+
+@FORMATS
 @pytest.mark.parametrize("layout", [ROW_MAJOR, COL_MAJOR], ids=["rows", "columns"])
 def test_quantize_strides_and_offsets(fmt, layout):
     """A view inside a larger matrix that starts anywhere, into codes with room behind each row."""
