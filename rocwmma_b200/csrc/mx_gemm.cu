@@ -418,9 +418,11 @@ namespace b200wmma
         // behind it, and the first MMA of a tile waits only until the tile before has drained the
         // columns that both accumulators share, which are drained first.
         constexpr uint32_t P_TILE      = 256;
-        constexpr uint32_t P_STAGES    = 5;
+        // With C, whose boxes come from memory, twice the boxes are worth more than a fifth slot: one
+        // 256 x 256 tile f32 is drained in 5.8 us instead of 8.3, its MMAs take 0.1 us longer.
+        constexpr uint32_t P_STAGES    = 5, P_STAGES_C = 4;
         constexpr uint32_t BOX_BYTES   = 128 * 64; // 128 rows x 64 bytes of D (or C)
-        constexpr uint32_t BOXES       = 4;
+        constexpr uint32_t BOXES = 4, BOXES_C = 8;
         constexpr uint32_t P_THREADS   = 352;
         constexpr uint32_t DRAIN_WARPS = 8;
 
@@ -430,13 +432,13 @@ namespace b200wmma
             void*       d;
             uint32_t    m, n, k, ldc, ldd;
             float       alpha, beta;
-            uint32_t    band;
+            uint32_t    band, stages, boxes;
             uint32_t*   status;
         };
         struct PairControl
         {
             uint64_t   full[P_STAGES], empty[P_STAGES], accFull[2], accShared;
-            uint64_t   cFull[BOXES], boxFull[BOXES], boxFree[BOXES];
+            uint64_t   cFull[BOXES_C], boxFull[BOXES_C], boxFree[BOXES_C];
             AbortState abort;
             uint32_t   tmemBase;
         };
@@ -446,9 +448,10 @@ namespace b200wmma
             return 2u * CODE_BYTES + 3u * slotGroups<KIND>() * MX_TILE_BYTES;
         }
         template <ScaleKind KIND>
-        constexpr uint32_t pairSmemBytes()
+        constexpr uint32_t pairSmemBytes(bool useC)
         {
-            return 1024u + P_STAGES * pairSlotBytes<KIND>() + BOXES * BOX_BYTES + uint32_t(sizeof(PairControl));
+            return 1024u + (useC ? P_STAGES_C : P_STAGES) * pairSlotBytes<KIND>() + (useC ? BOXES_C : BOXES) * BOX_BYTES
+                   + uint32_t(sizeof(PairControl));
         }
 
         // The boxes of one tile, 128 rows x 64 bytes of D each, in the order in which they are drained:
@@ -483,46 +486,45 @@ namespace b200wmma
         __device__ inline bool moveBoxes(PairControl* ctl, uint8_t* staging, CUtensorMap const* mapC, CUtensorMap const* mapD,
                                          PairParams const& p, uint32_t first, uint32_t row0, uint32_t col0, uint32_t& count)
         {
-            using B = Boxes<OutT>;
-            const B    boxes(p, col0, first);
-            const bool useC = p.c != nullptr;
+            using B                = Boxes<OutT>;
+            constexpr uint32_t LAG = 2;
+            const B            boxes(p, col0, first);
+            const bool         useC = p.c != nullptr;
             uint32_t   asked = 0, askedCount = count;
             auto       askForC = [&] {
                 while(asked < B::COUNT && !boxes.staged(boxes.at(asked)))
                     ++asked;
                 if(asked == B::COUNT)
                     return;
-                const uint32_t b = askedCount % BOXES;
+                const uint32_t b = askedCount & (p.boxes - 1u);
                 mbar_expect_tx(&ctl->cFull[b], BOX_BYTES);
                 tma_load_2d(staging + b * BOX_BYTES, mapC, &ctl->cFull[b], int32_t(col0 + boxes.at(asked) * B::COLS), int32_t(row0));
                 ++asked;
                 ++askedCount;
             };
             if(useC) // the boxes of the tile before have been read out
-                for(uint32_t b = 0; b < BOXES; ++b)
+                for(uint32_t b = 0; b < p.boxes; ++b)
                     askForC();
             for(uint32_t i = 0; i < B::COUNT; ++i)
             {
                 const uint32_t box = boxes.at(i);
                 if(!boxes.staged(box))
                     continue;
-                const uint32_t b = count % BOXES;
-                if(!mbar_wait(&ctl->boxFull[b], (count / BOXES) & 1u, &ctl->abort, WAIT_ACC_FULL))
+                const uint32_t b = count & (p.boxes - 1u);
+                if(!mbar_wait(&ctl->boxFull[b], (count & p.boxes) != 0u, &ctl->abort, WAIT_ACC_FULL))
                     return false;
                 tma_store_2d(mapD, staging + b * BOX_BYTES, int32_t(col0 + box * B::COLS), int32_t(row0));
                 tma_store_commit();
+                // The store two before has been read out.  (Waiting for the one just issued would make
+                // every box as long as a store takes to read its source, 0.4 us.)
+                tma_store_wait_read<LAG>();
                 if(useC)
                 {
-                    tma_store_wait_read<0>();
-                    askForC();
+                    if(askedCount + LAG <= count + p.boxes)
+                        askForC();
                 }
-                else
-                {
-                    // the store before has been read out (the first box of all has none before it)
-                    tma_store_wait_read<1>();
-                    if(count > 0u)
-                        mbar_arrive(&ctl->boxFree[(count - 1u) % BOXES]);
-                }
+                else if(count >= LAG)
+                    mbar_arrive(&ctl->boxFree[(count - LAG) & (p.boxes - 1u)]);
                 ++count;
             }
             if(useC)
@@ -533,7 +535,7 @@ namespace b200wmma
         // Drains one tile's accumulator: TMEM -> registers -> shared memory in the TMA's 64-byte
         // swizzle, in place of C's box where there is one.  Two sets of four warps take boxes in
         // turn.  (Four warps, with one of their threads moving the boxes as well: 4.7 us for the last
-        // tile of 256 columns bf16, 11 us f32 with C; so: DRAIN_US.)
+        // tile of 256 columns bf16, 11 us f32 with C; so: 3.0 and 5.8.)
         template <typename OutT, bool C>
         __device__ inline bool drainTile(PairControl* ctl, uint8_t* staging, PairParams const& p, uint32_t taddr, uint32_t set,
                                          uint32_t first, uint32_t shared, uint32_t accBar, uint32_t accPhase, uint32_t row0,
@@ -595,7 +597,7 @@ namespace b200wmma
                         }
                     continue;
                 }
-                const uint32_t b = mine % BOXES, use = (mine / BOXES) & 1u;
+                const uint32_t b = mine & (p.boxes - 1u), use = (mine & p.boxes) != 0u;
                 const bool     open = C ? mbar_wait(&ctl->cFull[b], use, &ctl->abort, WAIT_STAGE_FULL)
                                         : mbar_wait(&ctl->boxFree[b], use ^ 1u, &ctl->abort, WAIT_DRAIN);
                 if(!__all_sync(0xffffffffu, open))
@@ -638,8 +640,8 @@ namespace b200wmma
             static_assert(ACC1 + 256u + 2u * SCALE_COLS <= 512u, "tensor memory");
             extern __shared__ uint8_t smemRaw[];
             uint8_t*       ring    = smemRaw + ((1024u - (smem_addr(smemRaw) & 1023u)) & 1023u);
-            uint8_t*       staging = ring + P_STAGES * SLOT;
-            PairControl*   ctl     = reinterpret_cast<PairControl*>(staging + BOXES * BOX_BYTES);
+            uint8_t*       staging = ring + p.stages * SLOT;
+            PairControl*   ctl     = reinterpret_cast<PairControl*>(staging + p.boxes * BOX_BYTES);
             const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
             const uint32_t rank = cluster_cta_rank(), pairId = blockIdx.x / 2, pairs = gridDim.x / 2;
             const uint32_t numSlots = (p.k + SLOT_K - 1) / SLOT_K;
@@ -647,7 +649,7 @@ namespace b200wmma
 
             if(threadIdx.x == 0)
             {
-                for(uint32_t s = 0; s < P_STAGES; ++s)
+                for(uint32_t s = 0; s < p.stages; ++s)
                 {
                     mbar_init(&ctl->full[s], 1);
                     mbar_init(&ctl->empty[s], 1);
@@ -655,7 +657,7 @@ namespace b200wmma
                 for(uint32_t b = 0; b < 2u; ++b)
                     mbar_init(&ctl->accFull[b], 1);
                 mbar_init(&ctl->accShared, 2u * DRAIN_WARPS);
-                for(uint32_t b = 0; b < BOXES; ++b)
+                for(uint32_t b = 0; b < p.boxes; ++b)
                 {
                     mbar_init(&ctl->cFull[b], 1);
                     mbar_init(&ctl->boxFull[b], DRAIN_WARPS / 2u);
@@ -714,7 +716,7 @@ namespace b200wmma
                             tma_load_3d_pair(slot + 2u * CODE_BYTES, &mapScaleA, full, 0, group, tileA);
                             tma_load_3d_pair(slot + 2u * CODE_BYTES + GROUPS * MX_TILE_BYTES, &mapScaleB, full, 0, group,
                                              tileB);
-                            at.next(P_STAGES, SLOT);
+                            at.next(p.stages, SLOT);
                         }
                     }
                     if(!ok)
@@ -778,7 +780,7 @@ namespace b200wmma
                             const uint32_t swap = scale;
                             scale               = otherScale;
                             otherScale          = swap;
-                            at.next(P_STAGES, SLOT);
+                            at.next(p.stages, SLOT);
                         }
                         if(ok)
                             mma_commit_pair(&ctl->accFull[i & 1u], 0x3);
@@ -932,12 +934,13 @@ namespace b200wmma
                 rc = outputMap<OutT>(&mapC, q.c, q.m, q.n, q.ldc);
             if(rc != B200WMMA_OK)
                 return rc;
-            constexpr uint32_t smem = pairSmemBytes<KIND>();
-            static uint32_t    done[64] = {};
+            const uint32_t  smem = pairSmemBytes<KIND>(q.c != nullptr);
+            static uint32_t done[64] = {};
             rc = optInSharedMemory(mxGemmPairKernel<KIND, OutT>, smem, done);
             if(rc != B200WMMA_OK)
                 return rc;
-            const PairParams p{q.c, q.d, q.m, q.n, q.k, q.ldc, q.ldd, q.alpha, q.beta, 16u, q.status};
+            const PairParams p{q.c, q.d, q.m, q.n, q.k, q.ldc, q.ldd, q.alpha, q.beta, 16u, q.c ? P_STAGES_C : P_STAGES, q.c ? BOXES_C : BOXES,
+                               q.status};
             const uint32_t   pairs = uint32_t(tiles < uint64_t(sms / 2) ? tiles : uint64_t(sms / 2));
             return cudaToStatus(launchOverlapped(mxGemmPairKernel<KIND, OutT>, dim3(2u * pairs), dim3(P_THREADS), smem,
                                                  stream, mapA, mapB, mapScaleA, mapScaleB, mapC, mapD, p));
@@ -970,7 +973,7 @@ namespace b200wmma
             const uint32_t tiles    = mxRowTiles(p.rows);
             // K is split until the blocks fill the device: twice over for up to 32 thin rows (1 x 8192 x
             // 8192 MXF4: 8.5 us in the kernel with 4 parts, 9.3 with 2, 11.4 with 1), once for more,
-            // whose sums cost more to exchange (64 x 16384 x 4096 NVF4: TODO).
+            // whose sums cost more to exchange (64 x 16384 x 4096 NVF4: 11.3 us with 1 part, 12.0 with 2).
             const uint32_t resident = p.nq <= 32u ? 2u : 1u;
             p.parts                 = 8;
             while(p.parts > 1u && (uint64_t(tiles) * p.parts > resident * uint32_t(sms) || slots < 2u * p.parts))
