@@ -373,9 +373,11 @@ namespace b200wmma
 
         // ---- sorting many tokens -------------------------------------------------------------
         // Digits of up to ten bits: two passes for tables of up to a million rows.
-        constexpr uint32_t SORT_ITEMS = 16; // keys of a thread
-        constexpr uint32_t SORT_TILE  = THREADS * SORT_ITEMS;
+        // A block has a tile of THREADS x ITEMS keys: sixteen a thread, or four where that would leave
+        // SMs without one (a block's own latency is the kernels' time then: 74000 tokens in 4 columns
+        // of 2900 rows, whole call, 86 us with sixteen, 62 with four).
         constexpr uint32_t SORT_WARPS = THREADS / 32;
+        constexpr uint32_t FEW_ITEMS = 4, MANY_ITEMS = 16, MANY_TOKENS = 500000;
         constexpr uint32_t SORT_BITS  = 10;
         constexpr uint32_t SORT_RADIX = 1u << SORT_BITS;
         struct Digit
@@ -388,7 +390,8 @@ namespace b200wmma
         };
 
         // bins[digit] = keys of the tile
-        __device__ inline void countDigits(uint32_t* bins, uint32_t const (&key)[SORT_ITEMS], uint32_t first, uint32_t n,
+        template <uint32_t ITEMS>
+        __device__ inline void countDigits(uint32_t* bins, uint32_t const (&key)[ITEMS], uint32_t first, uint32_t n,
                                            Digit digit, uint32_t tiles, uint32_t* counts)
         {
             const uint32_t radix = 1u << digit.bits;
@@ -396,7 +399,7 @@ namespace b200wmma
                 bins[d] = 0;
             __syncthreads();
 #pragma unroll
-            for(uint32_t i = 0; i < SORT_ITEMS; ++i)
+            for(uint32_t i = 0; i < ITEMS; ++i)
             {
                 // one addition for the equal digits of a warp: a hot row would queue 32
                 const bool     in    = uint64_t(first) + i * THREADS < n;
@@ -410,23 +413,24 @@ namespace b200wmma
         }
 
         // Row of every token, and the first digit's counts[digit][tile].
+        template <uint32_t ITEMS>
         __global__ void __launch_bounds__(THREADS)
             keysKernel(const Tokens t, uint32_t* keys, uint32_t tiles, const Digit digit, uint32_t* counts)
         {
             __shared__ uint32_t bins[SORT_RADIX];
             grid_dependency_wait();
             grid_launch_dependents();
-            const uint32_t first = blockIdx.x * SORT_TILE + threadIdx.x;
-            uint32_t       key[SORT_ITEMS], outer, inner[SORT_ITEMS];
-            int64_t        id[SORT_ITEMS];
+            const uint32_t first = blockIdx.x * (THREADS * ITEMS) + threadIdx.x;
+            uint32_t       key[ITEMS], outer, inner[ITEMS];
+            int64_t        id[ITEMS];
 #pragma unroll
-            for(uint32_t i = 0; i < SORT_ITEMS; ++i)
+            for(uint32_t i = 0; i < ITEMS; ++i)
             {
                 const uint32_t token = first + i * THREADS;
                 id[i]                = token < t.count ? idOf(t, token, outer, inner[i]) : -1;
             }
 #pragma unroll
-            for(uint32_t i = 0; i < SORT_ITEMS; ++i)
+            for(uint32_t i = 0; i < ITEMS; ++i)
             {
                 const uint32_t token = first + i * THREADS;
                 key[i]               = t.rows; // behind every row
@@ -441,16 +445,17 @@ namespace b200wmma
             countDigits(bins, key, first, t.count, digit, tiles, counts);
         }
 
+        template <uint32_t ITEMS>
         __global__ void __launch_bounds__(THREADS)
             countKernel(uint2 const* pairs, uint32_t n, const Digit digit, uint32_t tiles, uint32_t* counts)
         {
             __shared__ uint32_t bins[SORT_RADIX];
             grid_dependency_wait();
             grid_launch_dependents();
-            const uint32_t first = blockIdx.x * SORT_TILE + threadIdx.x;
-            uint32_t       key[SORT_ITEMS];
+            const uint32_t first = blockIdx.x * (THREADS * ITEMS) + threadIdx.x;
+            uint32_t       key[ITEMS];
 #pragma unroll
-            for(uint32_t i = 0; i < SORT_ITEMS; ++i)
+            for(uint32_t i = 0; i < ITEMS; ++i)
                 key[i] = first + i * THREADS < n ? pairs[first + i * THREADS].x : 0u;
             countDigits(bins, key, first, n, digit, tiles, counts);
         }
@@ -509,33 +514,35 @@ namespace b200wmma
         // of smaller lanes come first.  The tile is put in order in shared memory first, so that
         // neighbouring threads write neighbouring places.  pairs == nullptr: the first pass, key i
         // of `keys` belongs to token i.
+        template <uint32_t ITEMS, uint32_t PER>
         struct ScatterShared
         {
-            uint2    tile[SORT_TILE];
-            uint16_t bins[SORT_WARPS][SORT_RADIX];
-            uint32_t shifts[SORT_RADIX]; // place of a digit's keys minus their place in the tile
+            uint2    tile[THREADS * ITEMS];
+            uint16_t bins[SORT_WARPS][THREADS * PER];
+            uint32_t shifts[THREADS * PER]; // place of a digit's keys minus their place in the tile
             uint32_t warps[SORT_WARPS];
         };
 
+        template <uint32_t ITEMS, uint32_t PER>
         __global__ void __launch_bounds__(THREADS)
             scatterKernel(uint32_t const* keys, uint2 const* pairs, uint32_t n, const Digit digit, uint32_t tiles,
                           uint32_t const* counts, uint32_t const* totals, uint2* out)
         {
-            constexpr uint32_t PER = SORT_RADIX / THREADS; // digits of a thread
+            constexpr uint32_t RADIX_HERE = THREADS * PER; // 2^bits or more; PER digits a thread
             extern __shared__ uint8_t smem[];
-            ScatterShared* sh   = reinterpret_cast<ScatterShared*>(smem);
+            auto*          sh   = reinterpret_cast<ScatterShared<ITEMS, PER>*>(smem);
             const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, radix = 1u << digit.bits;
             grid_dependency_wait();
             grid_launch_dependents();
-            for(uint32_t i = threadIdx.x; i < SORT_WARPS * SORT_RADIX / 2u; i += THREADS)
+            for(uint32_t i = threadIdx.x; i < SORT_WARPS * RADIX_HERE / 2u; i += THREADS)
                 reinterpret_cast<uint32_t*>(sh->bins)[i] = 0;
             __syncthreads();
-            const uint32_t tile0 = blockIdx.x * SORT_TILE, here = min(SORT_TILE, n - tile0);
-            const uint32_t first = warp * (32u * SORT_ITEMS) + lane;
-            uint2          pair[SORT_ITEMS];
-            uint32_t       rank[SORT_ITEMS];
+            const uint32_t tile0 = blockIdx.x * (THREADS * ITEMS), here = min(THREADS * ITEMS, n - tile0);
+            const uint32_t first = warp * (32u * ITEMS) + lane;
+            uint2          pair[ITEMS];
+            uint32_t       rank[ITEMS];
 #pragma unroll
-            for(uint32_t i = 0; i < SORT_ITEMS; ++i)
+            for(uint32_t i = 0; i < ITEMS; ++i)
             {
                 const uint32_t at = first + i * 32u;
                 pair[i]           = make_uint2(0u, tile0 + at);
@@ -548,7 +555,7 @@ namespace b200wmma
                 }
             }
 #pragma unroll
-            for(uint32_t i = 0; i < SORT_ITEMS; ++i)
+            for(uint32_t i = 0; i < ITEMS; ++i)
             {
                 const bool     in    = first + i * 32u < here;
                 const uint32_t d     = digit.of(pair[i].x);
@@ -597,7 +604,7 @@ namespace b200wmma
             }
             __syncthreads();
 #pragma unroll
-            for(uint32_t i = 0; i < SORT_ITEMS; ++i)
+            for(uint32_t i = 0; i < ITEMS; ++i)
                 if(first + i * 32u < here)
                     sh->tile[sh->bins[warp][digit.of(pair[i].x)] + rank[i]] = pair[i];
             __syncthreads();
@@ -678,7 +685,7 @@ namespace b200wmma
             // slot s of the calling thread; the threads of a block lie side by side
             static __device__ uint8_t* at(uint8_t* ring, uint32_t s, uint32_t part)
             {
-                return ring + ((s * (BYTES / PART) + part) * THREADS + threadIdx.x) * PART;
+                return ring + ((s * (BYTES / PART) + part) * blockDim.x + threadIdx.x) * PART;
             }
             static __device__ void load(uint8_t* ring, uint32_t s, T const* from)
             {
@@ -723,7 +730,8 @@ namespace b200wmma
             using R = Ring<T, V>;
             __shared__ uint32_t rows[SUM_ITEMS + 2]; // of the items, and one on each side
             __shared__ uint64_t places[SUM_ITEMS + 2]; // of their gradients, in elements
-            __shared__ alignas(16) uint8_t ring[R::DEPTH * R::BYTES * THREADS];
+            extern __shared__ uint4 ringWords[]; // R::DEPTH * R::BYTES of each thread
+            uint8_t* const ring = reinterpret_cast<uint8_t*>(ringWords);
             grid_dependency_wait();
             grid_launch_dependents();
             if(blockIdx.x >= p.blocks)
@@ -838,7 +846,7 @@ namespace b200wmma
         template <typename OutT, int V>
         __global__ void __launch_bounds__(THREADS) joinKernel(const SumParams p)
         {
-            constexpr uint32_t U = 8;
+            constexpr uint32_t U = 4;
             __shared__ uint32_t longs[THREADS], longCount, end;
             __shared__ float    sums[THREADS][V + 1];
             if(threadIdx.x == 0u)
@@ -1011,10 +1019,10 @@ namespace b200wmma
             return lookupTyped<T, float>(p, dim, stream);
         }
 
-        // Threads of a block of the sum.
+        // Threads of a block of the sum: sixteen rows side by side, a warp at least.
         uint32_t sumThreads(uint32_t lanesLog2)
         {
-            return lanesLog2 >= 3u ? THREADS : 32u << lanesLog2;
+            return lanesLog2 == 0u ? 32u : lanesLog2 >= 4u ? THREADS : 16u << lanesLog2;
         }
 
         // The workspace of the gradient; offsets in bytes.  The chunks go by the sizes alone.
@@ -1035,7 +1043,8 @@ namespace b200wmma
                 return here;
             };
             w.small    = count <= SMALL_TOKENS;
-            w.tiles    = uint32_t((uint64_t(count) + SORT_TILE - 1) / SORT_TILE);
+            const uint32_t tile = THREADS * (count < MANY_TOKENS ? FEW_ITEMS : MANY_ITEMS);
+            w.tiles    = uint32_t((uint64_t(count) + tile - 1u) / tile);
             const uint32_t bits = log2Up(rows + 1u), most1 = w.small ? 8u : SORT_BITS; // keys 0..rows
             w.passes    = (bits + most1 - 1u) / most1;
             w.digitBits = (bits + w.passes - 1u) / w.passes;
@@ -1047,13 +1056,14 @@ namespace b200wmma
                 w.totals   = take(SORT_RADIX * 4u);
                 w.counts   = take((uint64_t(w.tiles) << w.digitBits) * 4u);
             }
+            // (pieces of the widest kind; narrower ones put fewer rows into a block, and fewer items)
             const uint32_t pieces = dim % 8u == 0u ? dim / 8u : dim % 2u == 0u ? dim / 2u : dim;
             const uint32_t lanes  = rowLanesLog2(pieces);
             const uint32_t most   = SUM_ITEMS / (sumThreads(lanes) >> lanes); // that fit a block
-            // Long chunks leave fewer pieces of runs behind, short ones make more threads: twice
-            // what the device holds at once, so that the last ones do not wait long.
+            // Long chunks leave fewer pieces of runs behind, short ones make more threads: as many
+            // as the device could hold of them.
             w.chunk = 8;
-            while(w.chunk < 128u && w.chunk < most && uint64_t(count) * pieces > 2u * uint64_t(w.chunk) * DEVICE_THREADS)
+            while(w.chunk < 128u && w.chunk < most && uint64_t(count) * pieces > uint64_t(w.chunk) * DEVICE_THREADS)
                 w.chunk *= 2u;
             w.chunks = (count + w.chunk - 1u) / w.chunk;
             if(w.chunks > 1u)
@@ -1124,31 +1134,40 @@ namespace b200wmma
                                                  reinterpret_cast<uint2*>(g.workspace + w.pairs[0])));
         }
 
+        template <uint32_t ITEMS, uint32_t PER>
         int sortMany(GradientCall const& g, Plan const& w, uint2** sorted, cudaStream_t stream)
         {
             auto       words = [&](uint64_t at) { return reinterpret_cast<uint32_t*>(g.workspace + at); };
             auto       pairs = [&](uint32_t i) { return reinterpret_cast<uint2*>(g.workspace + w.pairs[i]); };
             static std::mutex mutex;
             static bool       done[64] = {};
-            B200WMMA_TRY(optIn(scatterKernel, sizeof(ScatterShared), mutex, done));
+            B200WMMA_TRY(optIn(scatterKernel<ITEMS, PER>, sizeof(ScatterShared<ITEMS, PER>), mutex, done));
             const dim3 grid(w.tiles);
             auto       digit = [&](uint32_t pass) { return Digit{w.digitBits * pass, w.digitBits}; };
-            B200WMMA_TRY(cudaToStatus(launchOverlapped(keysKernel, grid, dim3(THREADS), 0, stream, g.t, words(w.keys),
+            B200WMMA_TRY(cudaToStatus(launchOverlapped(keysKernel<ITEMS>, grid, dim3(THREADS), 0, stream, g.t, words(w.keys),
                                                        w.tiles, digit(0), words(w.counts))));
             for(uint32_t pass = 0; pass < w.passes; ++pass)
             {
                 uint2* from = pass ? pairs((pass - 1u) % 2u) : nullptr;
                 if(pass > 0u)
-                    B200WMMA_TRY(cudaToStatus(launchOverlapped(countKernel, grid, dim3(THREADS), 0, stream, from,
+                    B200WMMA_TRY(cudaToStatus(launchOverlapped(countKernel<ITEMS>, grid, dim3(THREADS), 0, stream, from,
                                                                g.t.count, digit(pass), w.tiles, words(w.counts))));
                 B200WMMA_TRY(cudaToStatus(launchOverlapped(scanKernel, dim3(1u << w.digitBits), dim3(THREADS), 0, stream,
                                                            words(w.counts), w.tiles, words(w.totals))));
-                B200WMMA_TRY(cudaToStatus(launchOverlapped(scatterKernel, grid, dim3(THREADS), sizeof(ScatterShared),
+                B200WMMA_TRY(cudaToStatus(launchOverlapped(scatterKernel<ITEMS, PER>, grid, dim3(THREADS), sizeof(ScatterShared<ITEMS, PER>),
                                                            stream, words(w.keys), from, g.t.count, digit(pass), w.tiles,
                                                            words(w.counts), words(w.totals), pairs(pass % 2u))));
             }
             *sorted = pairs((w.passes - 1u) % 2u);
             return B200WMMA_OK;
+        }
+
+        template <uint32_t ITEMS>
+        int sortDigits(GradientCall const& g, Plan const& w, uint2** sorted, cudaStream_t stream)
+        {
+            return w.digitBits <= 8u ? sortMany<ITEMS, 1>(g, w, sorted, stream)
+                                     : w.digitBits == 9u ? sortMany<ITEMS, 2>(g, w, sorted, stream)
+                                                         : sortMany<ITEMS, 4>(g, w, sorted, stream);
         }
 
         // The sums of chunks, with pieces of `V` values, and rows cleared beside them where the
@@ -1175,7 +1194,8 @@ namespace b200wmma
             if(blocks + c.blocks > 0x7fffffffull)
                 return B200WMMA_ERR_TOO_LARGE;
             p.blocks = uint32_t(blocks);
-            return cudaToStatus(launchOverlapped(sumKernel<T, OutT, V>, dim3(p.blocks + c.blocks), dim3(threads), 0, stream, p, c));
+            return cudaToStatus(launchOverlapped(sumKernel<T, OutT, V>, dim3(p.blocks + c.blocks), dim3(threads),
+                                                 threads * Ring<T, V>::DEPTH * Ring<T, V>::BYTES, stream, p, c));
         }
 
         template <typename OutT, int V>
@@ -1205,7 +1225,8 @@ namespace b200wmma
                 B200WMMA_TRY(vt == 8u ? (sortFew<OutT, 8>(g, w, stream))
                                       : vt == 2u ? (sortFew<OutT, 2>(g, w, stream)) : (sortFew<OutT, 1>(g, w, stream)));
             else
-                B200WMMA_TRY(sortMany(g, w, &sorted, stream));
+                B200WMMA_TRY(g.t.count < MANY_TOKENS ? sortDigits<FEW_ITEMS>(g, w, &sorted, stream)
+                                                     : sortDigits<MANY_ITEMS>(g, w, &sorted, stream));
             SumParams p{};
             p.sorted     = sorted;
             p.grad       = g.grad;
