@@ -208,13 +208,20 @@ namespace b200wmma
                         storePiece<OutT, V>(static_cast<OutT*>(c.table) + row * c.ldt + uint64_t(piece) * V, zero);
         }
 
-        // Lanes of the warp with the same digit of `bits` bits, among those that are `in`.  (A ballot
-        // for each bit: match.any took most of the scattering kernel's time.)
-        __device__ inline uint32_t sameDigit(uint32_t digit, bool in, uint32_t bits)
+        // Digits of eight, nine or ten bits: two passes for tables of up to a million rows.
+        template <uint32_t BITS>
+        __device__ inline uint32_t digitOf(uint32_t key, uint32_t pass)
+        {
+            return (key >> (BITS * pass)) & ((1u << BITS) - 1u);
+        }
+        // Lanes of the warp with the same digit, among those that are `in`.  (A ballot for each bit:
+        // match.any took most of the scattering kernel's time.)
+        template <uint32_t BITS>
+        __device__ inline uint32_t sameDigit(uint32_t digit, bool in)
         {
             uint32_t same = __ballot_sync(0xffffffffu, in);
-#pragma unroll 10
-            for(uint32_t b = 0; b < bits; ++b)
+#pragma unroll
+            for(uint32_t b = 0; b < BITS; ++b)
             {
                 const bool     set  = (digit >> b) & 1u;
                 const uint32_t vote = __ballot_sync(0xffffffffu, set);
@@ -228,25 +235,27 @@ namespace b200wmma
         constexpr uint32_t SMALL_ITEMS   = 16;
         constexpr uint32_t SMALL_TOKENS  = SMALL_THREADS * SMALL_ITEMS;
         constexpr uint32_t SMALL_WARPS   = SMALL_THREADS / 32;
-        constexpr uint32_t RADIX         = 256;
+        constexpr uint32_t SORT_BITS     = 10; // of a digit, at most
+        constexpr uint32_t SORT_RADIX    = 1u << SORT_BITS;
         constexpr uint32_t CLEAR_BITS    = 65536; // rows that a clearing block looks over at a time
+        template <uint32_t BITS>
         struct SmallShared
         {
             uint32_t keys[SMALL_TOKENS];
-            uint32_t bins[SMALL_WARPS][RADIX];
-            uint32_t sums[8];
+            uint32_t sums[SMALL_WARPS];
+            uint16_t bins[SMALL_WARPS][1u << BITS];
             uint16_t tokens[SMALL_TOKENS];
         };
-        static_assert(CLEAR_BITS / 8 <= sizeof(SmallShared::keys), "the clearing blocks' bits take the keys' place");
+        static_assert(CLEAR_BITS / 8 <= SMALL_TOKENS * 4, "the clearing blocks' bits take the keys' place");
 
         // Block 0 sorts all tokens in shared memory; the others clear a share of the rows each, for
         // which they look through the tokens themselves.
-        template <typename OutT, int V>
+        template <typename OutT, int V, uint32_t BITS>
         __global__ void __launch_bounds__(SMALL_THREADS)
             sortSmallKernel(const Tokens t, const ClearParams c, const uint32_t passes, uint2* sorted)
         {
             extern __shared__ uint8_t smem[];
-            SmallShared*   sh   = reinterpret_cast<SmallShared*>(smem);
+            auto*          sh   = reinterpret_cast<SmallShared<BITS>*>(smem);
             const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
             grid_dependency_wait();
             grid_launch_dependents();
@@ -276,70 +285,80 @@ namespace b200wmma
                 }
                 return;
             }
-            // A warp's keys are neighbours, 32 of them a step.
+            // A warp's keys are neighbours, 32 of them a step.  A key's token and its rank among the
+            // warp's keys of its digit share a register.
+            constexpr uint32_t RADIX = 1u << BITS, PER = RADIX <= SMALL_THREADS ? 1u : RADIX / SMALL_THREADS;
+            static_assert(PER == 1u, "a thread has a digit");
             const uint32_t items = (t.count + SMALL_THREADS - 1u) / SMALL_THREADS;
+            const uint32_t warps = (t.count + 32u * items - 1u) / (32u * items); // that have keys
             const uint32_t first = warp * 32u * items + lane;
-            uint32_t       key[SMALL_ITEMS], rank[SMALL_ITEMS];
-            uint16_t       token[SMALL_ITEMS];
-#pragma unroll
-            for(uint32_t i = 0; i < SMALL_ITEMS; ++i)
+            uint32_t       key[SMALL_ITEMS], token[SMALL_ITEMS]; // rank << 16 | token
             {
-                const uint32_t at = first + i * 32u;
-                key[i]            = 0;
-                token[i]          = uint16_t(at);
-                if(i < items && at < t.count)
+                int64_t id[SMALL_ITEMS];
+#pragma unroll
+                for(uint32_t i = 0; i < SMALL_ITEMS; ++i)
                 {
-                    const uint32_t row = rowOf(t, at, outer, inner);
+                    const uint32_t at = first + i * 32u;
+                    id[i]             = i < items && at < t.count ? idOf(t, at, outer, token[i]) : -1;
+                }
+#pragma unroll
+                for(uint32_t i = 0; i < SMALL_ITEMS; ++i)
+                {
+                    const uint32_t row = i < items && first + i * 32u < t.count ? rowOf(t, id[i], token[i]) : NO_ROW;
                     key[i]             = row == NO_ROW ? t.rows : row; // behind every row
+                    token[i]           = first + i * 32u;
                 }
             }
             for(uint32_t pass = 0; pass < passes; ++pass)
             {
-                const uint32_t shift = 8u * pass;
-                for(uint32_t i = threadIdx.x; i < SMALL_WARPS * RADIX; i += SMALL_THREADS)
-                    sh->bins[0][i] = 0;
+                for(uint32_t i = threadIdx.x; i < warps * (RADIX / 2u); i += SMALL_THREADS)
+                    reinterpret_cast<uint32_t*>(sh->bins)[i] = 0;
                 __syncthreads();
+                if(warp < warps)
+                {
 #pragma unroll
-                for(uint32_t i = 0; i < SMALL_ITEMS; ++i)
-                    if(i < items)
-                    {
-                        const bool     in    = first + i * 32u < t.count;
-                        const uint32_t digit = (key[i] >> shift) % RADIX;
-                        const uint32_t peers = sameDigit(digit, in, 8);
-                        rank[i]              = (in ? sh->bins[warp][digit] : 0u) + __popc(peers & ((1u << lane) - 1u));
-                        __syncwarp();
-                        if(in && (peers >> lane) == 1u) // the last of its digit
-                            sh->bins[warp][digit] = rank[i] + 1u;
-                        __syncwarp();
-                    }
+                    for(uint32_t i = 0; i < SMALL_ITEMS; ++i)
+                        if(i < items)
+                        {
+                            const bool     in    = first + i * 32u < t.count;
+                            const uint32_t d     = digitOf<BITS>(key[i], pass);
+                            const uint32_t peers = sameDigit<BITS>(d, in);
+                            const uint32_t rank  = sh->bins[warp][d] + __popc(peers & ((1u << lane) - 1u));
+                            token[i]             = rank << 16 | (token[i] & 0xffffu);
+                            __syncwarp();
+                            if(in && (peers >> lane) == 1u) // the last of its digit
+                                sh->bins[warp][d] = uint16_t(rank + 1u);
+                            __syncwarp();
+                        }
+                }
                 __syncthreads();
                 // thread = digit: where the keys of each warp go
-                uint32_t sum = 0, before = 0;
+                uint32_t sum = 0;
                 if(threadIdx.x < RADIX)
-                {
-                    for(uint32_t w = 0; w < SMALL_WARPS; ++w)
+#pragma unroll 8
+                    for(uint32_t w = 0; w < warps; ++w)
                         sum += sh->bins[w][threadIdx.x];
-                    before = sum;
+                uint32_t before = sum;
 #pragma unroll
-                    for(uint32_t d = 1; d < 32u; d *= 2u)
-                    {
-                        const uint32_t other = __shfl_up_sync(0xffffffffu, before, d);
-                        if(lane >= d)
-                            before += other;
-                    }
-                    if(lane == 31u)
-                        sh->sums[warp] = before;
-                    before -= sum;
+                for(uint32_t d = 1; d < 32u; d *= 2u)
+                {
+                    const uint32_t other = __shfl_up_sync(0xffffffffu, before, d);
+                    if(lane >= d)
+                        before += other;
                 }
+                if(lane == 31u)
+                    sh->sums[warp] = before;
+                before -= sum;
                 __syncthreads();
                 if(threadIdx.x < RADIX)
                 {
                     for(uint32_t w = 0; w < warp; ++w)
                         before += sh->sums[w];
-                    for(uint32_t w = 0; w < SMALL_WARPS; ++w)
+#pragma unroll 8
+                    for(uint32_t w = 0; w < warps; ++w)
                     {
-                        const uint32_t count      = sh->bins[w][threadIdx.x];
-                        sh->bins[w][threadIdx.x] = before;
+                        const uint32_t count     = sh->bins[w][threadIdx.x];
+                        sh->bins[w][threadIdx.x] = uint16_t(before);
                         before += count;
                     }
                 }
@@ -349,13 +368,13 @@ namespace b200wmma
                 for(uint32_t i = 0; i < SMALL_ITEMS; ++i)
                     if(i < items && first + i * 32u < t.count)
                     {
-                        const uint32_t to = sh->bins[warp][(key[i] >> shift) % RADIX] + rank[i];
+                        const uint32_t to = sh->bins[warp][digitOf<BITS>(key[i], pass)] + (token[i] >> 16);
                         if(last)
-                            sorted[to] = make_uint2(key[i], token[i]);
+                            sorted[to] = make_uint2(key[i], token[i] & 0xffffu);
                         else
                         {
                             sh->keys[to]   = key[i];
-                            sh->tokens[to] = token[i];
+                            sh->tokens[to] = uint16_t(token[i]);
                         }
                     }
                 if(last)
@@ -372,29 +391,18 @@ namespace b200wmma
         }
 
         // ---- sorting many tokens -------------------------------------------------------------
-        // Digits of up to ten bits: two passes for tables of up to a million rows.
         // A block has a tile of THREADS x ITEMS keys: sixteen a thread, or four where that would leave
         // SMs without one (a block's own latency is the kernels' time then: 74000 tokens in 4 columns
         // of 2900 rows, whole call, 86 us with sixteen, 62 with four).
         constexpr uint32_t SORT_WARPS = THREADS / 32;
         constexpr uint32_t FEW_ITEMS = 4, MANY_ITEMS = 16, MANY_TOKENS = 500000;
-        constexpr uint32_t SORT_BITS  = 10;
-        constexpr uint32_t SORT_RADIX = 1u << SORT_BITS;
-        struct Digit
-        {
-            uint32_t shift, bits;
-            __device__ uint32_t of(uint32_t key) const
-            {
-                return (key >> shift) & ((1u << bits) - 1u);
-            }
-        };
 
         // bins[digit] = keys of the tile
-        template <uint32_t ITEMS>
+        template <uint32_t ITEMS, uint32_t BITS>
         __device__ inline void countDigits(uint32_t* bins, uint32_t const (&key)[ITEMS], uint32_t first, uint32_t n,
-                                           Digit digit, uint32_t tiles, uint32_t* counts)
+                                           uint32_t pass, uint32_t* counts)
         {
-            const uint32_t radix = 1u << digit.bits;
+            constexpr uint32_t radix = 1u << BITS;
             for(uint32_t d = threadIdx.x; d < radix; d += THREADS)
                 bins[d] = 0;
             __syncthreads();
@@ -403,21 +411,21 @@ namespace b200wmma
             {
                 // one addition for the equal digits of a warp: a hot row would queue 32
                 const bool     in    = uint64_t(first) + i * THREADS < n;
-                const uint32_t peers = sameDigit(digit.of(key[i]), in, digit.bits);
+                const uint32_t digit = digitOf<BITS>(key[i], pass);
+                const uint32_t peers = sameDigit<BITS>(digit, in);
                 if(in && (peers & ((1u << (threadIdx.x % 32u)) - 1u)) == 0u)
-                    atomicAdd(&bins[digit.of(key[i])], uint32_t(__popc(peers)));
+                    atomicAdd(&bins[digit], uint32_t(__popc(peers)));
             }
             __syncthreads();
             for(uint32_t d = threadIdx.x; d < radix; d += THREADS)
-                counts[uint64_t(d) * tiles + blockIdx.x] = bins[d];
+                counts[uint64_t(blockIdx.x) * radix + d] = bins[d];
         }
 
-        // Row of every token, and the first digit's counts[digit][tile].
-        template <uint32_t ITEMS>
-        __global__ void __launch_bounds__(THREADS)
-            keysKernel(const Tokens t, uint32_t* keys, uint32_t tiles, const Digit digit, uint32_t* counts)
+        // Row of every token, and the first digit's counts[tile][digit].
+        template <uint32_t ITEMS, uint32_t BITS>
+        __global__ void __launch_bounds__(THREADS) keysKernel(const Tokens t, uint32_t* keys, uint32_t* counts)
         {
-            __shared__ uint32_t bins[SORT_RADIX];
+            __shared__ uint32_t bins[1u << BITS];
             grid_dependency_wait();
             grid_launch_dependents();
             const uint32_t first = blockIdx.x * (THREADS * ITEMS) + threadIdx.x;
@@ -442,14 +450,14 @@ namespace b200wmma
                     keys[token] = key[i];
                 }
             }
-            countDigits(bins, key, first, t.count, digit, tiles, counts);
+            countDigits<ITEMS, BITS>(bins, key, first, t.count, 0, counts);
         }
 
-        template <uint32_t ITEMS>
+        template <uint32_t ITEMS, uint32_t BITS>
         __global__ void __launch_bounds__(THREADS)
-            countKernel(uint2 const* pairs, uint32_t n, const Digit digit, uint32_t tiles, uint32_t* counts)
+            countKernel(uint2 const* pairs, uint32_t n, uint32_t pass, uint32_t* counts)
         {
-            __shared__ uint32_t bins[SORT_RADIX];
+            __shared__ uint32_t bins[1u << BITS];
             grid_dependency_wait();
             grid_launch_dependents();
             const uint32_t first = blockIdx.x * (THREADS * ITEMS) + threadIdx.x;
@@ -457,7 +465,7 @@ namespace b200wmma
 #pragma unroll
             for(uint32_t i = 0; i < ITEMS; ++i)
                 key[i] = first + i * THREADS < n ? pairs[first + i * THREADS].x : 0u;
-            countDigits(bins, key, first, n, digit, tiles, counts);
+            countDigits<ITEMS, BITS>(bins, key, first, n, pass, counts);
         }
 
         // Exclusive sum of a value over the block's threads, and the total.
@@ -487,26 +495,50 @@ namespace b200wmma
             return before + sum - v;
         }
 
-        // One block per digit: its row of counts becomes its exclusive sums, the total goes to
-        // totals[digit].
-        __global__ void __launch_bounds__(THREADS) scanKernel(uint32_t* counts, uint32_t tiles, uint32_t* totals)
+        // A block has 32 digits: their counts become exclusive sums over the tiles, their totals go to
+        // totals[digit].  A warp reads the counts of neighbouring digits, its lanes' columns; the 32
+        // warps have a stretch of tiles each.
+        constexpr uint32_t SCAN_THREADS = 1024;
+        __global__ void __launch_bounds__(SCAN_THREADS) scanKernel(uint32_t* counts, uint32_t tiles, uint32_t radix, uint32_t* totals)
         {
-            __shared__ uint32_t warps[SORT_WARPS];
+            __shared__ uint32_t sums[32][33];
             grid_dependency_wait();
             grid_launch_dependents();
-            uint32_t* row = counts + uint64_t(blockIdx.x) * tiles;
-            uint32_t  sum = 0;
-            for(uint32_t t0 = 0; t0 < tiles; t0 += THREADS)
+            const uint32_t lane = threadIdx.x % 32u, warp = threadIdx.x / 32u, digit = blockIdx.x * 32u + lane;
+            const uint32_t begin = uint32_t(uint64_t(tiles) * warp / 32u), end = uint32_t(uint64_t(tiles) * (warp + 1u) / 32u);
+            const bool     in    = digit < radix;
+            uint32_t       sum   = 0;
+#pragma unroll 8
+            for(uint32_t t = begin; t < end; ++t)
+                sum += in ? counts[uint64_t(t) * radix + digit] : 0u;
+            sums[warp][lane] = sum;
+            __syncthreads();
+            uint32_t before = 0, total = 0;
+#pragma unroll
+            for(uint32_t w = 0; w < 32u; ++w)
             {
-                const uint32_t t = t0 + threadIdx.x;
-                uint32_t       total;
-                const uint32_t before = blockScan(t < tiles ? row[t] : 0u, warps, total);
-                if(t < tiles)
-                    row[t] = sum + before;
-                sum += total;
+                before += w < warp ? sums[w][lane] : 0u;
+                total += sums[w][lane];
             }
-            if(threadIdx.x == 0)
-                totals[blockIdx.x] = sum;
+            if(!in)
+                return;
+            constexpr uint32_t BATCH = 8; // loaded together
+            for(uint32_t t0 = begin; t0 < end; t0 += BATCH)
+            {
+                uint32_t count[BATCH];
+#pragma unroll
+                for(uint32_t i = 0; i < BATCH; ++i)
+                    count[i] = t0 + i < end ? counts[uint64_t(t0 + i) * radix + digit] : 0u;
+#pragma unroll
+                for(uint32_t i = 0; i < BATCH; ++i)
+                {
+                    if(t0 + i < end)
+                        counts[uint64_t(t0 + i) * radix + digit] = before;
+                    before += count[i];
+                }
+            }
+            if(warp == 0u)
+                totals[digit] = total;
         }
 
         // Moves every key of a tile, with its token, to its place among the keys of this digit:
@@ -514,27 +546,27 @@ namespace b200wmma
         // of smaller lanes come first.  The tile is put in order in shared memory first, so that
         // neighbouring threads write neighbouring places.  pairs == nullptr: the first pass, key i
         // of `keys` belongs to token i.
-        template <uint32_t ITEMS, uint32_t PER>
+        template <uint32_t ITEMS, uint32_t BITS>
         struct ScatterShared
         {
             uint2    tile[THREADS * ITEMS];
-            uint16_t bins[SORT_WARPS][THREADS * PER];
-            uint32_t shifts[THREADS * PER]; // place of a digit's keys minus their place in the tile
+            uint16_t bins[SORT_WARPS][1u << BITS];
+            uint32_t shifts[1u << BITS]; // place of a digit's keys minus their place in the tile
             uint32_t warps[SORT_WARPS];
         };
 
-        template <uint32_t ITEMS, uint32_t PER>
+        template <uint32_t ITEMS, uint32_t BITS>
         __global__ void __launch_bounds__(THREADS)
-            scatterKernel(uint32_t const* keys, uint2 const* pairs, uint32_t n, const Digit digit, uint32_t tiles,
+            scatterKernel(uint32_t const* keys, uint2 const* pairs, uint32_t n, uint32_t pass,
                           uint32_t const* counts, uint32_t const* totals, uint2* out)
         {
-            constexpr uint32_t RADIX_HERE = THREADS * PER; // 2^bits or more; PER digits a thread
+            constexpr uint32_t RADIX = 1u << BITS, PER = RADIX / THREADS; // digits of a thread
             extern __shared__ uint8_t smem[];
-            auto*          sh   = reinterpret_cast<ScatterShared<ITEMS, PER>*>(smem);
-            const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, radix = 1u << digit.bits;
+            auto*          sh   = reinterpret_cast<ScatterShared<ITEMS, BITS>*>(smem);
+            const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
             grid_dependency_wait();
             grid_launch_dependents();
-            for(uint32_t i = threadIdx.x; i < SORT_WARPS * RADIX_HERE / 2u; i += THREADS)
+            for(uint32_t i = threadIdx.x; i < SORT_WARPS * RADIX / 2u; i += THREADS)
                 reinterpret_cast<uint32_t*>(sh->bins)[i] = 0;
             __syncthreads();
             const uint32_t tile0 = blockIdx.x * (THREADS * ITEMS), here = min(THREADS * ITEMS, n - tile0);
@@ -558,8 +590,8 @@ namespace b200wmma
             for(uint32_t i = 0; i < ITEMS; ++i)
             {
                 const bool     in    = first + i * 32u < here;
-                const uint32_t d     = digit.of(pair[i].x);
-                const uint32_t peers = sameDigit(d, in, digit.bits);
+                const uint32_t d     = digitOf<BITS>(pair[i].x, pass);
+                const uint32_t peers = sameDigit<BITS>(d, in);
                 rank[i]              = (in ? sh->bins[warp][d] : 0u) + __popc(peers & ((1u << lane) - 1u));
                 __syncwarp();
                 if(in && (peers >> lane) == 1u) // the last of its digit
@@ -580,7 +612,7 @@ namespace b200wmma
                     for(uint32_t w = 0; w < SORT_WARPS; ++w)
                         sums[j] += sh->bins[w][d0 + j];
                     mine += sums[j];
-                    all[j] = d0 + j < radix ? totals[d0 + j] : 0u;
+                    all[j] = totals[d0 + j];
                     whole += all[j];
                 }
                 uint32_t local  = blockScan(mine, sh->warps, total);
@@ -596,8 +628,7 @@ namespace b200wmma
                         sh->bins[w][d0 + j]  = uint16_t(at);
                         at += count;
                     }
-                    if(d0 + j < radix)
-                        sh->shifts[d0 + j] = global + counts[uint64_t(d0 + j) * tiles + blockIdx.x] - local;
+                    sh->shifts[d0 + j] = global + counts[uint64_t(blockIdx.x) * RADIX + d0 + j] - local;
                     local += sums[j];
                     global += all[j];
                 }
@@ -606,12 +637,12 @@ namespace b200wmma
 #pragma unroll
             for(uint32_t i = 0; i < ITEMS; ++i)
                 if(first + i * 32u < here)
-                    sh->tile[sh->bins[warp][digit.of(pair[i].x)] + rank[i]] = pair[i];
+                    sh->tile[sh->bins[warp][digitOf<BITS>(pair[i].x, pass)] + rank[i]] = pair[i];
             __syncthreads();
             for(uint32_t i = threadIdx.x; i < here; i += THREADS)
             {
                 const uint2 p = sh->tile[i];
-                out[sh->shifts[digit.of(p.x)] + i] = p;
+                out[sh->shifts[digitOf<BITS>(p.x, pass)] + i] = p;
             }
         }
 
@@ -1029,7 +1060,7 @@ namespace b200wmma
         struct Plan
         {
             uint64_t keys, pairs[2], counts, totals, pieceKeys, pieceSums, bytes;
-            uint32_t tiles, passes, digitBits, chunk, chunks; // digits: of many tokens
+            uint32_t tiles, passes, digitBits, chunk, chunks;
             bool     small;
         };
 
@@ -1045,9 +1076,10 @@ namespace b200wmma
             w.small    = count <= SMALL_TOKENS;
             const uint32_t tile = THREADS * (count < MANY_TOKENS ? FEW_ITEMS : MANY_ITEMS);
             w.tiles    = uint32_t((uint64_t(count) + tile - 1u) / tile);
-            const uint32_t bits = log2Up(rows + 1u), most1 = w.small ? 8u : SORT_BITS; // keys 0..rows
-            w.passes    = (bits + most1 - 1u) / most1;
+            const uint32_t bits = log2Up(rows + 1u); // keys 0..rows
+            w.passes    = (bits + SORT_BITS - 1u) / SORT_BITS;
             w.digitBits = (bits + w.passes - 1u) / w.passes;
+            w.digitBits = w.digitBits < 8u ? 8u : w.digitBits;
             w.pairs[0] = take(uint64_t(count) * 8u);
             if(!w.small)
             {
@@ -1119,8 +1151,8 @@ namespace b200wmma
 
         // (row, token) of every token into the workspace, sorted; few tokens: rows without one
         // cleared on the way.
-        template <typename OutT, int V>
-        int sortFew(GradientCall const& g, Plan const& w, cudaStream_t stream)
+        template <typename OutT, int V, uint32_t BITS>
+        int sortFewBits(GradientCall const& g, Plan const& w, cudaStream_t stream)
         {
             ClearParams c = clearParams(g.table, g.ldt, g.t.rows, g.dim / V);
             // a block to an SM, each with 16 KB of rows at least
@@ -1128,34 +1160,42 @@ namespace b200wmma
             c.blocks            = g.accumulate ? 0u : uint32_t(want < 147u ? want : 147u);
             static std::mutex mutex;
             static bool       done[64] = {};
-            B200WMMA_TRY(optIn(sortSmallKernel<OutT, V>, sizeof(SmallShared), mutex, done));
-            return cudaToStatus(launchOverlapped(sortSmallKernel<OutT, V>, dim3(1u + c.blocks), dim3(SMALL_THREADS),
-                                                 sizeof(SmallShared), stream, g.t, c, w.passes,
+            B200WMMA_TRY(optIn(sortSmallKernel<OutT, V, BITS>, sizeof(SmallShared<BITS>), mutex, done));
+            return cudaToStatus(launchOverlapped(sortSmallKernel<OutT, V, BITS>, dim3(1u + c.blocks), dim3(SMALL_THREADS),
+                                                 sizeof(SmallShared<BITS>), stream, g.t, c, w.passes,
                                                  reinterpret_cast<uint2*>(g.workspace + w.pairs[0])));
         }
 
-        template <uint32_t ITEMS, uint32_t PER>
+        template <typename OutT, int V>
+        int sortFew(GradientCall const& g, Plan const& w, cudaStream_t stream)
+        {
+            return w.digitBits == 8u ? sortFewBits<OutT, V, 8>(g, w, stream)
+                                     : w.digitBits == 9u ? sortFewBits<OutT, V, 9>(g, w, stream)
+                                                         : sortFewBits<OutT, V, 10>(g, w, stream);
+        }
+
+        template <uint32_t ITEMS, uint32_t BITS>
         int sortMany(GradientCall const& g, Plan const& w, uint2** sorted, cudaStream_t stream)
         {
             auto       words = [&](uint64_t at) { return reinterpret_cast<uint32_t*>(g.workspace + at); };
             auto       pairs = [&](uint32_t i) { return reinterpret_cast<uint2*>(g.workspace + w.pairs[i]); };
             static std::mutex mutex;
             static bool       done[64] = {};
-            B200WMMA_TRY(optIn(scatterKernel<ITEMS, PER>, sizeof(ScatterShared<ITEMS, PER>), mutex, done));
+            B200WMMA_TRY(optIn(scatterKernel<ITEMS, BITS>, sizeof(ScatterShared<ITEMS, BITS>), mutex, done));
             const dim3 grid(w.tiles);
-            auto       digit = [&](uint32_t pass) { return Digit{w.digitBits * pass, w.digitBits}; };
-            B200WMMA_TRY(cudaToStatus(launchOverlapped(keysKernel<ITEMS>, grid, dim3(THREADS), 0, stream, g.t, words(w.keys),
-                                                       w.tiles, digit(0), words(w.counts))));
+            B200WMMA_TRY(cudaToStatus(launchOverlapped(keysKernel<ITEMS, BITS>, grid, dim3(THREADS), 0, stream, g.t,
+                                                       words(w.keys), words(w.counts))));
             for(uint32_t pass = 0; pass < w.passes; ++pass)
             {
                 uint2* from = pass ? pairs((pass - 1u) % 2u) : nullptr;
                 if(pass > 0u)
-                    B200WMMA_TRY(cudaToStatus(launchOverlapped(countKernel<ITEMS>, grid, dim3(THREADS), 0, stream, from,
-                                                               g.t.count, digit(pass), w.tiles, words(w.counts))));
-                B200WMMA_TRY(cudaToStatus(launchOverlapped(scanKernel, dim3(1u << w.digitBits), dim3(THREADS), 0, stream,
-                                                           words(w.counts), w.tiles, words(w.totals))));
-                B200WMMA_TRY(cudaToStatus(launchOverlapped(scatterKernel<ITEMS, PER>, grid, dim3(THREADS), sizeof(ScatterShared<ITEMS, PER>),
-                                                           stream, words(w.keys), from, g.t.count, digit(pass), w.tiles,
+                    B200WMMA_TRY(cudaToStatus(launchOverlapped(countKernel<ITEMS, BITS>, grid, dim3(THREADS), 0, stream, from,
+                                                               g.t.count, pass, words(w.counts))));
+                constexpr uint32_t radix = 1u << BITS;
+                B200WMMA_TRY(cudaToStatus(launchOverlapped(scanKernel, dim3((radix + 31u) / 32u), dim3(SCAN_THREADS), 0, stream,
+                                                           words(w.counts), w.tiles, radix, words(w.totals))));
+                B200WMMA_TRY(cudaToStatus(launchOverlapped(scatterKernel<ITEMS, BITS>, grid, dim3(THREADS), sizeof(ScatterShared<ITEMS, BITS>),
+                                                           stream, words(w.keys), from, g.t.count, pass,
                                                            words(w.counts), words(w.totals), pairs(pass % 2u))));
             }
             *sorted = pairs((w.passes - 1u) % 2u);
@@ -1165,9 +1205,9 @@ namespace b200wmma
         template <uint32_t ITEMS>
         int sortDigits(GradientCall const& g, Plan const& w, uint2** sorted, cudaStream_t stream)
         {
-            return w.digitBits <= 8u ? sortMany<ITEMS, 1>(g, w, sorted, stream)
-                                     : w.digitBits == 9u ? sortMany<ITEMS, 2>(g, w, sorted, stream)
-                                                         : sortMany<ITEMS, 4>(g, w, sorted, stream);
+            return w.digitBits == 8u ? sortMany<ITEMS, 8>(g, w, sorted, stream)
+                                     : w.digitBits == 9u ? sortMany<ITEMS, 9>(g, w, sorted, stream)
+                                                         : sortMany<ITEMS, 10>(g, w, sorted, stream);
         }
 
         // The sums of chunks, with pieces of `V` values, and rows cleared beside them where the

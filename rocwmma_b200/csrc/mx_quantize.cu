@@ -242,19 +242,16 @@ namespace b200wmma
                 return uint32_t(reinterpret_cast<uintptr_t>(row) % 16u) / uint32_t(sizeof(T));
             }
         };
-        // Threads of the block move rows of `count` values, row r of the tile at global(r), to or
-        // from shared memory.
-        template <typename T, bool LOAD, typename Row>
-        __device__ inline void moveStaged(uint8_t* staged, uint32_t rows, uint32_t count, Row global)
+        // The eight threads of a row (`lane` 0 to 7) move `count` values of it to or from shared memory.
+        template <typename T, bool LOAD>
+        __device__ inline void moveStaged(uint8_t* staged, T* row, uint32_t shift, uint32_t count, uint32_t lane)
         {
             using S = StagedRow<T>;
-            for(uint32_t i = threadIdx.x; i < rows * S::PIECES; i += THREADS)
+#pragma unroll
+            for(uint32_t i = 0; i < (S::PIECES + 7u) / 8u; ++i)
             {
-                const uint32_t r = i / S::PIECES, piece = i % S::PIECES;
-                T*             row   = global(r);
-                const uint32_t shift = S::shift(row);
-                const uint32_t first = piece * S::PER; // of the piece, counted from the boundary
-                T*             here  = reinterpret_cast<T*>(staged + r * S::PITCH) + first;
+                const uint32_t first = (i * 8u + lane) * S::PER; // of the piece, counted from the boundary
+                T*             here  = reinterpret_cast<T*>(staged) + first;
                 T*             there = row + (int32_t(first) - int32_t(shift));
                 if(first >= shift && first + S::PER <= shift + count)
                 {
@@ -263,7 +260,7 @@ namespace b200wmma
                     else
                         *reinterpret_cast<uint4*>(there) = *reinterpret_cast<uint4 const*>(here);
                 }
-                else
+                else if(first < shift + count)
                 {
 #pragma unroll
                     for(uint32_t j = 0; j < S::PER; ++j)
@@ -337,17 +334,19 @@ namespace b200wmma
                 }
                 else
                 {
+                    // (a row's threads are in one warp)
                     const uint32_t count = min(TILE_K, p.k - (tile0 + t) * TILE_K);
-                    auto rowAt = [&](uint32_t i) {
-                        return const_cast<T*>(static_cast<T const*>(p.x)) + (row0 + i) * p.ldx + uint64_t(tile0 + t) * TILE_K;
-                    };
-                    __syncthreads();
-                    moveStaged<T, true>(staged, rows, count, rowAt);
-                    __syncthreads();
+                    T*             from  = const_cast<T*>(x) - col + done;
+                    const uint32_t shift = StagedRow<T>::shift(from);
+                    uint8_t*       here  = staged + r * StagedRow<T>::PITCH;
+                    __syncwarp();
+                    if(r < rows)
+                        moveStaged<T, true>(here, from, shift, count, threadIdx.x % 8u);
+                    __syncwarp();
                     raw = zeroRun<T>();
                     if(r < rows)
                     {
-                        T const* at = reinterpret_cast<T const*>(staged + r * StagedRow<T>::PITCH) + StagedRow<T>::shift(rowAt(r)) + col;
+                        T const* at = reinterpret_cast<T const*>(here) + shift + col;
 #pragma unroll
                         for(uint32_t j = 0; j < RUN; ++j)
                             if(col + j < count)
@@ -591,19 +590,20 @@ namespace b200wmma
                 else
                 {
                     const uint32_t count = min(TILE_K, p.k - (tile0 + t) * TILE_K);
-                    auto rowAt = [&](uint32_t i) {
-                        return static_cast<T*>(p.out) + (row0 + i) * p.ldo + uint64_t(tile0 + t) * TILE_K;
-                    };
-                    __syncthreads();
+                    T*             to    = out - col + done;
+                    const uint32_t shift = StagedRow<T>::shift(to);
+                    uint8_t*       here  = staged + r * StagedRow<T>::PITCH;
+                    __syncwarp();
                     if(r < rows)
                     {
-                        T* at = reinterpret_cast<T*>(staged + r * StagedRow<T>::PITCH) + StagedRow<T>::shift(rowAt(r)) + col;
+                        T* at = reinterpret_cast<T*>(here) + shift + col;
 #pragma unroll
                         for(uint32_t j = 0; j < RUN; ++j)
                             at[j] = o.v[j];
                     }
-                    __syncthreads();
-                    moveStaged<T, false>(staged, rows, count, rowAt);
+                    __syncwarp();
+                    if(r < rows)
+                        moveStaged<T, false>(here, to, shift, count, threadIdx.x % 8u);
                 }
             }
         }
