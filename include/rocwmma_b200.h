@@ -258,8 +258,8 @@ B200WMMA_API int b200wmma_embedding(int table_dtype, int out_dtype, uint64_t row
  *     table_grad[r * ldt + j] = scale * sum over the tokens of row r of grad[o * grad_outer + i * grad_inner + j]
  * (+ the old value where accumulate != 0, which leaves rows without tokens untouched; without it
  * those are set to zero).  Sums are fp32, the result is rounded once to table_dtype.  Tokens are
- * sorted by row and summed in an order that depends on outer, inner, dim and the ids alone: the
- * same call gives the same bits.  `workspace`: at least b200wmma_embedding_grad_workspace(...)
+ * sorted by row and summed in an order that depends on the sizes, the ids and the alignment of
+ * grad and table_grad alone: the same call gives the same bits.  `workspace`: at least b200wmma_embedding_grad_workspace(...)
  * bytes of device memory, 256-byte aligned, which the call may overwrite and leaves no state in;
  * calls that can run at the same time need one each.
  */

@@ -11,6 +11,7 @@
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "rocwmma_b200.h"
@@ -468,9 +469,9 @@ namespace
                 PyErr_SetString(PyExc_RuntimeError, s.where);
             Py_XDECREF(r);
         }
-        catch(std::exception const& e)
+        catch(...) // torch's own, such as no memory left
         {
-            PyErr_SetString(PyExc_RuntimeError, e.what());
+            torch::translate_exception_to_python(std::current_exception());
         }
         return nullptr;
     }

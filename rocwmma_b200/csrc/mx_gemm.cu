@@ -447,6 +447,7 @@ namespace b200wmma
         {
             return 2u * CODE_BYTES + 3u * slotGroups<KIND>() * MX_TILE_BYTES;
         }
+        // (Large enough that no block of the thin kernel fits beside it: see there.)
         template <ScaleKind KIND>
         constexpr uint32_t pairSmemBytes(bool useC)
         {
@@ -934,6 +935,8 @@ namespace b200wmma
                 rc = outputMap<OutT>(&mapC, q.c, q.m, q.n, q.ldc);
             if(rc != B200WMMA_OK)
                 return rc;
+            static_assert(pairSmemBytes<KIND>(true) >= 200u * 1024u && pairSmemBytes<KIND>(false) >= 200u * 1024u,
+                          "a thin block, 28 KB or more, must not fit beside a pair's");
             const uint32_t  smem = pairSmemBytes<KIND>(q.c != nullptr);
             static uint32_t done[64] = {};
             rc = optInSharedMemory(mxGemmPairKernel<KIND, OutT>, smem, done);
@@ -1002,7 +1005,15 @@ namespace b200wmma
                 rc = scaleMap(&mapScaleQ, thinA ? o.aScales : o.bScales, p.thin, groups, GROUPS, tilesOfQ);
             if(rc != B200WMMA_OK)
                 return rc;
-            const uint32_t  smem = 1024u + p.stages * p.slotBytes + uint32_t(sizeof(ThinControl));
+            // Blocks of a cluster wait for each other, and a block waits in tcgen05.alloc while its SM has
+            // no columns left: two clusters that each hold the columns that the other needs would wait
+            // for good.  So a block takes at least the share of its SM's shared memory that it takes of
+            // the 512 columns, and blocks that fit an SM always find theirs.  (The pair kernel, which
+            // takes all columns, leaves no room for the smallest block of this one.)
+            constexpr uint32_t SM_SMEM = 228u * 1024u, BLOCK_SMEM = 1024u; // of an SM; on top of each block's own
+            const uint32_t     share   = p.tmemCols * (SM_SMEM / 512u) - BLOCK_SMEM;
+            uint32_t           smem    = 1024u + p.stages * p.slotBytes + uint32_t(sizeof(ThinControl));
+            smem                       = smem < share ? share : smem;
             static uint32_t done[64] = {};
             rc = optInSharedMemory(mxGemmThinKernel<KIND, OutT>, smem, done);
             if(rc != B200WMMA_OK)

@@ -254,3 +254,24 @@ def test_quantize_and_product_in_a_graph_and_on_a_stream():
         bound = k * 2.0 ** -23 * (np.abs(xv) @ np.abs(wv).T)
         bound += 2.0 ** -8 * (np.abs(want) + bound)
         assert (np.abs(_host(d).reshape(m, n) - want) <= bound).all()
+
+
+def test_products_on_several_streams_at_once():
+    """Thin products, whose clusters hold tensor memory and wait for each other, and large ones beside
+    them: every block that fits an SM finds the columns it needs."""
+    g = torch.Generator().manual_seed(7)
+    work = []
+    for fmt, m, n, k in ((MXF4, 1, 4096, 1024), (NVF4, 100, 8192, 1024), (NVF4, 20, 2048, 2048), (MXF4, 400, 700, 512)):
+        (a, av), (b, bv) = _small(fmt, m, k, g), _small(fmt, n, k, g)
+        ld = (n + 7) // 8 * 8
+        want = torch.from_numpy(av @ bv.T).float().cuda()
+        work.append((fmt, m, n, k, a, b, ld, want, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    results = []
+    for _ in range(20):
+        for fmt, m, n, k, a, b, ld, want, stream in work:
+            results.append((m, n, api.mx_gemm(fmt, F32, m, n, k, a, b, None, 1.0, 0.0, ldd=ld, stream=stream), want))
+    torch.cuda.synchronize()
+    api.check_device()
+    for m, n, d, want in results:
+        assert torch.equal(d.view(m, -1)[:, :n], want)
