@@ -34,8 +34,11 @@ def np_dtype(code: int):
 def reference_dir() -> str:
     """Where the rocWMMA source tree is mounted (it need not exist).  The environment
     variable ROCWMMA_REFERENCE_DIR overrides the default location; the Makefile beside this
-    file receives it as REF."""
-    return os.environ.get("ROCWMMA_REFERENCE_DIR", "/root/reference")
+    file receives it as REF.  An empty mount point is not a tree: a path that does not exist then."""
+    path = os.environ.get("ROCWMMA_REFERENCE_DIR", "/root/reference")
+    if os.path.isdir(path) and not os.listdir(path):
+        return os.path.join(path, "library")
+    return path
 
 
 def _have_reference() -> bool:
