@@ -33,13 +33,32 @@ namespace b200wmma
         constexpr uint32_t NO_ROW  = 0x7fffffffu; // no token, or no row of the table
         constexpr uint32_t PASSES  = 0x80000000u; // with a row: a run that fills a chunk and goes on
 
+        // n / d for n < 2^31 by a multiplication: m = ceil(2^(31 + s) / d) with 2^s >= d is off by less
+        // than d / 2^(31 + s) of a quotient, too little to reach the next one.
+        struct Divisor
+        {
+            uint32_t d = 1, m = 0, s = 0;
+            Divisor() = default;
+            explicit Divisor(uint32_t by) : d(by)
+            {
+                while((1ull << s) < by)
+                    ++s;
+                m = uint32_t(((1ull << (31u + s)) + by - 1u) / by);
+            }
+            __device__ uint32_t of(uint32_t n) const // d > 1
+            {
+                return __umulhi(n, m) >> (s - 1u);
+            }
+        };
+
         // The tokens of a call.
         struct Tokens
         {
             void const*    ids;
             int64_t const* first;
             uint64_t       idsOuter, idsInner; // strides, elements
-            uint32_t       count, inner, rows;
+            uint32_t       count, rows;
+            Divisor        inner;
             uint32_t       wide; // 64-bit ids
         };
 
@@ -47,10 +66,10 @@ namespace b200wmma
         {
             outer = token;
             inner = 0;
-            if(t.inner > 1u)
+            if(t.inner.d > 1u)
             {
-                outer = token / t.inner;
-                inner = token - outer * t.inner;
+                outer = t.inner.of(token);
+                inner = token - outer * t.inner.d;
             }
             const uint64_t at = uint64_t(outer) * t.idsOuter + uint64_t(inner) * t.idsInner;
             return t.wide ? static_cast<int64_t const*>(t.ids)[at] : int64_t(static_cast<int32_t const*>(t.ids)[at]);
@@ -495,30 +514,41 @@ namespace b200wmma
             return before + sum - v;
         }
 
-        // A block has 32 digits: their counts become exclusive sums over the tiles, their totals go to
-        // totals[digit].  A warp reads the counts of neighbouring digits, its lanes' columns; the 32
-        // warps have a stretch of tiles each.
-        constexpr uint32_t SCAN_THREADS = 1024;
+        // A block has eight digits, a sector of each tile's counts: they become exclusive sums over the
+        // tiles, their totals go to totals[digit].  Four times 32 groups of eight threads have a
+        // stretch of tiles each.
+        constexpr uint32_t SCAN_THREADS = 1024, SCAN_DIGITS = 8;
         __global__ void __launch_bounds__(SCAN_THREADS) scanKernel(uint32_t* counts, uint32_t tiles, uint32_t radix, uint32_t* totals)
         {
-            __shared__ uint32_t sums[32][33];
+            constexpr uint32_t GROUPS = SCAN_THREADS / SCAN_DIGITS;
+            __shared__ uint32_t sums[32][SCAN_DIGITS];
             grid_dependency_wait();
             grid_launch_dependents();
-            const uint32_t lane = threadIdx.x % 32u, warp = threadIdx.x / 32u, digit = blockIdx.x * 32u + lane;
-            const uint32_t begin = uint32_t(uint64_t(tiles) * warp / 32u), end = uint32_t(uint64_t(tiles) * (warp + 1u) / 32u);
+            const uint32_t lane = threadIdx.x % 32u, warp = threadIdx.x / 32u, column = threadIdx.x % SCAN_DIGITS;
+            const uint32_t group = threadIdx.x / SCAN_DIGITS, digit = blockIdx.x * SCAN_DIGITS + column;
+            const uint32_t begin = uint32_t(uint64_t(tiles) * group / GROUPS), end = uint32_t(uint64_t(tiles) * (group + 1u) / GROUPS);
             const bool     in    = digit < radix;
             uint32_t       sum   = 0;
 #pragma unroll 8
             for(uint32_t t = begin; t < end; ++t)
                 sum += in ? counts[uint64_t(t) * radix + digit] : 0u;
-            sums[warp][lane] = sum;
+            uint32_t upTo = sum; // over the warp's groups so far
+#pragma unroll
+            for(uint32_t d = SCAN_DIGITS; d < 32u; d *= 2u)
+            {
+                const uint32_t other = __shfl_up_sync(0xffffffffu, upTo, d);
+                if(lane >= d)
+                    upTo += other;
+            }
+            if(lane >= 32u - SCAN_DIGITS)
+                sums[warp][column] = upTo;
             __syncthreads();
-            uint32_t before = 0, total = 0;
+            uint32_t before = upTo - sum, total = 0;
 #pragma unroll
             for(uint32_t w = 0; w < 32u; ++w)
             {
-                before += w < warp ? sums[w][lane] : 0u;
-                total += sums[w][lane];
+                before += w < warp ? sums[w][column] : 0u;
+                total += sums[w][column];
             }
             if(!in)
                 return;
@@ -537,7 +567,7 @@ namespace b200wmma
                     before += count[i];
                 }
             }
-            if(warp == 0u)
+            if(group == 0u)
                 totals[digit] = total;
         }
 
@@ -556,7 +586,7 @@ namespace b200wmma
         };
 
         template <uint32_t ITEMS, uint32_t BITS>
-        __global__ void __launch_bounds__(THREADS)
+        __global__ void __launch_bounds__(THREADS, 3)
             scatterKernel(uint32_t const* keys, uint2 const* pairs, uint32_t n, uint32_t pass,
                           uint32_t const* counts, uint32_t const* totals, uint2* out)
         {
@@ -654,15 +684,15 @@ namespace b200wmma
             uint2 const* sorted; // (row, token), equal rows next to each other
             void const*  grad;
             uint64_t     gradOuter, gradInner;
-            uint32_t     inner;
-            uint32_t     n, chunk, chunks, rows;
+            Divisor      inner;
+            uint32_t     n, chunk, parts, rows; // parts: blocks' worth of chunks
             uint32_t     pieces, lanesLog2, slices; // pieces of a row; threads side by side on it; blocks
             uint32_t     blocks; // that sum; those behind them clear
             void*        table;
             uint64_t     ldt;
             float        scale;
             uint32_t     accumulate;
-            uint32_t*    pieceKeys; // two of each chunk: run from the left, run to the right; nullptr: one chunk
+            uint32_t*    pieceKeys; // two of each part: run from the left, run to the right; nullptr: one part
             float*       pieceSums; // rows of `pieces * V`
         };
 
@@ -786,10 +816,10 @@ namespace b200wmma
                 const uint64_t at   = item0 + i; // of item at - 1
                 const uint2    pair = at >= 1u && at <= p.n ? p.sorted[at - 1u] : make_uint2(NO_ROW, 0u);
                 uint32_t       outer = pair.y, in = 0;
-                if(p.inner > 1u)
+                if(p.inner.d > 1u)
                 {
-                    outer = pair.y / p.inner;
-                    in    = pair.y - outer * p.inner;
+                    outer = p.inner.of(pair.y);
+                    in    = pair.y - outer * p.inner.d;
                 }
                 rows[i]   = pair.x;
                 places[i] = uint64_t(outer) * p.gradOuter + uint64_t(in) * p.gradInner;
@@ -797,21 +827,21 @@ namespace b200wmma
             __syncthreads();
             const uint32_t piece = slice * lanes + (threadIdx.x & (lanes - 1u));
             const uint32_t local = (threadIdx.x >> p.lanesLog2) * p.chunk; // first item in shared memory
-            const uint64_t begin = item0 + local, chunkIdx = begin / p.chunk;
-            if(piece >= p.pieces || begin >= p.n)
-                return;
-            const uint32_t  count  = uint32_t(min(uint64_t(p.chunk), p.n - begin));
-            const uint64_t  width  = uint64_t(p.pieces) * V;
+            const uint64_t begin = item0 + local;
+            const uint32_t count = piece < p.pieces && begin < p.n ? uint32_t(min(uint64_t(p.chunk), p.n - begin)) : 0u;
             const uint32_t  before = rows[local], after = rows[local + count + 1u];
             uint32_t const* rowAt  = rows + local + 1u;
             uint64_t const* place  = places + local + 1u;
             T const*        grad   = static_cast<T const*>(p.grad) + uint64_t(piece) * V;
 
-            float    sum[V];
+            float    sum[V], left[V]; // of the current run; of the one that came from the left
             uint32_t run      = NO_ROW; // row of the current run
             bool     fromLeft = false;
             uint32_t leftKey = NO_ROW, rightKey = NO_ROW;
-            auto     load = [&](uint32_t i) {
+#pragma unroll
+            for(int j = 0; j < V; ++j)
+                sum[j] = left[j] = 0.0f;
+            auto load = [&](uint32_t i) {
                 if(i < count && rowAt[i] < p.rows)
                     R::load(ring, i % R::DEPTH, grad + place[i]);
                 asm volatile("cp.async.commit_group;" ::: "memory");
@@ -832,13 +862,13 @@ namespace b200wmma
                             finishRow<OutT, V>(p, run, piece, sum);
                         else
                         {
-                            Piece<float, V> s;
-#pragma unroll
-                            for(int j = 0; j < V; ++j)
-                                s.v[j] = sum[j];
-                            storePiece<float, V>(p.pieceSums + (2u * chunkIdx + (fromLeft ? 0u : 1u)) * width + uint64_t(piece) * V, s);
                             if(fromLeft)
+                            {
                                 leftKey = run;
+#pragma unroll
+                                for(int j = 0; j < V; ++j)
+                                    left[j] = sum[j];
+                            }
                             if(toRight) // a piece of a run that starts here, or one that passes through
                                 rightKey = run | (fromLeft ? PASSES : 0u);
                         }
@@ -861,16 +891,85 @@ namespace b200wmma
                 }
                 load(i + R::DEPTH);
             }
-            if(piece == 0u && p.pieceKeys)
+            // The runs that cross the block's chunks: the pieces take the rings' place.
+            __shared__ uint32_t leftKeys[32], rightKeys[32], ends[2];
+            const uint32_t group = threadIdx.x >> p.lanesLog2, lane = threadIdx.x & (lanes - 1u);
+            auto           pieceAt = [&](uint32_t g, uint32_t side) {
+                return reinterpret_cast<float*>(ringWords) + ((2u * g + side) * lanes + lane) * V;
+            };
+            __syncthreads();
+            if(lane == 0u)
             {
-                p.pieceKeys[2u * chunkIdx]      = leftKey;
-                p.pieceKeys[2u * chunkIdx + 1u] = rightKey;
+                leftKeys[group]  = leftKey;
+                rightKeys[group] = rightKey;
             }
+            if(threadIdx.x < 2u)
+                ends[threadIdx.x] = NO_ROW;
+            if(leftKey < p.rows)
+            {
+#pragma unroll
+                for(int j = 0; j < V; ++j)
+                    pieceAt(group, 0)[j] = left[j];
+            }
+            if(rightKey < p.rows)
+            {
+#pragma unroll
+                for(int j = 0; j < V; ++j)
+                    pieceAt(group, 1)[j] = sum[j];
+            }
+            __syncthreads();
+            const uint64_t part = blockIdx.x / p.slices, width = uint64_t(p.pieces) * V;
+            // the run `row` whose piece of chunk g, on its `side`, comes first in the block
+            auto follow = [&](uint32_t row, uint32_t g, uint32_t side) {
+#pragma unroll
+                for(int j = 0; j < V; ++j)
+                    sum[j] = pieceAt(g, side)[j];
+                bool on = side == 1u || rightKeys[g] == (row | PASSES);
+                for(++g; on && g < groups; ++g)
+                {
+#pragma unroll
+                    for(int j = 0; j < V; ++j)
+                        sum[j] += pieceAt(g, 0)[j];
+                    on = rightKeys[g] == (row | PASSES);
+                }
+                if(side == 1u && !on)
+                {
+                    if(piece < p.pieces)
+                        finishRow<OutT, V>(p, row, piece, sum);
+                    return;
+                }
+                if(lane == 0u)
+                {
+                    if(side == 0u)
+                        ends[0] = row;
+                    if(on)
+                        ends[1] = row | (side == 0u ? PASSES : 0u);
+                }
+                if(piece < p.pieces)
+                {
+                    Piece<float, V> s;
+#pragma unroll
+                    for(int j = 0; j < V; ++j)
+                        s.v[j] = sum[j];
+                    storePiece<float, V>(p.pieceSums + (2u * part + side) * width + uint64_t(piece) * V, s);
+                }
+            };
+            const uint32_t starts = rightKeys[group];
+            if(starts < p.rows)
+                follow(starts, group, 1);
+            if(group == 0u && leftKeys[0] < p.rows)
+                follow(leftKeys[0], 0, 0);
+            if(!p.pieceKeys || slice != 0u)
+                return;
+            __syncthreads();
+            if(threadIdx.x < 2u)
+                p.pieceKeys[2u * part + threadIdx.x] = ends[threadIdx.x];
         }
 
-        // Joins the runs that cross chunks.  A group of threads side by side has a chunk: where a run
-        // starts there that goes on to the right, the row is the sum of that piece, of those of the
-        // chunks that the run passes through, and of the last one's, in this order.  Runs of more
+        // Joins the runs that cross parts, as a block's worth of chunks is called.  A group of threads side
+        // by side has a part: where a run starts there that goes on to the right, the row is the sum
+        // of that piece, of those of the parts that the run passes through, and of the last one's, in
+        // this order.  Runs of more
         // than JOIN_FEW pieces are left to the whole block: its groups take the pieces in turn.
         constexpr uint32_t JOIN_FEW = 16;
 
@@ -893,7 +992,7 @@ namespace b200wmma
             float const*   at    = p.pieceSums + uint64_t(piece) * V;
             auto           rightKey = [&](uint32_t c) { return p.pieceKeys[2u * uint64_t(c) + 1u]; };
             float          sum[V];
-            // pieces begin, begin + step, ... of a run of `count` that starts in chunk `first`
+            // pieces begin, begin + step, ... of a run of `count` that starts in part `first`
             auto add = [&](uint32_t first, uint32_t begin, uint32_t count, uint32_t step) {
 #pragma unroll
                 for(int j = 0; j < V; ++j)
@@ -919,7 +1018,7 @@ namespace b200wmma
                 }
             };
             const uint64_t mine = uint64_t(blockIdx.x / p.slices) * groups + group;
-            if(mine + 1u < p.chunks)
+            if(mine + 1u < p.parts)
             {
                 const uint32_t first = uint32_t(mine), row = rightKey(first);
                 if(row < p.rows) // a run starts here and goes on
@@ -943,14 +1042,14 @@ namespace b200wmma
             for(uint32_t l = 0; l < longCount; ++l)
             {
                 const uint32_t first = longs[l], row = rightKey(first);
-                for(uint32_t c0 = first + 1u;; c0 += THREADS) // the run's last chunk
+                for(uint32_t c0 = first + 1u;; c0 += THREADS) // the run's last part
                 {
                     __syncthreads();
                     if(threadIdx.x == 0u)
                         end = 0xffffffffu;
                     __syncthreads();
                     const uint32_t c = c0 + threadIdx.x;
-                    if(c >= p.chunks || rightKey(c) != (row | PASSES))
+                    if(c >= p.parts || rightKey(c) != (row | PASSES))
                         atomicMin(&end, c);
                     __syncthreads();
                     if(end != 0xffffffffu)
@@ -1056,11 +1155,18 @@ namespace b200wmma
             return lanesLog2 == 0u ? 32u : lanesLog2 >= 4u ? THREADS : 16u << lanesLog2;
         }
 
+        // Blocks along the tokens.
+        uint64_t partsOf(uint32_t count, uint32_t chunk, uint32_t lanesLog2)
+        {
+            const uint64_t per = uint64_t(sumThreads(lanesLog2) >> lanesLog2) * chunk;
+            return (count + per - 1u) / per;
+        }
+
         // The workspace of the gradient; offsets in bytes.  The chunks go by the sizes alone.
         struct Plan
         {
             uint64_t keys, pairs[2], counts, totals, pieceKeys, pieceSums, bytes;
-            uint32_t tiles, passes, digitBits, chunk, chunks;
+            uint32_t tiles, passes, digitBits, chunk;
             bool     small;
         };
 
@@ -1097,11 +1203,14 @@ namespace b200wmma
             w.chunk = 8;
             while(w.chunk < 128u && w.chunk < most && uint64_t(count) * pieces > uint64_t(w.chunk) * DEVICE_THREADS)
                 w.chunk *= 2u;
-            w.chunks = (count + w.chunk - 1u) / w.chunk;
-            if(w.chunks > 1u)
+            // pieces of runs: two of each part, of which there are most where a row is cut into single
+            // values and fewest of its pieces' threads fit a block
+            const uint32_t single = rowLanesLog2(dim);
+            const uint64_t parts  = partsOf(count, w.chunk, single);
+            if(parts > 1u)
             {
-                w.pieceKeys = take(uint64_t(w.chunks) * 8u);
-                w.pieceSums = take(uint64_t(w.chunks) * 2u * dim * 4u);
+                w.pieceKeys = take(parts * 8u);
+                w.pieceSums = take(parts * 2u * dim * 4u);
             }
             w.bytes = at;
             return w;
@@ -1192,7 +1301,7 @@ namespace b200wmma
                     B200WMMA_TRY(cudaToStatus(launchOverlapped(countKernel<ITEMS, BITS>, grid, dim3(THREADS), 0, stream, from,
                                                                g.t.count, pass, words(w.counts))));
                 constexpr uint32_t radix = 1u << BITS;
-                B200WMMA_TRY(cudaToStatus(launchOverlapped(scanKernel, dim3((radix + 31u) / 32u), dim3(SCAN_THREADS), 0, stream,
+                B200WMMA_TRY(cudaToStatus(launchOverlapped(scanKernel, dim3((radix + SCAN_DIGITS - 1u) / SCAN_DIGITS), dim3(SCAN_THREADS), 0, stream,
                                                            words(w.counts), w.tiles, radix, words(w.totals))));
                 B200WMMA_TRY(cudaToStatus(launchOverlapped(scatterKernel<ITEMS, BITS>, grid, dim3(THREADS), sizeof(ScatterShared<ITEMS, BITS>),
                                                            stream, words(w.keys), from, g.t.count, pass,
@@ -1219,8 +1328,7 @@ namespace b200wmma
             p.lanesLog2 = rowLanesLog2(p.pieces);
             p.slices    = (p.pieces + (1u << p.lanesLog2) - 1u) >> p.lanesLog2;
             const uint32_t threads = sumThreads(p.lanesLog2);
-            const uint64_t per     = uint64_t(threads >> p.lanesLog2) * p.chunk;
-            const uint64_t blocks  = (p.n + per - 1u) / per * p.slices;
+            const uint64_t blocks  = uint64_t(p.parts) * p.slices;
             // rows may lie on wider boundaries than those of the gradient: clear by the narrower
             ClearParams c = clearParams(g.table, g.ldt, g.t.rows, p.pieces);
             c.lanesLog2   = c.lanesLog2 < log2Up(threads) ? c.lanesLog2 : log2Up(threads);
@@ -1248,7 +1356,7 @@ namespace b200wmma
             p.lanesLog2 = rowLanesLog2(p.pieces) < 5u ? rowLanesLog2(p.pieces) : 5u;
             p.slices    = (p.pieces + (1u << p.lanesLog2) - 1u) >> p.lanesLog2;
             const uint32_t groups = THREADS >> p.lanesLog2;
-            const uint64_t blocks = (uint64_t(p.chunks) + groups - 1u) / groups * p.slices;
+            const uint64_t blocks = (uint64_t(p.parts) + groups - 1u) / groups * p.slices;
             if(blocks > 0x7fffffffull)
                 return B200WMMA_ERR_TOO_LARGE;
             return cudaToStatus(launchOverlapped(joinKernel<OutT, V>, dim3(uint32_t(blocks)), dim3(THREADS), 0, stream, p));
@@ -1275,20 +1383,20 @@ namespace b200wmma
             p.inner      = g.t.inner;
             p.n          = g.t.count;
             p.chunk      = w.chunk;
-            p.chunks     = w.chunks;
+            p.parts      = uint32_t(partsOf(g.t.count, w.chunk, rowLanesLog2(g.dim / vg)));
             p.rows       = g.t.rows;
             p.table      = g.table;
             p.ldt        = g.ldt;
             p.scale      = g.scale;
             p.accumulate = g.accumulate ? 1u : 0u;
-            if(w.chunks > 1u)
+            if(p.parts > 1u)
             {
                 p.pieceKeys = reinterpret_cast<uint32_t*>(g.workspace + w.pieceKeys);
                 p.pieceSums = reinterpret_cast<float*>(g.workspace + w.pieceSums);
             }
             B200WMMA_TRY(vg == 8u ? (sumChunks<T, OutT, 8>(g, w, p, stream))
                                   : vg == 2u ? (sumChunks<T, OutT, 2>(g, w, p, stream)) : (sumChunks<T, OutT, 1>(g, w, p, stream)));
-            if(w.chunks > 1u)
+            if(p.parts > 1u)
                 B200WMMA_TRY(vt == 8u ? (joinPieces<OutT, 8>(g, p, stream))
                                       : vt == 2u ? (joinPieces<OutT, 2>(g, p, stream)) : (joinPieces<OutT, 1>(g, p, stream)));
             return B200WMMA_OK;
@@ -1343,7 +1451,7 @@ int b200wmma_embedding(int table_dtype, int out_dtype, uint64_t rows, uint32_t d
     if(rc != B200WMMA_OK)
         return rc;
     LookupParams p{};
-    p.t = Tokens{ids, first, ids_outer, ids_inner, uint32_t(outer * inner), inner, uint32_t(rows), id_bytes == 8 ? 1u : 0u};
+    p.t = Tokens{ids, first, ids_outer, ids_inner, uint32_t(outer * inner), uint32_t(rows), Divisor(inner), id_bytes == 8 ? 1u : 0u};
     p.table    = table;
     p.out      = out;
     p.ldt      = ldt;
@@ -1382,7 +1490,7 @@ int b200wmma_embedding_grad(int grad_dtype, int table_dtype, uint64_t rows, uint
         return B200WMMA_ERR_INVALID_ARG;
     if(!aligned(workspace, 256))
         return B200WMMA_ERR_ALIGNMENT;
-    const GradientCall g{Tokens{ids, first, ids_outer, ids_inner, uint32_t(outer * inner), inner, uint32_t(rows), id_bytes == 8 ? 1u : 0u},
+    const GradientCall g{Tokens{ids, first, ids_outer, ids_inner, uint32_t(outer * inner), uint32_t(rows), Divisor(inner), id_bytes == 8 ? 1u : 0u},
                          grad, grad_outer, grad_inner, table_grad, ldt, dim, float(scale), accumulate != 0,
                          static_cast<uint8_t*>(workspace)};
     const cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -275,3 +275,23 @@ def test_products_on_several_streams_at_once():
     api.check_device()
     for m, n, d, want in results:
         assert torch.equal(d.view(m, -1)[:, :n], want)
+
+
+@FORMATS
+def test_linear_layer_and_its_gradients(fmt):
+    """y = x W^T, dx = dy W and dW = dy^T x, each from operands quantised along the index it sums over."""
+    m, n, k = 150, 200, 330
+    x, w, dy = _values(m, k, BF16, 1), _values(n, k, BF16, 2, 0.2), _values(m, n, BF16, 3)
+
+    def both(t, columns):
+        """(operand, its values): the rows of t, or its columns."""
+        rows, length = t.shape[::-1] if columns else t.shape
+        q = api.mx_quantize(fmt, BF16, rows, length, t.cuda(), layout=COL_MAJOR if columns else ROW_MAJOR)
+        return q, R.quantize(fmt, _host(t).T if columns else _host(t))[2]
+
+    for a, b in ((both(x, False), both(w, False)), (both(dy, False), both(w, True)), (both(dy, True), both(x, True))):
+        rows, cols, length = a[1].shape[0], b[1].shape[0], a[1].shape[1]
+        ld = (cols + 3) // 4 * 4
+        d = api.mx_gemm(fmt, F32, rows, cols, length, a[0], b[0], None, 1.0, 0.0, ldd=ld)
+        bound = length * 2.0 ** -23 * (np.abs(a[1]) @ np.abs(b[1]).T)
+        assert (np.abs(_host(d.view(rows, ld)[:, :cols]) - a[1] @ b[1].T) <= bound).all()
