@@ -414,7 +414,7 @@ namespace b200wmma
         // SMs without one (a block's own latency is the kernels' time then: 74000 tokens in 4 columns
         // of 2900 rows, whole call, 86 us with sixteen, 62 with four).
         constexpr uint32_t SORT_WARPS = THREADS / 32;
-        constexpr uint32_t FEW_ITEMS = 4, MANY_ITEMS = 16, MANY_TOKENS = 500000;
+        constexpr uint32_t FEW_ITEMS = 4, MANY_ITEMS = 16, MANY_TOKENS = 500000, FEW_TILES = 96;
 
         // bins[digit] = keys of the tile
         template <uint32_t ITEMS, uint32_t BITS>
@@ -587,7 +587,7 @@ namespace b200wmma
 
         template <uint32_t ITEMS, uint32_t BITS>
         __global__ void __launch_bounds__(THREADS, 3)
-            scatterKernel(uint32_t const* keys, uint2 const* pairs, uint32_t n, uint32_t pass,
+            scatterKernel(uint32_t const* keys, uint2 const* pairs, uint32_t n, uint32_t pass, uint32_t tiles,
                           uint32_t const* counts, uint32_t const* totals, uint2* out)
         {
             constexpr uint32_t RADIX = 1u << BITS, PER = RADIX / THREADS; // digits of a thread
@@ -633,7 +633,32 @@ namespace b200wmma
             // in the whole
             {
                 const uint32_t d0 = threadIdx.x * PER;
-                uint32_t       sums[PER], all[PER], total, mine = 0, whole = 0;
+                uint32_t       sums[PER], all[PER], earlier[PER], total, mine = 0, whole = 0;
+                if(tiles != 0u)
+                {
+                    // few tiles: their counts are added up here instead of by a kernel of its own
+#pragma unroll
+                    for(uint32_t j = 0; j < PER; ++j)
+                        all[j] = earlier[j] = 0;
+#pragma unroll 8
+                    for(uint32_t t = 0; t < tiles; ++t)
+#pragma unroll
+                        for(uint32_t j = 0; j < PER; ++j)
+                        {
+                            const uint32_t count = counts[uint64_t(t) * RADIX + d0 + j];
+                            all[j] += count;
+                            earlier[j] += t < blockIdx.x ? count : 0u;
+                        }
+                }
+                else
+                {
+#pragma unroll
+                    for(uint32_t j = 0; j < PER; ++j)
+                    {
+                        all[j]     = totals[d0 + j];
+                        earlier[j] = counts[uint64_t(blockIdx.x) * RADIX + d0 + j];
+                    }
+                }
 #pragma unroll
                 for(uint32_t j = 0; j < PER; ++j)
                 {
@@ -642,7 +667,6 @@ namespace b200wmma
                     for(uint32_t w = 0; w < SORT_WARPS; ++w)
                         sums[j] += sh->bins[w][d0 + j];
                     mine += sums[j];
-                    all[j] = totals[d0 + j];
                     whole += all[j];
                 }
                 uint32_t local  = blockScan(mine, sh->warps, total);
@@ -658,7 +682,7 @@ namespace b200wmma
                         sh->bins[w][d0 + j]  = uint16_t(at);
                         at += count;
                     }
-                    sh->shifts[d0 + j] = global + counts[uint64_t(blockIdx.x) * RADIX + d0 + j] - local;
+                    sh->shifts[d0 + j] = global + earlier[j] - local;
                     local += sums[j];
                     global += all[j];
                 }
@@ -1301,10 +1325,13 @@ namespace b200wmma
                     B200WMMA_TRY(cudaToStatus(launchOverlapped(countKernel<ITEMS, BITS>, grid, dim3(THREADS), 0, stream, from,
                                                                g.t.count, pass, words(w.counts))));
                 constexpr uint32_t radix = 1u << BITS;
-                B200WMMA_TRY(cudaToStatus(launchOverlapped(scanKernel, dim3((radix + SCAN_DIGITS - 1u) / SCAN_DIGITS), dim3(SCAN_THREADS), 0, stream,
-                                                           words(w.counts), w.tiles, radix, words(w.totals))));
+                if(w.tiles > FEW_TILES)
+                    B200WMMA_TRY(cudaToStatus(launchOverlapped(scanKernel, dim3((radix + SCAN_DIGITS - 1u) / SCAN_DIGITS),
+                                                               dim3(SCAN_THREADS), 0, stream, words(w.counts), w.tiles, radix,
+                                                               words(w.totals))));
                 B200WMMA_TRY(cudaToStatus(launchOverlapped(scatterKernel<ITEMS, BITS>, grid, dim3(THREADS), sizeof(ScatterShared<ITEMS, BITS>),
                                                            stream, words(w.keys), from, g.t.count, pass,
+                                                           w.tiles > FEW_TILES ? 0u : w.tiles,
                                                            words(w.counts), words(w.totals), pairs(pass % 2u))));
             }
             *sorted = pairs((w.passes - 1u) % 2u);

@@ -108,7 +108,8 @@ def test_gradient(kind, out_t, tokens, rows, dim, skew):
         _check_grad(got, grad, ids, rows, out_t, scale)
 
 
-@pytest.mark.parametrize("tokens,rows,dim", [(300000, 40, 8), (70000, 1, 16), (200000, 100000, 3)])
+@pytest.mark.parametrize("tokens,rows,dim", [(300000, 40, 8), (70000, 1, 16), (200000, 100000, 3), (60000, 5000, 8),
+                                             (16385, 300, 520), (700000, 3000, 4)])
 def test_gradient_of_long_runs(tokens, rows, dim):
     """Rows that most tokens share: runs over many chunks and levels; every bit the same again."""
     grad, ids = _randn((tokens, dim), BF16, 1), _ids((tokens,), rows, 2, 6.0)
