@@ -11,9 +11,10 @@
 // Both are bound by HBM.  The gradient is made without atomics on its values, so that a call's
 // result depends on its arguments alone: tokens are sorted by row (a stable radix sort), the
 // sorted tokens are cut into chunks, and every run of equal rows in a chunk is summed in token
-// order, in fp32.  A run inside one chunk is written at once; a run that crosses chunks leaves a
-// piece for each in the workspace, and a last kernel joins those.  Rows without a token are
-// cleared by blocks of their own beside the others.
+// order, in fp32.  A run inside one chunk is written at once; the pieces of one that crosses
+// chunks are added up by the block that has them, and where it crosses blocks too, each block
+// leaves a piece in the workspace and a last kernel joins those.  Rows without a token are cleared by
+// blocks of their own beside the others.
 #include "common.cuh"
 #include "mx_format.cuh"
 #include "rocwmma/rocwmma_block.hpp"
@@ -81,7 +82,7 @@ namespace b200wmma
             {
                 begin = t.first[inner];
                 end   = t.first[inner + 1];
-                if(begin < 0 || end > int64_t(t.rows))
+                if(begin < 0 || end < begin || end > int64_t(t.rows)) // (end - begin must not wrap)
                     return NO_ROW;
             }
             return id >= 0 && id < end - begin ? uint32_t(begin + id) : NO_ROW;
@@ -253,6 +254,11 @@ namespace b200wmma
         constexpr uint32_t SMALL_THREADS = 1024;
         constexpr uint32_t SMALL_ITEMS   = 16;
         constexpr uint32_t SMALL_TOKENS  = SMALL_THREADS * SMALL_ITEMS;
+        // One block sorts 4096 tokens in the time that the launches of the other way take (50000 rows of
+        // 32: 23 us either way; 16384 tokens: 47 and 30).  Beyond, it pays while the other SMs have rows
+        // to clear for as long: 16384 tokens and 192 MB of table 57 us either way, 537 MB 122 and 157.
+        constexpr uint32_t SMALL_ALWAYS      = 4096;
+        constexpr uint64_t SMALL_CLEAR_BYTES = 12288; // of the table, a token
         constexpr uint32_t SMALL_WARPS   = SMALL_THREADS / 32;
         constexpr uint32_t SORT_BITS     = 10; // of a digit, at most
         constexpr uint32_t SORT_RADIX    = 1u << SORT_BITS;
@@ -306,8 +312,8 @@ namespace b200wmma
             }
             // A warp's keys are neighbours, 32 of them a step.  A key's token and its rank among the
             // warp's keys of its digit share a register.
-            constexpr uint32_t RADIX = 1u << BITS, PER = RADIX <= SMALL_THREADS ? 1u : RADIX / SMALL_THREADS;
-            static_assert(PER == 1u, "a thread has a digit");
+            constexpr uint32_t RADIX = 1u << BITS;
+            static_assert(RADIX <= SMALL_THREADS, "a thread has a digit");
             const uint32_t items = (t.count + SMALL_THREADS - 1u) / SMALL_THREADS;
             const uint32_t warps = (t.count + 32u * items - 1u) / (32u * items); // that have keys
             const uint32_t first = warp * 32u * items + lane;
@@ -410,11 +416,15 @@ namespace b200wmma
         }
 
         // ---- sorting many tokens -------------------------------------------------------------
-        // A block has a tile of THREADS x ITEMS keys: sixteen a thread, or four where that would leave
-        // SMs without one (a block's own latency is the kernels' time then: 74000 tokens in 4 columns
-        // of 2900 rows, whole call, 86 us with sixteen, 62 with four).
+        // A block has a tile of THREADS x ITEMS keys.  Four a thread make the blocks that hide a block's
+        // own latency, sixteen write longer stretches and leave fewer counts to add up: whole calls
+        // take 57 us with four and 61 with sixteen at 200000 tokens, 160 and 161 at 1.7 million, 292
+        // and 264 at four million.
+        // Up to FEW_TILES tiles, the scattering blocks add up the tiles' counts themselves instead of
+        // a kernel of its own: 32.8 us so and 35.6 with the kernel at 20 tiles, 41.2 and 42.6 at 59,
+        // 47.4 and 44.2 at 79.
         constexpr uint32_t SORT_WARPS = THREADS / 32;
-        constexpr uint32_t FEW_ITEMS = 4, MANY_ITEMS = 16, MANY_TOKENS = 500000, FEW_TILES = 96;
+        constexpr uint32_t FEW_ITEMS = 4, MANY_ITEMS = 16, MANY_TOKENS = 2000000, FEW_TILES = 64;
 
         // bins[digit] = keys of the tile
         template <uint32_t ITEMS, uint32_t BITS>
@@ -990,11 +1000,11 @@ namespace b200wmma
                 p.pieceKeys[2u * part + threadIdx.x] = ends[threadIdx.x];
         }
 
-        // Joins the runs that cross parts, as a block's worth of chunks is called.  A group of threads side
-        // by side has a part: where a run starts there that goes on to the right, the row is the sum
-        // of that piece, of those of the parts that the run passes through, and of the last one's, in
-        // this order.  Runs of more
-        // than JOIN_FEW pieces are left to the whole block: its groups take the pieces in turn.
+        // Joins the runs that cross parts, as a block's worth of chunks is called.  A group of threads
+        // side by side has a part: where a run starts there that goes on to the right, the row is the
+        // sum of that piece, of those of the parts that the run passes through, and of the last one's,
+        // in this order.  Runs of more than JOIN_FEW pieces are left to the whole block: its groups
+        // take the pieces in turn.
         constexpr uint32_t JOIN_FEW = 16;
 
         template <typename OutT, int V>
@@ -1194,7 +1204,13 @@ namespace b200wmma
             bool     small;
         };
 
-        Plan planGradient(uint64_t rows, uint32_t dim, uint32_t count)
+        // Whether one block sorts: see SMALL_ALWAYS.  `clear`: bytes to be cleared, at most.
+        bool sortsSmall(uint32_t count, uint64_t clear)
+        {
+            return count <= SMALL_ALWAYS || (count <= SMALL_TOKENS && clear >= count * SMALL_CLEAR_BYTES);
+        }
+
+        Plan planGradient(uint64_t rows, uint32_t dim, uint32_t count, bool small)
         {
             Plan     w{};
             uint64_t at   = 0;
@@ -1203,7 +1219,7 @@ namespace b200wmma
                 at += (bytes + 255u) / 256u * 256u;
                 return here;
             };
-            w.small    = count <= SMALL_TOKENS;
+            w.small    = small;
             const uint32_t tile = THREADS * (count < MANY_TOKENS ? FEW_ITEMS : MANY_ITEMS);
             w.tiles    = uint32_t((uint64_t(count) + tile - 1u) / tile);
             const uint32_t bits = log2Up(rows + 1u); // keys 0..rows
@@ -1392,7 +1408,8 @@ namespace b200wmma
         template <typename T, typename OutT>
         int gradient(GradientCall const& g, cudaStream_t stream)
         {
-            const Plan     w  = planGradient(g.t.rows, g.dim, g.t.count);
+            const uint64_t clear = g.accumulate ? 0u : uint64_t(g.t.rows) * g.dim * sizeof(OutT);
+            const Plan     w  = planGradient(g.t.rows, g.dim, g.t.count, sortsSmall(g.t.count, clear));
             const uint32_t vt = pieceSize(g.dim, g.table, sizeof(OutT), 8, g.ldt);
             const uint32_t vg = pieceSize(g.dim, g.grad, sizeof(T), vt, g.gradOuter, g.gradInner);
             uint2*         sorted = reinterpret_cast<uint2*>(g.workspace + w.pairs[0]);
@@ -1456,7 +1473,7 @@ namespace b200wmma
             if(!aligned(table, dtypeSize(tableType)) || !aligned(values, dtypeSize(valuesType))
                || !aligned(ids, uint64_t(idBytes)) || !aligned(first, 8))
                 return B200WMMA_ERR_ALIGNMENT;
-            // rows and tokens are counted in 31 bits; a grid's second dimension has 16
+            // rows and tokens are counted in 31 bits
             if(rows >= NO_ROW || outer > 0x7ffff000ull / inner || dim > 0x100000u)
                 return B200WMMA_ERR_TOO_LARGE;
             return B200WMMA_OK;
@@ -1500,7 +1517,9 @@ uint64_t b200wmma_embedding_grad_workspace(uint64_t rows, uint32_t dim, uint64_t
 {
     if(rows == 0 || dim == 0 || outer == 0 || inner == 0 || rows >= NO_ROW || outer > 0x7ffff000ull / inner)
         return 0;
-    return planGradient(rows, dim, uint32_t(outer * inner)).bytes;
+    // (whichever way the call takes: that of many tokens needs more)
+    const uint32_t count = uint32_t(outer * inner);
+    return planGradient(rows, dim, count, sortsSmall(count, 0)).bytes;
 }
 
 int b200wmma_embedding_grad(int grad_dtype, int table_dtype, uint64_t rows, uint32_t dim, uint64_t outer,

@@ -482,7 +482,7 @@ namespace b200wmma
         };
 
         // Warp 10, one thread: boxes of D go out by TMA as the draining warps fill them; with C, boxes
-        // of it come in by TMA to where D's will be, up to four ahead.
+        // of it come in by TMA to where D's will be, as many ahead as there are boxes.
         template <typename OutT>
         __device__ inline bool moveBoxes(PairControl* ctl, uint8_t* staging, CUtensorMap const* mapC, CUtensorMap const* mapD,
                                          PairParams const& p, uint32_t first, uint32_t row0, uint32_t col0, uint32_t& count)

@@ -54,6 +54,24 @@ def test_lookup_of_several_tables_into_the_interaction(dtype, dim):
     assert torch.equal(x.cpu(), want)
 
 
+def test_tables_that_run_backwards_or_past_the_end_have_no_rows():
+    """Their ids read as zeros and have no gradient; also where the length would wrap in 64 bits."""
+    least, most = -2 ** 63, 2 ** 63 - 1
+    for first in ([10, least, 0, 30], [10, 5, 31, 12], [least, most, least, 30], [most, least, 1, most]):
+        legal = [0 <= a <= b <= 30 for a, b in zip(first, first[1:])]
+        table, ids = _randn((30, 8), F32, 1), torch.tensor([[0, 1, 2], [5, -1, 7], [most, least, 2 ** 40]])
+        at = torch.tensor(first, device="cuda")
+        got = api.embedding(table.cuda(), ids.cuda(), first=at).cpu()
+        grad = api.embedding_grad(torch.ones(3, 3, 8, device="cuda"), ids.cuda(), 30, first=at).cpu()
+        want, sums = torch.zeros(3, 3, 8), torch.zeros(30, 8)
+        for o in range(3):
+            for i in range(3):
+                if legal[i] and 0 <= int(ids[o, i]) < first[i + 1] - first[i]:
+                    want[o, i] = table[first[i] + ids[o, i]]
+                    sums[first[i] + ids[o, i]] += 1
+        assert torch.equal(got, want) and torch.equal(grad, sums)
+
+
 def test_lookup_strides():
     """Rows of a wider table, transposed ids, an output with room between its rows."""
     wide = _randn((40, 37), F32, 1)
@@ -100,7 +118,8 @@ def _check_grad(got, grad, ids, rows, kind, scale=1.0, old=None):
 @KINDS
 @pytest.mark.parametrize("out_t", [F16, BF16, F32], ids=["to_f16", "to_bf16", "to_f32"])
 @pytest.mark.parametrize("tokens,rows,dim,skew", [(1, 1, 1, 1), (1, 5, 8, 1), (40, 1, 3, 1), (33, 70, 264, 1), (513, 90, 1001, 4),
-                                                  (4097, 300, 64, 4), (5000, 70000, 24, 1), (9000, 2, 40, 1)])
+                                                  (4097, 300, 64, 4), (5000, 70000, 24, 1), (9000, 2, 40, 1),
+                                                  (4096, 300, 64, 4), (4100, 40000, 400, 2)])
 def test_gradient(kind, out_t, tokens, rows, dim, skew):
     grad, ids = _randn((tokens, dim), kind, 1), _ids((tokens,), rows, 2, skew)
     for scale in (1.0, 0.3):
@@ -109,7 +128,8 @@ def test_gradient(kind, out_t, tokens, rows, dim, skew):
 
 
 @pytest.mark.parametrize("tokens,rows,dim", [(300000, 40, 8), (70000, 1, 16), (200000, 100000, 3), (60000, 5000, 8),
-                                             (16385, 300, 520), (700000, 3000, 4)])
+                                             (16385, 300, 520), (65536, 5000, 8), (65537, 5000, 8),
+                                             (700000, 3000, 4), (2000001, 3000, 4)])
 def test_gradient_of_long_runs(tokens, rows, dim):
     """Rows that most tokens share: runs over many chunks and levels; every bit the same again."""
     grad, ids = _randn((tokens, dim), BF16, 1), _ids((tokens,), rows, 2, 6.0)
