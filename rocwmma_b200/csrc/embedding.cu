@@ -137,19 +137,29 @@ namespace b200wmma
             uint64_t    ldt, outOuter, outInner;
             uint32_t    pieces, lanesLog2; // pieces of a row; threads side by side on a row
             uint32_t    perBlock; // tokens
+            uint32_t    slices; // blocks to a row; 0: rows to a block
             float       scale;
         };
 
+        // Pieces that a thread has in flight.
+        constexpr uint32_t lookupUnroll(int V)
+        {
+            return V == 8 ? 4u : 8u;
+        }
+
         // A block finds the rows of its tokens first, one thread a token, then moves them, U pieces
-        // in flight a thread.
+        // in flight a thread: the same piece of U rows, or, where a block has fewer rows than that
+        // (p.slices != 0), U pieces of one row, of which a block has a slice.  (4000 rows of 4954 bf16,
+        // out of L2: 84 us the first way, 17 the second; one row of 16384 f16: 4.5 and 1.7.)
+        // Bound by HBM: 65536 x 26 x 128 f16 take 83 us, 5.5 TB/s of the 453 MB that are written.
         template <typename T, typename OutT, int V>
         __global__ void __launch_bounds__(THREADS) lookupKernel(const LookupParams p)
         {
-            constexpr uint32_t U = V == 8 ? 4 : 8;
+            constexpr uint32_t U = lookupUnroll(V);
             __shared__ uint32_t rows[THREADS];
             __shared__ uint64_t outs[THREADS];
-            const uint32_t token0 = blockIdx.x * p.perBlock;
-            const uint32_t here   = min(p.perBlock, p.t.count - token0);
+            const uint32_t token0 = p.slices ? blockIdx.x / p.slices : blockIdx.x * p.perBlock;
+            const uint32_t here   = p.slices ? 1u : min(p.perBlock, p.t.count - token0);
             grid_dependency_wait();
             grid_launch_dependents();
             if(threadIdx.x < here)
@@ -159,10 +169,43 @@ namespace b200wmma
                 outs[threadIdx.x] = uint64_t(outer) * p.outOuter + uint64_t(inner) * p.outInner;
             }
             __syncthreads();
+            auto get = [&](uint32_t row, uint32_t piece) {
+                return loadPiece<T, V>(static_cast<T const*>(p.table) + uint64_t(row) * p.ldt + uint64_t(piece) * V);
+            };
+            auto put = [&](uint32_t t, uint32_t row, uint32_t piece, Piece<T, V> const& v) {
+                Piece<OutT, V> o;
+                if(row == NO_ROW)
+                {
+#pragma unroll
+                    for(int i = 0; i < V; ++i)
+                        o.v[i] = OutT(0.0f);
+                }
+                else if(std::is_same<T, OutT>::value && p.scale == 1.0f)
+                    memcpy(&o, &v, sizeof(o)); // (65536 x 26 x 128 f16: 88 us with the conversions, 83 without)
+                else
+                {
+#pragma unroll
+                    for(int i = 0; i < V; ++i)
+                        o.v[i] = fromFloat<OutT>(toFloat(v.v[i]) * p.scale);
+                }
+                storePiece<OutT, V>(static_cast<OutT*>(p.out) + outs[t] + uint64_t(piece) * V, o);
+            };
+            if(p.slices)
+            {
+                const uint32_t first = (blockIdx.x % p.slices) * (THREADS * U) + threadIdx.x, row = rows[0];
+                Piece<T, V>    v[U];
+#pragma unroll
+                for(uint32_t u = 0; u < U; ++u)
+                    if(row != NO_ROW && first + u * THREADS < p.pieces)
+                        v[u] = get(row, first + u * THREADS);
+#pragma unroll
+                for(uint32_t u = 0; u < U; ++u)
+                    if(first + u * THREADS < p.pieces)
+                        put(0, row, first + u * THREADS, v[u]);
+                return;
+            }
             const uint32_t lanes = 1u << p.lanesLog2, step = THREADS >> p.lanesLog2;
             for(uint32_t piece = threadIdx.x & (lanes - 1u); piece < p.pieces; piece += lanes)
-            {
-                const uint64_t at = uint64_t(piece) * V;
                 for(uint32_t t0 = threadIdx.x >> p.lanesLog2; t0 < here; t0 += U * step)
                 {
                     Piece<T, V> v[U];
@@ -170,37 +213,15 @@ namespace b200wmma
 #pragma unroll
                     for(uint32_t u = 0; u < U; ++u)
                     {
-                        const uint32_t t = t0 + u * step;
-                        row[u]           = t < here ? rows[t] : NO_ROW;
+                        row[u] = t0 + u * step < here ? rows[t0 + u * step] : NO_ROW;
                         if(row[u] != NO_ROW)
-                            v[u] = loadPiece<T, V>(static_cast<T const*>(p.table) + uint64_t(row[u]) * p.ldt + at);
+                            v[u] = get(row[u], piece);
                     }
 #pragma unroll
                     for(uint32_t u = 0; u < U; ++u)
-                    {
-                        const uint32_t t = t0 + u * step;
-                        if(t < here)
-                        {
-                            Piece<OutT, V> o;
-                            if(row[u] == NO_ROW)
-                            {
-#pragma unroll
-                                for(int i = 0; i < V; ++i)
-                                    o.v[i] = OutT(0.0f);
-                            }
-                            else if(std::is_same<T, OutT>::value && p.scale == 1.0f)
-                                memcpy(&o, &v[u], sizeof(o)); // (65536 x 26 x 128 f16: 88 us with the conversions, 83 without)
-                            else
-                            {
-#pragma unroll
-                                for(int i = 0; i < V; ++i)
-                                    o.v[i] = fromFloat<OutT>(toFloat(v[u].v[i]) * p.scale);
-                            }
-                            storePiece<OutT, V>(static_cast<OutT*>(p.out) + outs[t] + at, o);
-                        }
-                    }
+                        if(t0 + u * step < here)
+                            put(t0 + u * step, row[u], piece, v[u]);
                 }
-            }
         }
 
         // ---- clearing rows without a token -------------------------------------------------
@@ -1157,8 +1178,17 @@ namespace b200wmma
             per          = per > THREADS ? THREADS : per;
             const uint32_t spread = (p.t.count + 4u * 148u - 1u) / (4u * 148u);
             p.perBlock            = per < spread ? per : spread;
-            return cudaToStatus(launchOverlapped(lookupKernel<T, OutT, V>, dim3((p.t.count + p.perBlock - 1u) / p.perBlock),
-                                                 dim3(THREADS), 0, stream, p));
+            p.slices              = 0;
+            constexpr uint32_t U  = lookupUnroll(V);
+            if(p.perBlock < U && p.pieces > THREADS)
+            {
+                p.perBlock = 1;
+                p.slices   = (p.pieces + THREADS * U - 1u) / (THREADS * U);
+            }
+            const uint64_t blocks = (uint64_t(p.t.count) + p.perBlock - 1u) / p.perBlock * (p.slices ? p.slices : 1u);
+            if(blocks > 0x7fffffffull)
+                return B200WMMA_ERR_TOO_LARGE;
+            return cudaToStatus(launchOverlapped(lookupKernel<T, OutT, V>, dim3(uint32_t(blocks)), dim3(THREADS), 0, stream, p));
         }
 
         template <typename T, typename OutT>

@@ -24,7 +24,8 @@ def _randn(shape, kind, seed):
 @KINDS
 @pytest.mark.parametrize("out_t", [F16, BF16, F32], ids=["to_f16", "to_bf16", "to_f32"])
 @pytest.mark.parametrize("tokens,rows,dim", [(1, 1, 1), (1, 7, 8), (5, 3, 3), (63, 100, 96), (64, 1000, 1001),
-                                             (1000, 50, 128), (257, 300, 2056), (20000, 40, 16)])
+                                             (1000, 50, 128), (257, 300, 2056), (20000, 40, 16),
+                                             (3, 5, 4954), (700, 9, 1030), (2, 3, 40000), (2500, 30, 2304)])
 def test_lookup(kind, out_t, tokens, rows, dim):
     table, ids = _randn((rows, dim), kind, 1), _ids((tokens,), rows, 2)
     for scale in (1.0, 0.3):
