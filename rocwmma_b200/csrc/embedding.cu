@@ -773,16 +773,28 @@ namespace b200wmma
             storePiece<OutT, V>(at, o);
         }
 
-        // First of the sorted items [low, high) whose row is not below `row`.
-        __device__ inline uint32_t lowerBound(uint2 const* sorted, uint32_t low, uint32_t high, uint64_t row)
+        // First of the n sorted items whose row is not below `row`.  Seven items are looked at together:
+        // the search is a chain of waits for memory, and three bits a link make it a third as long.
+        // (38000 tokens of 300 rows of 8: the kernel took @A us with one item at a time, @B so.)
+        __device__ inline uint32_t lowerBound(uint2 const* sorted, uint32_t n, uint64_t row)
         {
+            uint32_t low = 0, high = n;
             while(low < high)
             {
-                const uint32_t mid = low + (high - low) / 2u;
-                if(sorted[mid].x < row)
-                    low = mid + 1u;
-                else
-                    high = mid;
+                uint32_t at[7];
+#pragma unroll
+                for(uint32_t i = 0; i < 7u; ++i)
+                    at[i] = low + uint32_t(uint64_t(high - low) * (i + 1u) / 8u); // < high
+                bool less[7];
+#pragma unroll
+                for(uint32_t i = 0; i < 7u; ++i)
+                    less[i] = sorted[at[i]].x < row;
+#pragma unroll
+                for(uint32_t i = 0; i < 7u; ++i) // behind the last one that is below
+                    low = less[i] ? at[i] + 1u : low;
+#pragma unroll
+                for(uint32_t i = 7; i-- > 0u;) // up to the first one that is not
+                    high = less[i] ? high : at[i];
             }
             return low;
         }
@@ -854,11 +866,10 @@ namespace b200wmma
             {
                 const uint64_t begin = uint64_t(blockIdx.x - p.blocks) * c.rowsPerBlock;
                 const uint64_t end   = min(uint64_t(c.rows), begin + c.rowsPerBlock);
-                const uint32_t low = lowerBound(p.sorted, 0, p.n, begin), high = lowerBound(p.sorted, low, p.n, end);
                 for(uint32_t i = threadIdx.x; i < uint32_t(end - begin); i += blockDim.x)
                 {
-                    const uint32_t at = lowerBound(p.sorted, low, high, begin + i);
-                    rows[i]           = at < high && p.sorted[at].x == begin + i;
+                    const uint32_t at = lowerBound(p.sorted, p.n, begin + i);
+                    rows[i]           = at < p.n && p.sorted[at].x == begin + i;
                 }
                 __syncthreads();
                 return clearRows<OutT, V>(c, begin, end, [&](uint64_t row) { return rows[row - begin] != 0u; });
