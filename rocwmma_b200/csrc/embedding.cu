@@ -775,7 +775,7 @@ namespace b200wmma
 
         // First of the n sorted items whose row is not below `row`.  Seven items are looked at together:
         // the search is a chain of waits for memory, and three bits a link make it a third as long.
-        // (38000 tokens of 300 rows of 8: the kernel took @A us with one item at a time, @B so.)
+        // (38000 tokens of 300 rows of 8: the kernel took 23 us with one item at a time, 10 so.)
         __device__ inline uint32_t lowerBound(uint2 const* sorted, uint32_t n, uint64_t row)
         {
             uint32_t low = 0, high = n;
@@ -806,46 +806,32 @@ namespace b200wmma
         struct Ring
         {
             // (single 16-bit values travel in the aligned word that holds them)
-            static constexpr uint32_t BYTES = sizeof(T) * V < 4 ? 4 : sizeof(T) * V;
-            static constexpr uint32_t PART  = BYTES > 16 ? 16 : BYTES; // of one copy
+            static constexpr uint32_t BYTES = sizeof(T) * V < 4 ? 4 : sizeof(T) * V; // 4, 8 or 16: a copy
             static constexpr uint32_t DEPTH = RING_BYTES / BYTES > 16 ? 16 : RING_BYTES / BYTES;
 
             // slot s of the calling thread; the threads of a block lie side by side
-            static __device__ uint8_t* at(uint8_t* ring, uint32_t s, uint32_t part)
+            static __device__ uint8_t* at(uint8_t* ring, uint32_t s)
             {
-                return ring + ((s * (BYTES / PART) + part) * blockDim.x + threadIdx.x) * PART;
+                return ring + (s * blockDim.x + threadIdx.x) * BYTES;
             }
             static __device__ void load(uint8_t* ring, uint32_t s, T const* from)
             {
                 uint64_t src = reinterpret_cast<uint64_t>(from);
                 if constexpr(sizeof(T) * V < 4)
                     src &= ~uint64_t(3);
-#pragma unroll
-                for(uint32_t part = 0; part < BYTES / PART; ++part)
-                {
-                    const uint32_t to = uint32_t(__cvta_generic_to_shared(at(ring, s, part)));
-                    if constexpr(PART == 16) // past L1, which has no use for them
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(src + part * PART) : "memory");
-                    else
-                        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(src + part * PART), "n"(PART)
-                                     : "memory");
-                }
+                const uint32_t to = uint32_t(__cvta_generic_to_shared(at(ring, s)));
+                if constexpr(BYTES == 16) // past L1, which has no use for them
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(src) : "memory");
+                else
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(src), "n"(BYTES) : "memory");
             }
             static __device__ Piece<T, V> get(uint8_t* ring, uint32_t s, uint64_t place)
             {
                 Piece<T, V> p;
                 if constexpr(sizeof(T) * V < 4)
-                    p.v[0] = reinterpret_cast<T const*>(at(ring, s, 0))[place / sizeof(T) % 2u];
+                    p.v[0] = reinterpret_cast<T const*>(at(ring, s))[place / sizeof(T) % 2u];
                 else
-                {
-                    struct alignas(PART) Part
-                    {
-                        uint8_t b[PART];
-                    };
-#pragma unroll
-                    for(uint32_t part = 0; part < BYTES / PART; ++part)
-                        reinterpret_cast<Part*>(&p)[part] = *reinterpret_cast<Part const*>(at(ring, s, part));
-                }
+                    p = *reinterpret_cast<Piece<T, V> const*>(at(ring, s));
                 return p;
             }
         };
@@ -1165,12 +1151,12 @@ namespace b200wmma
             const uint32_t l = log2Up(pieces);
             return l > 8u ? 8u : l;
         }
-        // Values of a piece: 8, 2 or 1, whatever divides dim and keeps every piece of the given
+        // Values of a piece: 8, 4, 2 or 1, whatever divides dim and keeps every piece of the given
         // tensors on its boundary.  `strides`: distances of rows, in elements.
         template <typename... Strides>
         uint32_t pieceSize(uint32_t dim, void const* base, uint64_t elem, uint32_t most, Strides... strides)
         {
-            for(uint32_t v = most; v > 1u; v = v == 8u ? 2u : 1u)
+            for(uint32_t v = most; v > 1u; v /= 2u)
             {
                 const uint64_t bytes = v * elem;
                 if(dim % v == 0u && aligned(base, bytes) && ((strides * elem % bytes == 0) && ...))
@@ -1179,11 +1165,33 @@ namespace b200wmma
             return 1;
         }
 
+        // f(v) with v as a constant
+        template <typename F>
+        int withPiece(uint32_t v, F f)
+        {
+            switch(v)
+            {
+            case 8:
+                return f(std::integral_constant<int, 8>());
+            case 4:
+                return f(std::integral_constant<int, 4>());
+            case 2:
+                return f(std::integral_constant<int, 2>());
+            }
+            return f(std::integral_constant<int, 1>());
+        }
+
         template <typename T, typename OutT, int V>
         int lookup(LookupParams p, uint32_t dim, cudaStream_t stream)
         {
             p.pieces    = dim / V;
             p.lanesLog2 = rowLanesLog2(p.pieces);
+            // Fewer threads side by side where that leaves fewer of them without a piece, down to those of a
+            // line of 128 bytes (701000 rows of 82 f32, 41 pieces: 88 us with 64 threads to a row, 77 with
+            // 16; 122000 rows of 247 bf16, 247 pieces: 50 us with 256, 242 with 8).
+            auto rounded = [&](uint32_t lanes) { return (p.pieces + (1u << lanes) - 1u) >> lanes << lanes; };
+            for(uint32_t l = p.lanesLog2; (V * sizeof(OutT)) << l >= 128u; --l)
+                p.lanesLog2 = rounded(l) < rounded(p.lanesLog2) ? l : p.lanesLog2;
             // 4096 pieces to a block (16 a thread), but blocks for every SM first
             uint32_t per = p.pieces >= 4096u ? 1u : 4096u / p.pieces;
             per          = per > THREADS ? THREADS : per;
@@ -1207,8 +1215,7 @@ namespace b200wmma
         {
             const uint32_t v = pieceSize(dim, p.out, sizeof(OutT), pieceSize(dim, p.table, sizeof(T), 8, p.ldt), p.outOuter,
                                          p.outInner);
-            return v == 8u ? lookup<T, OutT, 8>(p, dim, stream)
-                           : v == 2u ? lookup<T, OutT, 2>(p, dim, stream) : lookup<T, OutT, 1>(p, dim, stream);
+            return withPiece(v, [&](auto V) { return lookup<T, OutT, V.value>(p, dim, stream); });
         }
 
         template <typename T>
@@ -1276,7 +1283,7 @@ namespace b200wmma
                 w.counts   = take((uint64_t(w.tiles) << w.digitBits) * 4u);
             }
             // (pieces of the widest kind; narrower ones put fewer rows into a block, and fewer items)
-            const uint32_t pieces = dim % 8u == 0u ? dim / 8u : dim % 2u == 0u ? dim / 2u : dim;
+            const uint32_t pieces = dim % 8u == 0u ? dim / 8u : dim % 4u == 0u ? dim / 4u : dim % 2u == 0u ? dim / 2u : dim;
             const uint32_t lanes  = rowLanesLog2(pieces);
             const uint32_t most   = SUM_ITEMS / (sumThreads(lanes) >> lanes); // that fit a block
             // Long chunks leave fewer pieces of runs behind, short ones make more threads: as many
@@ -1452,11 +1459,13 @@ namespace b200wmma
             const uint64_t clear = g.accumulate ? 0u : uint64_t(g.t.rows) * g.dim * sizeof(OutT);
             const Plan     w  = planGradient(g.t.rows, g.dim, g.t.count, sortsSmall(g.t.count, clear));
             const uint32_t vt = pieceSize(g.dim, g.table, sizeof(OutT), 8, g.ldt);
-            const uint32_t vg = pieceSize(g.dim, g.grad, sizeof(T), vt, g.gradOuter, g.gradInner);
+            // (the gradient comes in copies of 16 bytes at most; two for a piece of 32 would each touch half of
+            // a sector: 236000 rows of 208 f32 take 80 us with eight values to a piece, 61 with four)
+            const uint32_t most = sizeof(T) == 4 && vt == 8u ? 4u : vt;
+            const uint32_t vg   = pieceSize(g.dim, g.grad, sizeof(T), most, g.gradOuter, g.gradInner);
             uint2*         sorted = reinterpret_cast<uint2*>(g.workspace + w.pairs[0]);
             if(w.small)
-                B200WMMA_TRY(vt == 8u ? (sortFew<OutT, 8>(g, w, stream))
-                                      : vt == 2u ? (sortFew<OutT, 2>(g, w, stream)) : (sortFew<OutT, 1>(g, w, stream)));
+                B200WMMA_TRY(withPiece(vt, [&](auto V) { return sortFew<OutT, V.value>(g, w, stream); }));
             else
                 B200WMMA_TRY(g.t.count < MANY_TOKENS ? sortDigits<FEW_ITEMS>(g, w, &sorted, stream)
                                                      : sortDigits<MANY_ITEMS>(g, w, &sorted, stream));
@@ -1479,11 +1488,14 @@ namespace b200wmma
                 p.pieceKeys = reinterpret_cast<uint32_t*>(g.workspace + w.pieceKeys);
                 p.pieceSums = reinterpret_cast<float*>(g.workspace + w.pieceSums);
             }
-            B200WMMA_TRY(vg == 8u ? (sumChunks<T, OutT, 8>(g, w, p, stream))
-                                  : vg == 2u ? (sumChunks<T, OutT, 2>(g, w, p, stream)) : (sumChunks<T, OutT, 1>(g, w, p, stream)));
+            B200WMMA_TRY(withPiece(vg, [&](auto V) {
+                if constexpr(sizeof(T) * V.value > 16)
+                    return int(B200WMMA_ERR_INVALID_ARG); // never
+                else
+                    return sumChunks<T, OutT, V.value>(g, w, p, stream);
+            }));
             if(p.parts > 1u)
-                B200WMMA_TRY(vt == 8u ? (joinPieces<OutT, 8>(g, p, stream))
-                                      : vt == 2u ? (joinPieces<OutT, 2>(g, p, stream)) : (joinPieces<OutT, 1>(g, p, stream)));
+                B200WMMA_TRY(withPiece(vt, [&](auto V) { return joinPieces<OutT, V.value>(g, p, stream); }));
             return B200WMMA_OK;
         }
 #undef B200WMMA_TRY
