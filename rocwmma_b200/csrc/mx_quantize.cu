@@ -44,29 +44,48 @@ namespace b200wmma
                 r.v[i] = T(0.0f);
             return r;
         }
-        template <typename T>
+        // ... moved in words of WIDTH bytes, 32 or 16, whichever boundary the rows lie on.
+        template <typename T, int WIDTH>
         __device__ inline Run<T> loadRun(T const* p)
         {
-            Run<T>    r;
-            uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+            Run<T> r;
+            if constexpr(WIDTH == 32)
+            {
+                uint32_t* w = reinterpret_cast<uint32_t*>(&r);
 #pragma unroll
-            for(uint32_t i = 0; i < sizeof(r) / 4u; i += 8u)
-                asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                             : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]), "=r"(w[i + 4]),
-                               "=r"(w[i + 5]), "=r"(w[i + 6]), "=r"(w[i + 7])
-                             : "l"(reinterpret_cast<uint32_t const*>(p) + i));
+                for(uint32_t i = 0; i < sizeof(r) / 4u; i += 8u)
+                    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                                 : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]), "=r"(w[i + 4]),
+                                   "=r"(w[i + 5]), "=r"(w[i + 6]), "=r"(w[i + 7])
+                                 : "l"(reinterpret_cast<uint32_t const*>(p) + i));
+            }
+            else
+            {
+#pragma unroll
+                for(uint32_t i = 0; i < sizeof(r) / 16u; ++i)
+                    reinterpret_cast<uint4*>(&r)[i] = reinterpret_cast<uint4 const*>(p)[i];
+            }
             return r;
         }
-        template <typename T>
+        template <typename T, int WIDTH>
         __device__ inline void storeRun(T* p, Run<T> const& r)
         {
-            uint32_t const* w = reinterpret_cast<uint32_t const*>(&r);
+            if constexpr(WIDTH == 32)
+            {
+                uint32_t const* w = reinterpret_cast<uint32_t const*>(&r);
 #pragma unroll
-            for(uint32_t i = 0; i < sizeof(r) / 4u; i += 8u)
-                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<uint32_t*>(p) + i),
-                             "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]),
-                             "r"(w[i + 6]), "r"(w[i + 7])
-                             : "memory");
+                for(uint32_t i = 0; i < sizeof(r) / 4u; i += 8u)
+                    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<uint32_t*>(p) + i),
+                                 "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]),
+                                 "r"(w[i + 6]), "r"(w[i + 7])
+                                 : "memory");
+            }
+            else
+            {
+#pragma unroll
+                for(uint32_t i = 0; i < sizeof(r) / 16u; ++i)
+                    reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<uint4 const*>(&r)[i];
+            }
         }
 
         // Values are worked on as the 32-bit words they come in, two to a word if they have 16 bits:
@@ -300,7 +319,7 @@ namespace b200wmma
         // those with the scales of four blocks write them as a word.  The values of the next tile
         // are on their way while those of one are worked on.  (8192 x 8192 bf16 MXF4, 171 MB: 64 us
         // with eight values a thread and maxima found as integers, 40 so; 26 at the measured copy rate.)
-        template <typename T, bool NV, bool VEC>
+        template <typename T, bool NV, int WIDTH>
         __global__ void __launch_bounds__(THREADS) quantizeRowsKernel(const QuantizeParams p)
         {
             using W                   = Words<T>;
@@ -318,14 +337,14 @@ namespace b200wmma
             const uint32_t left  = r < rows && p.k > k0 ? uint32_t(p.k - k0) : 0u; // values from the first on
             const uint32_t pitch = r < rows && mxPitch(p.k) > k0 / 2u ? uint32_t(mxPitch(p.k) - k0 / 2u) : 0u; // bytes
             const uint32_t group = uint32_t(k0 / (4u * mxBlock(NV)));
-            __shared__ alignas(16) uint8_t staged[VEC ? 16 : SLAB_ROWS * StagedRow<T>::PITCH];
+            __shared__ alignas(16) uint8_t staged[WIDTH ? 16 : SLAB_ROWS * StagedRow<T>::PITCH];
             auto fetch = [&](uint32_t t) {
                 const uint32_t done = t * TILE_K;
                 Run<T>         raw;
-                if constexpr(VEC)
+                if constexpr(WIDTH != 0)
                 {
                     if(left >= done + RUN)
-                        return loadRun(x + done);
+                        return loadRun<T, WIDTH>(x + done);
                     raw = zeroRun<T>();
 #pragma unroll
                     for(uint32_t j = 0; j < RUN; ++j)
@@ -537,7 +556,7 @@ namespace b200wmma
 
         // A block takes 32 rows x 128 columns at a time, a thread sixteen codes; those of the next
         // tile are on their way meanwhile.
-        template <typename T, bool NV, bool VEC>
+        template <typename T, bool NV, int WIDTH>
         __global__ void __launch_bounds__(THREADS) dequantizeKernel(const DequantizeParams p)
         {
             constexpr uint32_t GROUPS = TILE_K / (4u * mxBlock(NV));
@@ -552,7 +571,7 @@ namespace b200wmma
             uint8_t const* scales = p.scales + (uint64_t(slab / 4u) * p.groups + k0 / (4u * mxBlock(NV))) * MX_TILE_BYTES
                                     + scaleOffset(slab % 4u * SLAB_ROWS + r, uint32_t(k0 / mxBlock(NV) % 4u));
             T*             out    = static_cast<T*>(p.out) + row * p.ldo + k0;
-            __shared__ alignas(16) uint8_t staged[VEC ? 16 : SLAB_ROWS * StagedRow<T>::PITCH];
+            __shared__ alignas(16) uint8_t staged[WIDTH ? 16 : SLAB_ROWS * StagedRow<T>::PITCH];
             grid_dependency_wait();
             grid_launch_dependents();
             uint2    nextCode{};
@@ -575,10 +594,10 @@ namespace b200wmma
                 Run<T> o;
                 values8<T>(code.x, s, p.factor, o.v);
                 values8<T>(code.y, s, p.factor, o.v + 8);
-                if constexpr(VEC)
+                if constexpr(WIDTH != 0)
                 {
                     if(left >= done + RUN)
-                        storeRun(out + done, o);
+                        storeRun<T, WIDTH>(out + done, o);
                     else
                     {
 #pragma unroll
@@ -620,12 +639,22 @@ namespace b200wmma
             return whole ? mxRowTiles(rows) * 4u : uint32_t((uint64_t(rows) + SLAB_ROWS - 1u) / SLAB_ROWS);
         }
 
+        // f(32), f(16) or f(0): the boundary that rows `pitch` bytes apart start on; none: through shared
+        // memory.  (5335 x 3604 f32 NVF4, rows on 16 bytes, quantised: 56 us through shared
+        // memory, 32 so.)
+        template <typename F>
+        int withWidth(void const* base, uint64_t pitch, F f)
+        {
+            if(aligned(base, 32) && pitch % 32 == 0)
+                return f(std::integral_constant<int, 32>());
+            if(aligned(base, 16) && pitch % 16 == 0)
+                return f(std::integral_constant<int, 16>());
+            return f(std::integral_constant<int, 0>());
+        }
+
         template <typename T>
         int quantize(bool nv, bool columns, QuantizeParams p, cudaStream_t stream)
         {
-            // Wide loads where every row (or pair of rows) starts on their boundary.
-            const uint64_t width = columns ? 2 * sizeof(T) : 32;
-            const bool     vec   = aligned(p.x, width) && p.ldx * sizeof(T) % width == 0;
             const uint32_t slabs = slabsOf(p.rows, true);
             p.tilesPerBlock      = tilesPerBlock(uint64_t(slabs) * p.tilesK, p.tilesK);
             const uint32_t blocks = columns ? mxRowTiles(p.rows) * p.groups
@@ -634,24 +663,28 @@ namespace b200wmma
                 return cudaToStatus(launchOverlapped(kernel, dim3(blocks), dim3(THREADS), 0, stream, p));
             };
             if(columns)
+            {
+                const bool vec = aligned(p.x, 2 * sizeof(T)) && p.ldx % 2 == 0; // pairs of rows
                 return nv ? (vec ? launch(quantizeColumnsKernel<T, true, true>) : launch(quantizeColumnsKernel<T, true, false>))
                           : (vec ? launch(quantizeColumnsKernel<T, false, true>) : launch(quantizeColumnsKernel<T, false, false>));
-            return nv ? (vec ? launch(quantizeRowsKernel<T, true, true>) : launch(quantizeRowsKernel<T, true, false>))
-                      : (vec ? launch(quantizeRowsKernel<T, false, true>) : launch(quantizeRowsKernel<T, false, false>));
+            }
+            return withWidth(p.x, p.ldx * sizeof(T), [&](auto width) {
+                return nv ? launch(quantizeRowsKernel<T, true, width.value>) : launch(quantizeRowsKernel<T, false, width.value>);
+            });
         }
 
         template <typename T>
         int dequantize(bool nv, DequantizeParams p, cudaStream_t stream)
         {
-            const bool     vec   = aligned(p.out, 32) && p.ldo * sizeof(T) % 32 == 0;
             const uint32_t slabs = slabsOf(p.rows, false);
             p.tilesPerBlock      = tilesPerBlock(uint64_t(slabs) * p.tilesK, p.tilesK);
             const uint32_t blocks = slabs * ((p.tilesK + p.tilesPerBlock - 1u) / p.tilesPerBlock);
             auto launch = [&](auto kernel) {
                 return cudaToStatus(launchOverlapped(kernel, dim3(blocks), dim3(THREADS), 0, stream, p));
             };
-            return nv ? (vec ? launch(dequantizeKernel<T, true, true>) : launch(dequantizeKernel<T, true, false>))
-                      : (vec ? launch(dequantizeKernel<T, false, true>) : launch(dequantizeKernel<T, false, false>));
+            return withWidth(p.out, p.ldo * sizeof(T), [&](auto width) {
+                return nv ? launch(dequantizeKernel<T, true, width.value>) : launch(dequantizeKernel<T, false, width.value>);
+            });
         }
 
         // What both directions check; OK or a status.

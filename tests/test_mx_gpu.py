@@ -39,7 +39,8 @@ def _check_operand(fmt, rows, k, operand, x, exponent=0):
 @FORMATS
 @KINDS
 @pytest.mark.parametrize("layout", [ROW_MAJOR, COL_MAJOR], ids=["rows", "columns"])
-@pytest.mark.parametrize("rows,k", [(1, 1), (1, 8192), (3, 31), (2, 33), (127, 64), (128, 128), (129, 257), (300, 1000)])
+@pytest.mark.parametrize("rows,k", [(1, 1), (1, 8192), (3, 31), (2, 33), (127, 64), (128, 128), (129, 257), (300, 1000),
+                                    (40, 1204), (1100, 4152)])
 def test_quantize(fmt, kind, layout, rows, k):
     x = _values(rows, k, kind, rows * 1000 + k)
     if rows > 2:
