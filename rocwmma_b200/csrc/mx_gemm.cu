@@ -92,6 +92,7 @@ namespace b200wmma
         // tile, each a stretch of K, so that the stream comes through all SMs; the partial sums
         // meet in shared memory across the cluster (each block adds up its share of the thin
         // rows, always in the order of the blocks) where the ring was.
+        // 1 x 8192 x 8192 MXF4: 9 us a call, 5.5 for its bytes; 64 x 16384 x 4096 NVF4: 13 and 6.
         struct ThinParams
         {
             void const* c;
@@ -417,6 +418,8 @@ namespace b200wmma
         // So the two overlap: the second starts at column ACC1, the scales of two ring slots lie
         // behind it, and the first MMA of a tile waits only until the tile before has drained the
         // columns that both accumulators share, which are drained first.
+        // 8192 x 8192 x 8192 MXF4: 182 us (6.0 PFLOP/s) in bursts, 216 under the power limit.  One tile to
+        // a pair, 1000 x 4100 x 4111 NVF4 with C: 19 us, of which the MMAs take 7.
         constexpr uint32_t P_TILE      = 256;
         // With C, whose boxes come from memory, twice the boxes are worth more than a fifth slot: one
         // 256 x 256 tile f32 is drained in 5.8 us instead of 8.3, its MMAs take 0.1 us longer.
@@ -1042,6 +1045,7 @@ namespace b200wmma
             if(sms < 2)
                 return B200WMMA_ERR_CUDA;
             const uint32_t thin = p.m < p.n ? p.m : p.n;
+            // (96 x 4096 x 4096: 7.6 us thin, 10.5 in pairs; 128 x 8192 x 8192: 16.9 both; 256 x 8192 x 8192: 22 and 17)
             return thin <= 128u ? launchThin<KIND, OutT>(o, p, sms, stream) : launchPairs<KIND, OutT>(o, p, sms, stream);
         }
 
