@@ -89,10 +89,17 @@ namespace b200wmma
         // One of m and n is small (a decoding batch; one token): the other operand, whose rows
         // are the MMA's M here, 128 to a block, streams from HBM once and bounds the call.  The
         // thin operand is the MMA's N, padded to 16 rows.  A cluster of `parts` blocks shares a
-        // tile, each a stretch of K, so that the stream comes through all SMs; the partial sums
-        // meet in shared memory across the cluster (each block adds up its share of the thin
-        // rows, always in the order of the blocks) where the ring was.
-        // 1 x 8192 x 8192 MXF4: 9 us a call, 5.5 for its bytes; 64 x 16384 x 4096 NVF4: 13 and 6.
+        // tile, each a stretch of K, so that the stream comes through all SMs.  Every block puts its
+        // partial sums where its ring was, and adds up its share of the thin rows out of the
+        // shared memory of the whole cluster, always in the order of the blocks.
+        //
+        // A block holds columns of tensor memory only while it needs nothing of another block: it gives
+        // them back before it waits for its cluster.  tcgen05.alloc waits, without a limit, until its SM
+        // has a contiguous range of that size, and how ranges are placed is the hardware's business; so
+        // clusters that waited for each other's blocks with columns in hand could wait for good.
+        // 1 x 8192 x 8192 MXF4: 9.1 us a call, 5.5 for its bytes; 64 x 16384 x 4096 NVF4: 12.4 and 6.
+        // (With the sums sent to the block that adds them up, and the columns held until the end: 9.5 and 13.8;
+        // 8192 x 64 x 2048 MXF4: 10.4 us so, 7.0 now.)
         struct ThinParams
         {
             void const* c;
@@ -112,9 +119,20 @@ namespace b200wmma
             uint32_t   tmemBase;
         };
 
-        __device__ inline void storeCluster(uint32_t addr, uint32_t v)
+        __device__ inline float4 loadCluster4(uint32_t addr)
         {
-            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+            float4 v;
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                         : "r"(addr)
+                         : "memory");
+            return v;
+        }
+        __device__ inline float loadCluster(uint32_t addr)
+        {
+            float v;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+            return v;
         }
 
         // Four neighbouring elements of D, or the first `count` of them.  `wide`: D and C lie on the
@@ -143,6 +161,88 @@ namespace b200wmma
                 for(uint32_t i = 0; i < 4u; ++i)
                     if(i < count)
                         d[i] = finish<OutT>(a[i], p.alpha, p.beta, c ? c + i : nullptr);
+            }
+        }
+
+        // The block's share of the thin rows, summed over the rings of the PARTS blocks of the cluster and
+        // finished.  ring: shared-memory address of [thin row][row of the tile], the same in each.
+        // A thread has eight loads in flight: one from another block's memory takes long.
+        template <typename OutT, uint32_t PARTS>
+        __device__ inline void finishShare(ThinParams const& p, uint32_t ring, uint32_t tile, uint32_t part)
+        {
+            constexpr uint32_t Q = 8u / PARTS; // thin rows at a time
+            const uint32_t     share = p.nq / PARTS, first = part * share; // thin row
+            const uint32_t     mine  = first < p.thin ? min(share, p.thin - first) : 0u;
+            const uint64_t     row0  = uint64_t(tile) * ROW_TILE;
+            const uint32_t     left  = uint32_t(min(uint64_t(ROW_TILE), p.rows - row0));
+            OutT*              d     = static_cast<OutT*>(p.d) + row0 * p.dRow + first * p.dThin;
+            OutT const*        c     = p.c ? static_cast<OutT const*>(p.c) + row0 * p.cRow + first * p.cThin : nullptr;
+            uint32_t           from[PARTS];
+#pragma unroll
+            for(uint32_t o = 0; o < PARTS; ++o)
+                from[o] = (PARTS > 1u ? map_to_cta(ring, o) : ring) + first * ROW_TILE * 4u;
+            if(p.dRow == 1u)
+            {
+                // a warp takes a row of D, a lane four columns
+                constexpr uint32_t WARPS = NUM_THREADS / 32u;
+                const uint32_t     warp = threadIdx.x / 32u, r = 4u * (threadIdx.x % 32u);
+                if(r >= left)
+                    return;
+                d += r;
+                c = c ? c + r : nullptr;
+                for(uint32_t q0 = warp; q0 < mine; q0 += Q * WARPS)
+                {
+                    float4 v[Q][PARTS];
+#pragma unroll
+                    for(uint32_t i = 0; i < Q; ++i)
+#pragma unroll
+                        for(uint32_t o = 0; o < PARTS; ++o)
+                            if(q0 + i * WARPS < mine)
+                                v[i][o] = loadCluster4(from[o] + ((q0 + i * WARPS) * ROW_TILE + r) * 4u);
+#pragma unroll
+                    for(uint32_t i = 0; i < Q; ++i)
+                    {
+                        const uint32_t q = q0 + i * WARPS;
+                        if(q >= mine)
+                            break;
+                        float4 acc = v[i][0];
+#pragma unroll
+                        for(uint32_t o = 1; o < PARTS; ++o)
+                        {
+                            acc.x += v[i][o].x;
+                            acc.y += v[i][o].y;
+                            acc.z += v[i][o].z;
+                            acc.w += v[i][o].w;
+                        }
+                        putFour<OutT>(d + q * p.dThin, c ? c + q * p.cThin : nullptr, p, true, left - r, acc);
+                    }
+                }
+            }
+            else if(threadIdx.x < left)
+            {
+                // a thread takes a row of D, four columns at a time
+                const uint32_t r = threadIdx.x;
+                d += r * p.dRow;
+                c = c ? c + r * p.cRow : nullptr;
+                for(uint32_t q0 = 0; q0 < mine; q0 += 4u)
+                {
+                    float v[4][PARTS], acc[4];
+#pragma unroll
+                    for(uint32_t i = 0; i < 4u; ++i)
+#pragma unroll
+                        for(uint32_t o = 0; o < PARTS; ++o)
+                            v[i][o] = q0 + i < mine ? loadCluster(from[o] + ((q0 + i) * ROW_TILE + r) * 4u) : 0.0f;
+#pragma unroll
+                    for(uint32_t i = 0; i < 4u; ++i)
+                    {
+                        acc[i] = v[i][0];
+#pragma unroll
+                        for(uint32_t o = 1; o < PARTS; ++o)
+                            acc[i] += v[i][o];
+                    }
+                    putFour<OutT>(d + q0, c ? c + q0 : nullptr, p, first % 4u == 0u, mine - q0,
+                                  make_float4(acc[0], acc[1], acc[2], acc[3]));
+                }
             }
         }
 
@@ -297,23 +397,19 @@ namespace b200wmma
                 }
             }
 
-            // Every block puts its sums, as [part][thin row of the share][row of the tile], into the
-            // ring of the block that finishes them (a lane has a row of the tile, registers hold thin
-            // rows); then four values that D has side by side are one thread's.
-            const bool     drains = warp >= 2u;
-            const uint32_t share  = p.nq / p.parts; // thin rows that a block finishes
-            bool           ready  = false;
+            // The sums go where the ring was, as [thin row][row of the tile] (a lane has a row of the tile,
+            // registers hold thin rows), the columns back to the SM, and only then the block waits
+            // for its cluster.
+            const bool drains = warp >= 2u;
+            bool       ready  = false;
             if(drains)
-                ready = mbar_wait(&ctl->accFull, 0, &ctl->abort, WAIT_ACC_FULL);
+                ready = mbar_wait(&ctl->accFull, 0, &ctl->abort, WAIT_ACC_FULL); // the last slot has been read
             __syncwarp();
-            if(p.parts > 1u)
-                cluster_sync(); // every block's MMAs have read their last slot
             if(drains && ready)
             {
                 tc_fence_after_sync();
                 const uint32_t inTile = warp % 4u * 32u + lane, taddr = tmem + ((warp % 4u * 32u) << 16);
-                const uint32_t mine   = smem_addr(ring) + (part * share * ROW_TILE + inTile) * 4u;
-                uint32_t       to = 0, local = 0, addr = p.parts > 1u ? map_to_cta(mine, 0) : mine;
+                uint32_t*      at     = reinterpret_cast<uint32_t*>(ring) + inTile;
                 for(uint32_t q0 = 0; q0 < p.nq; q0 += 16u)
                 {
                     uint32_t raw[16];
@@ -321,76 +417,7 @@ namespace b200wmma
                     tmem_load_wait();
 #pragma unroll
                     for(uint32_t j = 0; j < 16u; ++j)
-                    {
-                        storeCluster(addr, raw[j]);
-                        addr += ROW_TILE * 4u;
-                        if(p.parts > 1u && ++local == share && ++to < p.parts)
-                        {
-                            local = 0;
-                            addr  = map_to_cta(mine, to);
-                        }
-                    }
-                }
-                tc_fence_before_sync();
-            }
-            if(p.parts > 1u)
-                cluster_sync();
-            else
-                __syncthreads();
-            {
-                float const*   sums  = reinterpret_cast<float const*>(ring);
-                const uint32_t first = part * share; // thin row
-                const uint32_t mine  = first < p.thin ? min(share, p.thin - first) : 0u;
-                const uint64_t row0  = uint64_t(tile) * ROW_TILE;
-                const uint32_t left  = uint32_t(min(uint64_t(ROW_TILE), p.rows - row0));
-                OutT*          d     = static_cast<OutT*>(p.d) + row0 * p.dRow + first * p.dThin;
-                OutT const*    c     = p.c ? static_cast<OutT const*>(p.c) + row0 * p.cRow + first * p.cThin : nullptr;
-                if(p.dRow == 1u)
-                {
-                    // a warp takes a row of D, a lane four columns
-                    constexpr uint32_t WARPS = NUM_THREADS / 32u;
-                    const uint32_t     r     = 4u * lane;
-                    if(r < left)
-                    {
-                        d += r + warp * p.dThin;
-                        c = c ? c + r + warp * p.cThin : nullptr;
-                        float const* at = sums + warp * ROW_TILE + r;
-#pragma unroll 4
-                        for(uint32_t q = warp; q < mine; q += WARPS)
-                        {
-                            float4 acc = *reinterpret_cast<float4 const*>(at);
-                            for(uint32_t o = 1; o < p.parts; ++o)
-                            {
-                                const float4 more = *reinterpret_cast<float4 const*>(at + o * share * ROW_TILE);
-                                acc.x += more.x;
-                                acc.y += more.y;
-                                acc.z += more.z;
-                                acc.w += more.w;
-                            }
-                            putFour<OutT>(d, c, p, true, left - r, acc);
-                            at += WARPS * ROW_TILE;
-                            d += WARPS * p.dThin;
-                            c = c ? c + WARPS * p.cThin : nullptr;
-                        }
-                    }
-                }
-                else if(threadIdx.x < left)
-                {
-                    // a thread takes a row of D, four columns at a time
-                    const uint32_t r = threadIdx.x;
-                    d += r * p.dRow;
-                    c = c ? c + r * p.cRow : nullptr;
-                    auto total = [&](uint32_t q) {
-                        if(q >= mine)
-                            return 0.0f;
-                        float acc = sums[q * ROW_TILE + r];
-                        for(uint32_t o = 1; o < p.parts; ++o)
-                            acc += sums[(o * share + q) * ROW_TILE + r];
-                        return acc;
-                    };
-                    for(uint32_t q = 0; q < mine; q += 4u)
-                        putFour<OutT>(d + q, c ? c + q : nullptr, p, first % 4u == 0u, mine - q,
-                                      make_float4(total(q), total(q + 1u), total(q + 2u), total(q + 3u)));
+                        at[(q0 + j) * ROW_TILE] = raw[j];
                 }
             }
             tc_fence_before_sync();
@@ -400,6 +427,31 @@ namespace b200wmma
                 __syncwarp();
                 tc_fence_after_sync();
                 tmem_dealloc(tmem, p.tmemCols);
+            }
+            __syncwarp();
+            if(p.parts > 1u)
+                cluster_sync();
+            switch(p.parts)
+            {
+            case 1:
+                finishShare<OutT, 1>(p, smem_addr(ring), tile, part);
+                break;
+            case 2:
+                finishShare<OutT, 2>(p, smem_addr(ring), tile, part);
+                break;
+            case 4:
+                finishShare<OutT, 4>(p, smem_addr(ring), tile, part);
+                break;
+            default:
+                finishShare<OutT, 8>(p, smem_addr(ring), tile, part);
+            }
+            __syncwarp();
+            if(p.parts > 1u)
+            {
+                // no block leaves while another may still read its sums (what this one has read has arrived:
+                // it has been stored)
+                cluster_arrive_relaxed();
+                cluster_wait();
             }
             if(threadIdx.x == 0 && ctl->abort.flag != 0u && p.status != nullptr)
             {
@@ -450,7 +502,8 @@ namespace b200wmma
         {
             return 2u * CODE_BYTES + 3u * slotGroups<KIND>() * MX_TILE_BYTES;
         }
-        // (Large enough that no block of the thin kernel fits beside it: see there.)
+        // (Large enough that no block of the thin kernel fits beside it, which would leave it waiting for
+        // columns.)
         template <ScaleKind KIND>
         constexpr uint32_t pairSmemBytes(bool useC)
         {
@@ -1008,11 +1061,10 @@ namespace b200wmma
                 rc = scaleMap(&mapScaleQ, thinA ? o.aScales : o.bScales, p.thin, groups, GROUPS, tilesOfQ);
             if(rc != B200WMMA_OK)
                 return rc;
-            // Blocks of a cluster wait for each other, and a block waits in tcgen05.alloc while its SM has
-            // no columns left: two clusters that each hold the columns that the other needs would wait
-            // for good.  So a block takes at least the share of its SM's shared memory that it takes of
-            // the 512 columns, and blocks that fit an SM always find theirs.  (The pair kernel, which
-            // takes all columns, leaves no room for the smallest block of this one.)
+            // A block takes at least the share of its SM's shared memory that it takes of the 512 columns, so
+            // that an SM is not given more blocks than it has columns for, which would wait in
+            // tcgen05.alloc while other SMs have room.  (That such a wait ends does not rest on this:
+            // see the kernel.)
             constexpr uint32_t SM_SMEM = 228u * 1024u, BLOCK_SMEM = 1024u; // of an SM; on top of each block's own
             const uint32_t     share   = p.tmemCols * (SM_SMEM / 512u) - BLOCK_SMEM;
             uint32_t           smem    = 1024u + p.stages * p.slotBytes + uint32_t(sizeof(ThinControl));
@@ -1045,7 +1097,7 @@ namespace b200wmma
             if(sms < 2)
                 return B200WMMA_ERR_CUDA;
             const uint32_t thin = p.m < p.n ? p.m : p.n;
-            // (96 x 4096 x 4096: 7.6 us thin, 10.5 in pairs; 128 x 8192 x 8192: 16.9 both; 256 x 8192 x 8192: 22 and 17)
+            // (96 x 4096 x 4096: 7.3 us thin, 10.5 in pairs; 128 x 8192 x 8192: 14.5 and 16.9)
             return thin <= 128u ? launchThin<KIND, OutT>(o, p, sms, stream) : launchPairs<KIND, OutT>(o, p, sms, stream);
         }
 

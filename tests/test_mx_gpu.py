@@ -278,6 +278,27 @@ def test_products_on_several_streams_at_once():
         assert torch.equal(d.view(m, -1)[:, :n], want)
 
 
+def test_clusters_beside_blocks_that_take_other_widths_of_tensor_memory():
+    """Thin products of 64, 128 and 256 columns a block, K in one to eight parts, and a large one, all on
+    streams of their own: ranges of every size come and go on an SM while the blocks of a cluster start."""
+    g = torch.Generator().manual_seed(8)
+    work = []
+    for fmt, m, n, k in ((MXF4, 1, 2048, 4096), (MXF4, 40, 2048, 2048), (MXF4, 100, 2048, 4096), (MXF4, 3, 9000, 512),
+                         (NVF4, 20, 4096, 2048), (NVF4, 50, 20000, 512), (NVF4, 128, 1024, 4096), (NVF4, 500, 600, 512)):
+        (a, av), (b, bv) = _small(fmt, m, k, g), _small(fmt, n, k, g)
+        out = [torch.full((m, n), 7.0, device="cuda") for _ in range(30)]
+        work.append((fmt, m, n, k, a, b, torch.from_numpy(av @ bv.T).float().cuda(), out, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for i in range(30):
+        for fmt, m, n, k, a, b, _, out, stream in work:
+            api.mx_gemm(fmt, F32, m, n, k, a, b, None, 1.0, 0.0, out=out[i], stream=stream)
+    torch.cuda.synchronize()
+    api.check_device()
+    for *_, want, out, _ in work:
+        for d in out:
+            assert torch.equal(d, want)
+
+
 @FORMATS
 def test_linear_layer_and_its_gradients(fmt):
     """y = x W^T, dx = dy W and dW = dy^T x, each from operands quantised along the index it sums over."""
