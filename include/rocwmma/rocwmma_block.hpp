@@ -153,6 +153,16 @@ namespace rocwmma
             }
         }
 
+        // mbar_wait for a whole, converged warp: true if every lane's wait was.  Lanes read the clock and
+        // the abort flag at different times, so around the limit some may give up and some not;
+        // what follows as one instruction of the warp (tcgen05.ld) needs one answer.
+        ROCWMMA_DEVICE inline bool
+            mbar_wait_warp(uint64_t* bar, uint32_t parity, AbortState* abort, uint32_t code,
+                           long long limit = WAIT_LIMIT_CYCLES)
+        {
+            return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, code, limit));
+        }
+
         // ---- TMA (cp.async.bulk.tensor), no multicast --------------------------------
         ROCWMMA_DEVICE inline void tma_prefetch_descriptor(void const* tensorMap)
         {

@@ -403,8 +403,7 @@ namespace b200wmma
             const bool drains = warp >= 2u;
             bool       ready  = false;
             if(drains)
-                ready = mbar_wait(&ctl->accFull, 0, &ctl->abort, WAIT_ACC_FULL); // the last slot has been read
-            __syncwarp();
+                ready = mbar_wait_warp(&ctl->accFull, 0, &ctl->abort, WAIT_ACC_FULL); // the last slot has been read
             if(drains && ready)
             {
                 tc_fence_after_sync();
@@ -613,7 +612,7 @@ namespace b200wmma
                         prefetch_l2(c + at);
                 }
             }
-            if(!__all_sync(0xffffffffu, mbar_wait(&ctl->accFull[accBar], accPhase, &ctl->abort, WAIT_ACC_FULL)))
+            if(!mbar_wait_warp(&ctl->accFull[accBar], accPhase, &ctl->abort, WAIT_ACC_FULL))
                 return false;
             tc_fence_after_sync();
 #pragma unroll 1
@@ -655,9 +654,9 @@ namespace b200wmma
                     continue;
                 }
                 const uint32_t b = mine & (p.boxes - 1u), use = (mine & p.boxes) != 0u;
-                const bool     open = C ? mbar_wait(&ctl->cFull[b], use, &ctl->abort, WAIT_STAGE_FULL)
-                                        : mbar_wait(&ctl->boxFree[b], use ^ 1u, &ctl->abort, WAIT_DRAIN);
-                if(!__all_sync(0xffffffffu, open))
+                const bool     open = C ? mbar_wait_warp(&ctl->cFull[b], use, &ctl->abort, WAIT_STAGE_FULL)
+                                        : mbar_wait_warp(&ctl->boxFree[b], use ^ 1u, &ctl->abort, WAIT_DRAIN);
+                if(!open)
                     return false;
                 uint8_t* at = staging + b * BOX_BYTES + rowIn * 64u;
 #pragma unroll

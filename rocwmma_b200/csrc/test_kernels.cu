@@ -262,6 +262,31 @@ namespace
         out[3] = abortState.flag;
     }
 
+    // One warp, its lanes on two barriers: one that has completed a phase and, from lane `split` on,
+    // one that never will, in a block that is aborting already.  out[lane] = what the lane's own
+    // wait said, out[32 + lane] = what the warp's said.
+    __global__ void warpWaitKernel(uint32_t* out, uint32_t split)
+    {
+        __shared__ uint64_t                    bars[2];
+        __shared__ rocwmma::block::AbortState abortState;
+        namespace blk = rocwmma::block;
+        const uint32_t lane = threadIdx.x;
+        if(lane == 0)
+        {
+            blk::mbar_init(&bars[0], 1);
+            blk::mbar_init(&bars[1], 1);
+            abortState.flag = 1;
+            abortState.code = 0;
+            blk::mbar_init_fence();
+            blk::mbar_arrive(&bars[0]);
+        }
+        __syncwarp();
+        uint64_t* bar = &bars[lane < split ? 0 : 1];
+        out[lane]     = blk::mbar_wait(bar, 0, &abortState, blk::WAIT_ACC_FULL, 2000000ll);
+        __syncwarp();
+        out[32u + lane] = blk::mbar_wait_warp(bar, 0, &abortState, blk::WAIT_ACC_FULL, 2000000ll);
+    }
+
     // Untiled bulk copies: rows of `rowBytes` go global -> shared (one copy per lane, all
     // signalling one mbarrier that every lane arrives on once) and come back shared -> global
     // with every byte incremented, which shows that both directions and the proxy fence
@@ -431,6 +456,15 @@ TEST_API int b200wmma_test_bounded_wait(uint32_t* out4, long long limit_cycles, 
     if(limit_cycles <= 0 || limit_cycles > 20000000ll)
         return -1;
     boundedWaitKernel<<<1, 64, 0, static_cast<cudaStream_t>(stream)>>>(out4, limit_cycles);
+    return cudaGetLastError() == cudaSuccess ? 0 : -4;
+}
+
+// split <= 32: lanes that wait for a completed phase; 64 words come back.
+TEST_API int b200wmma_test_warp_wait(uint32_t* out64, uint32_t split, void* stream)
+{
+    if(split > 32u)
+        return -1;
+    warpWaitKernel<<<1, 32, 0, static_cast<cudaStream_t>(stream)>>>(out64, split);
     return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 

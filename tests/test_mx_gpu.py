@@ -278,6 +278,20 @@ def test_products_on_several_streams_at_once():
         assert torch.equal(d.view(m, -1)[:, :n], want)
 
 
+@pytest.mark.parametrize("split", [0, 16, 31, 32])
+def test_a_warp_gives_up_as_one(split):
+    """Where a wait's limit passes for some lanes only, the warp that drains an accumulator has one answer."""
+    import ctypes as C
+    from rocwmma_b200 import _lib as L
+    wait = C.CDLL(L.TEST_LIB_PATH).b200wmma_test_warp_wait
+    wait.argtypes = [C.c_void_p, C.c_uint32, C.c_void_p]
+    out = torch.full((64,), 7, dtype=torch.int32, device="cuda")
+    assert wait(out.data_ptr(), split, torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert out[:32].tolist() == [1] * split + [0] * (32 - split)
+    assert out[32:].tolist() == [int(split == 32)] * 32
+
+
 def test_clusters_beside_blocks_that_take_other_widths_of_tensor_memory():
     """Thin products of 64, 128 and 256 columns a block, K in one to eight parts, and a large one, all on
     streams of their own: ranges of every size come and go on an SM while the blocks of a cluster start."""
