@@ -528,8 +528,16 @@ namespace b200wmma
             uint64_t       ldo; // elements
             uint32_t       rows, k, groups, tilesK;
             uint32_t       tilesPerBlock;
-            float          factor; // 2^exponent
+            float          factor; // 2^exponent; MXF4: four times that, see scaleValue()
         };
+
+        // A block's scale s; MXF4: s / 4, since 6 * 2^127 is beyond fp32 where 2^exponent can bring it back.
+        // (Both s / 4 and half of it are fp32 numbers down to s = 2^-127.)
+        template <bool NV>
+        __device__ inline float scaleValue(uint32_t byte)
+        {
+            return NV ? fromE4m3(byte) : 0.25f * fromE8m0(byte);
+        }
 
         // Eight values: code * s is exact (three bits times at most four); so is the power of two, short
         // of the subnormals.
@@ -588,7 +596,7 @@ namespace b200wmma
             {
                 const uint32_t done = t * TILE_K;
                 const uint2    code = nextCode;
-                const float    s    = NV ? fromE4m3(nextByte) : fromE8m0(nextByte);
+                const float    s    = scaleValue<NV>(nextByte);
                 if(t + 1u < tiles)
                     fetch(t + 1u);
                 Run<T> o;
@@ -764,7 +772,8 @@ int b200wmma_mx_dequantize(int fmt, int out_dtype, uint32_t rows, uint32_t k, co
     const bool             nv = fmt == B200WMMA_NVF4;
     const DequantizeParams p{static_cast<uint8_t const*>(codes), static_cast<uint8_t const*>(scales),
                              out, ldq, ldo, rows, k, mxGroups(nv, k),
-                             uint32_t((uint64_t(k) + TILE_K - 1) / TILE_K), 0, ldexpf(1.0f, exponent)};
+                             uint32_t((uint64_t(k) + TILE_K - 1) / TILE_K), 0,
+                             ldexpf(1.0f, nv ? exponent : exponent + 2)};
     const cudaStream_t     s = static_cast<cudaStream_t>(stream);
     switch(out_dtype)
     {

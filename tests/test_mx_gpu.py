@@ -128,6 +128,21 @@ def test_quantize_strides_and_offsets(fmt, layout):
     assert (out[:, k:] == 7).all()
 
 
+@FORMATS
+@pytest.mark.parametrize("exponent", [-64, -10, 0, 5, 64])
+def test_dequantize_every_code_and_scale(fmt, exponent):
+    """All codes under all scales, those no quantisation writes among them: 6 * 2^127 times a small power
+    of two is a number again."""
+    block, scales = R.BLOCK[fmt], np.arange(256 if fmt == MXF4 else 128, dtype=np.uint8)
+    codes = np.tile(np.arange(16, dtype=np.uint8), (scales.size, block // 16))
+    packed = [torch.from_numpy(t).cuda() for t in R.pack(fmt, codes, scales[:, None])]
+    want = torch.from_numpy(R.values(fmt, codes, scales[:, None]) * 2.0 ** exponent)
+    for out in (F32, BF16):
+        got = api.mx_dequantize(fmt, out, scales.size, block, *packed, exponent=exponent).view(want.shape)
+        # (at most seven bits: fp32, and then bf16, round what lies below their subnormals' steps alike)
+        np.testing.assert_array_equal(_host(got), _host(want.float().to(TYPES[out])))
+
+
 # ---- products ------------------------------------------------------------------------------------
 
 def _small(fmt, rows, k, g):
