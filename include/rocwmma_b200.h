@@ -242,7 +242,8 @@ B200WMMA_API int b200wmma_dlrm_bwd(int dtype, const void* input, const void* ups
  * of the tokens picks from the i-th: row = first[i] + id, 0 <= id < first[i + 1] - first[i], with
  * first[0..inner] in device memory.  An id outside its table (-1 for padding) gives a row of
  * zeros.  With out_outer = 27 * dim and out 27 * dim-strided from the second row on, the call
- * writes the 26 categorical features of b200wmma_dlrm_fwd's input in place.
+ * writes the 26 categorical features of b200wmma_dlrm_fwd's input in place.  Rows of out that share
+ * an element are refused (INVALID_ARG).
  * Any alignment of whole elements; rows on 16-byte boundaries and dim a multiple of 8 are fast.
  * rows < 2^31 - 1, outer * inner < 2^31 - 4096, dim <= 2^20.
  */

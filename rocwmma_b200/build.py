@@ -74,7 +74,7 @@ def _bind(force):
     """The Python binding, linked with libb200wmma.so and with torch's libraries (which `import
     torch` has loaded before the binding is)."""
     src, so = os.path.join(CSRC, "bind.cpp"), os.path.join(HERE, "_bind.so")
-    if force or _stale(so, [src, os.path.join(ROOT, "include", "rocwmma_b200.h")]):
+    if force or _stale(so, [src, os.path.join(CSRC, "row_overlap.h"), os.path.join(ROOT, "include", "rocwmma_b200.h")]):
         torch = os.path.dirname(importlib.util.find_spec("torch").origin)
         cuda = os.path.dirname(os.path.dirname(NVCC))
         cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-fvisibility=hidden", "-shared",

@@ -15,6 +15,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "rocwmma_b200.h"
+#include "row_overlap.h"
 
 namespace
 {
@@ -380,8 +381,8 @@ namespace
         }
         int64_t outOuter, outInner;
         rowsOf(out, ids, dim, "out", outOuter, outInner);
-        if((outOuter == 0 && t.outer > 1) || (outInner == 0 && t.inner > 1))
-            refuse("out must not hold a row twice");
+        if(b200wmma::rowsOverlap(uint64_t(t.outer), uint64_t(outOuter), uint64_t(t.inner), uint64_t(outInner), uint64_t(dim)))
+            refuse("the rows of out must not overlap");
         const int outType = valueCode(out, "out");
         if(t.outer && t.inner)
             finish(b200wmma_embedding(tableCode, outType, uint64_t(rows), width(dim), uint64_t(t.outer), width(t.inner),

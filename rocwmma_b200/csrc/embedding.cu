@@ -18,6 +18,7 @@
 #include "common.cuh"
 #include "mx_format.cuh"
 #include "rocwmma/rocwmma_block.hpp"
+#include "row_overlap.h"
 #include <cstring>
 #include <mutex>
 #include <type_traits>
@@ -1548,6 +1549,8 @@ int b200wmma_embedding(int table_dtype, int out_dtype, uint64_t rows, uint32_t d
                                table_dtype, out_dtype);
     if(rc != B200WMMA_OK)
         return rc;
+    if(rowsOverlap(outer, out_outer, inner, out_inner, dim)) // which row would remain is nobody's choice
+        return B200WMMA_ERR_INVALID_ARG;
     LookupParams p{};
     p.t = Tokens{ids, first, ids_outer, ids_inner, uint32_t(outer * inner), uint32_t(rows), Divisor(inner), id_bytes == 8 ? 1u : 0u};
     p.table    = table;

@@ -88,6 +88,27 @@ def test_lookup_strides():
     assert torch.equal(got[:4], torch.zeros(4, 37)) and torch.equal(got[4], wide[39])
 
 
+def test_lookup_into_rows_that_interleave_and_rows_that_overlap():
+    """Any layout whose rows share no element is written; the others are refused."""
+    table, dim = _randn((9, 4), F32, 1), 4
+    for outer, inner in ((1, 5), (2, 3), (3, 2), (7, 2), (4, 1)):
+        ids = _ids((outer, inner), 9, outer)
+        want = torch.where(ids[..., None] >= 0, table[ids.clamp(min=0)], 0.0)
+        for a in range(0, 25):
+            for b in range(0, 25):
+                flat = torch.full((400,), 7.0, device="cuda")
+                out = flat.as_strided((outer, inner, dim), (a, b, 1))
+                starts = (torch.arange(outer)[:, None] * a + torch.arange(inner) * b).reshape(-1).sort().values
+                if (starts.diff() < dim).any():
+                    with pytest.raises(ValueError):
+                        api.embedding(table.cuda(), ids.cuda(), out=out)
+                    assert (flat == 7).all()
+                else:
+                    api.embedding(table.cuda(), ids.cuda(), out=out)
+                    assert torch.equal(out.cpu(), want)
+                    assert int((flat != 7).sum()) <= outer * inner * dim
+
+
 def _grad_reference(grad, ids, rows, scale=1.0, old=None):
     """(sum, sum of magnitudes, tokens) of every row in 64 bits."""
     flat, g = ids.reshape(-1).numpy(), grad.double().reshape(-1, grad.shape[-1]).numpy()

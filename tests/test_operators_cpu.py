@@ -82,6 +82,31 @@ def _gradient(table_t=L.F16, out_t=L.F16, rows=9, dim=8, outer=3, inner=2, table
                                            first, table, ldt, 1.0, 0, work, size, None)
 
 
+def _rows_share_an_element(outer, a, inner, b, dim):
+    starts = np.sort((np.arange(outer)[:, None] * a + np.arange(inner) * b).reshape(-1))
+    return bool((np.diff(starts) < dim).any())
+
+
+def test_lookup_refuses_rows_that_overlap():
+    """Every small layout, against the rows written out; only those that overlap are called (there is no
+    device to write to)."""
+    def call(outer, a, inner, b, dim):
+        return L.lib().b200wmma_embedding(L.F32, L.F32, 9, dim, outer, inner, P, dim, P, 8, inner, 1, None, P, a, b, 1.0, None)
+
+    seen = 0
+    for outer in (1, 2, 3, 7):
+        for inner in (1, 2, 5):
+            for a in range(0, 31):
+                for b in range(0, 31):
+                    if _rows_share_an_element(outer, a, inner, b, 4):
+                        assert call(outer, a, inner, b, 4) == L.ERR_INVALID_ARG, (outer, a, inner, b)
+                        seen += 1
+    assert seen > 1000
+    for outer, a, inner, b in ((2 ** 30, 3, 1, 0), (2, 2 ** 63, 2, 2 ** 63), (2 ** 15, 2 ** 15 * 4 - 1, 2 ** 15, 4),
+                               (2 ** 15, 4, 2 ** 15, 2 ** 15 * 4 - 1)):
+        assert call(outer, a, inner, b, 4) == L.ERR_INVALID_ARG
+
+
 @pytest.mark.parametrize("call", [_lookup, _gradient])
 def test_embedding_refusals(call):
     for bad in (dict(table=None), dict(ids=None), dict(out=None), dict(rows=0), dict(dim=0), dict(outer=0), dict(inner=0),
