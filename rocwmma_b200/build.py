@@ -6,11 +6,13 @@ Produces, next to this file:
     lib/libb200wmma.so        the product: kernels + C ABI (include/rocwmma_b200.h)
     lib/libb200wmma_test.so   device-API unit-test kernels used only by tests/
     _bind.so                  the Python binding of the calls where ctypes would take longer than
-                              the kernels (csrc/bind.cpp; g++, torch's headers)
+                              the kernels (csrc/bind.cpp; g++, torch's headers); left out where
+                              torch with CUDA is not installed, which the C ABI does not need
 """
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.metadata
 import importlib.util
 import os
 import subprocess
@@ -70,12 +72,33 @@ def _link(objs, name, force):
     return so
 
 
+def _built_for():
+    """What the binding's machine code depends on beside its sources: torch's and Python's ABI."""
+    try:
+        torch = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:
+        torch = "unknown"
+    return f"torch {torch}, {sysconfig.get_config_var('SOABI')}\n"
+
+
+def _read(path):
+    if not os.path.exists(path):
+        return None
+    with open(path) as f:
+        return f.read()
+
+
 def _bind(force):
     """The Python binding, linked with libb200wmma.so and with torch's libraries (which `import
-    torch` has loaded before the binding is)."""
-    src, so = os.path.join(CSRC, "bind.cpp"), os.path.join(HERE, "_bind.so")
-    if force or _stale(so, [src, os.path.join(CSRC, "row_overlap.h"), os.path.join(ROOT, "include", "rocwmma_b200.h")]):
-        torch = os.path.dirname(importlib.util.find_spec("torch").origin)
+    torch` has loaded before the binding is).  None without torch, or with one that has no CUDA."""
+    spec = importlib.util.find_spec("torch")
+    torch = os.path.dirname(spec.origin) if spec and spec.origin else None
+    if torch is None or not os.path.exists(os.path.join(torch, "lib", "libc10_cuda.so")):
+        print("torch with CUDA is not installed: the C libraries are built, rocwmma_b200/_bind.so is not")
+        return None
+    src, so, stamp = os.path.join(CSRC, "bind.cpp"), os.path.join(HERE, "_bind.so"), os.path.join(LIB, "_bind.stamp")
+    if (force or _stale(so, [src, os.path.join(CSRC, "row_overlap.h"), os.path.join(ROOT, "include", "rocwmma_b200.h")])
+            or _read(stamp) != _built_for()):
         cuda = os.path.dirname(os.path.dirname(NVCC))
         cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-fvisibility=hidden", "-shared",
                "-I", os.path.join(ROOT, "include"), "-I", os.path.join(cuda, "include"),
@@ -87,6 +110,8 @@ def _bind(force):
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"g++ failed for bind.cpp:\n{r.stdout}\n{r.stderr}")
+        with open(stamp, "w") as f:
+            f.write(_built_for())
     return so
 
 
@@ -97,10 +122,10 @@ def build(force: bool = False, verbose: bool = False):
     with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
         objs = dict(zip(srcs, ex.map(lambda s: _compile(s, force), srcs)))
     prod = _link([objs[s] for s in PRODUCT if s in objs], "libb200wmma.so", force)
-    _bind(force)
     test = None
     if all(s in objs for s in TESTLIB):
         test = _link([objs[s] for s in TESTLIB], "libb200wmma_test.so", force)
+    _bind(force)
     if verbose:
         print("built", prod, test)
     return prod, test
