@@ -189,6 +189,29 @@ def test_gradient_accumulates_into_views(dim):
     _check_grad(got, grad[:, 1:], flat, rows, F32, 0.5, old[:, :dim].double().numpy())
 
 
+@pytest.mark.parametrize("tokens,rows,dim,skew", [(70000, 300, 64, 6.0), (30000, 2000, 520, 2.0), (5000, 40, 1032, 4.0),
+                                                  (3000, 7, 2304, 1.0)])
+@pytest.mark.parametrize("grad_off,grad_ld,out_off,out_ld", [(1, 0, 0, 0), (0, 0, 1, 0), (0, 1, 0, 0), (0, 0, 0, 1), (4, 0, 2, 4),
+                                                             (2, 2, 1, 3)])
+def test_gradient_off_the_boundary(tokens, rows, dim, skew, grad_off, grad_ld, out_off, out_ld):
+    """Rows of a multiple of eight that start or follow each other off the boundary: pieces narrower than the
+    workspace is planned for, of the gradient and of the table apart, over many parts."""
+    grad, ids = _randn((tokens, dim), BF16, 1), _ids((tokens,), rows, 2, skew)
+    g = torch.full((grad_off + tokens * (dim + grad_ld),), float("nan"), dtype=torch.bfloat16, device="cuda")
+    g = g[grad_off:].view(tokens, dim + grad_ld)[:, :dim]
+    g.copy_(grad)
+    for kind in (F32, F16):
+        flat = torch.full((out_off + rows * (dim + out_ld) + 8,), 7.0, dtype=TYPES[kind], device="cuda")
+        out = flat[out_off:out_off + rows * (dim + out_ld)].view(rows, dim + out_ld)[:, :dim]
+        api.embedding_grad(g, ids.cuda(), rows, out=out)
+        _check_grad(out, grad, ids, rows, kind)
+        old = out.clone()
+        api.embedding_grad(g, ids.cuda(), rows, out=out, accumulate=True, scale=0.5)
+        _check_grad(out, grad, ids, rows, kind, 0.5, old.double().cpu().numpy())
+        out.fill_(7.0)
+        assert (flat == 7).all()
+
+
 def test_gradient_is_the_lookups():
     """<grad, embedding(table)> grows with the table as the gradient says: differences in 64 bits of a
     function that is linear in the table."""

@@ -194,6 +194,16 @@ def test_gemm_alpha_beta(fmt, kind, m, n, k):
 
 @FORMATS
 @KINDS
+@pytest.mark.parametrize("m,n,k", [(1, 264, 4096), (33, 260, 2100), (16, 1000, 1100), (100, 500, 3000), (300, 9, 4096),
+                                   (200, 72, 2100), (1030, 33, 1290)])
+def test_gemm_thin_in_parts_with_c(fmt, kind, m, n, k):
+    """K in two to eight parts, whose blocks each finish a share of the thin rows: C is read where D is written."""
+    _product(fmt, kind, m, n, k, 3, alpha=0.5, beta=-2.0, c=True)
+    _product(fmt, kind, m, n, k, 4, alpha=1.0, beta=1.0, c=True, ld=(n + 7) // 8 * 8 + 24)
+
+
+@FORMATS
+@KINDS
 @pytest.mark.parametrize("m,n,k", [(2570, 5000, 200), (300, 20001, 328)])
 def test_gemm_many_tiles(fmt, kind, m, n, k):
     """More tiles than the device has SMs: several to a block, the last ones ragged."""
