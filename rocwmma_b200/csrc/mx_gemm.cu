@@ -88,7 +88,7 @@ namespace b200wmma
         // ---- thin products -----------------------------------------------------------------
         // One of m and n is small (a decoding batch; one token): the other operand, whose rows
         // are the MMA's M here, 128 to a block, streams from HBM once and bounds the call.  The
-        // thin operand is the MMA's N, padded to 16 rows.  A cluster of `parts` blocks shares a
+        // thin operand is the MMA's N, padded to 16 rows; its scales are one tile of 128.  A cluster of `parts` blocks shares a
         // tile, each a stretch of K, so that the stream comes through all SMs.  Every block puts its
         // partial sums where its ring was, and adds up its share of the thin rows out of the
         // shared memory of the whole cluster, always in the order of the blocks.
@@ -100,6 +100,8 @@ namespace b200wmma
         // 1 x 8192 x 8192 MXF4: 9.1 us a call, 5.5 for its bytes; 64 x 16384 x 4096 NVF4: 12.4 and 6.
         // (With the sums sent to the block that adds them up, and the columns held until the end: 9.5 and 13.8;
         // 8192 x 64 x 2048 MXF4: 10.4 us so, 7.0 now.)
+        constexpr uint32_t THIN_ROWS = 128; // at most, of the thin operand
+        static_assert(THIN_ROWS <= MX_TILE_ROWS, "one scale tile to a ring slot's group");
         struct ThinParams
         {
             void const* c;
@@ -263,7 +265,6 @@ namespace b200wmma
             const uint32_t allSlots = (p.k + SLOT_K - 1) / SLOT_K;
             const uint32_t slot0 = uint32_t(uint64_t(part) * allSlots / p.parts);
             const uint32_t numSlots = uint32_t(uint64_t(part + 1u) * allSlots / p.parts) - slot0;
-            const uint32_t tilesOfQ = (p.nq + 127u) / 128u; // scale row tiles of the thin operand
             const uint32_t qBytes   = p.nq * 128u;
 
             if(threadIdx.x == 0)
@@ -339,7 +340,7 @@ namespace b200wmma
                 if(elect_one())
                 {
                     // accumulator, then the scales of two ring slots in turn
-                    const uint32_t scaleCols = 4u * GROUPS * (1u + tilesOfQ);
+                    const uint32_t scaleCols = 4u * GROUPS * 2u;
                     uint32_t       scale = tmem + (p.nq + 31u) / 32u * 32u, otherScale = scale + scaleCols;
                     const uint32_t base  = smem_addr(ring);
                     const uint64_t descR = smem_desc_kmajor_sw128(base), descQ = descAt(descR, CODE_BYTES);
@@ -361,12 +362,7 @@ namespace b200wmma
                         for(uint32_t g = 0; g < GROUPS; ++g)
                         {
                             tmem_copy_scales(scale + 4u * g, descAt(dS, g * MX_TILE_BYTES));
-                            if(tilesOfQ == 1u)
-                                tmem_copy_scales(scale + 4u * (GROUPS + g), descAt(dS, (GROUPS + g) * MX_TILE_BYTES));
-                            else
-                                for(uint32_t t = 0; t < tilesOfQ; ++t)
-                                    tmem_copy_scales(scale + 4u * (GROUPS + g * tilesOfQ + t),
-                                                     descAt(dS, (GROUPS * (1u + t) + g) * MX_TILE_BYTES));
+                            tmem_copy_scales(scale + 4u * (GROUPS + g), descAt(dS, (GROUPS + g) * MX_TILE_BYTES));
                         }
                         const uint64_t dR = descAt(descR, at.offset), dQ = descAt(descQ, at.offset);
                         auto step = [&](uint32_t ks) {
@@ -374,7 +370,7 @@ namespace b200wmma
                             const uint32_t g  = KIND == ScaleKind::E4M3_16 ? ks : ks / 2u;
                             const uint32_t id = KIND == ScaleKind::E4M3_16 ? 0u : (ks & 1u) * 2u;
                             mma_scaled<KIND>(tmem, descAt(dR, ks * 32u), descAt(dQ, ks * 32u), idesc | id << 4 | id << 29,
-                                             scale + 4u * g, scale + 4u * (GROUPS + g * tilesOfQ), more);
+                                             scale + 4u * g, scale + 4u * (GROUPS + g), more);
                             more = 1;
                         };
                         if(left >= SLOT_K)
@@ -1026,9 +1022,8 @@ namespace b200wmma
             p.r      = thinA ? o.b : o.a;
             p.ldr    = thinA ? o.ldb : o.lda;
             p.nq     = (p.thin + 15u) / 16u * 16u;
-            const uint32_t tilesOfQ = (p.nq + 127u) / 128u;
-            const uint32_t slots    = (q.k + SLOT_K - 1u) / SLOT_K;
-            const uint32_t tiles    = mxRowTiles(p.rows);
+            const uint32_t slots = (q.k + SLOT_K - 1u) / SLOT_K;
+            const uint32_t tiles = mxRowTiles(p.rows);
             // K is split until the blocks fill the device: twice over for up to 32 thin rows (1 x 8192 x
             // 8192 MXF4: 8.5 us in the kernel with 4 parts, 9.3 with 2, 11.4 with 1), once for more,
             // whose sums cost more to exchange (64 x 16384 x 4096 NVF4: 11.3 us with 1 part, 12.0 with 2).
@@ -1036,7 +1031,7 @@ namespace b200wmma
             p.parts                 = 8;
             while(p.parts > 1u && (uint64_t(tiles) * p.parts > resident * uint32_t(sms) || slots < 2u * p.parts))
                 p.parts /= 2u;
-            p.slotBytes = CODE_BYTES + p.nq * 128u + GROUPS * MX_TILE_BYTES * (1u + tilesOfQ);
+            p.slotBytes = CODE_BYTES + p.nq * 128u + GROUPS * MX_TILE_BYTES * 2u;
             // a block leaves room for another on its SM: of this kernel or of the next one
             const uint32_t room  = 112u * 1024u - uint32_t(sizeof(ThinControl)) - 1024u;
             const uint32_t mine  = (slots + p.parts - 1u) / p.parts;
@@ -1046,7 +1041,7 @@ namespace b200wmma
             // the sums take the ring's place
             while(p.stages * p.slotBytes < p.nq * ROW_TILE * 4u)
                 ++p.stages;
-            const uint32_t cols = (p.nq + 31u) / 32u * 32u + 2u * 4u * GROUPS * (1u + tilesOfQ);
+            const uint32_t cols = (p.nq + 31u) / 32u * 32u + 2u * 4u * GROUPS * 2u;
             p.tmemCols          = 32;
             while(p.tmemCols < cols)
                 p.tmemCols *= 2;
@@ -1057,7 +1052,7 @@ namespace b200wmma
             if(rc == B200WMMA_OK)
                 rc = scaleMap(&mapScaleR, thinA ? o.bScales : o.aScales, p.rows, groups, GROUPS, 1);
             if(rc == B200WMMA_OK)
-                rc = scaleMap(&mapScaleQ, thinA ? o.aScales : o.bScales, p.thin, groups, GROUPS, tilesOfQ);
+                rc = scaleMap(&mapScaleQ, thinA ? o.aScales : o.bScales, p.thin, groups, GROUPS, 1);
             if(rc != B200WMMA_OK)
                 return rc;
             // A block takes at least the share of its SM's shared memory that it takes of the 512 columns, so
@@ -1097,7 +1092,7 @@ namespace b200wmma
                 return B200WMMA_ERR_CUDA;
             const uint32_t thin = p.m < p.n ? p.m : p.n;
             // (96 x 4096 x 4096: 7.3 us thin, 10.5 in pairs; 128 x 8192 x 8192: 14.5 and 16.9)
-            return thin <= 128u ? launchThin<KIND, OutT>(o, p, sms, stream) : launchPairs<KIND, OutT>(o, p, sms, stream);
+            return thin <= THIN_ROWS ? launchThin<KIND, OutT>(o, p, sms, stream) : launchPairs<KIND, OutT>(o, p, sms, stream);
         }
 
         template <typename OutT>
