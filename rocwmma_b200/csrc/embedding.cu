@@ -1112,21 +1112,19 @@ namespace b200wmma
                 const uint32_t count = end - first + 1u;
                 if(piece < p.pieces)
                     add(first, group, count, groups);
-                if(groups > 1u)
+#pragma unroll
+                for(int j = 0; j < V; ++j)
+                    sums[threadIdx.x][j] = sum[j];
+                __syncthreads();
+                if(group != 0u)
+                    continue;
+                for(uint32_t g = 1; g < groups && g < count; ++g)
                 {
 #pragma unroll
                     for(int j = 0; j < V; ++j)
-                        sums[threadIdx.x][j] = sum[j];
-                    __syncthreads();
-                    if(group == 0u)
-                        for(uint32_t g = 1; g < groups && g < count; ++g)
-                        {
-#pragma unroll
-                            for(int j = 0; j < V; ++j)
-                                sum[j] += sums[(g << p.lanesLog2) + threadIdx.x][j];
-                        }
+                        sum[j] += sums[(g << p.lanesLog2) + threadIdx.x][j];
                 }
-                if(group == 0u && piece < p.pieces)
+                if(piece < p.pieces)
                     finishRow<OutT, V>(p, row, piece, sum);
             }
         }
