@@ -6,6 +6,7 @@
 #include <cstdint>
 #include <cstdlib>
 #include <cuda_runtime.h>
+#include <mutex>
 
 namespace b200wmma
 {
@@ -44,6 +45,24 @@ namespace b200wmma
             return 8;
         }
         return 0;
+    }
+
+    // Opts a kernel in to more than 48 KB of dynamic shared memory, which is a property of the kernel on
+    // each device.  done: the largest size set so far on each, one array to a kernel.
+    template <typename KernelT>
+    inline int optInSharedMemory(KernelT kernel, uint32_t bytes, uint32_t (&done)[64])
+    {
+        static std::mutex           mutex;
+        std::lock_guard<std::mutex> lock(mutex);
+        int                         dev = 0;
+        B200WMMA_CUDA_TRY(cudaGetDevice(&dev));
+        if(dev < 0 || dev >= 64 || done[dev] < bytes)
+        {
+            B200WMMA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
+            if(dev >= 0 && dev < 64)
+                done[dev] = bytes;
+        }
+        return B200WMMA_OK;
     }
 
     // Kernels of this library whose prologue touches no global data are launched with

@@ -20,7 +20,6 @@
 #include "rocwmma/rocwmma_block.hpp"
 #include "row_overlap.h"
 #include <cstring>
-#include <mutex>
 #include <type_traits>
 
 namespace b200wmma
@@ -1325,22 +1324,6 @@ namespace b200wmma
             return rc__;         \
     } while(0)
 
-        // More than 48 KB of shared memory: a property of the kernel on each device.
-        template <typename KernelT>
-        int optIn(KernelT kernel, size_t bytes, std::mutex& mutex, bool (&done)[64])
-        {
-            std::lock_guard<std::mutex> lock(mutex);
-            int                         dev = 0;
-            B200WMMA_CUDA_TRY(cudaGetDevice(&dev));
-            if(dev >= 64 || !done[dev])
-            {
-                B200WMMA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
-                if(dev < 64)
-                    done[dev] = true;
-            }
-            return B200WMMA_OK;
-        }
-
         ClearParams clearParams(void* table, uint64_t ldt, uint32_t rows, uint32_t pieces)
         {
             return ClearParams{table, ldt, pieces, rowLanesLog2(pieces), 0, rows, 0};
@@ -1355,9 +1338,8 @@ namespace b200wmma
             // a block to an SM, each with 16 KB of rows at least
             const uint64_t want = (uint64_t(g.t.rows) * g.dim * sizeof(OutT) + 16383u) / 16384u;
             c.blocks            = g.accumulate ? 0u : uint32_t(want < 147u ? want : 147u);
-            static std::mutex mutex;
-            static bool       done[64] = {};
-            B200WMMA_TRY(optIn(sortSmallKernel<OutT, V, BITS>, sizeof(SmallShared<BITS>), mutex, done));
+            static uint32_t done[64] = {};
+            B200WMMA_TRY(optInSharedMemory(sortSmallKernel<OutT, V, BITS>, sizeof(SmallShared<BITS>), done));
             return cudaToStatus(launchOverlapped(sortSmallKernel<OutT, V, BITS>, dim3(1u + c.blocks), dim3(SMALL_THREADS),
                                                  sizeof(SmallShared<BITS>), stream, g.t, c, w.passes,
                                                  reinterpret_cast<uint2*>(g.workspace + w.pairs[0])));
@@ -1376,9 +1358,8 @@ namespace b200wmma
         {
             auto       words = [&](uint64_t at) { return reinterpret_cast<uint32_t*>(g.workspace + at); };
             auto       pairs = [&](uint32_t i) { return reinterpret_cast<uint2*>(g.workspace + w.pairs[i]); };
-            static std::mutex mutex;
-            static bool       done[64] = {};
-            B200WMMA_TRY(optIn(scatterKernel<ITEMS, BITS>, sizeof(ScatterShared<ITEMS, BITS>), mutex, done));
+            static uint32_t done[64] = {};
+            B200WMMA_TRY(optInSharedMemory(scatterKernel<ITEMS, BITS>, sizeof(ScatterShared<ITEMS, BITS>), done));
             const dim3 grid(w.tiles);
             B200WMMA_TRY(cudaToStatus(launchOverlapped(keysKernel<ITEMS, BITS>, grid, dim3(THREADS), 0, stream, g.t,
                                                        words(w.keys), words(w.counts))));

@@ -1850,24 +1850,6 @@ namespace
         return on;
     }
 
-    template <typename KernelT>
-    int optInSharedMemory(KernelT kernel, uint32_t bytes, bool (&done)[64])
-    {
-        static std::mutex           attrMutex;
-        std::lock_guard<std::mutex> lock(attrMutex);
-        int                         dev = 0;
-        B200WMMA_CUDA_TRY(cudaGetDevice(&dev));
-        if(dev < 0 || dev >= 64 || !done[dev])
-        {
-            // the opt-in shared-memory size is a per-device property of the kernel
-            B200WMMA_CUDA_TRY(cudaFuncSetAttribute(
-                kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
-            if(dev >= 0 && dev < 64)
-                done[dev] = true;
-        }
-        return B200WMMA_OK;
-    }
-
     // `status`: device word that records a bounded wait giving up (may be nullptr).
     // Tile rows per raster band.  Tiles are walked band by band, column by column inside a
     // band, so the rows of A that a band needs stay in L2 while B streams past.  Measured on
@@ -2206,9 +2188,9 @@ namespace
                 }();
                 p.cViaTma = cdHintEnv ? 3u : 1u;
             }
-            auto        kernel = gemm_tcgen05_pair_kernel<InT, OutT, CompT>;
-            static bool done[64] = {};
-            rc = optInSharedMemory(kernel, P_SMEM_BYTES, done);
+            auto            kernel   = gemm_tcgen05_pair_kernel<InT, OutT, CompT>;
+            static uint32_t done[64] = {};
+            rc = b200wmma::optInSharedMemory(kernel, P_SMEM_BYTES, done);
             if(rc != B200WMMA_OK)
                 return rc;
             const uint32_t tiles = tilesM * (wideCols + tailCols) + p.splitTiles; // work items
@@ -2226,9 +2208,9 @@ namespace
                  : makeOperandMap(&mapB, dt, sizeof(InT), b, n, k, ldb, BN);
         if(rc != B200WMMA_OK)
             return rc;
-        auto        kernel = gemm_tcgen05_kernel<InT, OutT, CompT>;
-        static bool done[64] = {};
-        rc = optInSharedMemory(kernel, SMEM_BYTES, done);
+        auto            kernel   = gemm_tcgen05_kernel<InT, OutT, CompT>;
+        static uint32_t done[64] = {};
+        rc = b200wmma::optInSharedMemory(kernel, SMEM_BYTES, done);
         if(rc != B200WMMA_OK)
             return rc;
         const uint32_t tiles = ((m + BM - 1) / BM) * ((n + BN - 1) / BN);

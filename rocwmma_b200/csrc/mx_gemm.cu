@@ -11,7 +11,6 @@
 #include "runtime.cuh"
 #include "tile_schedule.cuh"
 #include <cuda.h>
-#include <mutex>
 
 namespace b200wmma
 {
@@ -938,23 +937,6 @@ namespace b200wmma
                                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
                                   CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
             return r == CUDA_SUCCESS ? B200WMMA_OK : B200WMMA_ERR_CUDA;
-        }
-
-        template <typename KernelT>
-        int optInSharedMemory(KernelT kernel, uint32_t bytes, uint32_t (&done)[64])
-        {
-            static std::mutex           attrMutex;
-            std::lock_guard<std::mutex> lock(attrMutex);
-            int                         dev = 0;
-            B200WMMA_CUDA_TRY(cudaGetDevice(&dev));
-            if(dev < 0 || dev >= 64 || done[dev] < bytes)
-            {
-                B200WMMA_CUDA_TRY(cudaFuncSetAttribute(
-                    kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
-                if(dev >= 0 && dev < 64)
-                    done[dev] = bytes;
-            }
-            return B200WMMA_OK;
         }
 
         struct Operands
