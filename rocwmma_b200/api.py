@@ -242,7 +242,7 @@ def embedding(table, ids, scale=1.0, first=None, out_t=None, out=None, stream=No
     apart) and int32 / int64 ids of any shape; ids outside the table (-1: padding) give zeros.
     first: int64 [inner + 1] on the device; ids are [outer, inner], column i counts from row
     first[i] up to first[i + 1].  out: [*ids.shape, dim], may be a strided view such as the
-    rows behind the dense one of dlrm_fwd's input; out_t: its type otherwise (the table's)."""
+    rows behind the dense one of dlrm_fwd's input, not one whose rows overlap; out_t: its type otherwise (the table's)."""
     return _bind().embedding(table, ids, scale, first, out_t, out, _handle(stream, table))
 
 

@@ -151,7 +151,7 @@ namespace b200wmma
         // in flight a thread: the same piece of U rows, or, where a block has fewer rows than that
         // (p.slices != 0), U pieces of one row, of which a block has a slice.  (4000 rows of 4954 bf16,
         // out of L2: 84 us the first way, 17 the second; one row of 16384 f16: 4.5 and 1.7.)
-        // Bound by HBM: 65536 x 26 x 128 f16 take 83 us, 5.5 TB/s of the 453 MB that are written.
+        // Bound by HBM: 65536 x 26 x 128 f16 take 83 us, 5.3 TB/s of the 436 MB that are written.
         template <typename T, typename OutT, int V>
         __global__ void __launch_bounds__(THREADS) lookupKernel(const LookupParams p)
         {
@@ -275,9 +275,17 @@ namespace b200wmma
         constexpr uint32_t SMALL_THREADS = 1024;
         constexpr uint32_t SMALL_ITEMS   = 16;
         constexpr uint32_t SMALL_TOKENS  = SMALL_THREADS * SMALL_ITEMS;
-        // One block sorts 4096 tokens in the time that the launches of the other way take (50000 rows of
-        // 32: 23 us either way; 16384 tokens: 47 and 30).  Beyond, it pays while the other SMs have rows
-        // to clear for as long: 16384 tokens and 192 MB of table 57 us either way, 537 MB 122 and 157.
+        // One block sorts up to SMALL_ALWAYS tokens, and more where there is so much table to clear for each
+        // that the other SMs have work beside it.  Whole calls, bf16 to f32, this way and the other:
+        //     rows x dim      tokens   us                rows x dim      tokens   us
+        //     50000 x 32          16   11.7  13.2        100000 x 16       4096   23.5  38.3
+        //     50000 x 32        4096   23.4  20.2        2000000 x 32     16384   56    70
+        //     32768 x 512         64   17.1  21.2        32768 x 512       4096   26.4  24.7
+        //     1000 x 128        1024   13.9  10.4        1000 x 128        4096   17.6  11.7
+        //     50000 x 128       1024   20.5  15.1        32768 x 4096     16384   131   115
+        // So it is a coarse rule: right for narrow rows and for few tokens of a long table; for wide rows
+        // the other way, whose search for rows without a token has become faster since, takes less
+        // from some hundred tokens on, and always where the table has one digit of rows.
         constexpr uint32_t SMALL_ALWAYS      = 4096;
         constexpr uint64_t SMALL_CLEAR_BYTES = 12288; // of the table, a token
         constexpr uint32_t SMALL_WARPS   = SMALL_THREADS / 32;

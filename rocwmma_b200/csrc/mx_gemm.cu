@@ -87,16 +87,16 @@ namespace b200wmma
         // ---- thin products -----------------------------------------------------------------
         // One of m and n is small (a decoding batch; one token): the other operand, whose rows
         // are the MMA's M here, 128 to a block, streams from HBM once and bounds the call.  The
-        // thin operand is the MMA's N, padded to 16 rows; its scales are one tile of 128.  A cluster of `parts` blocks shares a
-        // tile, each a stretch of K, so that the stream comes through all SMs.  Every block puts its
-        // partial sums where its ring was, and adds up its share of the thin rows out of the
-        // shared memory of the whole cluster, always in the order of the blocks.
+        // thin operand is the MMA's N, padded to 16 rows; its scales are one tile of 128.  A cluster of
+        // `parts` blocks shares a tile, each a stretch of K, so that the stream comes through all SMs.
+        // Every block puts its partial sums where its ring was, and adds up its share of the thin
+        // rows out of the shared memory of the whole cluster, always in the order of the blocks.
         //
         // A block holds columns of tensor memory only while it needs nothing of another block: it gives
         // them back before it waits for its cluster.  tcgen05.alloc waits, without a limit, until its SM
         // has a contiguous range of that size, and how ranges are placed is the hardware's business; so
         // clusters that waited for each other's blocks with columns in hand could wait for good.
-        // 1 x 8192 x 8192 MXF4: 9.1 us a call, 5.5 for its bytes; 64 x 16384 x 4096 NVF4: 12.4 and 6.
+        // 1 x 8192 x 8192 MXF4: 9.1 us a call, 5.5 for its bytes; 64 x 16384 x 4096 NVF4: 12.0 and 6.
         // (With the sums sent to the block that adds them up, and the columns held until the end: 9.5 and 13.8;
         // 8192 x 64 x 2048 MXF4: 10.4 us so, 7.0 now.)
         constexpr uint32_t THIN_ROWS = 128; // at most, of the thin operand
@@ -1007,8 +1007,9 @@ namespace b200wmma
             const uint32_t slots = (q.k + SLOT_K - 1u) / SLOT_K;
             const uint32_t tiles = mxRowTiles(p.rows);
             // K is split until the blocks fill the device: twice over for up to 32 thin rows (1 x 8192 x
-            // 8192 MXF4: 8.5 us in the kernel with 4 parts, 9.3 with 2, 11.4 with 1), once for more,
-            // whose sums cost more to exchange (64 x 16384 x 4096 NVF4: 11.3 us with 1 part, 12.0 with 2).
+            // 8192 MXF4: 8.9 us with 4 parts, 10.3 with 2, 11.5 with 1, 11.9 with 8), once for more, whose
+            // sums cost more to exchange (96 x 4096 x 4096 MXF4 f32: 7.1 us with 4 parts, 9.7 with 8; the
+            // border is coarse: 64 x 16384 x 4096 NVF4 takes 12.0 with 1 part and 10.9 with 2).
             const uint32_t resident = p.nq <= 32u ? 2u : 1u;
             p.parts                 = 8;
             while(p.parts > 1u && (uint64_t(tiles) * p.parts > resident * uint32_t(sms) || slots < 2u * p.parts))
@@ -1073,7 +1074,7 @@ namespace b200wmma
             if(sms < 2)
                 return B200WMMA_ERR_CUDA;
             const uint32_t thin = p.m < p.n ? p.m : p.n;
-            // (96 x 4096 x 4096: 7.3 us thin, 10.5 in pairs; 128 x 8192 x 8192: 14.5 and 16.9)
+            // (MXF4, 96 x 4096 x 4096 f32: 7.2 us thin, 12.1 in pairs; 128 x 8192 x 8192 bf16: 13.6 and 16.5)
             return thin <= THIN_ROWS ? launchThin<KIND, OutT>(o, p, sms, stream) : launchPairs<KIND, OutT>(o, p, sms, stream);
         }
 

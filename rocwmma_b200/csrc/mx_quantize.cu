@@ -317,8 +317,8 @@ namespace b200wmma
         // x row-major: k is contiguous.  A block takes 32 rows x 128 columns at a time: eight threads
         // have 128 values of a row, sixteen each, which is a block (NVF4) or half of one (MXF4);
         // those with the scales of four blocks write them as a word.  The values of the next tile
-        // are on their way while those of one are worked on.  (8192 x 8192 bf16 MXF4, 171 MB: 64 us
-        // with eight values a thread and maxima found as integers, 40 so; 26 at the measured copy rate.)
+        // are on their way while those of one are worked on.  (8192 x 8192 bf16 MXF4, 171 MB: 34 us; 26 at the
+        // measured copy rate; 64 with eight values a thread and maxima found as integers.)
         template <typename T, bool NV, int WIDTH>
         __global__ void __launch_bounds__(THREADS) quantizeRowsKernel(const QuantizeParams p)
         {
@@ -427,7 +427,7 @@ namespace b200wmma
         // x column-major: the rows are contiguous.  A block takes 128 rows x four blocks of k (a scale
         // tile), a thread two neighbouring rows and one block of k of each, so that a warp reads 64
         // consecutive values at a time and no maximum crosses a thread; the codes pass through
-        // shared memory to leave as rows, the scale tile to leave whole.  (5000 x 4099 f16 NVF4: 16 us.)
+        // shared memory to leave as rows, the scale tile to leave whole.  (5000 x 4099 f16 NVF4: 15.5 us.)
         template <typename T, bool NV, bool VEC>
         __global__ void __launch_bounds__(THREADS, NV ? 4 : 2) quantizeColumnsKernel(const QuantizeParams p)
         {
@@ -563,7 +563,7 @@ namespace b200wmma
         }
 
         // A block takes 32 rows x 128 columns at a time, a thread sixteen codes; those of the next
-        // tile are on their way meanwhile.  (8192 x 8192 MXF4 to bf16: 28 us, 26 for its bytes.)
+        // tile are on their way meanwhile.  (8192 x 8192 MXF4 to bf16: 31 us, 26 for its bytes.)
         template <typename T, bool NV, int WIDTH>
         __global__ void __launch_bounds__(THREADS) dequantizeKernel(const DequantizeParams p)
         {
@@ -648,8 +648,8 @@ namespace b200wmma
         }
 
         // f(32), f(16) or f(0): the boundary that rows `pitch` bytes apart start on; none: through shared
-        // memory.  (5335 x 3604 f32 NVF4, rows on 16 bytes, quantised: 56 us through shared
-        // memory, 32 so.)
+        // memory.  (Rows on 16 bytes, quantised, through shared memory and so: 5335 x 3604 f32 NVF4 51.5 and
+        // 24.1 us, 8192 x 8200 bf16 MXF4 65.9 and 37.6.)
         template <typename F>
         int withWidth(void const* base, uint64_t pitch, F f)
         {
@@ -692,7 +692,7 @@ namespace b200wmma
             };
             return withWidth(p.out, p.ldo * sizeof(T), [&](auto width) {
                 // (sixteen values of 32 bits are four pieces of 16 bytes a thread, 64 bytes apart in each store: half
-                // sectors.  5335 x 3604 f32: 24 us so, 19 through shared memory; 8192 x 8200 bf16: 44 and 49.)
+                // sectors.  5335 x 3604 f32: 24 us so, 19 through shared memory; 8192 x 8200 bf16: 41 and 48.)
                 if constexpr(width.value == 16 && sizeof(T) == 4)
                     return nv ? launch(dequantizeKernel<T, true, 0>) : launch(dequantizeKernel<T, false, 0>);
                 else
