@@ -227,6 +227,67 @@ def test_gradient_is_the_lookups():
     assert abs(((up - down) * g.double()).sum() - moved) <= 202 * 2.0 ** -24 * size
 
 
+def test_values_of_tokens_without_a_row_reach_nothing():
+    """Infinities and NaN beside ids of no row, in the gradient and in rows that nothing picks."""
+    for tokens, rows, dim in ((70, 9, 24), (5000, 40, 33), (20000, 3000, 64)):
+        ids = _ids((tokens,), rows, 1, 2.0, 0.3)
+        ids[3], ids[5] = rows, -2 ** 40
+        grad = _randn((tokens, dim), F32, 2)
+        grad[(ids < 0) | (ids >= rows)] = torch.tensor([float("nan"), float("inf")]).repeat(dim)[:dim]
+        got = api.embedding_grad(grad.cuda(), ids.cuda(), rows)
+        _check_grad(got, torch.nan_to_num(grad, 0, 0, 0), ids, rows, F32)
+        table = _randn((rows, dim), F32, 3)
+        table[rows // 2] = float("nan")
+        ids[ids == rows // 2] = -1
+        out = api.embedding(table.cuda(), ids.cuda(), scale=0.0)
+        assert not out.any()
+
+
+def test_gradients_and_lookups_on_several_streams_at_once():
+    """Calls that overlap, each with the workspace it allocates, give what they give alone."""
+    work = []
+    for i, (tokens, rows, dim) in enumerate(((300, 50, 64), (40000, 900, 40), (9000, 70000, 24), (2000, 3000, 128))):
+        grad, ids = _randn((tokens, dim), BF16, i).cuda(), _ids((tokens,), rows, i, 3.0).cuda()
+        table = _randn((rows, dim), F16, i).cuda()
+        alone = api.embedding_grad(grad, ids, rows, out_t=F32), api.embedding(table, ids, scale=3.0)
+        work.append((grad, ids, rows, table, alone, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        for grad, ids, rows, table, alone, stream in work:
+            got.append((alone, api.embedding_grad(grad, ids, rows, out_t=F32, stream=stream),
+                        api.embedding(table, ids, scale=3.0, stream=stream)))
+    torch.cuda.synchronize()
+    for alone, total, picked in got:
+        assert torch.equal(total, alone[0]) and torch.equal(picked, alone[1])
+
+
+def test_rows_behind_four_billion_values():
+    """Offsets that 32 bits do not hold: of the table, the output, the gradient and the table's gradient."""
+    rows, dim = 1050000, 4104
+    ids = torch.tensor([0, rows - 1, -1, rows - 2, rows - 1], device="cuda")
+    some = _randn((5, dim), F16, 1).cuda()
+    table = torch.zeros(rows, dim, dtype=torch.float16, device="cuda")
+    table[ids[[0, 1, 3]]] = some[:3]
+    picked = api.embedding(table, ids)
+    assert torch.equal(picked, torch.stack([some[0], some[1], torch.zeros_like(some[0]), some[2], some[1]]))
+    grad = api.embedding_grad(some, ids, rows, out=table)
+    want = torch.stack([some[0].float(), some[1].float() + some[4].float(), some[3].float()]).half()
+    assert torch.equal(grad[ids[[0, 1, 3]]], want)
+    grad[ids[[0, 1, 3]]] = 0
+    for r in range(0, rows, 50000):
+        assert not grad[r:r + 50000].any()
+    # as many tokens: the output, and the gradient that is read
+    many = torch.full((rows,), -1, device="cuda")
+    many[0], many[-1], many[-2] = 1, 2, 1
+    out = api.embedding(some, many, out=table)
+    assert torch.equal(out[[0, -2, -1]], some[[1, 1, 2]]) and not out[1:-2:1000].any()
+    total = api.embedding_grad(out, many, 5, out_t=F32)
+    want = torch.zeros(5, dim, device="cuda")
+    want[1], want[2] = 2 * some[1].float(), some[2].float()
+    assert torch.equal(total, want)
+
+
 def test_dlrm_step():
     """Lookup -> interaction -> 4-bit product, and back through the interaction to the tables."""
     from rocwmma_b200 import MXF4

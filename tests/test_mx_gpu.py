@@ -251,6 +251,83 @@ def test_gemm_beta_in_place_and_pitch(fmt):
     np.testing.assert_array_equal(_host(d).reshape(m, n), want)
 
 
+@FORMATS
+@pytest.mark.parametrize("m,n,k", [(1, 264, 4096), (300, 12, 4096), (100, 500, 3000), (1300, 2600, 200)])
+def test_gemm_in_place(fmt, m, n, k):
+    """D is C, in parts of K and over several tiles to a block."""
+    g = torch.Generator().manual_seed(4)
+    (a, av), (b, bv) = _small(fmt, m, k, g), _small(fmt, n, k, g)
+    d = torch.randint(-8, 8, (m * n,), generator=g).float().cuda()
+    want = 2 * (av @ bv.T) - _host(d).reshape(m, n)
+    api.mx_gemm(fmt, F32, m, n, k, a, b, d, 2.0, -1.0, out=d)
+    api.check_device()
+    np.testing.assert_array_equal(_host(d).reshape(m, n), want)
+
+
+@FORMATS
+def test_gemm_of_an_operand_with_itself(fmt):
+    g = torch.Generator().manual_seed(6)
+    for rows, k in ((24, 600), (400, 600)):
+        a, av = _small(fmt, rows, k, g)
+        d = api.mx_gemm(fmt, F32, rows, rows, k, a, a, None, 1.0, 0.0)
+        np.testing.assert_array_equal(_host(d).reshape(rows, rows), av @ av.T)
+
+
+@FORMATS
+@pytest.mark.parametrize("layout", [ROW_MAJOR, COL_MAJOR], ids=["rows", "columns"])
+def test_quantize_behind_four_billion_values(fmt, layout):
+    """Offsets that 32 bits do not hold; the last rows against the definition."""
+    rows, k, tail = 70001, 62000, 70
+    x = torch.zeros((rows, k) if layout == ROW_MAJOR else (k, rows), dtype=torch.bfloat16, device="cuda")
+    end = _values(tail, k, BF16, 1)
+    if layout == ROW_MAJOR:
+        x[-tail:] = end.cuda()
+    else:
+        x[:, -tail:] = end.cuda().t()
+    codes, scales = api.mx_quantize(fmt, BF16, rows, k, x, layout=layout)
+    want = R.quantize(fmt, _host(end))[2]
+    del x
+    got = api.mx_dequantize(fmt, BF16, rows, k, codes, scales).view(rows, k)
+    np.testing.assert_array_equal(_host(got[-tail:]), _host(torch.from_numpy(want).bfloat16()))
+    for r in range(0, rows - tail, 5000):
+        assert not got[r:min(r + 5000, rows - tail)].any()
+
+
+@FORMATS
+@pytest.mark.parametrize("m,n,k", [(70001, 62000, 96), (3, 2 ** 21 + 5, 4096), (2 ** 21 + 5, 20, 4096)])
+def test_gemm_behind_four_billion_values(fmt, m, n, k):
+    """D, or the codes of the streamed operand, of more than 2^32 values (4096 x 2^21 codes are 2^32 bytes)."""
+    g = torch.Generator().manual_seed(9)
+    tail = 40
+
+    def operand(rows):
+        """All rows zero but the last ones."""
+        last = min(rows, tail)
+        pitch, groups = api.mx_pitch(k), -(-k // (4 * R.BLOCK[fmt]))
+        codes = torch.zeros(rows, pitch, dtype=torch.uint8, device="cuda")
+        scales = torch.zeros(-(-rows // 128), groups, 32, 4, 4, dtype=torch.uint8, device="cuda")
+        (c, s), v = _small(fmt, last, k, g)
+        codes[-last:] = c.view(last, pitch)
+        plain = R.unpack(fmt, last, k, c.cpu().numpy(), s.cpu().numpy())[1]
+        for i in range(last):
+            r = rows - last + i
+            row = np.zeros(groups * 4, np.uint8)
+            row[:plain.shape[1]] = plain[i]
+            scales[r // 128, :, r % 32, r // 32 % 4] = torch.from_numpy(row.reshape(groups, 4)).cuda()
+        return (codes.view(-1), scales.view(-1)), v
+
+    (a, av), (b, bv) = operand(m), operand(n)
+    ld = (n + 7) // 8 * 8
+    d = api.mx_gemm(fmt, F16, m, n, k, a, b, None, 0.125, 0.0, ldd=ld).view(m, ld)
+    api.check_device()
+    want = torch.from_numpy(0.125 * (av @ bv.T)).half()
+    assert torch.equal(d[-av.shape[0]:, n - bv.shape[0]:n].cpu(), want)
+    if m > tail:
+        assert not d[:-tail, n - bv.shape[0]:n].any()
+    if n > tail:
+        assert not d[-av.shape[0]:, :n - tail].any()
+
+
 def test_quantize_and_product_in_a_graph_and_on_a_stream():
     """Captured once, replayed on new inputs; the same on a stream of its own."""
     m, n, k = 5, 640, 1024
